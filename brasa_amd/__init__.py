@@ -10,10 +10,13 @@ from .kernels import (DECODE_CHUNK, GQA_GROUPS, KV_ALIGN, AttnShape, Kernels, Kv
                       PrefillPrecision, RopeTable, decode_batch_partials_len, decode_partials_len, gqa_supported,
                       rope_table)
 from .kvcache import KvCache, kv_cache_bytes, kv_cache_len, kv_capacity, kv_offset
+from .kvpool import (KV_PAGE, KvPool, decode_paged_workspace_len, kv_pages_workspace_len,
+                     kv_pool_bytes)
 
 __all__ = [
     "AttnShape", "BrasaError", "DECODE_CHUNK", "GQA_GROUPS", "KV_ALIGN", "Kernels", "KvType",
     "LIB_PATH", "OutDType", "PrefillPrecision", "RopeTable", "build", "decode_batch_partials_len", "decode_partials_len",
     "gqa_supported", "rope_table", "KvCache", "kv_cache_bytes", "kv_cache_len", "kv_capacity",
-    "kv_offset",
+    "kv_offset", "KV_PAGE", "KvPool", "decode_paged_workspace_len", "kv_pages_workspace_len",
+    "kv_pool_bytes",
 ]

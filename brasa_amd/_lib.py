@@ -31,6 +31,13 @@ class RopeTableC(ctypes.Structure):
     _fields_ = [("cos", VP), ("sin", VP), ("dim", SZ), ("max_pos", SZ)]
 
 
+class KvPoolC(ctypes.Structure):
+    """``brasa_kv_pool``."""
+
+    _fields_ = [("k", VP), ("v", VP), ("k_exp", VP), ("v_exp", VP), ("layers", SZ), ("pages", SZ),
+                ("hkv", SZ), ("dim", SZ)]
+
+
 # name -> (restype, argtypes) for every symbol the two public headers declare
 SYMBOLS = {
     "brasa_decode_partials_len": (SZ, [SZ, SZ]),
@@ -51,6 +58,15 @@ SYMBOLS = {
     "brasa_flash_attention": (INT, [VP, VP, VP, VP, AttnShapeC, VP]),
     "brasa_flash_attention_workspace_len": (SZ, [AttnShapeC, INT]),
     "brasa_flash_attention_ws": (INT, [VP, VP, VP, VP, AttnShapeC, INT, VP, SZ, VP]),
+    "brasa_flash_attention_packed": (INT, [VP, VP, VP, VP, VP, SZ, AttnShapeC, INT, VP]),
+    "brasa_kv_pool_bytes": (SZ, [SZ, SZ, SZ, SZ]),
+    "brasa_store_kv_paged": (INT, [KvPoolC, SZ, VP, VP, VP, VP, VP, SZ, SZ, SZ, VP]),
+    "brasa_decode_paged_workspace_len": (SZ, [SZ, SZ]),
+    "brasa_decode_attention_paged": (INT, [VP, KvPoolC, SZ, VP, SZ, VP, SZ, VP, SZ, VP, INT, SZ, VP]),
+    "brasa_kv_pages_fork": (INT, [VP, VP, VP, VP, VP, VP, VP, SZ, SZ, SZ, VP]),
+    "brasa_kv_pages_workspace_len": (SZ, [SZ, SZ, SZ]),
+    "brasa_kv_pages_reserve": (INT, [KvPoolC, VP, VP, VP, VP, VP, VP, VP, SZ, SZ, VP, SZ, VP]),
+    "brasa_kv_pages_compact": (INT, [KvPoolC, VP, VP, VP, VP, VP, SZ, SZ, VP, SZ, VP]),
     "brasa_rope_table": (INT, [ctypes.c_double, SZ, SZ, VP, VP]),
     "brasa_rms_norm": (INT, [VP, VP, VP, SZ, SZ, ctypes.c_float, VP]),
     "brasa_rope_neox": (INT, [VP, RopeTableC, SZ, SZ, SZ, SZ, VP]),

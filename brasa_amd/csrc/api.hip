@@ -37,6 +37,24 @@ int prefill_launch(const float* q, const void* k, const void* v, void* o, int to
 size_t prefill_workspace_len(int tokens, int hq, int hkv, int pos0, int kv, int precision,
                              size_t* required);
 void prefill_release_workspaces();
+int packed_launch(const float* q, const void* k, const void* v, void* o, const int* cu, int n, int tokens,
+                  int hq, int hkv, int kv, int precision, hipStream_t stream);
+int store_paged_launch(const PoolArgs& pool, const float* k, const float* v, const int* cu,
+                       const int* pos, const int* table, int n, int width, int tokens,
+                       hipStream_t stream);
+size_t decode_paged_workspace_len(int hq, int hkv);
+int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, int width,
+                        const int* lk, int n, void* ws, void* o, int o_f16, int hq,
+                        hipStream_t stream);
+size_t kv_pages_workspace_len(int pages, int n, int width);
+int kv_pages_fork_launch(const int* parent, const int* table, const int* len, const int* ref,
+                         int* table_out, int* len_out, int* ref_out, int n, int width, int pages,
+                         hipStream_t stream);
+int kv_pages_reserve_launch(const PoolArgs& pool, const int* add, const int* table, const int* len,
+                            const int* ref, int* table_out, int* ref_out, int* status, int n, int width,
+                            void* ws, hipStream_t stream);
+int kv_pages_compact_launch(const PoolArgs& pool, const int* table, const int* ref, int* table_out,
+                            int* ref_out, int* live, int n, int width, void* ws, hipStream_t stream);
 
 namespace {
 thread_local char g_err[512] = "";
@@ -71,6 +89,8 @@ static bool valid_kv(int kv) {
 // Largest sizes the kernels index with 32-bit integers.
 static constexpr size_t kMaxPositions = (size_t)1 << 30;
 static constexpr size_t kMaxHeads = 1024;
+static constexpr size_t kMaxSeqs = (size_t)1 << 20;
+static constexpr size_t kMaxPages = (size_t)1 << 24;
 
 }  // namespace brasa
 
@@ -281,6 +301,171 @@ int brasa_flash_attention_ws(const float* q, const void* k, const void* v, void*
 int brasa_flash_attention(const float* q, const void* k, const void* v, void* o,
                           brasa_attn_shape shape, void* stream) {
     return brasa_flash_attention_with(q, k, v, o, shape, BRASA_PREFILL_F16, stream);
+}
+
+int brasa_flash_attention_packed(const float* q, const void* k, const void* v, void* o,
+                                 const int32_t* cu, size_t n, brasa_attn_shape s, int precision,
+                                 void* stream) {
+    g_err[0] = 0;
+    const char* what = "flash_attention_packed";
+    if (!valid_kv(s.kv)) return set_error(BRASA_ERR_ARG, "%s: invalid kv %d", what, s.kv);
+    if (precision != BRASA_PREFILL_F16 && precision != BRASA_PREFILL_F32 &&
+        precision != BRASA_PREFILL_F16_PF32)
+        return set_error(BRASA_ERR_ARG, "%s: invalid precision %d", what, precision);
+    if (s.kv == BRASA_KV_Q8_0)
+        return set_error(BRASA_ERR_UNSUPPORTED, "%s: K and V rows are f32 or f16", what);
+    if (s.dim != (size_t)kDim) return set_error(BRASA_ERR_SHAPE, "%s requires head_dim 128", what);
+    if (s.hq == 0 || s.hkv == 0 || s.hq % s.hkv != 0)
+        return set_error(BRASA_ERR_SHAPE, "hq must be a multiple of hkv");
+    if (s.pos0 != 0) return set_error(BRASA_ERR_SHAPE, "%s: whole prompts only (pos0 = %zu)", what, s.pos0);
+    if (s.hq > kMaxHeads || s.tokens > kMaxPositions / s.hq || n > kMaxSeqs)
+        return set_error(BRASA_ERR_SHAPE, "%s: shape too large", what);
+    if (s.tokens == 0 || n == 0) return BRASA_OK;
+    if (!q || !k || !v || !o || !cu) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    return packed_launch(q, k, v, o, cu, (int)n, (int)s.tokens, (int)s.hq, (int)s.hkv, s.kv, precision,
+                         as_stream(stream));
+}
+
+// The checks every call on a pool makes; `out` is the pool from `layer` on.
+static int pool_check(const char* what, brasa_kv_pool p, size_t layer, PoolArgs* out) {
+    if (p.dim != (size_t)kDim) return set_error(BRASA_ERR_SHAPE, "%s requires head_dim 128", what);
+    if (p.hkv == 0 || p.hkv > kMaxHeads) return set_error(BRASA_ERR_SHAPE, "%s: %zu KV heads", what, p.hkv);
+    if (p.pages == 0 || p.pages > kMaxPages || p.layers == 0 ||
+        p.layers > ((size_t)1 << 31) / (p.pages * p.hkv))
+        return set_error(BRASA_ERR_SHAPE, "%s: a pool of %zu layers of %zu pages", what, p.layers, p.pages);
+    if (layer >= p.layers) return set_error(BRASA_ERR_SHAPE, "%s: layer %zu of %zu", what, layer, p.layers);
+    if (!p.k || !p.v || !p.k_exp || !p.v_exp) return set_error(BRASA_ERR_ARG, "%s: null pool pointer", what);
+    if (((uintptr_t)p.k | (uintptr_t)p.v) % 16)
+        return set_error(BRASA_ERR_ARG, "%s: the codes must be 16-byte aligned", what);
+    const size_t at = layer * p.pages * p.hkv;
+    const size_t tile = (size_t)BRASA_KV_PAGE * kDim;
+    *out = PoolArgs{(uint8_t*)p.k + at * tile, (uint8_t*)p.v + at * tile, (uint8_t*)p.k_exp + at,
+                    (uint8_t*)p.v_exp + at, (int)(p.layers - layer), (int)p.pages, (int)p.hkv};
+    return BRASA_OK;
+}
+// n rows of `width` table entries
+static int table_check(const char* what, size_t n, size_t width) {
+    if (n > kMaxSeqs || width > kMaxPages || (n && width > ((size_t)1 << 30) / n))
+        return set_error(BRASA_ERR_SHAPE, "%s: a table of %zu x %zu pages is too large", what, n, width);
+    return BRASA_OK;
+}
+
+size_t brasa_kv_pool_bytes(size_t layers, size_t pages, size_t hkv, size_t dim) {
+    return layers * pages * hkv * BRASA_KV_PAGE * dim;
+}
+
+int brasa_store_kv_paged(brasa_kv_pool pool, size_t layer, const float* k, const float* v,
+                         const int32_t* cu, const int32_t* pos, const int32_t* table, size_t n,
+                         size_t width, size_t tokens, void* stream) {
+    g_err[0] = 0;
+    const char* what = "store_kv_paged";
+    PoolArgs p;
+    int st = pool_check(what, pool, layer, &p);
+    if (st == BRASA_OK) st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    if (tokens > kMaxPositions / pool.hkv) return set_error(BRASA_ERR_SHAPE, "%s: shape too large", what);
+    if (n == 0 || tokens == 0 || width == 0) return BRASA_OK;
+    if (!k || !v || !cu || !pos || !table) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if (((uintptr_t)k | (uintptr_t)v) % 16)
+        return set_error(BRASA_ERR_ARG, "%s: the rows must be 16-byte aligned", what);
+    return store_paged_launch(p, k, v, cu, pos, table, (int)n, (int)width, (int)tokens, as_stream(stream));
+}
+
+size_t brasa_decode_paged_workspace_len(size_t hq, size_t hkv) {
+    if (hkv == 0 || hq == 0 || hq % hkv != 0 || hq > kMaxHeads) return 0;
+    return decode_paged_workspace_len((int)hq, (int)hkv);
+}
+
+int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t layer,
+                                 const int32_t* table, size_t width, const int32_t* lk, size_t n,
+                                 void* workspace, size_t workspace_len, void* o, int o_dtype,
+                                 size_t hq, void* stream) {
+    g_err[0] = 0;
+    const char* what = "decode_attention_paged";
+    if (o_dtype != BRASA_OUT_F32 && o_dtype != BRASA_OUT_F16)
+        return set_error(BRASA_ERR_ARG, "%s: invalid output dtype %d", what, o_dtype);
+    PoolArgs p;
+    int st = pool_check(what, pool, layer, &p);
+    if (st == BRASA_OK) st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    if (hq == 0 || hq > kMaxHeads || hq % pool.hkv != 0)
+        return set_error(BRASA_ERR_SHAPE, "hq must be a multiple of hkv, at most %zu", kMaxHeads);
+    const size_t need = brasa_decode_paged_workspace_len(hq, pool.hkv);
+    if (workspace_len < need)
+        return set_error(BRASA_ERR_SCRATCH, "%s: workspace too small (%zu < %zu bytes)", what, workspace_len, need);
+    if (n == 0) return BRASA_OK;
+    if (!q || (!table && width) || !lk || !workspace || !o)
+        return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if ((uintptr_t)workspace % 256 || (uintptr_t)q % 16)
+        return set_error(BRASA_ERR_ARG, "%s: q must be 16-byte, the workspace 256-byte aligned", what);
+    return decode_paged_launch(q, p, table, (int)width, lk, (int)n, workspace, o,
+                               o_dtype == BRASA_OUT_F16, (int)hq, as_stream(stream));
+}
+
+int brasa_kv_pages_fork(const int32_t* parent, const int32_t* table, const int32_t* len,
+                        const int32_t* ref, int32_t* table_out, int32_t* len_out,
+                        int32_t* ref_out, size_t n, size_t width, size_t pages, void* stream) {
+    g_err[0] = 0;
+    const char* what = "kv_pages_fork";
+    const int st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    if (pages == 0 || pages > kMaxPages) return set_error(BRASA_ERR_SHAPE, "%s: %zu pages", what, pages);
+    if (n == 0 || width == 0) {
+        if (n == 0 && ref == ref_out) return BRASA_OK;
+        if (width == 0) return set_error(BRASA_ERR_SHAPE, "%s: a table without columns", what);
+    }
+    if (!parent || !table || !len || !ref || !table_out || !len_out || !ref_out)
+        return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if (table_out == table || len_out == len)
+        return set_error(BRASA_ERR_ARG, "%s: table_out and len_out must be arrays of their own", what);
+    return kv_pages_fork_launch(parent, table, len, ref, table_out, len_out, ref_out, (int)n, (int)width,
+                                (int)pages, as_stream(stream));
+}
+
+size_t brasa_kv_pages_workspace_len(size_t pages, size_t n, size_t width) {
+    if (pages > kMaxPages || n > kMaxSeqs || width > kMaxPages || (n && width > ((size_t)1 << 30) / n)) return 0;
+    return kv_pages_workspace_len((int)pages, (int)n, (int)width);
+}
+
+// What reserve and compact check alike.
+static int pages_check(const char* what, brasa_kv_pool pool, size_t n, size_t width, const void* workspace,
+                       size_t workspace_len, PoolArgs* p) {
+    int st = pool_check(what, pool, 0, p);
+    if (st == BRASA_OK) st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    const size_t need = brasa_kv_pages_workspace_len(pool.pages, n, width);
+    if (workspace_len < need)
+        return set_error(BRASA_ERR_SCRATCH, "%s: workspace too small (%zu < %zu bytes)", what, workspace_len, need);
+    if (!workspace) return set_error(BRASA_ERR_ARG, "%s: null workspace", what);
+    if ((uintptr_t)workspace % 256) return set_error(BRASA_ERR_ARG, "%s: the workspace must be 256-byte aligned", what);
+    return BRASA_OK;
+}
+
+int brasa_kv_pages_reserve(brasa_kv_pool pool, const int32_t* add, const int32_t* table,
+                           const int32_t* len, const int32_t* ref, int32_t* table_out,
+                           int32_t* ref_out, int32_t* status, size_t n, size_t width,
+                           void* workspace, size_t workspace_len, void* stream) {
+    g_err[0] = 0;
+    PoolArgs p;
+    const int st = pages_check("kv_pages_reserve", pool, n, width, workspace, workspace_len, &p);
+    if (st != BRASA_OK) return st;
+    if (!ref || !ref_out || !status || (n && (!add || !len)) || (n && width && (!table || !table_out)))
+        return set_error(BRASA_ERR_ARG, "kv_pages_reserve: null pointer");
+    return kv_pages_reserve_launch(p, add, table, len, ref, table_out, ref_out, status, (int)n, (int)width,
+                                   workspace, as_stream(stream));
+}
+
+int brasa_kv_pages_compact(brasa_kv_pool pool, const int32_t* table, const int32_t* ref,
+                           int32_t* table_out, int32_t* ref_out, int32_t* live, size_t n,
+                           size_t width, void* workspace, size_t workspace_len, void* stream) {
+    g_err[0] = 0;
+    PoolArgs p;
+    const int st = pages_check("kv_pages_compact", pool, n, width, workspace, workspace_len, &p);
+    if (st != BRASA_OK) return st;
+    if (!ref || !ref_out || !live || (n && width && (!table || !table_out)))
+        return set_error(BRASA_ERR_ARG, "kv_pages_compact: null pointer");
+    return kv_pages_compact_launch(p, table, ref, table_out, ref_out, live, (int)n, (int)width, workspace,
+                                   as_stream(stream));
 }
 
 int brasa_rope_table(double theta, size_t dim, size_t max_pos, float* cos_out, float* sin_out) {

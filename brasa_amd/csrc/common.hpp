@@ -55,6 +55,16 @@ __host__ __device__ inline SplitBlocks split_blocks(int lk, int splits, int spli
     return SplitBlocks{32 * split, 32 * splits, (nblocks - split + splits - 1) / splits};
 }
 
+// A pool of the paged cache as the launchers take it: the codes and scale bytes of K and V, the
+// layers, and the pages and KV heads of one (see brasa_kv_pool).
+struct PoolArgs {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* kx;  // scale bytes
+    uint8_t* vx;
+    int layers, pages, hkv;
+};
+
 // ---- f16 helpers --------------------------------------------------------------------------
 __device__ __forceinline__ float h2f(uint16_t h) {
     return static_cast<float>(__ushort_as_half(h));

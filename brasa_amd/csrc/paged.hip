@@ -1,0 +1,546 @@
+// The 8-bit paged KV cache: its writer and the decode attention that reads it.
+#include "paged.hpp"
+
+namespace brasa {
+namespace {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+
+// ---- store ------------------------------------------------------------------------------------
+//
+// Row t of the packed new rows belongs to sequence i with cu[i] <= t < cu[i + 1] and goes to
+// position pos[i] + t - cu[i]. A block (page) and head is written by one workgroup, K and V by one
+// each: it holds the block's new rows in registers, takes their largest magnitude, the scale
+// from it (and from the block's scale, where earlier rows of the block stay), rounds those
+// earlier rows to a larger scale, and writes the codes.
+//
+// Bound: HBM at 4 bytes in and 1 out a value for prompts; a decode step's few rows are bound by
+// the chain cu / pos -> page id -> scale -> codes.
+constexpr int kStoreThreads = 256;
+
+struct StoreArgs {
+    PoolArgs p;  // of one layer
+    const float* k;
+    const float* v;
+    const int* cu;
+    const int* pos;
+    const int* table;
+    int n, width, tokens;
+};
+
+// the blocks that sequence i's new rows touch: [first, first + count)
+__device__ __forceinline__ int touched_blocks(const StoreArgs& a, int i, int& c0, int& c1, int& pos) {
+    c0 = min(max(a.cu[i], 0), a.tokens);
+    c1 = min(max(a.cu[i + 1], c0), a.tokens);
+    pos = a.pos[i];
+    // (a negative position, or one past what the table can hold, has no block)
+    if (c1 == c0 || pos < 0 || pos >= a.width * kPage) return 0;
+    return min((pos + (c1 - c0) - 1) / kPage, a.width - 1) - pos / kPage + 1;
+}
+
+__global__ void __launch_bounds__(kStoreThreads)
+store_paged_kernel(StoreArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int item = blockIdx.x / a.p.hkv, kh = blockIdx.x % a.p.hkv;
+    const bool is_v = blockIdx.y;
+
+    // the sequence and block of this item: every wave walks the sequences' block counts, 64 at a
+    // time
+    int seq = -1, before = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 64) {
+        int c0, c1, pos, nb = 0;
+        if (i0 + lane < a.n) nb = touched_blocks(a, i0 + lane, c0, c1, pos);
+        const int incl = wave_scan(nb) + before;
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > item);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            seq = i0 + l;
+            before = __shfl(incl - nb, l);
+            break;
+        }
+        before = __shfl(incl, 63);
+    }
+    if (seq < 0) return;  // the grid's bound is loose
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    int c0, c1, pos;
+    touched_blocks(a, seq, c0, c1, pos);
+    const int block = pos / kPage + item - before;
+    const int page = a.table[(size_t)seq * a.width + block];
+    if (page < 0 || page >= a.p.pages) return;
+    // slots [s0, s1) of the block are new, [0, s0) hold earlier rows
+    const int s0 = max(pos - block * kPage, 0);
+    const int s1 = min(pos + (c1 - c0) - block * kPage, kPage);
+    const size_t tile = (size_t)page * a.p.hkv + kh;
+    uint8_t* codes = (is_v ? a.p.v : a.p.k) + tile * kTileBytes8;
+    uint8_t* scale = (is_v ? a.p.vx : a.p.kx) + tile;
+    const int row0 = c0 + block * kPage - pos;  // the packed row of slot 0
+    const float* src = (is_v ? a.v : a.k) + kh * kDim + 4 * (threadIdx.x & 31);
+
+    const int old = s0 > 0 ? *scale : 0;
+    f32x4 x[8];
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int s = 8 * j + (threadIdx.x >> 5);
+        x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (s >= s0 && s < s1)
+            x[j] = *reinterpret_cast<const f32x4*>(src + (size_t)(row0 + s) * a.p.hkv * kDim);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float m = fabsf(x[j][e]);
+            amax = fmaxf(amax, m < INFINITY ? m : 0.0f);  // NaN and inf take no part in the scale
+        }
+    __shared__ float s_max[kStoreThreads / 64];
+#pragma unroll
+    for (int d = 32; d; d /= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if (lane == 0) s_max[threadIdx.x >> 6] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kStoreThreads / 64; ++w) amax = fmaxf(amax, s_max[w]);
+    const int ex = max(e4m3_scale(amax), old);
+
+    if (s0 > 0 && ex > old) {
+        // the earlier rows, rounded to the larger scale (exact but where they leave e4m3's normal
+        // range)
+        for (int i = threadIdx.x; i < s0 * (kDim / 4); i += kStoreThreads) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
+            const uint32_t c = *w;
+            float y[4];
+            y[0] = __builtin_amdgcn_cvt_f32_fp8(c, 0);
+            y[1] = __builtin_amdgcn_cvt_f32_fp8(c, 1);
+            y[2] = __builtin_amdgcn_cvt_f32_fp8(c, 2);
+            y[3] = __builtin_amdgcn_cvt_f32_fp8(c, 3);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // (a NaN code keeps its sign too)
+                if ((c >> 8 * e & 0x7fu) == 0x7fu) y[e] = __uint_as_float(0x7fc00000u | (c >> 8 * e << 24 & 0x80000000u));
+            *w = e4m3_quad(y, old - ex);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int s = 8 * j + (threadIdx.x >> 5);
+        if (s >= s0 && s < s1) {
+            const float y[4] = {x[j][0], x[j][1], x[j][2], x[j][3]};
+            reinterpret_cast<uint32_t*>(codes)[s * (kDim / 4) + (threadIdx.x & 31)] = e4m3_quad(y, 127 - ex);
+        }
+    }
+    // (every thread that needed the old scale has read it before the barrier above)
+    if (threadIdx.x == 0) *scale = (uint8_t)ex;
+}
+
+// ---- decode -----------------------------------------------------------------------------------
+//
+// o[i, h] = sum_j p_j v_j / sum_j p_j over the lk[i] keys of sequence i, p_j = exp(q . k_j / sqrt(128)).
+//
+// Bound: HBM, 256 bytes of codes per (key, KV head). The pages of all sequences stand in one line,
+// and workgroup w of a head takes the w-th equal run of them, so every CU reads the same number
+// whatever the lengths, which only the device knows. A run's pieces of one sequence are its
+// segments; a segment that is not the whole sequence leaves (m, l, acc) in the workspace, and
+// the last workgroup of a sequence to arrive merges them in order (a fixed order: the result does
+// not depend on who arrives last).
+//
+// A wave takes every kWaves-th page of a segment, all of it in registers: S^T = K Q^T on 16x16x32
+// f16 MFMAs with the 16 columns holding the group's query heads (repeated), K's codes converted
+// exactly (an e4m3 value is an f16 value) right from the loaded 16-byte pieces, and Q as
+// f16 hi + lo halves, which keep 22 bits. A lane then holds four keys of each 16 for its head, which
+// is the layout P^T needs for O^T = V^T P^T, also in hi + lo halves. V's operand needs eight keys of one
+// dim in a lane: the lane loads 8 bytes of each of its eight keys' rows (dims 8 i .. 8 i + 7 of lane
+// row i) and byte permutes pair the keys before the conversion, so V needs no LDS either. The block's
+// scales are exponents: K's is added to the scores' exponent, V's multiplies the page's sum.
+constexpr int kWaves = 4;
+constexpr int kDecThreads = 64 * kWaves;
+constexpr int kMaxCols = 16;     // query heads of a workgroup
+constexpr int kSlots = 512;      // workgroups of a launch: two per CU
+constexpr int kMinPages = 8;     // pages of a run, at least (two per wave)
+constexpr int kPartFloats = kDim + 2;
+constexpr int kCounterStride = 16;  // words between two arrival counters
+
+struct DecodePagedArgs {
+    const float* q;
+    PoolArgs p;  // of one layer
+    const int* table;
+    const int* lk;
+    void* o;
+    float* part;
+    unsigned* ctr;
+    int n, width, hq, group, runs, o_f16;
+};
+
+__device__ __forceinline__ f32x4 mfma16(half8v a, half8v b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// 4 codes -> 4 f16 values, exact
+__device__ __forceinline__ half2v f16_of_lo(uint32_t w) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+}
+__device__ __forceinline__ half2v f16_of_hi(uint32_t w) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+}
+__device__ __forceinline__ half8v join(half2v a, half2v b, half2v c, half2v d) {
+    return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// x = hi + lo up to 2^-22 of x
+__device__ __forceinline__ void split2(float x, float y, half2v& hi, half2v& lo) {
+    x = as_f32(x);
+    y = as_f32(y);
+    hi = half2v{(_Float16)x, (_Float16)y};
+    lo = half2v{(_Float16)fmaf((float)hi.x, -1.0f, x), (_Float16)fmaf((float)hi.y, -1.0f, y)};
+}
+__device__ __forceinline__ float max_u(float x) {  // over the four lanes of a column
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_u(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+// pages of a sequence of lk keys in the line of pages: at least one, so that a sequence without
+// keys has a workgroup that writes its zeros, and a length the table cannot hold one that
+// writes its NaN
+__device__ __forceinline__ int line_pages(int lk, int width) {
+    return lk <= 0 || lk > width * kPage ? 1 : (lk + kPage - 1) / kPage;
+}
+__device__ __forceinline__ void st_part(float* p, float x) {
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float ld_part(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ void __launch_bounds__(kDecThreads, 2)
+decode_paged_kernel(DecodePagedArgs a) {
+    __shared__ float s_acc[kWaves][kMaxCols][kDim];
+    __shared__ float s_m[kWaves][kMaxCols], s_l[kWaves][kMaxCols];
+    __shared__ unsigned s_last;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, u = lane >> 4;
+    const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv;
+    const int h0 = kh * a.group + blockIdx.y * kMaxCols;          // first query head
+    const int cols = min(a.group - (int)blockIdx.y * kMaxCols, kMaxCols);
+    const int head_of_lane = h0 + min(c, cols - 1);
+
+    // ---- this workgroup's run of the line of pages -------------------------------------------
+    int total = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 64) {
+        const int i = i0 + lane;
+        total += i < a.n ? line_pages(a.lk[i], a.width) : 0;
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) total += __shfl_xor(total, d);
+    const int size = max((total + a.runs - 1) / a.runs, kMinPages);
+    int at = run * size;
+    const int end = min(at + size, total);
+    if (at >= end) return;
+    int seq = 0, seq_at = 0;  // the sequence that holds page `at`, and its first page in the line
+    for (int i0 = 0; i0 < a.n; i0 += 64) {
+        const int np = i0 + lane < a.n ? line_pages(a.lk[i0 + lane], a.width) : 0;
+        const int incl = wave_scan(np) + seq_at;
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            seq = i0 + l;
+            seq_at = __shfl(incl - np, l);
+            break;
+        }
+        seq_at = __shfl(incl, 63);
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    seq_at = __builtin_amdgcn_readfirstlane(seq_at);
+
+    for (; at < end; ++seq) {
+        const int lk_raw = a.lk[seq];
+        const int np = line_pages(lk_raw, a.width);
+        const bool bad_len = lk_raw < 0 || lk_raw > a.width * kPage;
+        const int lk = bad_len ? 0 : lk_raw;
+        const int b0 = at - seq_at;                        // pages [b0, b1) of the sequence
+        const int b1 = min(end - seq_at, np);
+        const bool whole = b0 == 0 && b1 == np;
+
+        // ---- Q: hi and lo halves of q / sqrt(128) * log2 e, its exponent taken out --------------
+        // k-step t = 2 hh + j holds dims 64 hh + 16 u + 8 j .. + 8, as K's 16-byte loads do
+        half8v qh[4], ql[4];
+        int qx;
+        {
+            const float* qrow = a.q + ((size_t)seq * a.hq + head_of_lane) * kDim + 16 * u;
+            const float scale = 0.08838834764831845f * kLog2e;
+            float x[4][8];
+            float qmax = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[t][e] = as_f32(qrow[64 * (t >> 1) + 8 * (t & 1) + e] * scale);
+                    qmax = fmaxf(qmax, fabsf(x[t][e]));
+                }
+            qmax = max_u(qmax);
+            qx = (int)(__float_as_uint(qmax) >> 23) - 127 - 8;  // the row's largest to [2^8, 2^9)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                half2v hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    split2(ldexpf(x[t][2 * e], -qx), ldexpf(x[t][2 * e + 1], -qx), hi[e], lo[e]);
+                qh[t] = join(hi[0], hi[1], hi[2], hi[3]);
+                ql[t] = join(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+
+        float m_used = -INFINITY, lsum = 0.0f;
+        f32x4 acc[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        bool bad = false;
+
+        const int* ids = a.table + (size_t)seq * a.width;
+        for (int b = b0 + wave; lk > 0 && b < b1; b += kWaves) {
+            int page = ids[b];
+            if (page < 0 || page >= a.p.pages) {  // never read: the sequence's output is NaN
+                bad = true;
+                continue;
+            }
+            const size_t tile = (size_t)page * a.p.hkv + kh;
+            const uint8_t* kt = a.p.k + tile * kTileBytes8 + c * kDim + 16 * u;
+            const uint8_t* vt = a.p.v + tile * kTileBytes8 + 4 * u * kDim + 8 * c;
+            u32x4 kr[4][2];
+            u32x2 vr[4][4];
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+                    kr[T][hh] = *reinterpret_cast<const u32x4*>(kt + 16 * T * kDim + 64 * hh);
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    vr[T][r] = *reinterpret_cast<const u32x2*>(vt + (16 * T + r) * kDim);
+            const int kx = a.p.kx[tile], vx = a.p.vx[tile];
+
+            // ---- scores: key 16 T + 4 u + r of head c, in units of log2 ---------------------------
+            f32x4 s[4];
+#pragma unroll
+            for (int T = 0; T < 4; ++T) {
+                s[T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t w0 = kr[T][t >> 1][2 * (t & 1)], w1 = kr[T][t >> 1][2 * (t & 1) + 1];
+                    const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
+                    s[T] = mfma16(ka, qh[t], s[T]);
+                    s[T] = mfma16(ka, ql[t], s[T]);
+                }
+            }
+            const int left = lk - b * kPage;  // live keys of the page
+            float tmax = -INFINITY;
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[T][r] = ldexpf(s[T][r], qx + kx - 127);
+                    if (left < kPage && 16 * T + 4 * u + r >= left) s[T][r] = -INFINITY;
+                    tmax = fmaxf(tmax, s[T][r]);
+                }
+            tmax = max_u(tmax);
+            // a reference point that moves only when the maximum has grown by 2^8: p stays below
+            // 2^15 with the bias of 2^7 that keeps the lo halves of small p out of f16's subnormals
+            const bool grow = tmax > m_used + 8.0f;
+            if (__builtin_amdgcn_ballot_w64(grow)) {
+                const float alpha = grow ? __builtin_amdgcn_exp2f(m_used - tmax) : 1.0f;
+                if (grow) m_used = tmax;
+                lsum *= alpha;
+#pragma unroll
+                for (int t = 0; t < 8; ++t) acc[t] *= alpha;
+            }
+            half8v ph[2], pl[2];
+            const float mb = m_used - 7.0f;
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                half2v hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int T = 2 * st + (e >> 1), r = 2 * (e & 1);
+                    const float p0 = __builtin_amdgcn_exp2f(s[T][r] - mb);
+                    const float p1 = __builtin_amdgcn_exp2f(s[T][r + 1] - mb);
+                    lsum += p0 + p1;
+                    split2(p0, p1, hi[e], lo[e]);
+                }
+                ph[st] = join(hi[0], hi[1], hi[2], hi[3]);
+                pl[st] = join(lo[0], lo[1], lo[2], lo[3]);
+            }
+            if (left < kPage) {  // codes behind the last key may be anything, NaN too
+#pragma unroll
+                for (int T = 0; T < 4; ++T)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * T + 4 * u + r >= left) vr[T][r] = u32x2{0, 0};
+            }
+            const float vs = ldexpf(1.0f, vx - 127);
+            // ---- O^T += V^T P^T: tile t's rows are dims 8 i + t ------------------------------------
+#pragma unroll
+            for (int t2 = 0; t2 < 4; ++t2) {  // tiles 2 t2, 2 t2 + 1
+                f32x4 pv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                const int d = t2 >> 1;
+                const uint32_t b = 2 * (t2 & 1);
+                const uint32_t sel = b | (4 + b) << 8 | (b + 1) << 16 | (5 + b) << 24;
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    half2v x0[4], x1[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int T = 2 * st + (e >> 1), r = 2 * (e & 1);
+                        const uint32_t w = __builtin_amdgcn_perm(vr[T][r + 1][d], vr[T][r][d], sel);
+                        x0[e] = f16_of_lo(w);
+                        x1[e] = f16_of_hi(w);
+                    }
+                    const half8v v0 = join(x0[0], x0[1], x0[2], x0[3]);
+                    const half8v v1 = join(x1[0], x1[1], x1[2], x1[3]);
+                    pv[0] = mfma16(v0, ph[st], pv[0]);
+                    pv[1] = mfma16(v1, ph[st], pv[1]);
+                    pv[0] = mfma16(v0, pl[st], pv[0]);
+                    pv[1] = mfma16(v1, pl[st], pv[1]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[2 * t2 + j][r] = fmaf(pv[j][r], vs, acc[2 * t2 + j][r]);
+            }
+        }
+
+        // ---- the waves' states into one ----------------------------------------------------------
+        if (bad || bad_len) lsum = NAN;
+        lsum = sum_u(lsum);
+        if (c < cols) {
+            if (u == 0) {
+                s_m[wave][c] = m_used;
+                s_l[wave][c] = lsum;
+            }
+            // the lane holds dims 32 u + 8 r + t of its head
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < 8; ++t) s_acc[wave][c][32 * u + 8 * r + t] = acc[t][r];
+        }
+        __syncthreads();
+        const size_t out0 = ((size_t)seq * a.hq + h0) * kDim;
+        const int wg = run * a.p.hkv + kh;  // of this blockIdx.y
+        const size_t planes = (size_t)a.runs * a.p.hkv;
+        auto part_of = [&](int r, int second, int col) {
+            return a.part + ((((size_t)blockIdx.y * planes + (size_t)r * a.p.hkv + kh) * 2 + second) *
+                                 kMaxCols + col) * kPartFloats;
+        };
+        for (int i = threadIdx.x; i < cols * kDim; i += kDecThreads) {
+            const int col = i / kDim, d = i % kDim;
+            float m = s_m[0][col];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][col]);
+            float l = 0.0f, x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                // a wave without a page has m = -inf, l = 0 (or NaN for a page that is not there)
+                const float f = s_m[w][col] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][col] - m);
+                l += s_m[w][col] == -INFINITY ? s_l[w][col] : s_l[w][col] * f;
+                x = fmaf(s_acc[w][col][d], f, x);
+            }
+            if (whole) {
+                // no keys: zeros (a length out of range has l = NaN)
+                const float y = l == 0.0f ? 0.0f : x / l;
+                if (a.o_f16) static_cast<uint16_t*>(a.o)[out0 + i] = f2h(y);
+                else static_cast<float*>(a.o)[out0 + i] = y;
+            } else {
+                float* p = part_of(run, b0 > 0 || at == run * size ? 0 : 1, col);
+                st_part(p + 2 + d, x);
+                if (d == 0) st_part(p, m);
+                if (d == 1) st_part(p + 1, l);
+            }
+        }
+        if (!whole) {
+            // ---- the last segment of the sequence to arrive merges all of them ------------------
+            const int r0 = seq_at / size, r1 = (seq_at + np - 1) / size;  // the runs that hold it
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                unsigned* ctr = a.ctr + ((size_t)blockIdx.y * planes + (size_t)r0 * a.p.hkv + kh) * kCounterStride;
+                s_last = atomicInc(ctr, r1 - r0) == (unsigned)(r1 - r0);
+            }
+            __syncthreads();
+            if (s_last) {
+                const int first = seq_at == r0 * size ? 0 : 1;
+                for (int i = threadIdx.x; i < cols * kDim; i += kDecThreads) {
+                    const int col = i / kDim, d = i % kDim;
+                    float m = -INFINITY;
+                    for (int r = r0; r <= r1; ++r) m = fmaxf(m, ld_part(part_of(r, r == r0 ? first : 0, col)));
+                    float l = 0.0f, x = 0.0f;
+                    for (int r = r0; r <= r1; ++r) {
+                        const float* p = part_of(r, r == r0 ? first : 0, col);
+                        const float mr = ld_part(p), lr = ld_part(p + 1);
+                        const float f = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - m);
+                        l += mr == -INFINITY ? lr : lr * f;
+                        x = fmaf(ld_part(p + 2 + d), f, x);
+                    }
+                    const float y = x / l;
+                    if (a.o_f16) static_cast<uint16_t*>(a.o)[out0 + i] = f2h(y);
+                    else static_cast<float*>(a.o)[out0 + i] = y;
+                }
+            }
+        }
+        (void)wg;
+        __syncthreads();  // the LDS is free for the next segment
+        at = seq_at + b1;
+        seq_at += np;
+    }
+}
+
+int decode_runs(int hkv, int chunks) { return std::max(kSlots / (hkv * chunks), 1); }
+
+}  // namespace
+
+int store_paged_launch(const PoolArgs& pool, const float* k, const float* v, const int* cu,
+                       const int* pos, const int* table, int n, int width, int tokens,
+                       hipStream_t stream) {
+    StoreArgs a{pool, k, v, cu, pos, table, n, width, tokens};
+    // blocks touched: a sequence of r rows touches (r - 1) / 64 + 2 at most
+    const long long m = std::min(n, tokens);
+    const long long items = (tokens - m) / kPage + 2 * m;
+    hipLaunchKernelGGL(store_paged_kernel, dim3((unsigned)(items * pool.hkv), 2), dim3(kStoreThreads), 0,
+                       stream, a);
+    return check_launch("store_paged_kernel");
+}
+
+static size_t decode_paged_ctr_bytes(int hkv, int chunks) {
+    return (size_t)chunks * decode_runs(hkv, chunks) * hkv * kCounterStride * sizeof(unsigned);
+}
+size_t decode_paged_workspace_len(int hq, int hkv) {
+    const int chunks = (hq / hkv + kMaxCols - 1) / kMaxCols;
+    return decode_paged_ctr_bytes(hkv, chunks) +
+           (size_t)chunks * decode_runs(hkv, chunks) * hkv * 2 * kMaxCols * kPartFloats * sizeof(float);
+}
+
+int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, int width,
+                        const int* lk, int n, void* ws, void* o, int o_f16, int hq,
+                        hipStream_t stream) {
+    DecodePagedArgs a;
+    a.q = q;
+    a.p = pool;
+    a.table = table;
+    a.lk = lk;
+    a.o = o;
+    a.n = n;
+    a.width = width;
+    a.hq = hq;
+    a.group = hq / pool.hkv;
+    a.o_f16 = o_f16;
+    const int chunks = (a.group + kMaxCols - 1) / kMaxCols;
+    a.runs = decode_runs(pool.hkv, chunks);
+    a.ctr = static_cast<unsigned*>(ws);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + decode_paged_ctr_bytes(pool.hkv, chunks));
+    hipLaunchKernelGGL(decode_paged_kernel, dim3((unsigned)(a.runs * pool.hkv), chunks), dim3(kDecThreads),
+                       0, stream, a);
+    return check_launch("decode_paged_kernel");
+}
+
+}  // namespace brasa

@@ -246,3 +246,49 @@ class Kernels:
         check(lib().brasa_flash_attention_ws(_ptr(q), _ptr(k), _ptr(v), _ptr(o), shape.c(),
                                              int(precision), _ptr(workspace), wlen,
                                              _stream(stream or self.stream)))
+
+    def flash_attention_packed(self, q, k, v, o, cu, n: int, shape: AttnShape,
+                               precision: PrefillPrecision = PrefillPrecision.F16,
+                               stream=None) -> None:
+        """Causal attention over ``n`` packed prompts (no reference counterpart): prompt i holds rows
+        ``cu[i] .. cu[i + 1]`` of the ``shape.tokens`` rows of q, k, v and o; ``cu`` is a device
+        array of n + 1 int32. ``shape.kv`` is the type of k and v (F32 or F16)."""
+        check(lib().brasa_flash_attention_packed(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(cu), n,
+                                                 shape.c(), int(precision),
+                                                 _stream(stream or self.stream)))
+
+    # The paged 8-bit cache (no reference counterpart). ``pool`` is a KvPool; table, lengths and
+    # counts are device arrays of int32 (brasa_attn.h says what each call reads and writes).
+
+    def store_kv_paged(self, pool, layer: int, k, v, cu, pos, table, n: int, width: int,
+                       tokens: int, stream=None) -> None:
+        check(lib().brasa_store_kv_paged(pool.c(), layer, _ptr(k), _ptr(v), _ptr(cu), _ptr(pos),
+                                         _ptr(table), n, width, tokens,
+                                         _stream(stream or self.stream)))
+
+    def decode_attention_paged(self, q, pool, layer: int, table, lk, n: int, width: int, workspace,
+                               workspace_len: int, o, hq: int, out: OutDType = OutDType.F32,
+                               stream=None) -> None:
+        check(lib().brasa_decode_attention_paged(_ptr(q), pool.c(), layer, _ptr(table), width,
+                                                 _ptr(lk), n, _ptr(workspace), workspace_len,
+                                                 _ptr(o), int(out), hq,
+                                                 _stream(stream or self.stream)))
+
+    def kv_pages_fork(self, parent, table, lens, ref, table_out, lens_out, ref_out, n: int,
+                      width: int, pages: int, stream=None) -> None:
+        check(lib().brasa_kv_pages_fork(_ptr(parent), _ptr(table), _ptr(lens), _ptr(ref),
+                                        _ptr(table_out), _ptr(lens_out), _ptr(ref_out), n, width,
+                                        pages, _stream(stream or self.stream)))
+
+    def kv_pages_reserve(self, pool, add, table, lens, ref, table_out, ref_out, status, n: int,
+                         width: int, workspace, workspace_len: int, stream=None) -> None:
+        check(lib().brasa_kv_pages_reserve(pool.c(), _ptr(add), _ptr(table), _ptr(lens), _ptr(ref),
+                                           _ptr(table_out), _ptr(ref_out), _ptr(status), n, width,
+                                           _ptr(workspace), workspace_len,
+                                           _stream(stream or self.stream)))
+
+    def kv_pages_compact(self, pool, table, ref, table_out, ref_out, live, n: int, width: int,
+                         workspace, workspace_len: int, stream=None) -> None:
+        check(lib().brasa_kv_pages_compact(pool.c(), _ptr(table), _ptr(ref), _ptr(table_out),
+                                           _ptr(ref_out), _ptr(live), n, width, _ptr(workspace),
+                                           workspace_len, _stream(stream or self.stream)))

@@ -359,6 +359,143 @@ int brasa_decode_trace_read(unsigned long long* dst, size_t n);
 int brasa_prefill_trace_read(unsigned long long* dst, size_t n);
 #endif
 
+/* ---- packed prompts -------------------------------------------------------------------------- */
+
+/*
+ * Causal attention over n whole prompts packed one behind the other (no counterpart in the
+ * reference, which prefills one sequence per call, lib.rs:1185-1248). q: [tokens, hq, 128] f32;
+ * k, v: [tokens, hkv, 128] rows of the type shape.kv (BRASA_KV_F32 or BRASA_KV_F16; a prompt's own
+ * rows are not read back from an 8-bit cache: BRASA_ERR_UNSUPPORTED for q8_0); o: [tokens, hq, 128],
+ * f16 for BRASA_PREFILL_F16 / _F16_PF32, f32 for _F32, with brasa_flash_attention_with's numerics
+ * (softmax and sums in f32). cu: DEVICE array of n + 1 row numbers, 0 <= cu[0] <= ... <= cu[n] <=
+ * tokens: prompt i holds rows cu[i] .. cu[i + 1], none where the two are equal, and its row t attends
+ * to its rows up to t. Rows before cu[0] and from cu[n] on are neither read for another row's
+ * result nor written. The lengths are read on the device: a captured graph may be replayed with other
+ * cu. Values of cu outside that order are clamped to it (no access leaves the arrays); two prompts
+ * that would then overlap give unspecified values. K and V of a prompt must be finite (a row's V
+ * that is not spoils earlier rows of its prompt, never another prompt's). Any hq a multiple of
+ * hkv; dim 128; shape.pos0 must be 0. Allocates nothing, needs no workspace.
+ */
+int brasa_flash_attention_packed(const float* q, const void* k, const void* v, void* o,
+                                 const int32_t* cu, size_t n, brasa_attn_shape shape,
+                                 int precision, void* stream);
+
+/* ---- the paged 8-bit cache ------------------------------------------------------------------- */
+
+/* Positions of a page. */
+#define BRASA_KV_PAGE 64
+
+/*
+ * A pool of cache pages (no counterpart in the reference, whose caches are one run of rows per
+ * sequence). A page holds BRASA_KV_PAGE positions of every KV head in each layer. k, v: codes
+ * [layers][pages][hkv][64][128], one e4m3 byte each (OCP: largest value 448, 0x7f and 0xff NaN);
+ * k_exp, v_exp: scale bytes [layers][pages][hkv]. A code c of a (page, head) with scale byte x
+ * stands for e4m3(c) * 2^(x - 127). Pointers are 16-byte aligned (the scale bytes' need not be);
+ * dim must be 128.
+ *
+ * The scale: x is the least byte with amax <= 448 * 2^(x - 127), amax the largest finite
+ * magnitude among the values the block has been written with since its first position was (so a
+ * scale never shrinks while its block grows); a block whose scale grows has its earlier codes rounded
+ * to the new one, exactly except below 2^-6 of it. A power of two costs an e4m3 code no
+ * accuracy, and the attention adds it to an exponent. NaN and infinities become the NaN code.
+ */
+typedef struct brasa_kv_pool {
+    void* k;
+    void* v;
+    void* k_exp;
+    void* v_exp;
+    size_t layers;
+    size_t pages;
+    size_t hkv;
+    size_t dim;
+} brasa_kv_pool;
+
+/* layers * pages * hkv * 64 * 128: code bytes of k (or v); a 64th of a 128th of it in k_exp. */
+size_t brasa_kv_pool_bytes(size_t layers, size_t pages, size_t hkv, size_t dim);
+
+/*
+ * The tables, lengths and counts of the calls below are DEVICE arrays of int32, so a step whose
+ * sequences grow, fork or end replays one captured graph. table: [n, width] page ids, row i the
+ * pages of sequence i in order (position p in entry p / 64), -1 where it has none. Ids out of
+ * [0, pages) are never followed.
+ */
+
+/*
+ * Writes packed new rows k, v ([tokens, hkv, 128] f32; sequence i's are cu[i] .. cu[i + 1], as in
+ * brasa_flash_attention_packed, cu: [n + 1]) into the pages of `layer`, at positions pos[i],
+ * pos[i] + 1, ... of sequence i (pos: [n]). A prompt's rows and a decode step's (one per
+ * sequence) take the same call. Positions from a block's first to pos[i] keep their values (see the
+ * scale above); a block written from its first position on starts anew. Positions behind the
+ * last one written are left as they were. Rows whose position has no page (a negative pos, past the
+ * table's width, an id out of range) are dropped. A page that a call writes must belong to one
+ * sequence only (brasa_kv_pages_reserve). Rows of k and v 16-byte aligned.
+ */
+int brasa_store_kv_paged(brasa_kv_pool pool, size_t layer, const float* k, const float* v,
+                         const int32_t* cu, const int32_t* pos, const int32_t* table, size_t n,
+                         size_t width, size_t tokens, void* stream);
+
+/*
+ * Decode attention over the paged cache: query q[i] ([n, hq, 128] f32) of sequence i over its first
+ * lk[i] positions (lk: [n]; the new token's included) in `layer`. o: [n, hq, 128] in o_dtype. Any
+ * hq a multiple of hkv. Codes behind position lk[i] are never used, whatever they hold. lk[i] == 0
+ * gives zeros; a negative lk[i], one past 64 * width, or a page id out of range among the pages it
+ * reads gives NaN in that sequence's rows.
+ *
+ * All sequences' pages are cut into equal runs, one per workgroup, so a launch is balanced whatever
+ * the lengths; a sequence in several runs is merged in the launch, in a fixed order. The result
+ * bits of a sequence depend on the lengths of all (as brasa_decode_attention_batch's do), not on
+ * timing. workspace: brasa_decode_paged_workspace_len(hq, pool.hkv) bytes, 256-byte aligned; its arrival
+ * counters must be zero before its first use (clear it once, e.g. brasa_rt_fill_u8) and every
+ * call leaves them zero. Calls that may run at the same time (other streams, replays of other graphs)
+ * need workspaces of their own. Nothing else is shared between calls.
+ */
+size_t brasa_decode_paged_workspace_len(size_t hq, size_t hkv);
+int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t layer,
+                                 const int32_t* table, size_t width, const int32_t* lk, size_t n,
+                                 void* workspace, size_t workspace_len, void* o, int o_dtype,
+                                 size_t hq, void* stream);
+
+/*
+ * Forks and frees: row i of table_out / len_out becomes row parent[i] of table / len (a beam
+ * search's choice; i itself: it goes on), or empty (-1 throughout, length 0) where parent[i] is
+ * outside [0, n): the sequence that had the row has ended. ref_out[p] (counts of the table
+ * entries that name page p, [pages]) follows: a page loses an owner for each old entry and gains
+ * one for each new; a page with ref 0 is free. No page is copied: rows share them until
+ * brasa_kv_pages_reserve. ref_out may be ref; table_out and len_out must not be table and len.
+ */
+int brasa_kv_pages_fork(const int32_t* parent, const int32_t* table, const int32_t* len,
+                        const int32_t* ref, int32_t* table_out, int32_t* len_out,
+                        int32_t* ref_out, size_t n, size_t width, size_t pages, void* stream);
+
+/*
+ * Reserves add[i] positions behind the len[i] that row i holds (none where add[i] <= 0): afterwards
+ * positions len[i] .. len[i] + add[i] lie in pages that only row i owns, so they may be written. A
+ * block among them without a page, or whose page other rows own too, gets a free page (ref 0),
+ * the lowest first, in the order of rows and blocks; where every owner of a shared page reserves it,
+ * the first of them keeps it. The positions below len[i] of such a block are copied, in every layer
+ * (copy on write). status[0] = pages taken, status[1] = 0; or, when there are too few free pages,
+ * nothing is changed, status[0] = 0 and status[1] = how many are missing; when a row's positions do
+ * not fit its table row, nothing is changed and status[1] = -1 (table_out and ref_out are then
+ * copies). table_out may be table, ref_out may be ref. workspace:
+ * brasa_kv_pages_workspace_len bytes, 256-byte aligned, any contents; not shared by calls that may
+ * run at the same time.
+ */
+size_t brasa_kv_pages_workspace_len(size_t pages, size_t n, size_t width);
+int brasa_kv_pages_reserve(brasa_kv_pool pool, const int32_t* add, const int32_t* table,
+                           const int32_t* len, const int32_t* ref, int32_t* table_out,
+                           int32_t* ref_out, int32_t* status, size_t n, size_t width,
+                           void* workspace, size_t workspace_len, void* stream);
+
+/*
+ * Compacts the pool: *live = L pages have ref > 0, and afterwards they are pages 0 .. L: the k-th
+ * of them at or past L moves, in every layer, to the k-th free one below L, and table_out and
+ * ref_out name it there (pages from L on: ref 0, codes as they were). table: every row that owns
+ * pages. table_out may be table, ref_out may be ref. workspace as for brasa_kv_pages_reserve.
+ */
+int brasa_kv_pages_compact(brasa_kv_pool pool, const int32_t* table, const int32_t* ref,
+                           int32_t* table_out, int32_t* ref_out, int32_t* live, size_t n,
+                           size_t width, void* workspace, size_t workspace_len, void* stream);
+
 /* Description of the last error on this thread ("" if none). */
 const char* brasa_last_error(void);
 
