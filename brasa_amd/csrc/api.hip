@@ -322,6 +322,8 @@ int brasa_flash_attention_packed(const float* q, const void* k, const void* v, v
         return set_error(BRASA_ERR_SHAPE, "%s: shape too large", what);
     if (s.tokens == 0 || n == 0) return BRASA_OK;
     if (!q || !k || !v || !o || !cu) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 16)
+        return set_error(BRASA_ERR_ARG, "%s: q, k, v and o must be 16-byte aligned", what);
     return packed_launch(q, k, v, o, cu, (int)n, (int)s.tokens, (int)s.hq, (int)s.hkv, s.kv, precision,
                          as_stream(stream));
 }

@@ -1288,22 +1288,20 @@ prefill_q8_kernel4(PrefillArgs a) {
 // the light ones to CUs as they free up.
 constexpr int kTileS = 32;                    // keys per stage
 constexpr int kStageHalvesS = kTileS * kDim;  // one 32 x 128 f16 tile
-template <int HW, bool PS>
-__global__ void __launch_bounds__(kThreads, 3)
-prefill_f16_kernel4s(PrefillArgs a) {
+// PACKED: the rows behind the last key belong to another prompt, or to nobody: a stage that
+// reaches past it copies the last key's row in their place (masked like any key past the query).
+template <int HW, bool PS, bool PACKED>
+__device__ __forceinline__ void f16_tile4s(const PrefillArgs& a, const int hg, const int tile,
+                                           uint16_t (&s_k)[3][kStageHalvesS],
+                                           uint16_t (&s_vv)[3][kStageHalvesS]) {
     constexpr int TPW = 32 * 4 / HW;
     constexpr int kTileBytes = kStageHalvesS * 2;
-    // three-stage ring: the copies of stage i + 2 are issued when stage i starts (48 KB)
-    __shared__ __attribute__((aligned(16))) uint16_t s_k[3][kStageHalvesS];
-    __shared__ __attribute__((aligned(16))) uint16_t s_vv[3][kStageHalvesS];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31;
     const int u = lane >> 5;
 
-    const int hg = blockIdx.x;
-    const int tile = a.ntiles - 1 - (int)blockIdx.y;
     const int h = hg * HW + (wave % HW);
     const int kh = (hg * HW) / a.group;
     const int t0 = tile * TPW;
@@ -1348,6 +1346,16 @@ prefill_f16_kernel4s(PrefillArgs a) {
     auto dma = [&](int kb, int buf) {
         const uint8_t* kg = sgpr_offset(kbase, (size_t)kb * rstride);
         const uint8_t* vg = sgpr_offset(vbase, (size_t)kb * rstride);
+        if (PACKED && kb + kTileS > lk) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = 8 * wave + 4 * r + (lane >> 4), lc = lane & 15;
+                const uint32_t off = (uint32_t)(min(row, lk - 1 - kb) * (int)rstride);
+                lds_dma16_s(kg, off + 16 * kswz(row, lc), lds_k + buf * kTileBytes + r * 1024);
+                lds_dma16_s(vg, off + 16 * vswz(row, lc), lds_v + buf * kTileBytes + r * 1024);
+            }
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             lds_dma16_s(kg, kso[r], lds_k + buf * kTileBytes + r * 1024);
@@ -1462,6 +1470,15 @@ prefill_f16_kernel4s(PrefillArgs a) {
                  a.o, tw0, a.tokens, a.hq, h);
 }
 
+template <int HW, bool PS>
+__global__ void __launch_bounds__(kThreads, 3)
+prefill_f16_kernel4s(PrefillArgs a) {
+    // three-stage ring: the copies of stage i + 2 are issued when stage i starts (48 KB)
+    __shared__ __attribute__((aligned(16))) uint16_t s_k[3][kStageHalvesS];
+    __shared__ __attribute__((aligned(16))) uint16_t s_vv[3][kStageHalvesS];
+    f16_tile4s<HW, PS, false>(a, blockIdx.x, a.ntiles - 1 - (int)blockIdx.y, s_k, s_vv);
+}
+
 // One 8-dim chunk of a cache row as the staging threads hold it: loaded into registers one stage
 // ahead, then split into the f16 hi (and, unless the cache is f16, lo) halves the tiles hold.
 // Plain loads: the other query tiles of the head read the same rows.
@@ -1522,16 +1539,21 @@ template <> struct Chunk8<BRASA_KV_Q8_0> {
 // bytes at a time; 32 heads over 8): f32 cache, F32 precision, T = 1000 206 -> 49 us (39 -> 167
 // TFLOP/s of the 3x as many that the splits contract), T = 2000 402 -> 119 us; q8_0 cache,
 // F16_PF32, T = 600 89 -> 33 us; f16 cache, F32 precision, T = 600 57 -> 26 us.
-template <int KV, int HW, bool QS, bool PS, bool OF32>
-__global__ void __launch_bounds__(2 * kThreads, 1)
-prefill_split_kernel(PrefillArgs a) {
+// PACKED: rows past the last key are another prompt's, or nobody's: the last key's row is read in
+// their place.
+template <int KV>
+constexpr int kSplitBuf = 2 * (KV != BRASA_KV_F16 ? 2 : 1) * kStageHalvesS;  // a stage: K hi, K lo, V hi, V lo
+constexpr int kXchHalves = 4 * 17 * 64 * 8;                                 // the group merge's exchange
+template <int KV>
+constexpr int kSplitHalves = 4 * kSplitBuf<KV> > kXchHalves ? 4 * kSplitBuf<KV> : kXchHalves;
+template <int KV, int HW, bool QS, bool PS, bool OF32, bool PACKED>
+__device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, const int tile,
+                                           const int part, uint16_t* s_kv) {
     constexpr bool KS = KV != BRASA_KV_F16;  // cache values need hi / lo
     constexpr int NK = KS ? 2 : 1;
     constexpr int TPW = 32 * 4 / HW;         // query tokens per workgroup
     constexpr int RB = KvTraits<KV>::row_bytes;
-    constexpr int kBuf = 2 * NK * kStageHalvesS;  // one stage: K hi, K lo, V hi, V lo
-    constexpr int kXchHalves = 4 * 17 * 64 * 8;   // the group merge's exchange
-    __shared__ __attribute__((aligned(16))) uint16_t s_kv[4 * kBuf > kXchHalves ? 4 * kBuf : kXchHalves];
+    constexpr int kBuf = kSplitBuf<KV>;
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1540,9 +1562,6 @@ prefill_split_kernel(PrefillArgs a) {
     const int col = lane & 31;       // query column of the MFMA tiles
     const int u = lane >> 5;         // lane half
 
-    const int hg = blockIdx.x;                            // head group (fastest: spreads XCDs)
-    const int tile = a.ntiles - 1 - (int)blockIdx.y / a.kparts;  // heaviest query tiles first
-    const int part = (int)blockIdx.y % a.kparts;          // key part of the tile
     const int h = hg * HW + (qw % HW);
     const int kh = (hg * HW) / a.group;
     const int t0 = tile * TPW;
@@ -1570,6 +1589,12 @@ prefill_split_kernel(PrefillArgs a) {
         const size_t row = (size_t)(stage_of(i) * kTileS + r0) * kstride;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            if (PACKED) {
+                const size_t at = (size_t)min(stage_of(i) * kTileS + r0 + 16 * j, lk - 1) * kstride;
+                rk[j].load(kbase + at, ch);
+                rv[j].load(vbase + at, ch);
+                continue;
+            }
             rk[j].load(kbase + row + 16 * j * kstride, ch);
             rv[j].load(vbase + row + 16 * j * kstride, ch);
         }
@@ -1771,6 +1796,15 @@ prefill_split_kernel(PrefillArgs a) {
     }
 }
 
+template <int KV, int HW, bool QS, bool PS, bool OF32>
+__global__ void __launch_bounds__(2 * kThreads, 1)
+prefill_split_kernel(PrefillArgs a) {
+    __shared__ __attribute__((aligned(16))) uint16_t s_kv[kSplitHalves<KV>];
+    // head groups fastest (they spread over the XCDs), heaviest query tiles first, then key parts
+    split_tile<KV, HW, QS, PS, OF32, false>(a, blockIdx.x, a.ntiles - 1 - (int)blockIdx.y / a.kparts,
+                                            (int)blockIdx.y % a.kparts, s_kv);
+}
+
 // The merge of a key split as a launch of its own. A split over many parts leaves more partials
 // per query tile than the one CU of the last part to arrive can load in good time (64 KB per part
 // at ~64 bytes a clock; parts waiting for each other could deadlock): here every wave loads one
@@ -1850,6 +1884,98 @@ prefill_merge_kernel(PrefillArgs a) {
         w.y = (uint32_t)f2h(as_f32(y[2])) | ((uint32_t)f2h(as_f32(y[3])) << 16);
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + ob) = w;
     }
+}
+
+// ---- packed prompts -----------------------------------------------------------------------------
+// A workgroup finds its prompt and query tile from the row numbers, which only the device knows, and
+// runs the tile code above on that prompt alone. Order: the heaviest query tiles of 64
+// prompts first (the y-th in descending tile number), so that the launch ends with light ones.
+struct PackedTile {
+    int start, len, tile;
+};
+__device__ __forceinline__ int wave_sum(int x) {
+    auto add = [](int v, int w) { return v + w; };
+    x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false));  // row_mirror
+    x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false));  // row_half_mirror
+    x = add(x, __builtin_amdgcn_update_dpp(0, x, 0x1B, 0xF, 0xF, false));
+    x = add(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = a[0] + a[1];
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return b[0] + b[1];
+}
+template <int TPW>
+__device__ __forceinline__ bool packed_tile(const int* cu, int n, int tokens, int y, PackedTile& out) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const int i = i0 + lane;
+        int c0 = 0, c1 = 0;
+        if (i < n) {  // clamped: whatever stands there, no access leaves the arrays
+            c0 = min(max(cu[i], 0), tokens);
+            c1 = min(max(cu[i + 1], c0), tokens);
+        }
+        const int nt = (c1 - c0 + TPW - 1) / TPW;
+        const int total = __builtin_amdgcn_readfirstlane(wave_sum(nt));
+        if (y >= total) {
+            y -= total;
+            continue;
+        }
+        // the tile number t with count(t) > y >= count(t + 1), count(t) the tiles from t on
+        int lo = 0, hi = tokens / TPW + 1;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (__builtin_amdgcn_readfirstlane(wave_sum(max(nt - mid, 0))) > y) lo = mid;
+            else hi = mid;
+        }
+        const int rank = y - __builtin_amdgcn_readfirstlane(wave_sum(max(nt - lo - 1, 0)));
+        // the rank-th prompt that has such a tile
+        const unsigned long long has = __builtin_amdgcn_ballot_w64(nt > lo);
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(nt > lo && before == rank));
+        out.start = __builtin_amdgcn_readlane(c0, l);
+        out.len = __builtin_amdgcn_readlane(c1, l) - out.start;
+        out.tile = lo;
+        return true;
+    }
+    return false;  // the grid's bound is loose
+}
+
+struct PackedArgs {
+    PrefillArgs a;  // tokens: rows of all prompts
+    const int* cu;
+    int n;
+};
+
+// The arguments of one prompt, as a call of its own would have them.
+template <int KV, bool OF32>
+__device__ __forceinline__ PrefillArgs prompt_args(const PackedArgs& p, const PackedTile& t) {
+    PrefillArgs a = p.a;
+    a.q += (size_t)t.start * a.hq * kDim;
+    a.k += (size_t)t.start * a.hkv * KvTraits<KV>::row_bytes;
+    a.v += (size_t)t.start * a.hkv * KvTraits<KV>::row_bytes;
+    a.o = static_cast<uint8_t*>(a.o) + (size_t)t.start * a.hq * kDim * (OF32 ? 4 : 2);
+    a.tokens = t.len;
+    return a;
+}
+
+template <int HW, bool PS>
+__global__ void __launch_bounds__(kThreads, 3)
+packed_f16_kernel(PackedArgs p) {
+    __shared__ __attribute__((aligned(16))) uint16_t s_k[3][kStageHalvesS];
+    __shared__ __attribute__((aligned(16))) uint16_t s_vv[3][kStageHalvesS];
+    PackedTile t;
+    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    f16_tile4s<HW, PS, true>(prompt_args<BRASA_KV_F16, false>(p, t), blockIdx.x, t.tile, s_k, s_vv);
+}
+
+template <int KV, int HW, bool QS, bool PS, bool OF32>
+__global__ void __launch_bounds__(2 * kThreads, 1)
+packed_split_kernel(PackedArgs p) {
+    __shared__ __attribute__((aligned(16))) uint16_t s_kv[kSplitHalves<KV>];
+    PackedTile t;
+    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    split_tile<KV, HW, QS, PS, OF32, true>(prompt_args<KV, OF32>(p, t), blockIdx.x, t.tile, 0, s_kv);
 }
 
 // Kernel choice by workgroup count (one per query tile and head group), measured on one box at
@@ -2287,7 +2413,38 @@ int run(PfCtx& c, PrefillArgs& a, int kv, int precision) {
     return set_error(BRASA_ERR_ARG, "flash_attention: invalid kv type %d", kv);
 }
 
+template <int HW>
+int launch_packed(const PackedArgs& p, int kv, int precision, hipStream_t stream) {
+    constexpr int TPW = 32 * 4 / HW;
+    // query tiles: a prompt of r > 0 rows has (r + TPW - 1) / TPW
+    const long long prompts = std::min(p.n, p.a.tokens);
+    const long long tiles = ((long long)p.a.tokens + prompts * (TPW - 1)) / TPW;
+    const dim3 grid(p.a.hq / HW, (unsigned)tiles);
+    auto go = [&](auto kernel, int threads, const char* name) {
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, p);
+        return check_launch(name);
+    };
+    if (kv == BRASA_KV_F16) {
+        if (precision == BRASA_PREFILL_F16) return go(packed_f16_kernel<HW, false>, kThreads, "packed_f16_kernel");
+        if (precision == BRASA_PREFILL_F16_PF32) return go(packed_f16_kernel<HW, true>, kThreads, "packed_f16_kernel");
+        return go(packed_split_kernel<BRASA_KV_F16, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
+    }
+    if (precision == BRASA_PREFILL_F32)
+        return go(packed_split_kernel<BRASA_KV_F32, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
+    if (precision == BRASA_PREFILL_F16_PF32)
+        return go(packed_split_kernel<BRASA_KV_F32, HW, false, true, false>, 2 * kThreads, "packed_split_kernel");
+    return go(packed_split_kernel<BRASA_KV_F32, HW, false, false, false>, 2 * kThreads, "packed_split_kernel");
+}
+
 }  // namespace
+
+int packed_launch(const float* q, const void* k, const void* v, void* o, const int* cu, int n, int tokens,
+                  int hq, int hkv, int kv, int precision, hipStream_t stream) {
+    PackedArgs p{make_args(q, k, v, o, tokens, hq, hkv, 0), cu, n};
+    if (p.a.group % 4 == 0) return launch_packed<4>(p, kv, precision, stream);
+    if (p.a.group % 2 == 0) return launch_packed<2>(p, kv, precision, stream);
+    return launch_packed<1>(p, kv, precision, stream);
+}
 
 void prefill_release_workspaces() {
     for (auto& o : g_pf_static_owner) o.store(0, std::memory_order_relaxed);

@@ -373,8 +373,10 @@ int brasa_prefill_trace_read(unsigned long long* dst, size_t n);
  * result nor written. The lengths are read on the device: a captured graph may be replayed with other
  * cu. Values of cu outside that order are clamped to it (no access leaves the arrays); two prompts
  * that would then overlap give unspecified values. K and V of a prompt must be finite (a row's V
- * that is not spoils earlier rows of its prompt, never another prompt's). Any hq a multiple of
- * hkv; dim 128; shape.pos0 must be 0. Allocates nothing, needs no workspace.
+ * that is not spoils earlier rows of its prompt, never another prompt's); f32 rows, and q / sqrt(128),
+ * are contracted as two f16 halves where the precision keeps them (22 bits, 2^-25 at least,
+ * magnitudes up to 65504). Any hq a multiple of
+ * hkv; dim 128; shape.pos0 must be 0; q, k, v and o 16-byte aligned. Allocates nothing, needs no workspace.
  */
 int brasa_flash_attention_packed(const float* q, const void* k, const void* v, void* o,
                                  const int32_t* cu, size_t n, brasa_attn_shape shape,

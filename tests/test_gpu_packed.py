@@ -8,7 +8,11 @@ numerator and denominator both carry it, so o errs by twice that times the weigh
 lk keys in f32 add at most lk * 2^-24 of it (a lane adds its keys one by one). f16 rows of v are exact,
 f32 rows of v in two halves 2^-21. An f16 result adds half a step, 2^-11 of it (2^-25 below f16's normal
 range). A weight below f16's normal range errs by half of f16's smallest step, 2^-25, where the row's
-largest weight is at least 1: o by 2^-25 of the sum of |v|.
+largest weight is at least 1: o by 2^-25 of the sum of |v|. The halves have the same floor: the lo half of an
+f32 value x errs by 2^-22 |x| or, where it is below f16's normal range, by 2^-25 (x = hi + lo + e with
+|lo| <= 2^-11 |x|, and f16 steps by 2^-24 below 2^-14). That is 2^-25 in every v (o errs by as much, the
+weights' sum being 1), in every k (a score by 2^-25 of the sum of |q| / sqrt(128)) and in every
+q / sqrt(128) (a score by 2^-25 of the largest sum of |k|).
 """
 import numpy as np
 import pytest
@@ -73,6 +77,9 @@ class Case:
                                     self.v[a:b].astype(np.float64), True)
             tol = av * (2 * (top * e_s + e_p) + 2.0 ** -21 + (b - a + 64) * 2.0 ** -24) + 1e-30
             tol += 2.0 ** -25 * np.abs(self.v[a:b].astype(np.float64)).sum(0).repeat(self.hq // self.hkv, 0)
+            floor = np.abs(self.q[a:b]).sum(-1, keepdims=True) / np.sqrt(128.0) + \
+                np.abs(self.k[a:b]).sum(-1).max()
+            tol += 2.0 ** -25 * (2 * floor * av + 1)
             if f16:
                 tol += np.abs(o) * 2.0 ** -11 + 2.0 ** -25
             err = np.abs(got[a:b] - o)

@@ -26,7 +26,7 @@ def _refused(code, call):
     (UNSUPPORTED, {"kv": KvType.Q8_0}), (SHAPE, {"dim": 64}), (SHAPE, {"hkv": 5}), (SHAPE, {"hkv": 0}),
     (SHAPE, {"hq": 0}), (SHAPE, {"pos0": 1}), (SHAPE, {"tokens": 1 << 30}), (SHAPE, {"n": 1 << 21}),
     (ARG, {"precision": 7}), (ARG, {"kv": 9}), (ARG, {"q": 0}), (ARG, {"k": 0}), (ARG, {"v": 0}),
-    (ARG, {"o": 0}), (ARG, {"cu": 0}),
+    (ARG, {"o": 0}), (ARG, {"cu": 0}), (ARG, {"q": P + 4}), (ARG, {"o": P + 8}),
 ])
 def test_packed_refusals(code, over):
     a = {**dict(q=P, k=P, v=P, o=P, cu=P, n=2, tokens=5, hq=32, hkv=8, dim=128, pos0=0, kv=KvType.F16,
