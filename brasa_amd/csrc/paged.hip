@@ -156,7 +156,7 @@ constexpr int kDecThreads = 64 * kWaves;
 constexpr int kMaxCols = 16;     // query heads of a workgroup
 constexpr int kSlots = 512;      // workgroups of a launch: two per CU
 constexpr int kMinPages = 8;     // pages of a run, at least (two per wave)
-constexpr int kPartFloats = kDim + 2;
+constexpr int kPartFloats = kMaxCols * (kDim + 2);  // a part: (m, l) of each column, then its sums
 constexpr int kCounterStride = 16;  // words between two arrival counters
 
 struct DecodePagedArgs {
@@ -190,13 +190,18 @@ __device__ __forceinline__ void split2(float x, float y, half2v& hi, half2v& lo)
     hi = half2v{(_Float16)x, (_Float16)y};
     lo = half2v{(_Float16)fmaf((float)hi.x, -1.0f, x), (_Float16)fmaf((float)hi.y, -1.0f, y)};
 }
-__device__ __forceinline__ float max_u(float x) {  // over the four lanes of a column
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+// over the four lanes c, c + 16, c + 32, c + 48 of a column
+__device__ __forceinline__ float max_u(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
 }
 __device__ __forceinline__ float sum_u(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = __int_as_float(a[0]) + __int_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return __int_as_float(b[0]) + __int_as_float(b[1]);
 }
 // pages of a sequence of lk keys in the line of pages: at least one, so that a sequence without
 // keys has a workgroup that writes its zeros, and a length the table cannot hold one that
@@ -204,16 +209,52 @@ __device__ __forceinline__ float sum_u(float x) {
 __device__ __forceinline__ int line_pages(int lk, int width) {
     return lk <= 0 || lk > width * kPage ? 1 : (lk + kPage - 1) / kPage;
 }
-__device__ __forceinline__ void st_part(float* p, float x) {
-    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Parts cross XCDs: stores written through, loads past the L2 (relaxed atomics of the device's
+// scope; the arrival counter orders them).
+typedef unsigned long long u64;
+__device__ __forceinline__ void st_part(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<u64*>(p), (u64)__float_as_uint(y) << 32 | __float_as_uint(x),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float ld_part(const float* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ u64 ld_part(const float* p) {
+    return __hip_atomic_load(reinterpret_cast<const u64*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ float lo_f32(u64 x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi_f32(u64 x) { return __uint_as_float((uint32_t)(x >> 32)); }
+
+// weight of a part whose largest score is m in a sum whose largest is top (a part without a key has
+// m = -inf)
+__device__ __forceinline__ float part_weight(float m, float top) {
+    return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// x / l of four dims (no key: l = 0 and zeros; a NaN l stays one)
+__device__ __forceinline__ void write_o(const DecodePagedArgs& a, size_t at, f32x4 x, float l) {
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0.0f : x[e] / l;
+    if (a.o_f16) {
+        u32x2 w = {f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + at) = w;
+    } else {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + at) = y;
+    }
+}
+
+// A wave's page in registers: 8 KB each of K and V.
+struct PageK {
+    u32x4 w[4][2];  // key 16 T + c, bytes 64 hh + 16 u .. + 16
+    int x;          // scale byte
+};
+struct PageV {
+    u32x2 w[4][4];  // key 16 T + 4 u + r, bytes 8 c .. + 8
+    int x;
+};
 
 __global__ void __launch_bounds__(kDecThreads, 2)
 decode_paged_kernel(DecodePagedArgs a) {
-    __shared__ float s_acc[kWaves][kMaxCols][kDim];
+    __shared__ __attribute__((aligned(16))) float s_acc[kWaves][kMaxCols][kDim];  // or the parts' weights
+    __shared__ __attribute__((aligned(16))) f32x4 s_sum[kDecThreads];
     __shared__ float s_m[kWaves][kMaxCols], s_l[kWaves][kMaxCols];
     __shared__ unsigned s_last;
 
@@ -226,20 +267,17 @@ decode_paged_kernel(DecodePagedArgs a) {
     const int head_of_lane = h0 + min(c, cols - 1);
 
     // ---- this workgroup's run of the line of pages -------------------------------------------
-    int total = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 64) {
-        const int i = i0 + lane;
-        total += i < a.n ? line_pages(a.lk[i], a.width) : 0;
-    }
-#pragma unroll
-    for (int d = 32; d; d /= 2) total += __shfl_xor(total, d);
+    const int np0 = lane < a.n ? line_pages(a.lk[lane], a.width) : 0;
+    int total = np0;
+    for (int i = 64 + lane; i < a.n; i += 64) total += line_pages(a.lk[i], a.width);
+    total = __builtin_amdgcn_readfirstlane(__shfl(wave_scan(total), 63));
     const int size = max((total + a.runs - 1) / a.runs, kMinPages);
     int at = run * size;
     const int end = min(at + size, total);
     if (at >= end) return;
     int seq = 0, seq_at = 0;  // the sequence that holds page `at`, and its first page in the line
     for (int i0 = 0; i0 < a.n; i0 += 64) {
-        const int np = i0 + lane < a.n ? line_pages(a.lk[i0 + lane], a.width) : 0;
+        const int np = i0 == 0 ? np0 : i0 + lane < a.n ? line_pages(a.lk[i0 + lane], a.width) : 0;
         const int incl = wave_scan(np) + seq_at;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > at);
         if (past) {
@@ -261,6 +299,48 @@ decode_paged_kernel(DecodePagedArgs a) {
         const int b0 = at - seq_at;                        // pages [b0, b1) of the sequence
         const int b1 = min(end - seq_at, np);
         const bool whole = b0 == 0 && b1 == np;
+        const int blast = lk > 0 ? b1 : 0;                 // no keys: no pages
+
+        // ---- this wave's first page on its way ---------------------------------------------------
+        const int* ids = a.table + (size_t)seq * a.width;
+        bool bad = false;
+        PageK k;
+        PageV v;
+        // a page that is not there reads page 0 in its place, and the sequence's output is NaN
+        auto tile_of = [&](int page) {
+            const bool there = page >= 0 && page < a.p.pages;
+            bad |= !there;
+            return (size_t)(there ? page : 0) * a.p.hkv + kh;
+        };
+        auto load_k = [&](size_t tile) {
+            const uint8_t* p = a.p.k + tile * kTileBytes8 + c * kDim + 16 * u;
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+                    k.w[T][hh] = *reinterpret_cast<const u32x4*>(p + 16 * T * kDim + 64 * hh);
+            k.x = a.p.kx[tile];
+        };
+        auto load_v = [&](size_t tile) {
+            const uint8_t* p = a.p.v + tile * kTileBytes8 + 4 * u * kDim + 8 * c;
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    v.w[T][r] = *reinterpret_cast<const u32x2*>(p + (16 * T + r) * kDim);
+            v.x = a.p.vx[tile];
+        };
+        int b = b0 + wave;
+        int next_id = 0;  // the next page's id, loaded a page ahead of its codes
+        size_t next = 0;
+        if (b < blast) {
+            const int id = ids[b];
+            if (b + kWaves < blast) next_id = ids[b + kWaves];
+            const size_t tile = tile_of(id);
+            load_k(tile);
+            load_v(tile);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 
         // ---- Q: hi and lo halves of q / sqrt(128) * log2 e, its exponent taken out --------------
         // k-step t = 2 hh + j holds dims 64 hh + 16 u + 8 j .. + 8, as K's 16-byte loads do
@@ -295,32 +375,9 @@ decode_paged_kernel(DecodePagedArgs a) {
         f32x4 acc[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        bool bad = false;
 
-        const int* ids = a.table + (size_t)seq * a.width;
-        for (int b = b0 + wave; lk > 0 && b < b1; b += kWaves) {
-            int page = ids[b];
-            if (page < 0 || page >= a.p.pages) {  // never read: the sequence's output is NaN
-                bad = true;
-                continue;
-            }
-            const size_t tile = (size_t)page * a.p.hkv + kh;
-            const uint8_t* kt = a.p.k + tile * kTileBytes8 + c * kDim + 16 * u;
-            const uint8_t* vt = a.p.v + tile * kTileBytes8 + 4 * u * kDim + 8 * c;
-            u32x4 kr[4][2];
-            u32x2 vr[4][4];
-#pragma unroll
-            for (int T = 0; T < 4; ++T)
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh)
-                    kr[T][hh] = *reinterpret_cast<const u32x4*>(kt + 16 * T * kDim + 64 * hh);
-#pragma unroll
-            for (int T = 0; T < 4; ++T)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    vr[T][r] = *reinterpret_cast<const u32x2*>(vt + (16 * T + r) * kDim);
-            const int kx = a.p.kx[tile], vx = a.p.vx[tile];
-
+        for (; b < blast; b += kWaves) {
+            const bool more = b + kWaves < blast;
             // ---- scores: key 16 T + 4 u + r of head c, in units of log2 ---------------------------
             f32x4 s[4];
 #pragma unroll
@@ -328,19 +385,28 @@ decode_paged_kernel(DecodePagedArgs a) {
                 s[T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const uint32_t w0 = kr[T][t >> 1][2 * (t & 1)], w1 = kr[T][t >> 1][2 * (t & 1) + 1];
+                    const uint32_t w0 = k.w[T][t >> 1][2 * (t & 1)], w1 = k.w[T][t >> 1][2 * (t & 1) + 1];
                     const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
                     s[T] = mfma16(ka, qh[t], s[T]);
                     s[T] = mfma16(ka, ql[t], s[T]);
                 }
             }
+            const int sx = qx + k.x - 127;
+            // the next page's K takes this one's registers, its V later V's: a wave always has a
+            // load on its way
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+                next = tile_of(next_id);
+                load_k(next);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             const int left = lk - b * kPage;  // live keys of the page
             float tmax = -INFINITY;
 #pragma unroll
             for (int T = 0; T < 4; ++T)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[T][r] = ldexpf(s[T][r], qx + kx - 127);
+                    s[T][r] = ldexpf(s[T][r], sx);
                     if (left < kPage && 16 * T + 4 * u + r >= left) s[T][r] = -INFINITY;
                     tmax = fmaxf(tmax, s[T][r]);
                 }
@@ -376,23 +442,23 @@ decode_paged_kernel(DecodePagedArgs a) {
                 for (int T = 0; T < 4; ++T)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (16 * T + 4 * u + r >= left) vr[T][r] = u32x2{0, 0};
+                        if (16 * T + 4 * u + r >= left) v.w[T][r] = u32x2{0, 0};
             }
-            const float vs = ldexpf(1.0f, vx - 127);
+            const float vs = ldexpf(1.0f, v.x - 127);
             // ---- O^T += V^T P^T: tile t's rows are dims 8 i + t ------------------------------------
 #pragma unroll
             for (int t2 = 0; t2 < 4; ++t2) {  // tiles 2 t2, 2 t2 + 1
                 f32x4 pv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
                 const int d = t2 >> 1;
-                const uint32_t b = 2 * (t2 & 1);
-                const uint32_t sel = b | (4 + b) << 8 | (b + 1) << 16 | (5 + b) << 24;
+                const uint32_t by = 2 * (t2 & 1);
+                const uint32_t sel = by | (4 + by) << 8 | (by + 1) << 16 | (5 + by) << 24;
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     half2v x0[4], x1[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int T = 2 * st + (e >> 1), r = 2 * (e & 1);
-                        const uint32_t w = __builtin_amdgcn_perm(vr[T][r + 1][d], vr[T][r][d], sel);
+                        const uint32_t w = __builtin_amdgcn_perm(v.w[T][r + 1][d], v.w[T][r][d], sel);
                         x0[e] = f16_of_lo(w);
                         x1[e] = f16_of_hi(w);
                     }
@@ -409,6 +475,11 @@ decode_paged_kernel(DecodePagedArgs a) {
                     for (int r = 0; r < 4; ++r)
                         acc[2 * t2 + j][r] = fmaf(pv[j][r], vs, acc[2 * t2 + j][r]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+                load_v(next);
+                if (b + 2 * kWaves < blast) next_id = ids[b + 2 * kWaves];
+            }
         }
 
         // ---- the waves' states into one ----------------------------------------------------------
@@ -423,72 +494,111 @@ decode_paged_kernel(DecodePagedArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int t = 0; t < 8; ++t) s_acc[wave][c][32 * u + 8 * r + t] = acc[t][r];
+                for (int t = 0; t < 8; t += 4)
+                    *reinterpret_cast<f32x4*>(&s_acc[wave][c][32 * u + 8 * r + t]) =
+                        f32x4{acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]};
         }
         __syncthreads();
         const size_t out0 = ((size_t)seq * a.hq + h0) * kDim;
-        const int wg = run * a.p.hkv + kh;  // of this blockIdx.y
-        const size_t planes = (size_t)a.runs * a.p.hkv;
-        auto part_of = [&](int r, int second, int col) {
-            return a.part + ((((size_t)blockIdx.y * planes + (size_t)r * a.p.hkv + kh) * 2 + second) *
-                                 kMaxCols + col) * kPartFloats;
+        const size_t plane = (size_t)blockIdx.y * a.runs;  // of this chunk of columns
+        auto part_of = [&](int r, int second) {
+            return a.part + (((plane + r) * a.p.hkv + kh) * 2 + second) * kPartFloats;
         };
-        for (int i = threadIdx.x; i < cols * kDim; i += kDecThreads) {
-            const int col = i / kDim, d = i % kDim;
+        for (int i = threadIdx.x; i < cols * (kDim / 4); i += kDecThreads) {
+            const int col = i / (kDim / 4), d = 4 * (i % (kDim / 4));
             float m = s_m[0][col];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][col]);
-            float l = 0.0f, x = 0.0f;
+            float l = 0.0f;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 // a wave without a page has m = -inf, l = 0 (or NaN for a page that is not there)
-                const float f = s_m[w][col] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][col] - m);
+                const float f = part_weight(s_m[w][col], m);
                 l += s_m[w][col] == -INFINITY ? s_l[w][col] : s_l[w][col] * f;
-                x = fmaf(s_acc[w][col][d], f, x);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(&s_acc[w][col][d]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
             }
             if (whole) {
-                // no keys: zeros (a length out of range has l = NaN)
-                const float y = l == 0.0f ? 0.0f : x / l;
-                if (a.o_f16) static_cast<uint16_t*>(a.o)[out0 + i] = f2h(y);
-                else static_cast<float*>(a.o)[out0 + i] = y;
+                write_o(a, out0 + 4 * i, x, l);
             } else {
-                float* p = part_of(run, b0 > 0 || at == run * size ? 0 : 1, col);
-                st_part(p + 2 + d, x);
-                if (d == 0) st_part(p, m);
-                if (d == 1) st_part(p + 1, l);
+                float* p = part_of(run, at == run * size ? 0 : 1);
+                st_part(p + 2 * kMaxCols + 4 * i, x[0], x[1]);
+                st_part(p + 2 * kMaxCols + 4 * i + 2, x[2], x[3]);
+                if (d == 0) st_part(p + 2 * col, m, l);
             }
         }
         if (!whole) {
             // ---- the last segment of the sequence to arrive merges all of them ------------------
-            const int r0 = seq_at / size, r1 = (seq_at + np - 1) / size;  // the runs that hold it
+            const int r0 = seq_at / size, parts = (seq_at + np - 1) / size - r0 + 1;
+            const int first = seq_at == r0 * size ? 0 : 1;  // a run's parts: its first segment's, then another
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (threadIdx.x == 0) {
-                unsigned* ctr = a.ctr + ((size_t)blockIdx.y * planes + (size_t)r0 * a.p.hkv + kh) * kCounterStride;
-                s_last = atomicInc(ctr, r1 - r0) == (unsigned)(r1 - r0);
+                unsigned* ctr = a.ctr + ((plane + r0) * a.p.hkv + kh) * kCounterStride;
+                s_last = atomicInc(ctr, parts - 1) == (unsigned)(parts - 1);
             }
             __syncthreads();
             if (s_last) {
-                const int first = seq_at == r0 * size ? 0 : 1;
-                for (int i = threadIdx.x; i < cols * kDim; i += kDecThreads) {
-                    const int col = i / kDim, d = i % kDim;
-                    float m = -INFINITY;
-                    for (int r = r0; r <= r1; ++r) m = fmaxf(m, ld_part(part_of(r, r == r0 ? first : 0, col)));
-                    float l = 0.0f, x = 0.0f;
-                    for (int r = r0; r <= r1; ++r) {
-                        const float* p = part_of(r, r == r0 ? first : 0, col);
-                        const float mr = ld_part(p), lr = ld_part(p + 1);
-                        const float f = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - m);
-                        l += mr == -INFINITY ? lr : lr * f;
-                        x = fmaf(ld_part(p + 2 + d), f, x);
+                // weights: a wave per column, a lane per part
+                float* s_w = &s_acc[0][0][0];  // [column][part]
+                for (int col = wave; col < cols; col += kWaves) {
+                    float m = -INFINITY, l = 0.0f;
+                    for (int r = lane; r < parts; r += 64)
+                        m = fmaxf(m, lo_f32(ld_part(part_of(r0 + r, r ? 0 : first) + 2 * col)));
+#pragma unroll
+                    for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+                    for (int r = lane; r < parts; r += 64) {
+                        const u64 ml = ld_part(part_of(r0 + r, r ? 0 : first) + 2 * col);
+                        const float f = part_weight(lo_f32(ml), m);
+                        s_w[col * parts + r] = f;
+                        l += lo_f32(ml) == -INFINITY ? hi_f32(ml) : hi_f32(ml) * f;
                     }
-                    const float y = x / l;
-                    if (a.o_f16) static_cast<uint16_t*>(a.o)[out0 + i] = f2h(y);
-                    else static_cast<float*>(a.o)[out0 + i] = y;
+#pragma unroll
+                    for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
+                    if (lane == 0) s_l[0][col] = l;
+                }
+                __syncthreads();
+                // sums: a thread per four dims; where the columns leave threads over, these share
+                // the parts
+                const int chunks = cols * (kDim / 4);
+                const int share = max(kDecThreads / chunks, 1);
+                for (int i0 = 0; i0 < chunks; i0 += kDecThreads) {
+                    const int i = i0 + threadIdx.x % chunks, g = chunks < kDecThreads ? threadIdx.x / chunks : 0;
+                    const int col = i / (kDim / 4);
+                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (i < chunks && g < share) {
+                        constexpr int kAhead = 8;  // parts whose loads are in flight together
+                        for (int r = g; r < parts; r += share * kAhead) {
+                            u64 w[kAhead][2];
+#pragma unroll
+                            for (int j = 0; j < kAhead; ++j) {
+                                const int rj = min(r + j * share, parts - 1);
+                                const float* p = part_of(r0 + rj, rj ? 0 : first) + 2 * kMaxCols + 4 * i;
+                                w[j][0] = ld_part(p);
+                                w[j][1] = ld_part(p + 2);
+                            }
+#pragma unroll
+                            for (int j = 0; j < kAhead; ++j) {
+                                if (r + j * share >= parts) continue;
+                                const float f = s_w[col * parts + r + j * share];
+                                x[0] = fmaf(lo_f32(w[j][0]), f, x[0]);
+                                x[1] = fmaf(hi_f32(w[j][0]), f, x[1]);
+                                x[2] = fmaf(lo_f32(w[j][1]), f, x[2]);
+                                x[3] = fmaf(hi_f32(w[j][1]), f, x[3]);
+                            }
+                        }
+                    }
+                    if (share > 1) {
+                        s_sum[threadIdx.x] = x;
+                        __syncthreads();
+                        for (int j = 1; j < share && threadIdx.x < chunks; ++j) x += s_sum[threadIdx.x + j * chunks];
+                    }
+                    if (i < chunks && g == 0) write_o(a, out0 + 4 * i, x, s_l[0][col]);
                 }
             }
         }
-        (void)wg;
         __syncthreads();  // the LDS is free for the next segment
         at = seq_at + b1;
         seq_at += np;
@@ -517,7 +627,7 @@ static size_t decode_paged_ctr_bytes(int hkv, int chunks) {
 size_t decode_paged_workspace_len(int hq, int hkv) {
     const int chunks = (hq / hkv + kMaxCols - 1) / kMaxCols;
     return decode_paged_ctr_bytes(hkv, chunks) +
-           (size_t)chunks * decode_runs(hkv, chunks) * hkv * 2 * kMaxCols * kPartFloats * sizeof(float);
+           (size_t)chunks * decode_runs(hkv, chunks) * hkv * 2 * kPartFloats * sizeof(float);
 }
 
 int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, int width,
