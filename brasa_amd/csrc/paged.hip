@@ -153,7 +153,7 @@ store_paged_kernel(StoreArgs a) {
 // scales are exponents: K's is added to the scores' exponent, V's multiplies the page's sum.
 constexpr int kWaves = 4;
 constexpr int kDecThreads = 64 * kWaves;
-constexpr int kMaxCols = 16;     // query heads of a workgroup
+constexpr int kMaxCols = 8;      // query heads of a workgroup
 constexpr int kSlots = 512;      // workgroups of a launch: two per CU
 constexpr int kMinPages = 8;     // pages of a run, at least (two per wave)
 constexpr int kPartFloats = kMaxCols * (kDim + 2);  // a part: (m, l) of each column, then its sums
@@ -183,12 +183,12 @@ __device__ __forceinline__ half2v f16_of_hi(uint32_t w) {
 __device__ __forceinline__ half8v join(half2v a, half2v b, half2v c, half2v d) {
     return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-// x = hi + lo up to 2^-22 of x
-__device__ __forceinline__ void split2(float x, float y, half2v& hi, half2v& lo) {
+// This lane's half of x = hi + lo (up to 2^-22 of x): hi where less = 0, lo where it is -1.
+__device__ __forceinline__ half2v half_of(float x, float y, float less) {
     x = as_f32(x);
     y = as_f32(y);
-    hi = half2v{(_Float16)x, (_Float16)y};
-    lo = half2v{(_Float16)fmaf((float)hi.x, -1.0f, x), (_Float16)fmaf((float)hi.y, -1.0f, y)};
+    const half2v hi = {(_Float16)x, (_Float16)y};
+    return half2v{(_Float16)fmaf((float)hi.x, less, x), (_Float16)fmaf((float)hi.y, less, y)};
 }
 // over the four lanes c, c + 16, c + 32, c + 48 of a column
 __device__ __forceinline__ float max_u(float x) {
@@ -261,13 +261,15 @@ decode_paged_kernel(DecodePagedArgs a) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, u = lane >> 4;
+    const float less = c < kMaxCols ? 0.0f : -1.0f;  // columns of hi halves, then of lo halves
     const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv;
     const int h0 = kh * a.group + blockIdx.y * kMaxCols;          // first query head
     const int cols = min(a.group - (int)blockIdx.y * kMaxCols, kMaxCols);
-    const int head_of_lane = h0 + min(c, cols - 1);
+    const int head_of_lane = h0 + min(c < kMaxCols ? c : 15 - c, cols - 1);
 
     // ---- this workgroup's run of the line of pages -------------------------------------------
-    const int np0 = lane < a.n ? line_pages(a.lk[lane], a.width) : 0;
+    const int lk0 = lane < a.n ? a.lk[lane] : 0;
+    const int np0 = lane < a.n ? line_pages(lk0, a.width) : 0;
     int total = np0;
     for (int i = 64 + lane; i < a.n; i += 64) total += line_pages(a.lk[i], a.width);
     total = __builtin_amdgcn_readfirstlane(__shfl(wave_scan(total), 63));
@@ -292,7 +294,7 @@ decode_paged_kernel(DecodePagedArgs a) {
     seq_at = __builtin_amdgcn_readfirstlane(seq_at);
 
     for (; at < end; ++seq) {
-        const int lk_raw = a.lk[seq];
+        const int lk_raw = seq < 64 ? __builtin_amdgcn_readlane(lk0, seq) : a.lk[seq];
         const int np = line_pages(lk_raw, a.width);
         const bool bad_len = lk_raw < 0 || lk_raw > a.width * kPage;
         const int lk = bad_len ? 0 : lk_raw;
@@ -333,21 +335,34 @@ decode_paged_kernel(DecodePagedArgs a) {
         int b = b0 + wave;
         int next_id = 0;  // the next page's id, loaded a page ahead of its codes
         size_t next = 0;
+        int id = 0;
         if (b < blast) {
-            const int id = ids[b];
+            id = ids[b];
             if (b + kWaves < blast) next_id = ids[b + kWaves];
+        }
+        // Q's loads go out before the page's, which they would wait behind
+        // k-step t = 2 hh + j holds dims 64 hh + 16 u + 8 j .. + 8, as K's 16-byte loads do
+        f32x4 qraw[4][2];
+        {
+            const float* qrow = a.q + ((size_t)seq * a.hq + head_of_lane) * kDim + 16 * u;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    qraw[t][e] = *reinterpret_cast<const f32x4*>(qrow + 64 * (t >> 1) + 8 * (t & 1) + 4 * e);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (b < blast) {
             const size_t tile = tile_of(id);
             load_k(tile);
             load_v(tile);
         }
         __builtin_amdgcn_sched_barrier(0);
 
-        // ---- Q: hi and lo halves of q / sqrt(128) * log2 e, its exponent taken out --------------
-        // k-step t = 2 hh + j holds dims 64 hh + 16 u + 8 j .. + 8, as K's 16-byte loads do
-        half8v qh[4], ql[4];
+        // ---- Q: this lane's halves of q / sqrt(128) * log2 e, its exponent taken out -------------
+        half8v q[4];
         int qx;
         {
-            const float* qrow = a.q + ((size_t)seq * a.hq + head_of_lane) * kDim + 16 * u;
             const float scale = 0.08838834764831845f * kLog2e;
             float x[4][8];
             float qmax = 0.0f;
@@ -355,19 +370,18 @@ decode_paged_kernel(DecodePagedArgs a) {
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[t][e] = as_f32(qrow[64 * (t >> 1) + 8 * (t & 1) + e] * scale);
+                    x[t][e] = as_f32(qraw[t][e >> 2][e & 3] * scale);
                     qmax = fmaxf(qmax, fabsf(x[t][e]));
                 }
             qmax = max_u(qmax);
             qx = (int)(__float_as_uint(qmax) >> 23) - 127 - 8;  // the row's largest to [2^8, 2^9)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                half2v hi[4], lo[4];
+                half2v h[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    split2(ldexpf(x[t][2 * e], -qx), ldexpf(x[t][2 * e + 1], -qx), hi[e], lo[e]);
-                qh[t] = join(hi[0], hi[1], hi[2], hi[3]);
-                ql[t] = join(lo[0], lo[1], lo[2], lo[3]);
+                    h[e] = half_of(ldexpf(x[t][2 * e], -qx), ldexpf(x[t][2 * e + 1], -qx), less);
+                q[t] = join(h[0], h[1], h[2], h[3]);
             }
         }
 
@@ -387,11 +401,14 @@ decode_paged_kernel(DecodePagedArgs a) {
                 for (int t = 0; t < 4; ++t) {
                     const uint32_t w0 = k.w[T][t >> 1][2 * (t & 1)], w1 = k.w[T][t >> 1][2 * (t & 1) + 1];
                     const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
-                    s[T] = mfma16(ka, qh[t], s[T]);
-                    s[T] = mfma16(ka, ql[t], s[T]);
+                    s[T] = mfma16(ka, q[t], s[T]);
                 }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[T][r] += dpp<0x140>(s[T][r]);  // hi + lo: column 15 - c
             }
-            const int sx = qx + k.x - 127;
+            // 2^sx times the products of the codes and the scaled q. (Past the clamp every score is
+            // 0, or so far from the next that one key takes all.)
+            const float sc = ldexpf(1.0f, min(max(qx + k.x - 127, -127), 127));
             // the next page's K takes this one's registers, its V later V's: a wave always has a
             // load on its way
             __builtin_amdgcn_sched_barrier(0);
@@ -406,11 +423,10 @@ decode_paged_kernel(DecodePagedArgs a) {
             for (int T = 0; T < 4; ++T)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[T][r] = ldexpf(s[T][r], sx);
                     if (left < kPage && 16 * T + 4 * u + r >= left) s[T][r] = -INFINITY;
                     tmax = fmaxf(tmax, s[T][r]);
                 }
-            tmax = max_u(tmax);
+            tmax = max_u(tmax) * sc;
             // a reference point that moves only when the maximum has grown by 2^8: p stays below
             // 2^15 with the bias of 2^7 that keeps the lo halves of small p out of f16's subnormals
             const bool grow = tmax > m_used + 8.0f;
@@ -421,21 +437,20 @@ decode_paged_kernel(DecodePagedArgs a) {
 #pragma unroll
                 for (int t = 0; t < 8; ++t) acc[t] *= alpha;
             }
-            half8v ph[2], pl[2];
-            const float mb = m_used - 7.0f;
+            half8v p[2];
+            const float mb = 7.0f - m_used;
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                half2v hi[4], lo[4];
+                half2v h[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int T = 2 * st + (e >> 1), r = 2 * (e & 1);
-                    const float p0 = __builtin_amdgcn_exp2f(s[T][r] - mb);
-                    const float p1 = __builtin_amdgcn_exp2f(s[T][r + 1] - mb);
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[T][r], sc, mb));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[T][r + 1], sc, mb));
                     lsum += p0 + p1;
-                    split2(p0, p1, hi[e], lo[e]);
+                    h[e] = half_of(p0, p1, less);
                 }
-                ph[st] = join(hi[0], hi[1], hi[2], hi[3]);
-                pl[st] = join(lo[0], lo[1], lo[2], lo[3]);
+                p[st] = join(h[0], h[1], h[2], h[3]);
             }
             if (left < kPage) {  // codes behind the last key may be anything, NaN too
 #pragma unroll
@@ -464,10 +479,8 @@ decode_paged_kernel(DecodePagedArgs a) {
                     }
                     const half8v v0 = join(x0[0], x0[1], x0[2], x0[3]);
                     const half8v v1 = join(x1[0], x1[1], x1[2], x1[3]);
-                    pv[0] = mfma16(v0, ph[st], pv[0]);
-                    pv[1] = mfma16(v1, ph[st], pv[1]);
-                    pv[0] = mfma16(v0, pl[st], pv[0]);
-                    pv[1] = mfma16(v1, pl[st], pv[1]);
+                    pv[0] = mfma16(v0, p[st], pv[0]);
+                    pv[1] = mfma16(v1, p[st], pv[1]);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
@@ -485,6 +498,10 @@ decode_paged_kernel(DecodePagedArgs a) {
         // ---- the waves' states into one ----------------------------------------------------------
         if (bad || bad_len) lsum = NAN;
         lsum = sum_u(lsum);
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] += dpp<0x140>(acc[t][r]);  // P's hi + lo halves
         if (c < cols) {
             if (u == 0) {
                 s_m[wave][c] = m_used;
@@ -541,62 +558,65 @@ decode_paged_kernel(DecodePagedArgs a) {
             }
             __syncthreads();
             if (s_last) {
+                // A thread sums four dims over the parts; where the columns leave threads over,
+                // these share the parts. The first loads go out before the weights are known.
+                constexpr int kAhead = 16;  // parts whose loads are in flight together
+                const int chunks = cols * (kDim / 4);
+                const int share = kDecThreads / chunks;
+                const int i = threadIdx.x % chunks, g = threadIdx.x / chunks;
+                const int col = i / (kDim / 4);
+                u64 w[kAhead][2];
+                auto load = [&](int r) {
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        const int rj = min(r + j * share, parts - 1);
+                        const float* p = part_of(r0 + rj, rj ? 0 : first) + 2 * kMaxCols + 4 * i;
+                        w[j][0] = ld_part(p);
+                        w[j][1] = ld_part(p + 2);
+                    }
+                };
+                load(g);
+                __builtin_amdgcn_sched_barrier(0);
                 // weights: a wave per column, a lane per part
                 float* s_w = &s_acc[0][0][0];  // [column][part]
-                for (int col = wave; col < cols; col += kWaves) {
+                for (int cw = wave; cw < cols; cw += kWaves) {
                     float m = -INFINITY, l = 0.0f;
-                    for (int r = lane; r < parts; r += 64)
-                        m = fmaxf(m, lo_f32(ld_part(part_of(r0 + r, r ? 0 : first) + 2 * col)));
+                    u64 ml = ld_part(part_of(r0 + min(lane, parts - 1), lane ? 0 : first) + 2 * cw);
+                    for (int r = lane + 64; r < parts; r += 64)
+                        m = fmaxf(m, lo_f32(ld_part(part_of(r0 + r, 0) + 2 * cw)));
+                    if (lane < parts) m = fmaxf(m, lo_f32(ml));
 #pragma unroll
                     for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
                     for (int r = lane; r < parts; r += 64) {
-                        const u64 ml = ld_part(part_of(r0 + r, r ? 0 : first) + 2 * col);
+                        if (r >= 64) ml = ld_part(part_of(r0 + r, 0) + 2 * cw);
                         const float f = part_weight(lo_f32(ml), m);
-                        s_w[col * parts + r] = f;
+                        s_w[cw * parts + r] = f;
                         l += lo_f32(ml) == -INFINITY ? hi_f32(ml) : hi_f32(ml) * f;
                     }
 #pragma unroll
                     for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
-                    if (lane == 0) s_l[0][col] = l;
+                    if (lane == 0) s_l[0][cw] = l;
                 }
                 __syncthreads();
-                // sums: a thread per four dims; where the columns leave threads over, these share
-                // the parts
-                const int chunks = cols * (kDim / 4);
-                const int share = max(kDecThreads / chunks, 1);
-                for (int i0 = 0; i0 < chunks; i0 += kDecThreads) {
-                    const int i = i0 + threadIdx.x % chunks, g = chunks < kDecThreads ? threadIdx.x / chunks : 0;
-                    const int col = i / (kDim / 4);
-                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (i < chunks && g < share) {
-                        constexpr int kAhead = 8;  // parts whose loads are in flight together
-                        for (int r = g; r < parts; r += share * kAhead) {
-                            u64 w[kAhead][2];
+                f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int r = g; r < parts; r += share * kAhead) {
+                    if (r != g) load(r);
 #pragma unroll
-                            for (int j = 0; j < kAhead; ++j) {
-                                const int rj = min(r + j * share, parts - 1);
-                                const float* p = part_of(r0 + rj, rj ? 0 : first) + 2 * kMaxCols + 4 * i;
-                                w[j][0] = ld_part(p);
-                                w[j][1] = ld_part(p + 2);
-                            }
-#pragma unroll
-                            for (int j = 0; j < kAhead; ++j) {
-                                if (r + j * share >= parts) continue;
-                                const float f = s_w[col * parts + r + j * share];
-                                x[0] = fmaf(lo_f32(w[j][0]), f, x[0]);
-                                x[1] = fmaf(hi_f32(w[j][0]), f, x[1]);
-                                x[2] = fmaf(lo_f32(w[j][1]), f, x[2]);
-                                x[3] = fmaf(hi_f32(w[j][1]), f, x[3]);
-                            }
-                        }
+                    for (int j = 0; j < kAhead; ++j) {
+                        if (r + j * share >= parts) continue;
+                        const float f = s_w[col * parts + r + j * share];
+                        x[0] = fmaf(lo_f32(w[j][0]), f, x[0]);
+                        x[1] = fmaf(hi_f32(w[j][0]), f, x[1]);
+                        x[2] = fmaf(lo_f32(w[j][1]), f, x[2]);
+                        x[3] = fmaf(hi_f32(w[j][1]), f, x[3]);
                     }
-                    if (share > 1) {
-                        s_sum[threadIdx.x] = x;
-                        __syncthreads();
-                        for (int j = 1; j < share && threadIdx.x < chunks; ++j) x += s_sum[threadIdx.x + j * chunks];
-                    }
-                    if (i < chunks && g == 0) write_o(a, out0 + 4 * i, x, s_l[0][col]);
                 }
+                if (share > 1) {
+                    s_sum[threadIdx.x] = x;
+                    __syncthreads();
+                    for (int j = 1; j < share && threadIdx.x < chunks; ++j) x += s_sum[threadIdx.x + j * chunks];
+                }
+                if (threadIdx.x < chunks) write_o(a, out0 + 4 * i, x, s_l[0][col]);
             }
         }
         __syncthreads();  // the LDS is free for the next segment
