@@ -156,7 +156,7 @@ constexpr int kDecThreads = 64 * kWaves;
 constexpr int kMaxCols = 8;      // query heads of a workgroup
 constexpr int kSlots = 512;      // workgroups of a launch: two per CU
 constexpr int kMinPages = 8;     // pages of a run, at least (two per wave)
-constexpr int kPartFloats = kMaxCols * (kDim + 2);  // a part: (m, l) of each column, then its sums
+constexpr int kPartBytes = kMaxCols * (kDim + 2) * 4;  // a part: (m, l) of each column, then its sums
 constexpr int kCounterStride = 16;  // words between two arrival counters
 
 struct DecodePagedArgs {
@@ -167,7 +167,7 @@ struct DecodePagedArgs {
     void* o;
     float* part;
     unsigned* ctr;
-    int n, width, hq, group, runs, o_f16;
+    int n, width, hq, group, runs, o_f16, part_bytes;
 };
 
 __device__ __forceinline__ f32x4 mfma16(half8v a, half8v b, f32x4 c) {
@@ -209,18 +209,22 @@ __device__ __forceinline__ float sum_u(float x) {
 __device__ __forceinline__ int line_pages(int lk, int width) {
     return lk <= 0 || lk > width * kPage ? 1 : (lk + kPage - 1) / kPage;
 }
-// Parts cross XCDs: stores written through, loads past the L2 (relaxed atomics of the device's
-// scope; the arrival counter orders them).
-typedef unsigned long long u64;
-__device__ __forceinline__ void st_part(float* p, float x, float y) {
-    __hip_atomic_store(reinterpret_cast<u64*>(p), (u64)__float_as_uint(y) << 32 | __float_as_uint(x),
-                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Parts cross XCDs: stores written through, loads past the L2 (sc1; the arrival counter orders
+// them), through a buffer descriptor of the workspace's parts and byte offsets into it.
+constexpr int kSc1 = 16;
+typedef __amdgpu_buffer_rsrc_t Parts;
+__device__ __forceinline__ void st_part(Parts p, int at, f32x4 x) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), p, at, 0, kSc1);
 }
-__device__ __forceinline__ u64 ld_part(const float* p) {
-    return __hip_atomic_load(reinterpret_cast<const u64*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void st_part2(Parts p, int at, float x, float y) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(x), __float_as_uint(y)}, p, at, 0, kSc1);
 }
-__device__ __forceinline__ float lo_f32(u64 x) { return __uint_as_float((uint32_t)x); }
-__device__ __forceinline__ float hi_f32(u64 x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ f32x4 ld_part(Parts p, int at) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(p, at, 0, kSc1));
+}
+__device__ __forceinline__ f32x2 ld_part2(Parts p, int at) {
+    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(p, at, 0, kSc1));
+}
 
 // weight of a part whose largest score is m in a sum whose largest is top (a part without a key has
 // m = -inf)
@@ -270,9 +274,13 @@ decode_paged_kernel(DecodePagedArgs a) {
     // ---- this workgroup's run of the line of pages -------------------------------------------
     const int lk0 = lane < a.n ? a.lk[lane] : 0;
     const int np0 = lane < a.n ? line_pages(lk0, a.width) : 0;
-    int total = np0;
-    for (int i = 64 + lane; i < a.n; i += 64) total += line_pages(a.lk[i], a.width);
-    total = __builtin_amdgcn_readfirstlane(__shfl(wave_scan(total), 63));
+    const int incl0 = wave_scan(np0);
+    int total = __builtin_amdgcn_readlane(incl0, 63);
+    if (a.n > 64) {
+        int more = 0;
+        for (int i = 64 + lane; i < a.n; i += 64) more += line_pages(a.lk[i], a.width);
+        total += __builtin_amdgcn_readlane(wave_scan(more), 63);
+    }
     const int size = max((total + a.runs - 1) / a.runs, kMinPages);
     int at = run * size;
     const int end = min(at + size, total);
@@ -280,18 +288,16 @@ decode_paged_kernel(DecodePagedArgs a) {
     int seq = 0, seq_at = 0;  // the sequence that holds page `at`, and its first page in the line
     for (int i0 = 0; i0 < a.n; i0 += 64) {
         const int np = i0 == 0 ? np0 : i0 + lane < a.n ? line_pages(a.lk[i0 + lane], a.width) : 0;
-        const int incl = wave_scan(np) + seq_at;
+        const int incl = (i0 == 0 ? incl0 : wave_scan(np)) + seq_at;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             seq = i0 + l;
-            seq_at = __shfl(incl - np, l);
+            seq_at = __builtin_amdgcn_readlane(incl - np, l);
             break;
         }
-        seq_at = __shfl(incl, 63);
+        seq_at = __builtin_amdgcn_readlane(incl, 63);
     }
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    seq_at = __builtin_amdgcn_readfirstlane(seq_at);
 
     for (; at < end; ++seq) {
         const int lk_raw = seq < 64 ? __builtin_amdgcn_readlane(lk0, seq) : a.lk[seq];
@@ -518,9 +524,11 @@ decode_paged_kernel(DecodePagedArgs a) {
         __syncthreads();
         const size_t out0 = ((size_t)seq * a.hq + h0) * kDim;
         const size_t plane = (size_t)blockIdx.y * a.runs;  // of this chunk of columns
+        const Parts parts_at = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, a.part_bytes, 0x00027000);
         auto part_of = [&](int r, int second) {
-            return a.part + (((plane + r) * a.p.hkv + kh) * 2 + second) * kPartFloats;
+            return (int)(((plane + r) * a.p.hkv + kh) * 2 + second) * kPartBytes;
         };
+        constexpr int kSums = 2 * kMaxCols * 4;  // where a part's sums start
         for (int i = threadIdx.x; i < cols * (kDim / 4); i += kDecThreads) {
             const int col = i / (kDim / 4), d = 4 * (i % (kDim / 4));
             float m = s_m[0][col];
@@ -540,10 +548,9 @@ decode_paged_kernel(DecodePagedArgs a) {
             if (whole) {
                 write_o(a, out0 + 4 * i, x, l);
             } else {
-                float* p = part_of(run, at == run * size ? 0 : 1);
-                st_part(p + 2 * kMaxCols + 4 * i, x[0], x[1]);
-                st_part(p + 2 * kMaxCols + 4 * i + 2, x[2], x[3]);
-                if (d == 0) st_part(p + 2 * col, m, l);
+                const int p = part_of(run, at == run * size ? 0 : 1);
+                st_part(parts_at, p + kSums + 16 * i, x);
+                if (d == 0) st_part2(parts_at, p + 8 * col, m, l);
             }
         }
         if (!whole) {
@@ -565,33 +572,33 @@ decode_paged_kernel(DecodePagedArgs a) {
                 const int share = kDecThreads / chunks;
                 const int i = threadIdx.x % chunks, g = threadIdx.x / chunks;
                 const int col = i / (kDim / 4);
-                u64 w[kAhead][2];
+                f32x4 w[kAhead];
                 auto load = [&](int r) {
 #pragma unroll
                     for (int j = 0; j < kAhead; ++j) {
                         const int rj = min(r + j * share, parts - 1);
-                        const float* p = part_of(r0 + rj, rj ? 0 : first) + 2 * kMaxCols + 4 * i;
-                        w[j][0] = ld_part(p);
-                        w[j][1] = ld_part(p + 2);
+                        w[j] = ld_part(parts_at, part_of(r0 + rj, rj ? 0 : first) + kSums + 16 * i);
                     }
                 };
+                // (m, l) of this wave's first column's parts go ahead of the sums
+                f32x2 ml = ld_part2(parts_at, part_of(r0 + min(lane, parts - 1), lane ? 0 : first) + 8 * min(wave, cols - 1));
+                __builtin_amdgcn_sched_barrier(0);
                 load(g);
                 __builtin_amdgcn_sched_barrier(0);
                 // weights: a wave per column, a lane per part
                 float* s_w = &s_acc[0][0][0];  // [column][part]
                 for (int cw = wave; cw < cols; cw += kWaves) {
-                    float m = -INFINITY, l = 0.0f;
-                    u64 ml = ld_part(part_of(r0 + min(lane, parts - 1), lane ? 0 : first) + 2 * cw);
+                    if (cw != wave) ml = ld_part2(parts_at, part_of(r0 + min(lane, parts - 1), lane ? 0 : first) + 8 * cw);
+                    float m = lane < parts ? ml[0] : -INFINITY, l = 0.0f;
                     for (int r = lane + 64; r < parts; r += 64)
-                        m = fmaxf(m, lo_f32(ld_part(part_of(r0 + r, 0) + 2 * cw)));
-                    if (lane < parts) m = fmaxf(m, lo_f32(ml));
+                        m = fmaxf(m, ld_part2(parts_at, part_of(r0 + r, 0) + 8 * cw)[0]);
 #pragma unroll
                     for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
                     for (int r = lane; r < parts; r += 64) {
-                        if (r >= 64) ml = ld_part(part_of(r0 + r, 0) + 2 * cw);
-                        const float f = part_weight(lo_f32(ml), m);
+                        if (r >= 64) ml = ld_part2(parts_at, part_of(r0 + r, 0) + 8 * cw);
+                        const float f = part_weight(ml[0], m);
                         s_w[cw * parts + r] = f;
-                        l += lo_f32(ml) == -INFINITY ? hi_f32(ml) : hi_f32(ml) * f;
+                        l += ml[0] == -INFINITY ? ml[1] : ml[1] * f;
                     }
 #pragma unroll
                     for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
@@ -605,10 +612,8 @@ decode_paged_kernel(DecodePagedArgs a) {
                     for (int j = 0; j < kAhead; ++j) {
                         if (r + j * share >= parts) continue;
                         const float f = s_w[col * parts + r + j * share];
-                        x[0] = fmaf(lo_f32(w[j][0]), f, x[0]);
-                        x[1] = fmaf(hi_f32(w[j][0]), f, x[1]);
-                        x[2] = fmaf(lo_f32(w[j][1]), f, x[2]);
-                        x[3] = fmaf(hi_f32(w[j][1]), f, x[3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = fmaf(w[j][e], f, x[e]);
                     }
                 }
                 if (share > 1) {
@@ -641,13 +646,17 @@ int store_paged_launch(const PoolArgs& pool, const float* k, const float* v, con
     return check_launch("store_paged_kernel");
 }
 
-static size_t decode_paged_ctr_bytes(int hkv, int chunks) {
-    return (size_t)chunks * decode_runs(hkv, chunks) * hkv * kCounterStride * sizeof(unsigned);
+// the workspace: arrival counters, then two parts for each workgroup
+static size_t decode_paged_wgs(int hq, int hkv) {
+    const int chunks = (hq / hkv + kMaxCols - 1) / kMaxCols;
+    return (size_t)chunks * decode_runs(hkv, chunks) * hkv;
+}
+static size_t decode_paged_ctr_bytes(size_t wgs) {
+    return (wgs * kCounterStride * sizeof(unsigned) + 255) / 256 * 256;
 }
 size_t decode_paged_workspace_len(int hq, int hkv) {
-    const int chunks = (hq / hkv + kMaxCols - 1) / kMaxCols;
-    return decode_paged_ctr_bytes(hkv, chunks) +
-           (size_t)chunks * decode_runs(hkv, chunks) * hkv * 2 * kPartFloats * sizeof(float);
+    const size_t wgs = decode_paged_wgs(hq, hkv);
+    return decode_paged_ctr_bytes(wgs) + wgs * 2 * kPartBytes;
 }
 
 int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, int width,
@@ -666,8 +675,10 @@ int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, 
     a.o_f16 = o_f16;
     const int chunks = (a.group + kMaxCols - 1) / kMaxCols;
     a.runs = decode_runs(pool.hkv, chunks);
+    const size_t wgs = decode_paged_wgs(hq, pool.hkv);
     a.ctr = static_cast<unsigned*>(ws);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + decode_paged_ctr_bytes(pool.hkv, chunks));
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + decode_paged_ctr_bytes(wgs));
+    a.part_bytes = (int)(wgs * 2 * kPartBytes);
     hipLaunchKernelGGL(decode_paged_kernel, dim3((unsigned)(a.runs * pool.hkv), chunks), dim3(kDecThreads),
                        0, stream, a);
     return check_launch("decode_paged_kernel");

@@ -14,14 +14,15 @@ constexpr int kPage = BRASA_KV_PAGE;        // positions of a page
 constexpr int kTileBytes8 = kPage * kDim;   // codes of one head's page
 
 // ---- wave64 helpers -------------------------------------------------------------------------
-// inclusive sum over the lanes of a wave
+// inclusive sum over the lanes of a wave: within rows of 16 (row_shr), then row 0 into 1 and 2 into
+// 3 (row_bcast 15), then the lower half into the upper (row_bcast 31)
 __device__ __forceinline__ int wave_scan(int x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
     return x;
 }
 
