@@ -190,6 +190,11 @@ __device__ __forceinline__ half2v half_of(float x, float y, float less) {
     const half2v hi = {(_Float16)x, (_Float16)y};
     return half2v{(_Float16)fmaf((float)hi.x, less, x), (_Float16)fmaf((float)hi.y, less, y)};
 }
+// x plus that of column 15 - c: the same bits in both. (as_f32 keeps the addition here, where
+// row_mirror folds into it; sunk into a later block it would leave its move behind.)
+__device__ __forceinline__ float add_mirror(float x) {
+    return as_f32(x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true)));
+}
 // over the four lanes c, c + 16, c + 32, c + 48 of a column
 __device__ __forceinline__ float max_u(float x) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
@@ -410,7 +415,7 @@ decode_paged_kernel(DecodePagedArgs a) {
                     s[T] = mfma16(ka, q[t], s[T]);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[T][r] += dpp<0x140>(s[T][r]);  // hi + lo: column 15 - c
+                for (int r = 0; r < 4; ++r) s[T][r] = add_mirror(s[T][r]);  // q's hi + lo halves
             }
             // 2^sx times the products of the codes and the scaled q. (Past the clamp every score is
             // 0, or so far from the next that one key takes all.)
@@ -424,14 +429,21 @@ decode_paged_kernel(DecodePagedArgs a) {
             }
             __builtin_amdgcn_sched_barrier(0);
             const int left = lk - b * kPage;  // live keys of the page
+            if (left < kPage) {  // the codes behind the last key may be anything, NaN too
+#pragma unroll
+                for (int T = 0; T < 4; ++T)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool live = 16 * T + 4 * u + r < left;
+                        s[T][r] = live ? s[T][r] : -INFINITY;
+                        v.w[T][r] = live ? v.w[T][r] : u32x2{0, 0};
+                    }
+            }
             float tmax = -INFINITY;
 #pragma unroll
             for (int T = 0; T < 4; ++T)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (left < kPage && 16 * T + 4 * u + r >= left) s[T][r] = -INFINITY;
-                    tmax = fmaxf(tmax, s[T][r]);
-                }
+                for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, s[T][r]);
             tmax = max_u(tmax) * sc;
             // a reference point that moves only when the maximum has grown by 2^8: p stays below
             // 2^15 with the bias of 2^7 that keeps the lo halves of small p out of f16's subnormals
@@ -457,13 +469,6 @@ decode_paged_kernel(DecodePagedArgs a) {
                     h[e] = half_of(p0, p1, less);
                 }
                 p[st] = join(h[0], h[1], h[2], h[3]);
-            }
-            if (left < kPage) {  // codes behind the last key may be anything, NaN too
-#pragma unroll
-                for (int T = 0; T < 4; ++T)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (16 * T + 4 * u + r >= left) v.w[T][r] = u32x2{0, 0};
             }
             const float vs = ldexpf(1.0f, v.x - 127);
             // ---- O^T += V^T P^T: tile t's rows are dims 8 i + t ------------------------------------
@@ -507,7 +512,7 @@ decode_paged_kernel(DecodePagedArgs a) {
 #pragma unroll
         for (int t = 0; t < 8; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][r] += dpp<0x140>(acc[t][r]);  // P's hi + lo halves
+            for (int r = 0; r < 4; ++r) acc[t][r] = add_mirror(acc[t][r]);  // P's hi + lo halves
         if (c < cols) {
             if (u == 0) {
                 s_m[wave][c] = m_used;
