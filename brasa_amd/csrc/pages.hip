@@ -15,27 +15,54 @@ namespace {
 constexpr int kPagesThreads = 1024;
 constexpr int kPagesWaves = kPagesThreads / 64;
 
-// exclusive sum over the workgroup's threads; `sum` is the total. s: kPagesWaves + 1 ints of LDS.
-__device__ __forceinline__ int block_scan(int x, int* s, int& sum) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int incl = wave_scan(x);
+// exclusive sum over the workgroup's threads; `sum` is the total. s: kPagesWaves ints of LDS, free
+// again after the next barrier.
+__device__ __forceinline__ int across_waves(int mine, int* s, int& sum) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __syncthreads();  // s is free
-    if (lane == 63) s[wave] = incl;
+    if (lane == 0) s[wave] = mine;
     __syncthreads();
-    if (wave == 0) {
-        const int w = lane < kPagesWaves ? s[lane] : 0;
-        const int i = wave_scan(w);
-        if (lane < kPagesWaves) s[lane] = i - w;
-        if (lane == kPagesWaves - 1) s[kPagesWaves] = i;
-    }
+    static_assert(kPagesWaves == 16, "a row of 16 lanes scans the waves");
+    int w = s[lane & 15];
+    w += __builtin_amdgcn_update_dpp(0, w, 0x111, 0xF, 0xF, true);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x112, 0xF, 0xF, true);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x114, 0xF, 0xF, true);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x118, 0xF, 0xF, true);
+    sum = __builtin_amdgcn_readlane(w, 15);
+    return __builtin_amdgcn_readlane(w, wave) - mine;
+}
+__device__ __forceinline__ int block_scan(int x, int* s, int& sum) {
+    const int incl = wave_scan(x);
+    return across_waves(__builtin_amdgcn_readlane(incl, 63), s, sum) + incl - x;
+}
+// the same for truth values
+__device__ __forceinline__ int block_rank(bool on, int* s, int& sum) {
+    const unsigned long long b = __builtin_amdgcn_ballot_w64(on);
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+    return across_waves(__builtin_popcountll(b), s, sum) + before;
+}
+// Workgroup barrier after which the workgroup's earlier global stores and atomics have reached the L2,
+// where its later atomics and device-scope loads see them.
+__device__ __forceinline__ void stores_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    sum = s[kPagesWaves];
-    return s[wave] + incl - x;
+}
+__device__ __forceinline__ int ld_l2(const int* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__device__ __forceinline__ void copy_ints(int* dst, const int* src, long long n) {
+// dst = src by `threads` threads, this one the tid-th, eight loads in flight
+__device__ __forceinline__ void copy_ints(int* dst, const int* src, long long n, int tid, int threads) {
     if (dst == src) return;
-    for (long long i = threadIdx.x; i < n; i += kPagesThreads) dst[i] = src[i];
+    for (long long i = tid; i < n; i += 8LL * threads) {
+        int x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = i + (long long)j * threads < n ? src[i + (long long)j * threads] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + (long long)j * threads < n) dst[i + (long long)j * threads] = x[j];
+    }
 }
 
 // ---- fork ---------------------------------------------------------------------------------------
@@ -49,58 +76,81 @@ struct ForkArgs {
     int n, width, pages;
 };
 
-// entries [i0, n * width) by `step`: row i takes row parent[i]; the old row's pages lose an owner,
-// the new one's gain one
-__device__ __forceinline__ void fork_entries(const ForkArgs& a, long long i0, long long step) {
-    const long long all = (long long)a.n * a.width;
-    for (long long i = i0; i < all; i += step) {
-        const int row = (int)(i / a.width), col = (int)(i - (long long)row * a.width);
-        int parent = a.parent[row];
-        if (parent < 0 || parent >= a.n) parent = -1;
-        const int old = a.table[i];
-        const int now = parent < 0 ? -1 : a.table[(long long)parent * a.width + col];
-        a.table_out[i] = now;
-        if (col == 0) a.len_out[row] = parent < 0 ? 0 : a.len[parent];
-        if (parent == row) continue;
-        if (old >= 0 && old < a.pages) atomicAdd(a.ref + old, -1);
-        if (now >= 0 && now < a.pages) atomicAdd(a.ref + now, 1);
+// Rows row0, row0 + rows, ...; a wave per row, a lane per entry, kForkRows rows' loads in flight
+// together. Row i takes row parent[i]; the old row's pages lose an owner, the new one's gain one.
+constexpr int kForkRows = 8;
+__device__ __forceinline__ void fork_rows(const ForkArgs& a, int row0, int rows) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = row0; i0 < a.n; i0 += rows * kForkRows) {
+        int parent[kForkRows];
+#pragma unroll
+        for (int j = 0; j < kForkRows; ++j) {
+            const int i = i0 + j * rows;
+            const int p = i < a.n ? a.parent[i] : -1;
+            parent[j] = p < 0 || p >= a.n ? -1 : p;
+        }
+        for (int c0 = 0; c0 < a.width; c0 += 64) {
+            const int col = c0 + lane;
+            int old[kForkRows], now[kForkRows];
+#pragma unroll
+            for (int j = 0; j < kForkRows; ++j) {
+                const int i = i0 + j * rows;
+                old[j] = i < a.n && col < a.width ? a.table[(size_t)i * a.width + col] : -1;
+                now[j] = parent[j] >= 0 && col < a.width ? a.table[(size_t)parent[j] * a.width + col] : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < kForkRows; ++j) {
+                const int i = i0 + j * rows;
+                if (i >= a.n) break;
+                if (col < a.width) a.table_out[(size_t)i * a.width + col] = now[j];
+                if (parent[j] == i) continue;
+                if (old[j] >= 0 && old[j] < a.pages) atomicAdd(a.ref + old[j], -1);
+                if (now[j] >= 0 && now[j] < a.pages) atomicAdd(a.ref + now[j], 1);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kForkRows; ++j) {
+            const int i = i0 + j * rows;
+            if (i < a.n && lane == 0) a.len_out[i] = parent[j] < 0 ? 0 : a.len[parent[j]];
+        }
     }
 }
 
 __global__ void __launch_bounds__(kPagesThreads)
 fork_small_kernel(ForkArgs a, const int* ref_in) {
-    copy_ints(a.ref, ref_in, a.pages);
-    __threadfence();
-    __syncthreads();
-    fork_entries(a, threadIdx.x, kPagesThreads);
+    copy_ints(a.ref, ref_in, a.pages, threadIdx.x, kPagesThreads);
+    stores_barrier();
+    fork_rows(a, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kPagesWaves);
 }
 __global__ void __launch_bounds__(256)
 fork_kernel(ForkArgs a) {
-    fork_entries(a, (long long)blockIdx.x * 256 + threadIdx.x, (long long)gridDim.x * 256);
+    fork_rows(a, __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), gridDim.x * 4);
 }
 __global__ void __launch_bounds__(256)
 copy_ints_kernel(int* dst, const int* src, int n) {
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) dst[i] = src[i];
+    copy_ints(dst, src, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ---- the moves of pages -----------------------------------------------------------------------
-// The workspace of reserve and compact: the moves' count, then the lists.
+// The workspace of reserve and compact: what the first launch decides and the second carries out.
 struct MoveList {
-    int* count;
-    int* src;
+    int* count;     // [0] moves, [1] edits
+    int* src;       // moves: page src to dst, its first `held` positions
     int* dst;
-    int* held;   // live positions of the page (kPage: all)
-    int* tmp;    // reserve: claims and first claim of each page; compact: unused
+    int* held;
+    int* entry;     // reserve, edits: table entry, its new page (and the one it held, or -1)
+    int* page;
+    int* was;
+    int* tmp;       // reserve: claims and first claim of each page; compact: each moved page's new id
     int* free_ids;
     uint8_t* take;
 };
 
 // One head's page (8 KB each of K and V) per workgroup and step: 16-byte pieces, all of a step's
 // loads in flight at once.
-__global__ void __launch_bounds__(256)
-move_pages_kernel(PoolArgs p, MoveList m, bool whole) {
+__device__ __forceinline__ void move_pages(const PoolArgs& p, const MoveList& m, bool whole) {
     const int heads = p.layers * p.hkv;
-    const long long units = (long long)*m.count * heads;
+    const long long units = (long long)m.count[0] * heads;
     for (long long w = blockIdx.x; w < units; w += gridDim.x) {
         const int i = (int)(w / heads), lh = (int)(w % heads);
         const int layer = lh / p.hkv, kh = lh % p.hkv;
@@ -128,6 +178,7 @@ move_pages_kernel(PoolArgs p, MoveList m, bool whole) {
 
 // ---- reserve ------------------------------------------------------------------------------------
 struct ReserveArgs {
+    PoolArgs p;
     const int* add;
     const int* table;
     const int* len;
@@ -139,18 +190,49 @@ struct ReserveArgs {
     MoveList m;
 };
 
-// Calls f(valid, row, block, len, claim number) in rounds of the whole workgroup, the claims in order:
-// blocks [len / 64, (len + add) / 64 up) of each row with add > 0.
+// The claims of a row: blocks [len / 64, (len + add) / 64 up), none where add <= 0.
+__device__ __forceinline__ int row_claims(const ReserveArgs& a, int len, int add) {
+    if (add <= 0) return 0;
+    return max(min((int)(((long long)len + add + kPage - 1) / kPage), a.width) - len / kPage, 0);
+}
+__device__ __forceinline__ int owned_page(const ReserveArgs& a, size_t entry) {
+    const int e = a.table[entry];
+    return e >= 0 && e < a.pages ? e : -1;
+}
+// Claim k of `rows` rows whose claims end at s_end[row]: its row (the first whose claims end past k)
+// and its place among the row's.
+__device__ __forceinline__ int claim_row(const int* s_end, int rows, int k, int& nth) {
+    int lo = 0, hi = rows - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (s_end[mid] > k) hi = mid;
+        else lo = mid + 1;
+    }
+    nth = k - (lo ? s_end[lo - 1] : 0);
+    return lo;
+}
+// What one granted claim changes: the second launch's edit, and a move where the page it leaves
+// holds positions of the row.
+__device__ __forceinline__ void grant(const ReserveArgs& a, int k, int entry, int page, int was, int held,
+                                      int* s_moves) {
+    a.m.entry[k] = entry;
+    a.m.page[k] = page;
+    a.m.was[k] = was;
+    if (was >= 0 && held > 0) {
+        const int i = atomicAdd(s_moves, 1);
+        a.m.src[i] = was;
+        a.m.dst[i] = page;
+        a.m.held[i] = held;
+    }
+}
+
+// Calls f(valid, row, block, len, claim number) in rounds of the whole workgroup, the claims in order.
 template <typename F>
 __device__ __forceinline__ void for_claims(const ReserveArgs& a, int* s_scan, int* s_end, F f) {
-    long long base = 0;
+    int base = 0;
     for (int r0 = 0; r0 < a.n; r0 += kPagesThreads) {
         const int r = r0 + threadIdx.x;
-        int c = 0;
-        if (r < a.n && a.add[r] > 0) {
-            const int len = max(a.len[r], 0);
-            c = max(min((int)(((long long)len + a.add[r] + kPage - 1) / kPage), a.width) - len / kPage, 0);
-        }
+        const int c = r < a.n ? row_claims(a, max(a.len[r], 0), a.add[r]) : 0;
         int sum;
         const int excl = block_scan(c, s_scan, sum);
         s_end[threadIdx.x] = excl + c;
@@ -158,69 +240,45 @@ __device__ __forceinline__ void for_claims(const ReserveArgs& a, int* s_scan, in
         const int rows = min(a.n - r0, kPagesThreads);
         for (int i0 = 0; i0 < sum; i0 += kPagesThreads) {
             const int i = i0 + threadIdx.x;
-            int lo = 0, hi = rows - 1;  // the first row whose claims end past i
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (s_end[mid] > i) hi = mid;
-                else lo = mid + 1;
-            }
-            const int row = r0 + lo;
+            int nth;
+            const int row = r0 + claim_row(s_end, rows, i, nth);
             const int len = i < sum ? max(a.len[row], 0) : 0;
-            const int block = len / kPage + i - (lo ? s_end[lo - 1] : 0);
-            f(i < sum, row, block, len, base + i);
+            f(i < sum, row, len / kPage + nth, len, base + i);
         }
         base += sum;
         __syncthreads();
     }
 }
 
-__global__ void __launch_bounds__(kPagesThreads)
-reserve_kernel(ReserveArgs a) {
-    __shared__ int s_scan[kPagesWaves + 1];
-    __shared__ int s_end[kPagesThreads];
-    __shared__ int s_moves, s_refused;
+// The general path: any number of rows and claims, in rounds of the workgroup, with the claims of each
+// page counted in the workspace.
+__device__ __forceinline__ void reserve_many(const ReserveArgs& a, bool refused, int* s_scan, int* s_end,
+                                             int* s_moves) {
     int* count = a.m.tmp;
     int* first = a.m.tmp + a.pages;
-    auto page_of = [&](int row, int block) {
-        const int e = a.table[(size_t)row * a.width + block];
-        return e >= 0 && e < a.pages ? e : -1;
-    };
-    if (threadIdx.x == 0) s_moves = s_refused = 0;
-    __syncthreads();
-    copy_ints(a.table_out, a.table, (long long)a.n * a.width);
-    copy_ints(a.ref_out, a.ref, a.pages);
-    for (int r = threadIdx.x; r < a.n; r += kPagesThreads)
-        if (a.add[r] > 0 && (long long)max(a.len[r], 0) + a.add[r] > (long long)a.width * kPage)
-            s_refused = 1;  // more than the row's table holds
-    // claims of each page that is claimed, and the first of them
-    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int, long long) {
-        const int e = on ? page_of(row, block) : -1;
+    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int, int) {
+        const int e = on ? owned_page(a, (size_t)row * a.width + block) : -1;
         if (e >= 0) {
             count[e] = 0;
             first[e] = 0x7fffffff;
         }
     });
-    __threadfence();
-    __syncthreads();
-    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int, long long i) {
-        const int e = on ? page_of(row, block) : -1;
+    stores_barrier();
+    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int, int i) {
+        const int e = on ? owned_page(a, (size_t)row * a.width + block) : -1;
         if (e >= 0) {
             atomicAdd(count + e, 1);
-            atomicMin(first + e, (int)i);
+            atomicMin(first + e, i);
         }
     });
-    __threadfence();
-    __syncthreads();
+    stores_barrier();
     int need = 0;
-    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int, long long i) {
-        const int e = on ? page_of(row, block) : -1;
-        bool take = on;
+    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int, int i) {
+        const int e = on ? owned_page(a, (size_t)row * a.width + block) : -1;
         // every owner claims it: the first keeps it
-        if (e >= 0)
-            take = !(a.ref[e] <= __hip_atomic_load(count + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) &&
-                     __hip_atomic_load(first + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)i);
-        if (on) a.m.take[i] = take;
-        need += take;
+        const bool keeps = e >= 0 && a.ref[e] <= ld_l2(count + e) && ld_l2(first + e) == i;
+        if (on) a.m.take[i] = !keeps;
+        need += on && !keeps;
     });
     int all;
     block_scan(need, s_scan, all);
@@ -230,46 +288,143 @@ reserve_kernel(ReserveArgs a) {
         const int p = p0 + threadIdx.x;
         const bool free = p < a.pages && a.ref[p] <= 0;
         int sum;
-        const int at = found + block_scan(free, s_scan, sum);
+        const int at = found + block_rank(free, s_scan, sum);
         if (free && at < all) a.m.free_ids[at] = p;
         found += sum;
     }
-    __threadfence();
-    __syncthreads();
-    const bool fits = found >= all && !s_refused;
+    stores_barrier();
+    const bool fits = found >= all && !refused;
     if (threadIdx.x == 0) {
         a.status[0] = fits ? all : 0;
-        a.status[1] = s_refused ? -1 : max(all - found, 0);
+        a.status[1] = refused ? -1 : max(all - found, 0);
+        a.m.count[1] = fits ? all : 0;
     }
-    if (fits) {
-        int before = 0;
-        for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int len, long long i) {
-            const bool take = on && a.m.take[i];
-            int sum;
-            const int rank = before + block_scan(take, s_scan, sum);
-            before += sum;
-            if (!take) return;
-            const int e = page_of(row, block);
-            const int page = a.m.free_ids[rank];
-            a.ref_out[page] = 1;
-            if (e >= 0) {
-                atomicAdd(a.ref_out + e, -1);
-                if (len > block * kPage) {  // the rows it holds are copied
-                    const int k = atomicAdd(&s_moves, 1);
-                    a.m.src[k] = e;
-                    a.m.dst[k] = page;
-                    a.m.held[k] = len - block * kPage;
-                }
-            }
-            a.table_out[(size_t)row * a.width + block] = page;
-        });
+    if (!fits) return;
+    int before = 0;
+    for_claims(a, s_scan, s_end, [&](bool on, int row, int block, int len, int i) {
+        const bool take = on && a.m.take[i];
+        int sum;
+        const int rank = before + block_rank(take, s_scan, sum);
+        before += sum;
+        if (!take) return;
+        const int entry = row * a.width + block;
+        grant(a, rank, entry, ld_l2(a.m.free_ids + rank), owned_page(a, entry), len - block * kPage, s_moves);
+    });
+}
+
+// Up to kPagesThreads rows and claims, as in a decode step: a claim per thread, the claims of a page
+// counted in a hash table in LDS, free pages listed in LDS.
+constexpr int kHash = 4 * kPagesThreads;  // slots: at most a quarter is taken, so a probe ends
+struct ReserveLds {
+    int scan[kPagesWaves];
+    int end[kPagesThreads];
+    int key[kHash], count[kHash], first[kHash];
+    int free_ids[kPagesThreads];
+    int moves, refused;
+};
+
+__device__ __forceinline__ void reserve_few(const ReserveArgs& a, ReserveLds& s, int claims, bool refused,
+                                            int free0) {
+    const int k = threadIdx.x;
+    const bool on = k < claims;
+    int nth, entry = 0, held = 0, e = -1;
+    {
+        const int row = claim_row(s.end, a.n, k, nth);
+        if (on) {
+            const int len = max(a.len[row], 0);
+            entry = row * a.width + len / kPage + nth;
+            held = nth ? 0 : len % kPage;
+            e = owned_page(a, entry);
+        }
+    }
+    const int owners = e >= 0 ? a.ref[e] : 0;
+    int slot = -1;
+    if (e >= 0) {
+        slot = (int)((uint32_t)e * 2654435761u >> 20) & (kHash - 1);
+        while (true) {
+            const int was = atomicCAS(&s.key[slot], -1, e);
+            if (was == -1 || was == e) break;
+            slot = (slot + 1) & (kHash - 1);
+        }
+        atomicAdd(&s.count[slot], 1);
+        atomicMin(&s.first[slot], k);
     }
     __syncthreads();
-    if (threadIdx.x == 0) *a.m.count = s_moves;
+    // every owner claims it: the first keeps it
+    const bool take = on && !(e >= 0 && owners <= s.count[slot] && s.first[slot] == k);
+    int all;
+    const int rank = block_rank(take, s.scan, all);
+    int found = 0;
+    for (int p0 = 0; p0 < a.pages && found < all; p0 += kPagesThreads) {
+        const int p = p0 + threadIdx.x;
+        const bool free = p < a.pages && (p0 ? a.ref[p] : free0) <= 0;
+        int sum;
+        const int at = found + block_rank(free, s.scan, sum);
+        if (free && at < all) s.free_ids[at] = p;
+        found += sum;
+    }
+    __syncthreads();
+    const bool fits = found >= all && !refused;
+    if (threadIdx.x == 0) {
+        a.status[0] = fits ? all : 0;
+        a.status[1] = refused ? -1 : max(all - found, 0);
+        a.m.count[1] = fits ? all : 0;
+    }
+    if (fits && take) grant(a, rank, entry, s.free_ids[rank], e, held, &s.moves);
+}
+
+// Workgroup 0 decides; the others copy the table and the counts meanwhile.
+__global__ void __launch_bounds__(kPagesThreads)
+reserve_kernel(ReserveArgs a) {
+    __shared__ ReserveLds s;
+    if (blockIdx.x > 0) {
+        const int tid = (blockIdx.x - 1) * kPagesThreads + threadIdx.x, threads = (gridDim.x - 1) * kPagesThreads;
+        copy_ints(a.table_out, a.table, (long long)a.n * a.width, tid, threads);
+        copy_ints(a.ref_out, a.ref, a.pages, tid, threads);
+        return;
+    }
+    const int free0 = threadIdx.x < a.pages ? a.ref[threadIdx.x] : 1;
+    if (threadIdx.x == 0) s.moves = s.refused = 0;
+    for (int i = threadIdx.x; i < kHash; i += kPagesThreads) {
+        s.key[i] = -1;
+        s.count[i] = 0;
+        s.first[i] = 0x7fffffff;
+    }
+    __syncthreads();
+    int claims = 0;
+    for (int r0 = 0; r0 < a.n; r0 += kPagesThreads) {
+        const int r = r0 + threadIdx.x;
+        const int len = r < a.n ? max(a.len[r], 0) : 0, add = r < a.n ? a.add[r] : 0;
+        if (add > 0 && (long long)len + add > (long long)a.width * kPage) s.refused = 1;  // past the row's table
+        const int c = row_claims(a, len, add);
+        int sum;
+        const int excl = block_scan(c, s.scan, sum);
+        s.end[threadIdx.x] = excl + c;
+        claims += sum;
+    }
+    __syncthreads();
+    const bool refused = s.refused;
+    if (a.n <= kPagesThreads && claims <= kPagesThreads) reserve_few(a, s, claims, refused, free0);
+    else reserve_many(a, refused, s.scan, s.end, &s.moves);
+    __syncthreads();
+    if (threadIdx.x == 0) a.m.count[0] = s.moves;
+}
+
+__global__ void __launch_bounds__(256)
+reserve_apply_kernel(ReserveArgs a) {
+    const int edits = a.m.count[1];
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < edits; i += gridDim.x * 256) {
+        const int was = a.m.was[i], page = a.m.page[i];
+        a.table_out[a.m.entry[i]] = page;
+        a.ref_out[page] = 1;
+        if (was >= 0) atomicAdd(a.ref_out + was, -1);
+    }
+    move_pages(a.p, a.m, false);
 }
 
 // ---- compact ------------------------------------------------------------------------------------
 struct CompactArgs {
+    PoolArgs p;
     const int* table;
     const int* ref;
     int* table_out;
@@ -281,14 +436,15 @@ struct CompactArgs {
 
 __global__ void __launch_bounds__(kPagesThreads)
 compact_kernel(CompactArgs a) {
-    __shared__ int s_scan[kPagesWaves + 1];
-    int mine = 0, live;
-    for (int p = threadIdx.x; p < a.pages; p += kPagesThreads) mine += a.ref[p] > 0;
+    __shared__ int s_scan[kPagesWaves];
+    const int ref0 = threadIdx.x < a.pages ? a.ref[threadIdx.x] : 0;
+    int mine = ref0 > 0, live;
+    for (int p = kPagesThreads + threadIdx.x; p < a.pages; p += kPagesThreads) mine += a.ref[p] > 0;
     block_scan(mine, s_scan, live);
     int moves = 0, holes = 0;
     for (int p0 = 0; p0 < a.pages; p0 += kPagesThreads) {
         const int p = p0 + threadIdx.x;
-        const bool used = p < a.pages && a.ref[p] > 0;
+        const bool used = p < a.pages && (p0 ? a.ref[p] : ref0) > 0;
         int sum;
         // pages in use at or past `live` go down, free ones below it are filled
         const int at = block_scan(p >= live ? used : (p < a.pages && !used) << 16, s_scan, sum);
@@ -297,35 +453,35 @@ compact_kernel(CompactArgs a) {
         moves += sum & 0xffff;
         holes += sum >> 16;
     }
-    __threadfence();
-    __syncthreads();
+    copy_ints(a.ref_out, a.ref, a.pages, threadIdx.x, kPagesThreads);
     if (threadIdx.x == 0) {
-        *a.m.count = moves;
+        a.m.count[0] = moves;
         *a.live = live;
     }
-    for (int k = threadIdx.x; k < moves; k += kPagesThreads) a.m.tmp[a.m.src[k]] = a.m.dst[k];
-    copy_ints(a.ref_out, a.ref, a.pages);
-    __syncthreads();
+    stores_barrier();
     for (int k = threadIdx.x; k < moves; k += kPagesThreads) {
-        const int s = a.m.src[k], d = a.m.dst[k];
+        const int s = ld_l2(a.m.src + k), d = ld_l2(a.m.dst + k);
+        a.m.tmp[s] = d;
         a.ref_out[d] = a.ref[s];
         a.ref_out[s] = 0;
     }
 }
 
 __global__ void __launch_bounds__(256)
-remap_kernel(CompactArgs a) {
+compact_apply_kernel(CompactArgs a) {
     const int live = *a.live;
     const long long all = (long long)a.n * a.width;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
         const int e = a.table[i];
         a.table_out[i] = e >= live && e < a.pages ? a.m.tmp[e] : e;
     }
+    move_pages(a.p, a.m, true);
 }
 
 size_t ints(size_t n) { return (n * sizeof(int) + 255) / 256 * 256; }
 
-MoveList carve(void* ws, int n, int pages) {
+// most: moves (compact: of pages; reserve: one per row); claims: entries of the table, or pages
+MoveList carve(void* ws, int n, int width, int pages) {
     uint8_t* w = static_cast<uint8_t*>(ws);
     MoveList m;
     auto take = [&](size_t count) {
@@ -334,27 +490,28 @@ MoveList carve(void* ws, int n, int pages) {
         return p;
     };
     const size_t most = (size_t)std::max(n, pages);
-    m.count = take(1);
+    const size_t edits = std::min((size_t)n * width, (size_t)pages);  // an edit takes a page
+    m.count = take(2);
     m.src = take(most);
     m.dst = take(most);
     m.held = take(most);
+    m.entry = take(edits);
+    m.page = take(edits);
+    m.was = take(edits);
     m.tmp = take(2 * (size_t)pages);
     m.free_ids = take(pages);
     m.take = w;
     return m;
 }
 
-int launch_moves(const PoolArgs& pool, const MoveList& m, long long most, bool whole, hipStream_t stream) {
-    const long long units = most * pool.layers * pool.hkv;
-    const unsigned grid = (unsigned)std::min<long long>(std::max<long long>(units, 1), 2048);
-    hipLaunchKernelGGL(move_pages_kernel, dim3(grid), dim3(256), 0, stream, pool, m, whole);
-    return check_launch("move_pages_kernel");
-}
+// workgroups of a launch that has `units` pieces of work at most
+unsigned grid_of(long long units) { return (unsigned)std::min<long long>(std::max<long long>(units, 1), 2048); }
 
 }  // namespace
 
 size_t kv_pages_workspace_len(int pages, int n, int width) {
-    return ints(1) + 3 * ints(std::max(n, pages)) + ints(2 * (size_t)pages) + ints(pages) +
+    const size_t edits = std::min((size_t)n * width, (size_t)pages);
+    return ints(2) + 3 * ints(std::max(n, pages)) + 3 * ints(edits) + ints(2 * (size_t)pages) + ints(pages) +
            ((size_t)n * width + 255) / 256 * 256;
 }
 
@@ -368,41 +525,43 @@ int kv_pages_fork_launch(const int* parent, const int* table, const int* len, co
         return check_launch("fork_small_kernel");
     }
     if (ref_out != ref) {
-        hipLaunchKernelGGL(copy_ints_kernel, dim3(std::min((pages + 255) / 256, 1024)), dim3(256), 0, stream,
+        hipLaunchKernelGGL(copy_ints_kernel, dim3(grid_of((pages + 2047) / 2048)), dim3(256), 0, stream,
                            ref_out, ref, pages);
         const int st = check_launch("copy_ints_kernel");
         if (st != BRASA_OK) return st;
     }
-    hipLaunchKernelGGL(fork_kernel, dim3((unsigned)std::min<long long>((all + 255) / 256, 2048)), dim3(256), 0,
-                       stream, a);
+    hipLaunchKernelGGL(fork_kernel, dim3(grid_of((n + 3) / 4)), dim3(256), 0, stream, a);
     return check_launch("fork_kernel");
 }
 
 int kv_pages_reserve_launch(const PoolArgs& pool, const int* add, const int* table, const int* len,
                             const int* ref, int* table_out, int* ref_out, int* status, int n, int width,
                             void* ws, hipStream_t stream) {
-    ReserveArgs a{add, table, len, ref, table_out, ref_out, status, n, width, pool.pages,
-                  carve(ws, n, pool.pages)};
-    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kPagesThreads), 0, stream, a);
+    ReserveArgs a{pool, add, table, len, ref, table_out, ref_out, status, n, width, pool.pages,
+                  carve(ws, n, width, pool.pages)};
+    long long copies = 0;
+    if (table_out != table) copies += (long long)n * width;
+    if (ref_out != ref) copies += pool.pages;
+    const unsigned others = copies ? grid_of((copies + 8 * kPagesThreads - 1) / (8 * kPagesThreads)) : 0;
+    hipLaunchKernelGGL(reserve_kernel, dim3(1 + others), dim3(kPagesThreads), 0, stream, a);
     const int st = check_launch("reserve_kernel");
     if (st != BRASA_OK) return st;
-    return launch_moves(pool, a.m, n, false, stream);
+    hipLaunchKernelGGL(reserve_apply_kernel, dim3(grid_of((long long)n * pool.layers * pool.hkv)), dim3(256), 0,
+                       stream, a);
+    return check_launch("reserve_apply_kernel");
 }
 
 int kv_pages_compact_launch(const PoolArgs& pool, const int* table, const int* ref, int* table_out,
                             int* ref_out, int* live, int n, int width, void* ws, hipStream_t stream) {
-    CompactArgs a{table, ref, table_out, ref_out, live, n, width, pool.pages, carve(ws, n, pool.pages)};
+    CompactArgs a{pool, table, ref, table_out, ref_out, live, n, width, pool.pages,
+                  carve(ws, n, width, pool.pages)};
     hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kPagesThreads), 0, stream, a);
-    int st = check_launch("compact_kernel");
+    const int st = check_launch("compact_kernel");
     if (st != BRASA_OK) return st;
-    const long long all = (long long)n * width;
-    if (all > 0) {
-        hipLaunchKernelGGL(remap_kernel, dim3((unsigned)std::min<long long>((all + 255) / 256, 2048)), dim3(256),
-                           0, stream, a);
-        st = check_launch("remap_kernel");
-        if (st != BRASA_OK) return st;
-    }
-    return launch_moves(pool, a.m, pool.pages / 2, true, stream);
+    const long long units = (long long)(pool.pages / 2) * pool.layers * pool.hkv;
+    hipLaunchKernelGGL(compact_apply_kernel, dim3(grid_of(std::max(units, ((long long)n * width + 255) / 256))),
+                       dim3(256), 0, stream, a);
+    return check_launch("compact_apply_kernel");
 }
 
 }  // namespace brasa
