@@ -97,6 +97,8 @@ def decode_partials_len(hq: int, lk: int) -> int:
 
 
 def _ptr(x) -> int:
+    if type(x) is int:
+        return x
     if x is None:
         return 0
     if isinstance(x, tuple):
