@@ -481,7 +481,9 @@ __device__ __forceinline__ bool merge_key_parts(const PrefillArgs& a, int tile, 
 // qraw: this wave's raw half Q row. With q_ready it already holds the tile's Q, loaded by the
 // previous tile's call (next_tile) while that tile merged and stored; next_tile >= 0 loads the
 // next tile's Q into it the same way.
-template <int HW, bool PS>
+// PACKED: the rows behind the last key are another prompt's, or nobody's: a tile that reaches past it
+// copies the last key's row in their place (masked like any key past the query).
+template <int HW, bool PS, bool PACKED = false>
 __device__ __forceinline__ void f16_pp_tile(const PrefillArgs& a, const int tile, const int part,
                                             const int ti, uint16_t (&s_kv)[2][2][2][kStageHalves],
                                             u32x4 (&qraw)[8], const bool q_ready,
@@ -564,13 +566,30 @@ __device__ __forceinline__ void f16_pp_tile(const PrefillArgs& a, const int tile
         kso[r] = kdo(r, lrow, lchunk);
         vso[r] = vdo(r, lrow, lchunk);
     }
+    // byte distance from a tile's row quad r to the last key's row, where that is nearer than the row
+    auto clamped = [&](int i, int r) {
+        const int row = 16 * qw + 4 * r + lrow;
+        return (uint32_t)((min(row, lk - 1 - kb_of(i)) - row) * (int)rstride);
+    };
     auto dma_k = [&](int i) {
         const uint8_t* g = sgpr_offset(kbase, (size_t)kb_of(i) * rstride);
+        if (PACKED && kb_of(i) + kTile > lk) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                lds_dma16_s(g, kso[r] + clamped(i, r), lds_k + (i & 1) * kTileBytes + r * 1024);
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds_dma16_s(g, kso[r], lds_k + (i & 1) * kTileBytes + r * 1024);
     };
     auto dma_v = [&](int i) {
         const uint8_t* g = sgpr_offset(vbase, (size_t)kb_of(i) * rstride);
+        if (PACKED && kb_of(i) + kTile > lk) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                lds_dma16_s(g, vso[r] + clamped(i, r), lds_v + (i & 1) * kTileBytes + r * 1024);
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds_dma16_s(g, vso[r], lds_v + (i & 1) * kTileBytes + r * 1024);
     };
@@ -1921,7 +1940,8 @@ __device__ __forceinline__ bool packed_tile(const int* cu, int n, int tokens, in
             continue;
         }
         // the tile number t with count(t) > y >= count(t + 1), count(t) the tiles from t on
-        int lo = 0, hi = tokens / TPW + 1;
+        int lo = 0, hi = 1;
+        while (__builtin_amdgcn_ballot_w64(nt > hi)) hi *= 2;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
             if (__builtin_amdgcn_readfirstlane(wave_sum(max(nt - mid, 0))) > y) lo = mid;
@@ -1967,6 +1987,17 @@ packed_f16_kernel(PackedArgs p) {
     PackedTile t;
     if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
     f16_tile4s<HW, PS, true>(prompt_args<BRASA_KV_F16, false>(p, t), blockIdx.x, t.tile, s_k, s_vv);
+}
+
+// The two-group kernel (8 waves, one workgroup per CU), which halves the longest prompt's chain of stages.
+template <int HW, bool PS>
+__global__ void __launch_bounds__(2 * kThreads, 1)
+packed_pp_kernel(PackedArgs p) {
+    __shared__ __attribute__((aligned(16))) uint16_t s_kv[2][2][2][kStageHalves];
+    PackedTile t;
+    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    u32x4 qraw[8];
+    f16_pp_tile<HW, PS, true>(prompt_args<BRASA_KV_F16, false>(p, t), t.tile, 0, 0, s_kv, qraw, false, -1);
 }
 
 template <int KV, int HW, bool QS, bool PS, bool OF32>
@@ -2425,9 +2456,20 @@ int launch_packed(const PackedArgs& p, int kv, int precision, hipStream_t stream
         return check_launch(name);
     };
     if (kv == BRASA_KV_F16) {
-        if (precision == BRASA_PREFILL_F16) return go(packed_f16_kernel<HW, false>, kThreads, "packed_f16_kernel");
-        if (precision == BRASA_PREFILL_F16_PF32) return go(packed_f16_kernel<HW, true>, kThreads, "packed_f16_kernel");
-        return go(packed_split_kernel<BRASA_KV_F16, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
+        // The two-group kernel where each workgroup has a CU of its own (one prompt of 501 rows, 32 heads
+        // over 8: 15.6 us against 17.3; 1000 rows: 23.5 and 29.4); beyond that three workgroups per
+        // CU hide each other's prologues and chains (2000 rows 54 and 60, but twelve prompts of 2030
+        // rows 31.7 and 21.1, forty of 200 rows 103 and 50).
+        const bool few = tiles * (p.a.hq / HW) <= 256;
+        if (precision == BRASA_PREFILL_F32)
+            return go(packed_split_kernel<BRASA_KV_F16, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
+        if (few)
+            return precision == BRASA_PREFILL_F16
+                       ? go(packed_pp_kernel<HW, false>, 2 * kThreads, "packed_pp_kernel")
+                       : go(packed_pp_kernel<HW, true>, 2 * kThreads, "packed_pp_kernel");
+        return precision == BRASA_PREFILL_F16
+                   ? go(packed_f16_kernel<HW, false>, kThreads, "packed_f16_kernel")
+                   : go(packed_f16_kernel<HW, true>, kThreads, "packed_f16_kernel");
     }
     if (precision == BRASA_PREFILL_F32)
         return go(packed_split_kernel<BRASA_KV_F32, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
