@@ -1559,25 +1559,32 @@ template <> struct Chunk8<BRASA_KV_Q8_0> {
 // TFLOP/s of the 3x as many that the splits contract), T = 2000 402 -> 119 us; q8_0 cache,
 // F16_PF32, T = 600 89 -> 33 us; f16 cache, F32 precision, T = 600 57 -> 26 us.
 // PACKED: rows past the last key are another prompt's, or nobody's: the last key's row is read in
-// their place.
+// their place. CB: column blocks of the workgroup, and waves of a key group. NG: key groups; two take
+// turns with two stage buffers each, four have one, written while nobody reads.
 template <int KV>
 constexpr int kSplitBuf = 2 * (KV != BRASA_KV_F16 ? 2 : 1) * kStageHalvesS;  // a stage: K hi, K lo, V hi, V lo
 constexpr int kXchHalves = 4 * 17 * 64 * 8;                                 // the group merge's exchange
+template <int KV>  // four key groups of two column blocks
+constexpr int kSplitHalves4 = 4 * kSplitBuf<KV> > 6 * 17 * 64 * 8 ? 4 * kSplitBuf<KV> : 6 * 17 * 64 * 8;
 template <int KV>
 constexpr int kSplitHalves = 4 * kSplitBuf<KV> > kXchHalves ? 4 * kSplitBuf<KV> : kXchHalves;
-template <int KV, int HW, bool QS, bool PS, bool OF32, bool PACKED>
+template <int KV, int HW, bool QS, bool PS, bool OF32, bool PACKED, int CB = 4, int NG = 2>
 __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, const int tile,
                                            const int part, uint16_t* s_kv) {
     constexpr bool KS = KV != BRASA_KV_F16;  // cache values need hi / lo
     constexpr int NK = KS ? 2 : 1;
-    constexpr int TPW = 32 * 4 / HW;         // query tokens per workgroup
+    constexpr int TPW = 32 * CB / HW;        // query tokens per workgroup
+    constexpr int kRows = 4 * CB;            // rows a key group stages at a time
+    constexpr int kSteps = kTileS / kRows;
+    constexpr int NB = 4 / NG;               // stage buffers of a group
+    static_assert(HW <= CB && CB * NG <= 8, "a wave per column block and group");
     constexpr int RB = KvTraits<KV>::row_bytes;
     constexpr int kBuf = kSplitBuf<KV>;
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int grp = wave >> 2;
-    const int qw = wave & 3;
+    const int grp = wave / CB;
+    const int qw = wave % CB;
     const int col = lane & 31;       // query column of the MFMA tiles
     const int u = lane >> 5;         // lane half
 
@@ -1593,36 +1600,36 @@ __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, c
     const int sb = (int)((long long)nst_all * part / a.kparts);
     const int nst = (int)((long long)nst_all * (part + 1) / a.kparts) - sb;
     // up to 64 keys: one group takes them all (a merge costs more than a stage)
-    const int ngrp = nst <= 2 ? 1 : 2;
+    const int ngrp = nst <= 2 ? 1 : NG;
     if (grp >= ngrp) return;
     const int ng = (nst - grp + ngrp - 1) / ngrp;          // this group's
     auto stage_of = [&](int i) { return sb + ngrp * i + grp; };
 
-    // ---- staging: thread (row r0, chunk ch) of the group takes rows r0 and r0 + 16 ------------
+    // ---- staging: thread (row r0, chunk ch) of the group takes rows r0, r0 + kRows, ... --------
     const size_t kstride = (size_t)a.hkv * RB;
     const uint8_t* kbase = a.k + (size_t)kh * RB;
     const uint8_t* vbase = a.v + (size_t)kh * RB;
-    const int r0 = (threadIdx.x & 255) >> 4, ch = threadIdx.x & 15;
-    Chunk8<KV> rk[2], rv[2];
+    const int r0 = (threadIdx.x & (64 * CB - 1)) >> 4, ch = threadIdx.x & 15;
+    Chunk8<KV> rk[kSteps], rv[kSteps];
     auto load_rows = [&](int i) {
         const size_t row = (size_t)(stage_of(i) * kTileS + r0) * kstride;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < kSteps; ++j) {
             if (PACKED) {
-                const size_t at = (size_t)min(stage_of(i) * kTileS + r0 + 16 * j, lk - 1) * kstride;
+                const size_t at = (size_t)min(stage_of(i) * kTileS + r0 + kRows * j, lk - 1) * kstride;
                 rk[j].load(kbase + at, ch);
                 rv[j].load(vbase + at, ch);
                 continue;
             }
-            rk[j].load(kbase + row + 16 * j * kstride, ch);
-            rv[j].load(vbase + row + 16 * j * kstride, ch);
+            rk[j].load(kbase + row + kRows * j * kstride, ch);
+            rv[j].load(vbase + row + kRows * j * kstride, ch);
         }
     };
     auto write_rows = [&](int i) {
-        uint16_t* t = s_kv + (2 * grp + (i & 1)) * kBuf;
+        uint16_t* t = s_kv + (NB * grp + (NB == 2 ? i & 1 : 0)) * kBuf;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int row = r0 + 16 * j;
+        for (int j = 0; j < kSteps; ++j) {
+            const int row = r0 + kRows * j;
             half8 hi, lo;
             rk[j].split(hi, lo);
             *reinterpret_cast<half8*>(t + row * kDim + 8 * kswz(row, ch)) = hi;
@@ -1681,7 +1688,7 @@ __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, c
     const float kGrow = PS ? 8.0f / kLog2e : 0.0f;
 
     auto scores = [&](int i, f32x16& s) {
-        const uint8_t* kt = reinterpret_cast<const uint8_t*>(s_kv + (2 * grp + (i & 1)) * kBuf);
+        const uint8_t* kt = reinterpret_cast<const uint8_t*>(s_kv + (NB * grp + (NB == 2 ? i & 1 : 0)) * kBuf);
         int c = c14;
         asm volatile("" : "+v"(c));
 #pragma unroll
@@ -1723,7 +1730,8 @@ __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, c
         }
         // a column without a key so far has m = -inf and every s = -inf: P = 0
         const float m = m_used == -INFINITY ? 0.0f : m_used;
-        const uint8_t* vt = reinterpret_cast<const uint8_t*>(s_kv + (2 * grp + (i & 1)) * kBuf + NK * kStageHalvesS);
+        const uint8_t* vt = reinterpret_cast<const uint8_t*>(s_kv + (NB * grp + (NB == 2 ? i & 1 : 0)) * kBuf +
+                                                             NK * kStageHalvesS);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             float p[8];
@@ -1745,9 +1753,22 @@ __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, c
         }
     };
 
+    const int niter = (nst + ngrp - 1) / ngrp;  // group 0's stages: the groups pass the same barriers
+    if constexpr (NB == 1) {
+        for (int i = 0; i < niter; ++i) {
+            if (i > 0) lds_sync();  // the stage before has been read
+            if (i < ng) write_rows(i);
+            if (i + 1 < ng) load_rows(i + 1);
+            lds_sync();
+            if (i < ng && stage_of(i) * kTileS < kend_w) {
+                f32x16 s;
+                scores(i, s);
+                contract(i, s);
+            }
+        }
+    } else {
     if (0 < ng) write_rows(0);
     if (1 < ng) load_rows(1);
-    const int niter = (nst + ngrp - 1) / ngrp;  // group 0's stages: both groups pass the same barriers
     for (int i = 0; i < niter; ++i) {
         // stage i written by every wave of the group; its last reads of stage i - 1 returned
         lds_sync();
@@ -1760,22 +1781,25 @@ __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, c
         }
         if (on) contract(i, s);
     }
+    }
     lds_sync();  // every stage read
 
-    // ---- merge the two groups' key halves: group 1 hands (m, l, O) to group 0 through LDS -----
+    // ---- merge the groups' keys: the others hand (m, l, O) to group 0 through LDS -------------
     // (17 16-byte chunks per lane, chunk-major: conflict-free 128-bit accesses)
-    f32x4* xch = reinterpret_cast<f32x4*>(s_kv) + qw * 17 * 64 + lane;
-    if (grp == 1) {
+    auto xch = [&](int g) { return reinterpret_cast<f32x4*>(s_kv) + ((g - 1) * CB + qw) * 17 * 64 + lane; };
+    if (grp > 0) {
+        f32x4* x = xch(grp);
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-            xch[64 * c] = f32x4{acc[c >> 2][4 * (c & 3)], acc[c >> 2][4 * (c & 3) + 1],
-                                acc[c >> 2][4 * (c & 3) + 2], acc[c >> 2][4 * (c & 3) + 3]};
-        xch[64 * 16] = f32x4{m_used, lsum, 0.0f, 0.0f};
+            x[64 * c] = f32x4{acc[c >> 2][4 * (c & 3)], acc[c >> 2][4 * (c & 3) + 1],
+                              acc[c >> 2][4 * (c & 3) + 2], acc[c >> 2][4 * (c & 3) + 3]};
+        x[64 * 16] = f32x4{m_used, lsum, 0.0f, 0.0f};
     }
-    if (ngrp == 2) lds_sync();
-    if (grp == 1) return;
-    if (ngrp == 2) {
-        const f32x4 ml = xch[64 * 16];
+    if (ngrp > 1) lds_sync();
+    if (grp > 0) return;
+    for (int g = 1; g < ngrp; ++g) {
+        const f32x4* x = xch(g);
+        const f32x4 ml = x[64 * 16];
         const float M = fmaxf(m_used, ml[0]);
         // a group that saw no key of this column (a later key part's) has m = -inf, weight 0
         const float wa = (m_used == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f((m_used - M) * kLog2e);
@@ -1783,7 +1807,7 @@ __device__ __forceinline__ void split_tile(const PrefillArgs& a, const int hg, c
         lsum = lsum * wa + ml[1] * wb;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-            const f32x4 o1 = xch[64 * c];
+            const f32x4 o1 = x[64 * c];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 acc[c >> 2][4 * (c & 3) + j] = acc[c >> 2][4 * (c & 3) + j] * wa + o1[j] * wb;
@@ -1979,6 +2003,13 @@ __device__ __forceinline__ PrefillArgs prompt_args(const PackedArgs& p, const Pa
     return a;
 }
 
+// The first query tiles of a prompt carry P in f32 accuracy (two halves) in F16 precision too: rows
+// below 128, or the first eighth of a long prompt. Over few keys outputs are largest, so much of a
+// result's error (f16's rounding of P beside that of Q and of the result) is theirs, and their few
+// stages cost little: prompts of 100 / 600 / 8000 rows err by 1.29 / 1.43 / 1.44 times the result's own
+// rounding, 1.44 / 1.55 / 1.60 without (1.29 / 1.33 / 1.35 with two halves throughout, a third slower).
+__device__ __forceinline__ bool full_p(int row, int len) { return row < max(len / 8, 128); }
+
 template <int HW, bool PS>
 __global__ void __launch_bounds__(kThreads, 3)
 packed_f16_kernel(PackedArgs p) {
@@ -1986,7 +2017,9 @@ packed_f16_kernel(PackedArgs p) {
     __shared__ __attribute__((aligned(16))) uint16_t s_vv[3][kStageHalvesS];
     PackedTile t;
     if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
-    f16_tile4s<HW, PS, true>(prompt_args<BRASA_KV_F16, false>(p, t), blockIdx.x, t.tile, s_k, s_vv);
+    const PrefillArgs a = prompt_args<BRASA_KV_F16, false>(p, t);
+    if (PS || full_p(t.tile * (32 * 4 / HW), t.len)) f16_tile4s<HW, true, true>(a, blockIdx.x, t.tile, s_k, s_vv);
+    else f16_tile4s<HW, PS, true>(a, blockIdx.x, t.tile, s_k, s_vv);
 }
 
 // The two-group kernel (8 waves, one workgroup per CU), which halves the longest prompt's chain of stages.
@@ -1997,16 +2030,18 @@ packed_pp_kernel(PackedArgs p) {
     PackedTile t;
     if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
     u32x4 qraw[8];
-    f16_pp_tile<HW, PS, true>(prompt_args<BRASA_KV_F16, false>(p, t), t.tile, 0, 0, s_kv, qraw, false, -1);
+    const PrefillArgs a = prompt_args<BRASA_KV_F16, false>(p, t);
+    if (PS || full_p(t.tile * (32 * 4 / HW), t.len)) f16_pp_tile<HW, true, true>(a, t.tile, 0, 0, s_kv, qraw, false, -1);
+    else f16_pp_tile<HW, PS, true>(a, t.tile, 0, 0, s_kv, qraw, false, -1);
 }
 
-template <int KV, int HW, bool QS, bool PS, bool OF32>
+template <int KV, int HW, bool QS, bool PS, bool OF32, int CB>
 __global__ void __launch_bounds__(2 * kThreads, 1)
 packed_split_kernel(PackedArgs p) {
-    __shared__ __attribute__((aligned(16))) uint16_t s_kv[kSplitHalves<KV>];
+    __shared__ __attribute__((aligned(16))) uint16_t s_kv[CB == 4 ? kSplitHalves<KV> : kSplitHalves4<KV>];
     PackedTile t;
-    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
-    split_tile<KV, HW, QS, PS, OF32, true>(prompt_args<KV, OF32>(p, t), blockIdx.x, t.tile, 0, s_kv);
+    if (!packed_tile<32 * CB / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    split_tile<KV, HW, QS, PS, OF32, true, CB, 8 / CB>(prompt_args<KV, OF32>(p, t), blockIdx.x, t.tile, 0, s_kv);
 }
 
 // Kernel choice by workgroup count (one per query tile and head group), measured on one box at
@@ -2444,38 +2479,57 @@ int run(PfCtx& c, PrefillArgs& a, int kv, int precision) {
     return set_error(BRASA_ERR_ARG, "flash_attention: invalid kv type %d", kv);
 }
 
+// A launch of `kernel`, whose workgroups serve TPW tokens of HW heads: one for each query tile of each
+// head group, of which a prompt of r > 0 rows has (r + TPW - 1) / TPW.
+long long packed_tiles(const PackedArgs& p, int tpw) {
+    const long long prompts = std::min(p.n, p.a.tokens);
+    return ((long long)p.a.tokens + prompts * (tpw - 1)) / tpw;
+}
+template <typename K>
+int launch_tiles(const PackedArgs& p, K kernel, int hw, int tpw, int threads, const char* name,
+                 hipStream_t stream) {
+    hipLaunchKernelGGL(kernel, dim3(p.a.hq / hw, (unsigned)packed_tiles(p, tpw)), dim3(threads), 0, stream, p);
+    return check_launch(name);
+}
+
+template <int HW, bool PS>
+int launch_packed_f16(const PackedArgs& p, hipStream_t stream) {
+    constexpr int TPW = 32 * 4 / HW;
+    // The two-group kernel where each workgroup has a CU of its own (one prompt of 501 rows, 32 heads
+    // over 8: 15.6 us against 17.3; 1000 rows: 23.5 and 29.4); beyond that three workgroups per
+    // CU hide each other's prologues and chains (2000 rows 54 and 60, but twelve prompts of 2030
+    // rows 31.7 and 21.1, forty of 200 rows 103 and 50).
+    if (packed_tiles(p, TPW) * (p.a.hq / HW) <= 256)
+        return launch_tiles(p, packed_pp_kernel<HW, PS>, HW, TPW, 2 * kThreads, "packed_pp_kernel", stream);
+    return launch_tiles(p, packed_f16_kernel<HW, PS>, HW, TPW, kThreads, "packed_f16_kernel", stream);
+}
+template <int KV, int HW, bool QS, bool PS, bool OF32>
+int launch_packed_split(const PackedArgs& p, hipStream_t stream) {
+    constexpr int TPW = 32 * 4 / HW;
+    // Four key groups of two column blocks where workgroups of four blocks leave CUs idle: half as many
+    // serial stages, twice the workgroups (f32 rows: prompts of 130, 257, 1 and 600 rows, 16 heads over
+    // 8, 34.6 -> 29.3 us; one of 501, 32 over 8, 30.6 -> 25.9; not with 272 workgroups, 37.2 and 43.0,
+    // nor on short prompts, ten of 50 rows 8.9 and 9.6).
+    if (packed_tiles(p, TPW) * (p.a.hq / HW) <= 192 && p.a.tokens / 100 >= p.n) {
+        constexpr int H2 = HW < 2 ? HW : 2;
+        return launch_tiles(p, packed_split_kernel<KV, H2, QS, PS, OF32, 2>, H2, 32 * 2 / H2, 512,
+                            "packed_split_kernel", stream);
+    }
+    return launch_tiles(p, packed_split_kernel<KV, HW, QS, PS, OF32, 4>, HW, TPW, 512, "packed_split_kernel",
+                        stream);
+}
+
 template <int HW>
 int launch_packed(const PackedArgs& p, int kv, int precision, hipStream_t stream) {
-    constexpr int TPW = 32 * 4 / HW;
-    // query tiles: a prompt of r > 0 rows has (r + TPW - 1) / TPW
-    const long long prompts = std::min(p.n, p.a.tokens);
-    const long long tiles = ((long long)p.a.tokens + prompts * (TPW - 1)) / TPW;
-    const dim3 grid(p.a.hq / HW, (unsigned)tiles);
-    auto go = [&](auto kernel, int threads, const char* name) {
-        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, p);
-        return check_launch(name);
-    };
     if (kv == BRASA_KV_F16) {
-        // The two-group kernel where each workgroup has a CU of its own (one prompt of 501 rows, 32 heads
-        // over 8: 15.6 us against 17.3; 1000 rows: 23.5 and 29.4); beyond that three workgroups per
-        // CU hide each other's prologues and chains (2000 rows 54 and 60, but twelve prompts of 2030
-        // rows 31.7 and 21.1, forty of 200 rows 103 and 50).
-        const bool few = tiles * (p.a.hq / HW) <= 256;
-        if (precision == BRASA_PREFILL_F32)
-            return go(packed_split_kernel<BRASA_KV_F16, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
-        if (few)
-            return precision == BRASA_PREFILL_F16
-                       ? go(packed_pp_kernel<HW, false>, 2 * kThreads, "packed_pp_kernel")
-                       : go(packed_pp_kernel<HW, true>, 2 * kThreads, "packed_pp_kernel");
-        return precision == BRASA_PREFILL_F16
-                   ? go(packed_f16_kernel<HW, false>, kThreads, "packed_f16_kernel")
-                   : go(packed_f16_kernel<HW, true>, kThreads, "packed_f16_kernel");
+        if (precision == BRASA_PREFILL_F16) return launch_packed_f16<HW, false>(p, stream);
+        if (precision == BRASA_PREFILL_F16_PF32) return launch_packed_f16<HW, true>(p, stream);
+        return launch_packed_split<BRASA_KV_F16, HW, true, true, true>(p, stream);
     }
-    if (precision == BRASA_PREFILL_F32)
-        return go(packed_split_kernel<BRASA_KV_F32, HW, true, true, true>, 2 * kThreads, "packed_split_kernel");
+    if (precision == BRASA_PREFILL_F32) return launch_packed_split<BRASA_KV_F32, HW, true, true, true>(p, stream);
     if (precision == BRASA_PREFILL_F16_PF32)
-        return go(packed_split_kernel<BRASA_KV_F32, HW, false, true, false>, 2 * kThreads, "packed_split_kernel");
-    return go(packed_split_kernel<BRASA_KV_F32, HW, false, false, false>, 2 * kThreads, "packed_split_kernel");
+        return launch_packed_split<BRASA_KV_F32, HW, false, true, false>(p, stream);
+    return launch_packed_split<BRASA_KV_F32, HW, false, false, false>(p, stream);
 }
 
 }  // namespace
