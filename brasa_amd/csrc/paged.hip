@@ -155,7 +155,8 @@ constexpr int kWaves = 4;
 constexpr int kDecThreads = 64 * kWaves;
 constexpr int kMaxCols = 8;      // query heads of a workgroup
 constexpr int kSlots = 512;      // workgroups of a launch: two per CU
-constexpr int kMinPages = 8;     // pages of a run, at least (two per wave)
+constexpr int kMinPages = 8;     // pages of a run that may split a sequence (two per wave)
+constexpr int kWholePages = 12;  // pages of a sequence that is not worth splitting
 constexpr int kPartBytes = kMaxCols * (kDim + 2) * 4;  // a part: (m, l) of each column, then its sums
 constexpr int kCounterStride = 16;  // words between two arrival counters
 
@@ -281,12 +282,21 @@ decode_paged_kernel(DecodePagedArgs a) {
     const int np0 = lane < a.n ? line_pages(lk0, a.width) : 0;
     const int incl0 = wave_scan(np0);
     int total = __builtin_amdgcn_readlane(incl0, 63);
+    bool lengthy = __builtin_amdgcn_ballot_w64(np0 > kWholePages);  // a sequence worth splitting
     if (a.n > 64) {
-        int more = 0;
-        for (int i = 64 + lane; i < a.n; i += 64) more += line_pages(a.lk[i], a.width);
+        int more = 0, most = 0;
+        for (int i = 64 + lane; i < a.n; i += 64) {
+            const int np = line_pages(a.lk[i], a.width);
+            more += np;
+            most = max(most, np);
+        }
         total += __builtin_amdgcn_readlane(wave_scan(more), 63);
+        lengthy |= (bool)__builtin_amdgcn_ballot_w64(most > kWholePages);
     }
-    const int size = max((total + a.runs - 1) / a.runs, kMinPages);
+    // Few pages, in sequences of few: a run takes the sequences that start in it, whole (128 sequences of
+    // 100 keys 19.0 us cut into runs of kMinPages, 13.7 in runs of 4).
+    const bool whole_only = total <= a.runs * kMinPages && !lengthy;
+    const int size = max((total + a.runs - 1) / a.runs, whole_only ? (total + a.n - 1) / a.n : kMinPages);
     int at = run * size;
     const int end = min(at + size, total);
     if (at >= end) return;
@@ -303,72 +313,91 @@ decode_paged_kernel(DecodePagedArgs a) {
         }
         seq_at = __builtin_amdgcn_readlane(incl, 63);
     }
+    auto keys_of = [&](int i) { return i < 64 ? __builtin_amdgcn_readlane(lk0, i) : a.lk[i]; };
+    if (whole_only && seq_at < at) {  // that one is the run's before
+        seq_at += line_pages(keys_of(seq), a.width);
+        ++seq;
+        at = seq_at;
+        if (at >= end) return;
+    }
 
-    for (; at < end; ++seq) {
-        const int lk_raw = seq < 64 ? __builtin_amdgcn_readlane(lk0, seq) : a.lk[seq];
-        const int np = line_pages(lk_raw, a.width);
-        const bool bad_len = lk_raw < 0 || lk_raw > a.width * kPage;
-        const int lk = bad_len ? 0 : lk_raw;
-        const int b0 = at - seq_at;                        // pages [b0, b1) of the sequence
-        const int b1 = min(end - seq_at, np);
-        const bool whole = b0 == 0 && b1 == np;
-        const int blast = lk > 0 ? b1 : 0;                 // no keys: no pages
-
-        // ---- this wave's first page on its way ---------------------------------------------------
-        const int* ids = a.table + (size_t)seq * a.width;
-        bool bad = false;
-        PageK k;
-        PageV v;
-        // a page that is not there reads page 0 in its place, and the sequence's output is NaN
-        auto tile_of = [&](int page) {
-            const bool there = page >= 0 && page < a.p.pages;
-            bad |= !there;
-            return (size_t)(there ? page : 0) * a.p.hkv + kh;
-        };
-        auto load_k = [&](size_t tile) {
-            const uint8_t* p = a.p.k + tile * kTileBytes8 + c * kDim + 16 * u;
+    // ---- a segment: pages [b0, b1) of a sequence of np --------------------------------------------
+    struct Segment {
+        int seq, seq_at, np, lk, b0, b1, blast;
+        bool whole, bad;  // bad: a length or page that is not there, the output is NaN
+    };
+    auto segment = [&](int seq, int seq_at, int at) {
+        Segment g;
+        const int lk = keys_of(seq);
+        const bool bad_len = lk < 0 || lk > a.width * kPage;
+        g.seq = seq;
+        g.seq_at = seq_at;
+        g.np = line_pages(lk, a.width);
+        g.lk = bad_len ? 0 : lk;
+        g.b0 = at - seq_at;
+        g.b1 = whole_only ? g.np : min(end - seq_at, g.np);
+        g.blast = g.lk > 0 ? g.b1 : 0;  // no keys: no pages
+        g.whole = g.b0 == 0 && g.b1 == g.np;
+        g.bad = bad_len;
+        return g;
+    };
+    PageK k;
+    PageV v;
+    f32x4 qraw[4][2];
+    int next_id = 0;  // the next page's id, loaded a page ahead of its codes
+    // a page that is not there reads page 0 in its place
+    auto tile_of = [&](int page, bool& bad) {
+        const bool there = page >= 0 && page < a.p.pages;
+        bad |= !there;
+        return (size_t)(there ? page : 0) * a.p.hkv + kh;
+    };
+    auto load_k = [&](size_t tile) {
+        const uint8_t* p = a.p.k + tile * kTileBytes8 + c * kDim + 16 * u;
 #pragma unroll
-            for (int T = 0; T < 4; ++T)
+        for (int T = 0; T < 4; ++T)
 #pragma unroll
-                for (int hh = 0; hh < 2; ++hh)
-                    k.w[T][hh] = *reinterpret_cast<const u32x4*>(p + 16 * T * kDim + 64 * hh);
-            k.x = a.p.kx[tile];
-        };
-        auto load_v = [&](size_t tile) {
-            const uint8_t* p = a.p.v + tile * kTileBytes8 + 4 * u * kDim + 8 * c;
+            for (int hh = 0; hh < 2; ++hh)
+                k.w[T][hh] = *reinterpret_cast<const u32x4*>(p + 16 * T * kDim + 64 * hh);
+        k.x = a.p.kx[tile];
+    };
+    auto load_v = [&](size_t tile) {
+        const uint8_t* p = a.p.v + tile * kTileBytes8 + 4 * u * kDim + 8 * c;
 #pragma unroll
-            for (int T = 0; T < 4; ++T)
+        for (int T = 0; T < 4; ++T)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    v.w[T][r] = *reinterpret_cast<const u32x2*>(p + (16 * T + r) * kDim);
-            v.x = a.p.vx[tile];
-        };
-        int b = b0 + wave;
-        int next_id = 0;  // the next page's id, loaded a page ahead of its codes
-        size_t next = 0;
+            for (int r = 0; r < 4; ++r)
+                v.w[T][r] = *reinterpret_cast<const u32x2*>(p + (16 * T + r) * kDim);
+        v.x = a.p.vx[tile];
+    };
+    // Q and this wave's first page on their way, Q ahead: it would wait behind the page.
+    // k-step t = 2 hh + j holds dims 64 hh + 16 u + 8 j .. + 8, as K's 16-byte loads do
+    auto begin = [&](Segment& g, const int* ids) {
+        const int b = g.b0 + wave;
         int id = 0;
-        if (b < blast) {
+        if (b < g.blast) {
             id = ids[b];
-            if (b + kWaves < blast) next_id = ids[b + kWaves];
+            if (b + kWaves < g.blast) next_id = ids[b + kWaves];
         }
-        // Q's loads go out before the page's, which they would wait behind
-        // k-step t = 2 hh + j holds dims 64 hh + 16 u + 8 j .. + 8, as K's 16-byte loads do
-        f32x4 qraw[4][2];
-        {
-            const float* qrow = a.q + ((size_t)seq * a.hq + head_of_lane) * kDim + 16 * u;
+        const float* qrow = a.q + ((size_t)g.seq * a.hq + head_of_lane) * kDim + 16 * u;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    qraw[t][e] = *reinterpret_cast<const f32x4*>(qrow + 64 * (t >> 1) + 8 * (t & 1) + 4 * e);
-        }
+            for (int e = 0; e < 2; ++e)
+                qraw[t][e] = *reinterpret_cast<const f32x4*>(qrow + 64 * (t >> 1) + 8 * (t & 1) + 4 * e);
         __builtin_amdgcn_sched_barrier(0);
-        if (b < blast) {
-            const size_t tile = tile_of(id);
+        if (b < g.blast) {
+            const size_t tile = tile_of(id, g.bad);
             load_k(tile);
             load_v(tile);
         }
         __builtin_amdgcn_sched_barrier(0);
+    };
+
+    while (true) {
+        Segment g = segment(seq, seq_at, at);
+        const int* ids = a.table + (size_t)g.seq * a.width;
+        const int lk = g.lk, blast = g.blast;
+        begin(g, ids);
 
         // ---- Q: this lane's halves of q / sqrt(128) * log2 e, its exponent taken out -------------
         half8v q[4];
@@ -401,7 +430,8 @@ decode_paged_kernel(DecodePagedArgs a) {
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-        for (; b < blast; b += kWaves) {
+        size_t next = 0;
+        for (int b = g.b0 + wave; b < blast; b += kWaves) {
             const bool more = b + kWaves < blast;
             // ---- scores: key 16 T + 4 u + r of head c, in units of log2 ---------------------------
             f32x4 s[4];
@@ -424,7 +454,7 @@ decode_paged_kernel(DecodePagedArgs a) {
             // load on its way
             __builtin_amdgcn_sched_barrier(0);
             if (more) {
-                next = tile_of(next_id);
+                next = tile_of(next_id, g.bad);
                 load_k(next);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -507,7 +537,7 @@ decode_paged_kernel(DecodePagedArgs a) {
         }
 
         // ---- the waves' states into one ----------------------------------------------------------
-        if (bad || bad_len) lsum = NAN;
+        if (g.bad) lsum = NAN;
         lsum = sum_u(lsum);
 #pragma unroll
         for (int t = 0; t < 8; ++t)
@@ -527,7 +557,7 @@ decode_paged_kernel(DecodePagedArgs a) {
                         f32x4{acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]};
         }
         __syncthreads();
-        const size_t out0 = ((size_t)seq * a.hq + h0) * kDim;
+        const size_t out0 = ((size_t)g.seq * a.hq + h0) * kDim;
         const size_t plane = (size_t)blockIdx.y * a.runs;  // of this chunk of columns
         const Parts parts_at = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, a.part_bytes, 0x00027000);
         auto part_of = [&](int r, int second) {
@@ -550,18 +580,18 @@ decode_paged_kernel(DecodePagedArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
             }
-            if (whole) {
+            if (g.whole) {
                 write_o(a, out0 + 4 * i, x, l);
             } else {
-                const int p = part_of(run, at == run * size ? 0 : 1);
+                const int p = part_of(run, g.seq_at + g.b0 == run * size ? 0 : 1);
                 st_part(parts_at, p + kSums + 16 * i, x);
                 if (d == 0) st_part2(parts_at, p + 8 * col, m, l);
             }
         }
-        if (!whole) {
+        if (!g.whole) {
             // ---- the last segment of the sequence to arrive merges all of them ------------------
-            const int r0 = seq_at / size, parts = (seq_at + np - 1) / size - r0 + 1;
-            const int first = seq_at == r0 * size ? 0 : 1;  // a run's parts: its first segment's, then another
+            const int r0 = g.seq_at / size, parts = (g.seq_at + g.np - 1) / size - r0 + 1;
+            const int first = g.seq_at == r0 * size ? 0 : 1;  // a run's parts: its first segment's, then another
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -629,9 +659,11 @@ decode_paged_kernel(DecodePagedArgs a) {
                 if (threadIdx.x < chunks) write_o(a, out0 + 4 * i, x, s_l[0][col]);
             }
         }
+        at = g.seq_at + g.b1;
+        if (at >= end) return;
         __syncthreads();  // the LDS is free for the next segment
-        at = seq_at + b1;
-        seq_at += np;
+        ++seq;
+        seq_at = at;
     }
 }
 
