@@ -297,13 +297,27 @@ decode_paged_kernel(DecodePagedArgs a) {
     // 100 keys 19.0 us cut into runs of kMinPages, 13.7 in runs of 4).
     const bool whole_only = total <= a.runs * kMinPages && !lengthy;
     const int size = max((total + a.runs - 1) / a.runs, whole_only ? (total + a.n - 1) / a.n : kMinPages);
-    int at = run * size;
-    const int end = min(at + size, total);
+    // Few sequences: each is cut into parts of its own, `cut` pages or a little less, and a run is one
+    // part; the line is one of parts. With more of them that would leave runs idle or uneven.
+    int cut = 0, incl1 = incl0, np1 = np0;
+    if (!whole_only && a.n <= 64 && a.n <= a.runs / 4) {
+        cut = size;
+        while (true) {
+            np1 = (np0 + cut - 1) / cut;
+            incl1 = wave_scan(np1);
+            total = __builtin_amdgcn_readlane(incl1, 63);
+            if (total <= a.runs) break;
+            cut += (cut + 7) / 8;  // (every sequence whole is n <= runs parts)
+        }
+    }
+    const int run_size = cut ? 1 : size;
+    int at = run * run_size;
+    const int end = min(at + run_size, total);
     if (at >= end) return;
-    int seq = 0, seq_at = 0;  // the sequence that holds page `at`, and its first page in the line
+    int seq = 0, seq_at = 0;  // the sequence that holds page (or part) `at`, and its first in the line
     for (int i0 = 0; i0 < a.n; i0 += 64) {
-        const int np = i0 == 0 ? np0 : i0 + lane < a.n ? line_pages(a.lk[i0 + lane], a.width) : 0;
-        const int incl = (i0 == 0 ? incl0 : wave_scan(np)) + seq_at;
+        const int np = i0 == 0 ? np1 : i0 + lane < a.n ? line_pages(a.lk[i0 + lane], a.width) : 0;
+        const int incl = (i0 == 0 ? incl1 : wave_scan(np)) + seq_at;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > at);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -323,7 +337,7 @@ decode_paged_kernel(DecodePagedArgs a) {
 
     // ---- a segment: pages [b0, b1) of a sequence of np --------------------------------------------
     struct Segment {
-        int seq, seq_at, np, lk, b0, b1, blast;
+        int seq, np, lk, b0, b1, blast;
         bool whole, bad;  // bad: a length or page that is not there, the output is NaN
     };
     auto segment = [&](int seq, int seq_at, int at) {
@@ -331,11 +345,17 @@ decode_paged_kernel(DecodePagedArgs a) {
         const int lk = keys_of(seq);
         const bool bad_len = lk < 0 || lk > a.width * kPage;
         g.seq = seq;
-        g.seq_at = seq_at;
         g.np = line_pages(lk, a.width);
         g.lk = bad_len ? 0 : lk;
-        g.b0 = at - seq_at;
-        g.b1 = whole_only ? g.np : min(end - seq_at, g.np);
+        if (cut) {  // part at - seq_at of the sequence's, as equal as they can be
+            const int parts = __builtin_amdgcn_readlane(np1, seq), i = at - seq_at;
+            const int each = g.np / parts, more = g.np - each * parts;
+            g.b0 = i * each + min(i, more);
+            g.b1 = g.b0 + each + (i < more ? 1 : 0);
+        } else {
+            g.b0 = at - seq_at;
+            g.b1 = whole_only ? g.np : min(end - seq_at, g.np);
+        }
         g.blast = g.lk > 0 ? g.b1 : 0;  // no keys: no pages
         g.whole = g.b0 == 0 && g.b1 == g.np;
         g.bad = bad_len;
@@ -583,15 +603,16 @@ decode_paged_kernel(DecodePagedArgs a) {
             if (g.whole) {
                 write_o(a, out0 + 4 * i, x, l);
             } else {
-                const int p = part_of(run, g.seq_at + g.b0 == run * size ? 0 : 1);
+                const int p = part_of(run, at == run * run_size ? 0 : 1);
                 st_part(parts_at, p + kSums + 16 * i, x);
                 if (d == 0) st_part2(parts_at, p + 8 * col, m, l);
             }
         }
         if (!g.whole) {
             // ---- the last segment of the sequence to arrive merges all of them ------------------
-            const int r0 = g.seq_at / size, parts = (g.seq_at + g.np - 1) / size - r0 + 1;
-            const int first = g.seq_at == r0 * size ? 0 : 1;  // a run's parts: its first segment's, then another
+            const int r0 = seq_at / run_size;
+            const int parts = cut ? __builtin_amdgcn_readlane(np1, seq) : (seq_at + g.np - 1) / size - r0 + 1;
+            const int first = seq_at == r0 * run_size ? 0 : 1;  // a run's parts: its first segment's, then another
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -659,7 +680,8 @@ decode_paged_kernel(DecodePagedArgs a) {
                 if (threadIdx.x < chunks) write_o(a, out0 + 4 * i, x, s_l[0][col]);
             }
         }
-        at = g.seq_at + g.b1;
+        if (cut) return;
+        at = seq_at + g.b1;
         if (at >= end) return;
         __syncthreads();  // the LDS is free for the next segment
         ++seq;
