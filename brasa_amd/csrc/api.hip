@@ -89,7 +89,7 @@ static bool valid_kv(int kv) {
 // Largest sizes the kernels index with 32-bit integers.
 static constexpr size_t kMaxPositions = (size_t)1 << 30;
 static constexpr size_t kMaxHeads = 1024;
-static constexpr size_t kMaxSeqs = (size_t)1 << 20;
+static constexpr size_t kMaxSeqs = 65536;  // (a workgroup walks them to find its own)
 static constexpr size_t kMaxPages = (size_t)1 << 24;
 
 }  // namespace brasa
@@ -398,8 +398,8 @@ int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t laye
     if (n == 0) return BRASA_OK;
     if (!q || (!table && width) || !lk || !workspace || !o)
         return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
-    if ((uintptr_t)workspace % 256 || (uintptr_t)q % 16)
-        return set_error(BRASA_ERR_ARG, "%s: q must be 16-byte, the workspace 256-byte aligned", what);
+    if ((uintptr_t)workspace % 256 || ((uintptr_t)q | (uintptr_t)o) % 16)
+        return set_error(BRASA_ERR_ARG, "%s: q and o must be 16-byte, the workspace 256-byte aligned", what);
     return decode_paged_launch(q, p, table, (int)width, lk, (int)n, workspace, o,
                                o_dtype == BRASA_OUT_F16, (int)hq, as_stream(stream));
 }

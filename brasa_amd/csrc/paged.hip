@@ -705,17 +705,17 @@ int store_paged_launch(const PoolArgs& pool, const float* k, const float* v, con
     return check_launch("store_paged_kernel");
 }
 
-// the workspace: arrival counters, then two parts for each workgroup
+// The workspace: arrival counters, then two parts for each workgroup. The counters take the same room
+// whatever the heads (hkv * chunks is at most 1024 where hq is), so that calls of other heads on one
+// workspace leave them alone.
+constexpr size_t kCounterBytes = 1024 * kCounterStride * sizeof(unsigned);
 static size_t decode_paged_wgs(int hq, int hkv) {
     const int chunks = (hq / hkv + kMaxCols - 1) / kMaxCols;
     return (size_t)chunks * decode_runs(hkv, chunks) * hkv;
 }
-static size_t decode_paged_ctr_bytes(size_t wgs) {
-    return (wgs * kCounterStride * sizeof(unsigned) + 255) / 256 * 256;
-}
 size_t decode_paged_workspace_len(int hq, int hkv) {
     const size_t wgs = decode_paged_wgs(hq, hkv);
-    return decode_paged_ctr_bytes(wgs) + wgs * 2 * kPartBytes;
+    return kCounterBytes + wgs * 2 * kPartBytes;
 }
 
 int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, int width,
@@ -736,7 +736,7 @@ int decode_paged_launch(const float* q, const PoolArgs& pool, const int* table, 
     a.runs = decode_runs(pool.hkv, chunks);
     const size_t wgs = decode_paged_wgs(hq, pool.hkv);
     a.ctr = static_cast<unsigned*>(ws);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + decode_paged_ctr_bytes(wgs));
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kCounterBytes);
     a.part_bytes = (int)(wgs * 2 * kPartBytes);
     hipLaunchKernelGGL(decode_paged_kernel, dim3((unsigned)(a.runs * pool.hkv), chunks), dim3(kDecThreads),
                        0, stream, a);

@@ -1989,6 +1989,7 @@ struct PackedArgs {
     PrefillArgs a;  // tokens: rows of all prompts
     const int* cu;
     int n;
+    int y0;  // first query tile of the launch
 };
 
 // The arguments of one prompt, as a call of its own would have them.
@@ -2016,7 +2017,7 @@ packed_f16_kernel(PackedArgs p) {
     __shared__ __attribute__((aligned(16))) uint16_t s_k[3][kStageHalvesS];
     __shared__ __attribute__((aligned(16))) uint16_t s_vv[3][kStageHalvesS];
     PackedTile t;
-    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, p.y0 + blockIdx.y, t)) return;
     const PrefillArgs a = prompt_args<BRASA_KV_F16, false>(p, t);
     if (PS || full_p(t.tile * (32 * 4 / HW), t.len)) f16_tile4s<HW, true, true>(a, blockIdx.x, t.tile, s_k, s_vv);
     else f16_tile4s<HW, PS, true>(a, blockIdx.x, t.tile, s_k, s_vv);
@@ -2028,7 +2029,7 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
 packed_pp_kernel(PackedArgs p) {
     __shared__ __attribute__((aligned(16))) uint16_t s_kv[2][2][2][kStageHalves];
     PackedTile t;
-    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    if (!packed_tile<32 * 4 / HW>(p.cu, p.n, p.a.tokens, p.y0 + blockIdx.y, t)) return;
     u32x4 qraw[8];
     const PrefillArgs a = prompt_args<BRASA_KV_F16, false>(p, t);
     if (PS || full_p(t.tile * (32 * 4 / HW), t.len)) f16_pp_tile<HW, true, true>(a, t.tile, 0, 0, s_kv, qraw, false, -1);
@@ -2040,7 +2041,7 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
 packed_split_kernel(PackedArgs p) {
     __shared__ __attribute__((aligned(16))) uint16_t s_kv[CB == 4 ? kSplitHalves<KV> : kSplitHalves4<KV>];
     PackedTile t;
-    if (!packed_tile<32 * CB / HW>(p.cu, p.n, p.a.tokens, blockIdx.y, t)) return;
+    if (!packed_tile<32 * CB / HW>(p.cu, p.n, p.a.tokens, p.y0 + blockIdx.y, t)) return;
     split_tile<KV, HW, QS, PS, OF32, true, CB, 8 / CB>(prompt_args<KV, OF32>(p, t), blockIdx.x, t.tile, 0, s_kv);
 }
 
@@ -2486,10 +2487,18 @@ long long packed_tiles(const PackedArgs& p, int tpw) {
     return ((long long)p.a.tokens + prompts * (tpw - 1)) / tpw;
 }
 template <typename K>
-int launch_tiles(const PackedArgs& p, K kernel, int hw, int tpw, int threads, const char* name,
+int launch_tiles(PackedArgs p, K kernel, int hw, int tpw, int threads, const char* name,
                  hipStream_t stream) {
-    hipLaunchKernelGGL(kernel, dim3(p.a.hq / hw, (unsigned)packed_tiles(p, tpw)), dim3(threads), 0, stream, p);
-    return check_launch(name);
+    constexpr long long kMostRows = 32768;  // of a grid (its y dimension has 16 bits)
+    const long long tiles = packed_tiles(p, tpw);
+    for (long long y0 = 0; y0 < tiles; y0 += kMostRows) {
+        p.y0 = (int)y0;
+        hipLaunchKernelGGL(kernel, dim3(p.a.hq / hw, (unsigned)std::min(tiles - y0, kMostRows)), dim3(threads), 0,
+                           stream, p);
+        const int st = check_launch(name);
+        if (st != BRASA_OK) return st;
+    }
+    return BRASA_OK;
 }
 
 template <int HW, bool PS>
@@ -2536,7 +2545,7 @@ int launch_packed(const PackedArgs& p, int kv, int precision, hipStream_t stream
 
 int packed_launch(const float* q, const void* k, const void* v, void* o, const int* cu, int n, int tokens,
                   int hq, int hkv, int kv, int precision, hipStream_t stream) {
-    PackedArgs p{make_args(q, k, v, o, tokens, hq, hkv, 0), cu, n};
+    PackedArgs p{make_args(q, k, v, o, tokens, hq, hkv, 0), cu, n, 0};
     if (p.a.group % 4 == 0) return launch_packed<4>(p, kv, precision, stream);
     if (p.a.group % 2 == 0) return launch_packed<2>(p, kv, precision, stream);
     return launch_packed<1>(p, kv, precision, stream);

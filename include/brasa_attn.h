@@ -376,7 +376,7 @@ int brasa_prefill_trace_read(unsigned long long* dst, size_t n);
  * that is not spoils earlier rows of its prompt, never another prompt's); f32 rows, and q / sqrt(128),
  * are contracted as two f16 halves where the precision keeps them (22 bits, 2^-25 at least,
  * magnitudes up to 65504). Any hq a multiple of
- * hkv; dim 128; shape.pos0 must be 0; q, k, v and o 16-byte aligned. Allocates nothing, needs no workspace.
+ * hkv; dim 128; shape.pos0 must be 0; n up to 65536; q, k, v and o 16-byte aligned. Allocates nothing, needs no workspace.
  */
 int brasa_flash_attention_packed(const float* q, const void* k, const void* v, void* o,
                                  const int32_t* cu, size_t n, brasa_attn_shape shape,
@@ -419,7 +419,7 @@ size_t brasa_kv_pool_bytes(size_t layers, size_t pages, size_t hkv, size_t dim);
  * The tables, lengths and counts of the calls below are DEVICE arrays of int32, so a step whose
  * sequences grow, fork or end replays one captured graph. table: [n, width] page ids, row i the
  * pages of sequence i in order (position p in entry p / 64), -1 where it has none. Ids out of
- * [0, pages) are never followed.
+ * [0, pages) are never followed. n up to 65536, n * width up to 2^30.
  */
 
 /*
@@ -447,8 +447,9 @@ int brasa_store_kv_paged(brasa_kv_pool pool, size_t layer, const float* k, const
  * the lengths; a sequence in several runs is merged in the launch, in a fixed order. The result
  * bits of a sequence depend on the lengths of all (as brasa_decode_attention_batch's do), not on
  * timing. workspace: brasa_decode_paged_workspace_len(hq, pool.hkv) bytes, 256-byte aligned; its arrival
- * counters must be zero before its first use (clear it once, e.g. brasa_rt_fill_u8) and every
- * call leaves them zero. Calls that may run at the same time (other streams, replays of other graphs)
+ * counters (its first 64 KB) must be zero before its first use (clear it once, e.g.
+ * brasa_rt_fill_u8) and every call leaves them zero; calls of other lengths and other heads may take
+ * turns on one workspace. q and o 16-byte aligned. Calls that may run at the same time (other streams, replays of other graphs)
  * need workspaces of their own. Nothing else is shared between calls.
  */
 size_t brasa_decode_paged_workspace_len(size_t hq, size_t hkv);

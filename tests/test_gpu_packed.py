@@ -123,6 +123,21 @@ def test_packed_many_short(precision, kv):
 
 
 @pytest.mark.parametrize("precision,kv", [(F16, KvType.F16), (F32, KvType.F32)])
+def test_packed_most_prompts(precision, kv):
+    """As many prompts as a call takes, of one row each: more query tiles than one grid holds. Each
+    row's result is its own v, weight 1."""
+    n = 65536
+    c = Case([1] * n, 1, 1, kv, precision, 11)
+    c.upload()
+    c.call(Kernels())
+    synchronize()
+    raw = c.raw()
+    got = (raw if c.f32_out else oracle.f16_to_f32(raw)).reshape(n, 128)
+    # f32 rows: two halves, 2^-22 of the value or 2^-25; f16 rows are exact
+    assert np.all(np.abs(got - c.v[:, 0]) <= (0 if kv == KvType.F16 else 2.0 ** -22 * np.abs(c.v[:, 0]) + 2.0 ** -25))
+
+
+@pytest.mark.parametrize("precision,kv", [(F16, KvType.F16), (F32, KvType.F32)])
 def test_packed_long(precision, kv):
     _run(Case([1500, 40, 2100], 4, 1, kv, precision, 6), "long")
 

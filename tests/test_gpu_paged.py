@@ -291,6 +291,18 @@ def test_decode_one_workspace_for_many_shapes():
         assert np.array_equal(a, b) and np.array_equal(a, c)
 
 
+def test_decode_one_workspace_for_many_heads():
+    """Calls of other heads take turns on one workspace, each splitting its sequences."""
+    ds = [Decode(lens=[3000, 700], hq=hq, hkv=hkv, seed=hq) for hq, hkv in ((32, 8), (4, 1), (40, 1), (6, 3))]
+    ds.append(Decode(lens=[900], hq=1024, hkv=1024, seed=1))
+    ws = DeviceBuffer(max(d.wlen for d in ds))
+    ws.fill(0)
+    for d in ds + ds[::-1] + ds:
+        d.call(ws=ws)
+        synchronize()
+        d.check()
+
+
 def test_decode_replays_with_other_lengths():
     """A captured step whose lengths grow, on its own workspace, beside eager calls on another stream."""
     s, other = Stream(), Stream()

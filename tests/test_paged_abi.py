@@ -24,7 +24,7 @@ def _refused(code, call):
 
 @pytest.mark.parametrize("code,over", [
     (UNSUPPORTED, {"kv": KvType.Q8_0}), (SHAPE, {"dim": 64}), (SHAPE, {"hkv": 5}), (SHAPE, {"hkv": 0}),
-    (SHAPE, {"hq": 0}), (SHAPE, {"pos0": 1}), (SHAPE, {"tokens": 1 << 30}), (SHAPE, {"n": 1 << 21}),
+    (SHAPE, {"hq": 0}), (SHAPE, {"pos0": 1}), (SHAPE, {"tokens": 1 << 30}), (SHAPE, {"n": 65537}),
     (ARG, {"precision": 7}), (ARG, {"kv": 9}), (ARG, {"q": 0}), (ARG, {"k": 0}), (ARG, {"v": 0}),
     (ARG, {"o": 0}), (ARG, {"cu": 0}), (ARG, {"q": P + 4}), (ARG, {"o": P + 8}),
 ])
@@ -45,7 +45,7 @@ def test_packed_nothing_to_do():
     (SHAPE, {"dim": 64}, {}), (SHAPE, {"hkv": 0}, {}), (SHAPE, {"hkv": 2000}, {}), (SHAPE, {"pages": 0}, {}),
     (SHAPE, {"layers": 0}, {}), (SHAPE, {"pages": 1 << 25}, {}), (SHAPE, {"layers": 1 << 40}, {}),
     (SHAPE, {}, {"layer": 2}), (ARG, {"k": 0}, {}), (ARG, {"v_exp": 0}, {}), (ARG, {"v": P + 8}, {}),
-    (SHAPE, {}, {"n": 1 << 21}), (SHAPE, {}, {"width": 1 << 25}), (SHAPE, {}, {"n": 1 << 15, "width": 1 << 16}),
+    (SHAPE, {}, {"n": 65537}), (SHAPE, {}, {"width": 1 << 25}), (SHAPE, {}, {"n": 1 << 15, "width": 1 << 16}),
 ])
 def test_pool_refusals(code, pool, over):
     a = {**dict(layer=0, n=2, width=4), **over}
@@ -81,6 +81,7 @@ def test_decode_refusals():
     _refused(ARG, lambda: call(out=3))
     _refused(ARG, lambda: call(ws=P + 16))
     _refused(ARG, lambda: call(q=P + 4))
+    _refused(ARG, lambda: call(o=P + 8))
     _refused(SCRATCH, lambda: call(wlen=w - 1))
     _refused(SHAPE, lambda: call(hq=30))
     _refused(SHAPE, lambda: call(hq=0))
