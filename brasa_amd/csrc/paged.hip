@@ -15,8 +15,9 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 // from it (and from the block's scale, where earlier rows of the block stay), rounds those
 // earlier rows to a larger scale, and writes the codes.
 //
-// Bound: HBM at 4 bytes in and 1 out a value for prompts; a decode step's few rows are bound by
-// the chain cu / pos -> page id -> scale -> codes.
+// Bound: HBM at 4 bytes in and 1 out a value for prompts (7K rows of 8 heads 14.2 us, 5.1 TB/s); a
+// decode step's few rows are bound by the chain cu / pos -> page id -> scale -> codes (64 sequences
+// 4.9 us in the kernel, 7.8 from call to call).
 constexpr int kStoreThreads = 256;
 
 struct StoreArgs {
@@ -136,21 +137,34 @@ store_paged_kernel(StoreArgs a) {
 //
 // o[i, h] = sum_j p_j v_j / sum_j p_j over the lk[i] keys of sequence i, p_j = exp(q . k_j / sqrt(128)).
 //
-// Bound: HBM, 256 bytes of codes per (key, KV head). The pages of all sequences stand in one line,
-// and workgroup w of a head takes the w-th equal run of them, so every CU reads the same number
-// whatever the lengths, which only the device knows. A run's pieces of one sequence are its
-// segments; a segment that is not the whole sequence leaves (m, l, acc) in the workspace, and
+// Bound: HBM, 256 bytes of codes per (key, KV head), where a launch has a few pages for every wave; the
+// chain lengths -> page ids -> codes -> merge where it has not. The pages of all sequences stand in
+// one line, and workgroup w of a head takes the w-th equal run of them, so every CU reads the same
+// number whatever the lengths, which only the device knows. A run's pieces of one sequence are its
+// segments; a segment that is not the whole sequence leaves (m, l, sums) in the workspace, and
 // the last workgroup of a sequence to arrive merges them in order (a fixed order: the result does
-// not depend on who arrives last).
+// not depend on who arrives last). A few sequences are cut into parts of their own instead, one
+// a workgroup, and short ones are left whole.
 //
-// A wave takes every kWaves-th page of a segment, all of it in registers: S^T = K Q^T on 16x16x32
-// f16 MFMAs with the 16 columns holding the group's query heads (repeated), K's codes converted
-// exactly (an e4m3 value is an f16 value) right from the loaded 16-byte pieces, and Q as
-// f16 hi + lo halves, which keep 22 bits. A lane then holds four keys of each 16 for its head, which
-// is the layout P^T needs for O^T = V^T P^T, also in hi + lo halves. V's operand needs eight keys of one
-// dim in a lane: the lane loads 8 bytes of each of its eight keys' rows (dims 8 i .. 8 i + 7 of lane
-// row i) and byte permutes pair the keys before the conversion, so V needs no LDS either. The block's
-// scales are exponents: K's is added to the scores' exponent, V's multiplies the page's sum.
+// A wave takes every kWaves-th page of a segment, all of it in registers, the next page's codes loaded as
+// soon as this one's are used. S^T = K Q^T on 16x16x32 f16 MFMAs: K's codes are converted exactly (an
+// e4m3 value is an f16 value) right from the loaded 16-byte pieces; columns 0 .. 7 hold the f16 hi
+// halves of the heads' q, columns 15 .. 8 the lo halves (22 bits together), so one MFMA does both
+// and a mirrored addition joins them. Both lanes of a head then hold its scores of four keys of each 16,
+// which is the layout P^T needs for O^T = V^T P^T, again hi halves in one lane and lo halves in the other.
+// V's operand needs eight keys of one dim in a lane: the lane loads 8 bytes of each of its eight
+// keys' rows (dims 8 i .. 8 i + 7 of lane row i) and byte permutes pair the keys before the
+// conversion, so neither K nor V goes through LDS. The blocks' scales are exponents: K's is
+// folded into the exponential's argument, V's multiplies the page's sum.
+//
+// Measured at 32 heads over 8: one sequence of 257 keys 8.0 us, 4096 12.0, 16384 15.4 (a layer of
+// many, 2.2 TB/s), 32768 23.5 (2.9); 64 sequences of 300 to 16000 110 us (5.0 TB/s, an ordinary copy
+// 4.7); 200 of 300 to 1000 63 us (3.8). Where the 15 us at 16384 go: 2 until a wave's first page is asked
+// for, 7 for the codes (32 workgroups of 8 pages a head), 1.5 for the waves' sums, parts and arrivals,
+// 4 for the last workgroup's merge, whose one CU has 64 KB of parts to fetch. Two workgroups per CU, 256
+// registers a wave: with 256 or 1024 workgroups in place of 512 the batch takes 137 and 143 us, with
+// eight waves in each 138 (of 128 then). The parts' loads, (m, l) first and 16 ahead, took 52 us to
+// 18; the columns of halves 18.1 to 16.8.
 constexpr int kWaves = 4;
 constexpr int kDecThreads = 64 * kWaves;
 constexpr int kMaxCols = 8;      // query heads of a workgroup

@@ -5,8 +5,11 @@
 // All of it is whole numbers, and every choice goes by order (lowest free page, first owner), so the
 // results do not depend on how the atomics of a launch interleave.
 //
-// Bound: latency for the tables (a few thousand entries; one workgroup walks them, so that no launch
-// waits for another), HBM for the pages that move.
+// Bound: latency for the tables (a few thousand entries), HBM for the pages that move. What has an order
+// is decided by one workgroup in one launch, with its lists in LDS where they fit; what has none
+// (copies of tables and counts, edits, moves) is spread over the chip. 128 sequences of 100 to 4000
+// positions: fork 2.0 + 3.2 us, reserve 4.6 + 5.5; compaction of 1000 pages in 12 layers (364 of them
+// move) 4.9 us of decisions and 150 of copies, 4.7 TB/s in and out, as an ordinary copy.
 #include "paged.hpp"
 
 namespace brasa {
@@ -505,7 +508,7 @@ MoveList carve(void* ws, int n, int width, int pages) {
 }
 
 // workgroups of a launch that has `units` pieces of work at most
-unsigned grid_of(long long units) { return (unsigned)std::min<long long>(std::max<long long>(units, 1), 2048); }
+unsigned grid_of(long long units) { return (unsigned)std::min<long long>(std::max<long long>(units, 1), 16384); }
 
 }  // namespace
 

@@ -1933,6 +1933,13 @@ prefill_merge_kernel(PrefillArgs a) {
 // A workgroup finds its prompt and query tile from the row numbers, which only the device knows, and
 // runs the tile code above on that prompt alone. Order: the heaviest query tiles of 64
 // prompts first (the y-th in descending tile number), so that the launch ends with light ones.
+//
+// Bound: the matrix cores for long prompts (15876 rows in seven prompts, 32 heads over 8: 715 to 735 us,
+// 1.0 PFLOP/s; a large f16 matrix product reaches 1.2 to 1.3), HBM and the longest prompt's chain of
+// stages for chats (twelve prompts of 2030 rows 20.8 us, 58 MB). Tried and slower on one or the other: 64
+// queries a wave (half the LDS reads; 737 us, chats 33), the same with S and P V of neighbouring
+// stages interleaved (its accumulators leave the vector registers), one barrier a stage (751),
+// raised wave priority around the products (no difference).
 struct PackedTile {
     int start, len, tile;
 };
