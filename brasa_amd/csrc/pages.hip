@@ -144,7 +144,7 @@ struct MoveList {
     int* entry;     // reserve, edits: table entry, its new page (and the one it held, or -1)
     int* page;
     int* was;
-    int* tmp;       // reserve: claims and first claim of each page; compact: each moved page's new id
+    int* tmp;       // reserve: claims and first claim of each page; compact: new ids
     int* free_ids;
     uint8_t* take;
 };
@@ -434,7 +434,7 @@ struct CompactArgs {
     int* ref_out;
     int* live;
     int n, width, pages;
-    MoveList m;  // tmp: the new id of each page that moves
+    MoveList m;  // tmp: the new id of each page at or past *live
 };
 
 __global__ void __launch_bounds__(kPagesThreads)
@@ -451,7 +451,10 @@ compact_kernel(CompactArgs a) {
         int sum;
         // pages in use at or past `live` go down, free ones below it are filled
         const int at = block_scan(p >= live ? used : (p < a.pages && !used) << 16, s_scan, sum);
-        if (p < a.pages && p >= live && used) a.m.src[moves + (at & 0xffff)] = p;
+        if (p < a.pages && p >= live) {
+            if (used) a.m.src[moves + (at & 0xffff)] = p;
+            else a.m.tmp[p] = p;  // an entry that names a free page stays as it is
+        }
         if (p < a.pages && p < live && !used) a.m.dst[holes + (at >> 16)] = p;
         moves += sum & 0xffff;
         holes += sum >> 16;

@@ -493,7 +493,8 @@ int brasa_kv_pages_reserve(brasa_kv_pool pool, const int32_t* add, const int32_t
  * Compacts the pool: *live = L pages have ref > 0, and afterwards they are pages 0 .. L: the k-th
  * of them at or past L moves, in every layer, to the k-th free one below L, and table_out and
  * ref_out name it there (pages from L on: ref 0, codes as they were). table: every row that owns
- * pages. table_out may be table, ref_out may be ref. workspace as for brasa_kv_pages_reserve.
+ * pages; entries that name a page with ref 0, or no page, stay as they are. table_out may be table,
+ * ref_out may be ref. workspace as for brasa_kv_pages_reserve.
  */
 int brasa_kv_pages_compact(brasa_kv_pool pool, const int32_t* table, const int32_t* ref,
                            int32_t* table_out, int32_t* ref_out, int32_t* live, size_t n,
