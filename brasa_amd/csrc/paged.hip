@@ -28,6 +28,7 @@ struct StoreArgs {
     const int* pos;
     const int* table;
     int n, width, tokens;
+    int item0;  // first item of the launch
 };
 
 // the blocks that sequence i's new rows touch: [first, first + count)
@@ -43,7 +44,7 @@ __device__ __forceinline__ int touched_blocks(const StoreArgs& a, int i, int& c0
 __global__ void __launch_bounds__(kStoreThreads)
 store_paged_kernel(StoreArgs a) {
     const int lane = threadIdx.x & 63;
-    const int item = blockIdx.x / a.p.hkv, kh = blockIdx.x % a.p.hkv;
+    const int item = a.item0 + blockIdx.x / a.p.hkv, kh = blockIdx.x % a.p.hkv;
     const bool is_v = blockIdx.y;
 
     // the sequence and block of this item: every wave walks the sequences' block counts, 64 at a
@@ -710,13 +711,20 @@ int decode_runs(int hkv, int chunks) { return std::max(kSlots / (hkv * chunks), 
 int store_paged_launch(const PoolArgs& pool, const float* k, const float* v, const int* cu,
                        const int* pos, const int* table, int n, int width, int tokens,
                        hipStream_t stream) {
-    StoreArgs a{pool, k, v, cu, pos, table, n, width, tokens};
+    StoreArgs a{pool, k, v, cu, pos, table, n, width, tokens, 0};
     // blocks touched: a sequence of r rows touches (r - 1) / 64 + 2 at most
     const long long m = std::min(n, tokens);
     const long long items = (tokens - m) / kPage + 2 * m;
-    hipLaunchKernelGGL(store_paged_kernel, dim3((unsigned)(items * pool.hkv), 2), dim3(kStoreThreads), 0,
-                       stream, a);
-    return check_launch("store_paged_kernel");
+    // A launch of 2^32 threads or more runs fewer, without an error: at most 2^31 in each.
+    const long long most = (1LL << 31) / kStoreThreads / pool.hkv;
+    for (long long i = 0; i < items; i += most) {
+        a.item0 = (int)i;
+        hipLaunchKernelGGL(store_paged_kernel, dim3((unsigned)(std::min(items - i, most) * pool.hkv), 2),
+                           dim3(kStoreThreads), 0, stream, a);
+        const int st = check_launch("store_paged_kernel");
+        if (st != BRASA_OK) return st;
+    }
+    return BRASA_OK;
 }
 
 // The workspace: arrival counters, then two parts for each workgroup. The counters take the same room

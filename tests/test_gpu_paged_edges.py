@@ -1,14 +1,16 @@
-"""GPU: calls of the paged cache at the ends of what they allow: tables whose entries name free pages."""
+"""GPU: calls of the paged cache at the ends of what they allow: tables whose entries name free pages, and
+the most workgroups that a write can ask for."""
 import numpy as np
 import pytest
 
 import paged_ref as ref
 from brasa_amd import Kernels
-from brasa_amd.device import synchronize
-from test_gpu_paged import assert_pool, ints
+from brasa_amd.device import DeviceBuffer, synchronize
+from test_gpu_paged import assert_pool, ints, upload_pool
 from test_gpu_pages import State, down
 
 pytestmark = pytest.mark.gpu
+PAGE = ref.PAGE
 
 
 @pytest.mark.parametrize("in_place", [False, True])
@@ -32,3 +34,32 @@ def test_compact_leaves_entries_of_free_pages(lens, pages, in_place):
     assert np.array_equal(table[row], s.table[row])
     assert np.array_equal(down(t2, table), table) and np.array_equal(down(r2, counts), counts)
     assert_pool(s.dev, s.pool)
+
+
+def test_store_of_most_workgroups():
+    """8200 sequences of two rows that cross a page, 1024 heads: more than 2^24 workgroups of 256 threads,
+    past what one launch takes. All but a few sequences have no page (their rows are dropped and
+    never read); of the few, some are the last ones."""
+    n, hkv, per = 8200, 1024, 2
+    some = [0, 1, 4095, 4096, n - 2, n - 1]
+    rng = np.random.default_rng(12)
+    pool = ref.Pool(1, 2 * len(some), hkv, rng)
+    pool.k_exp[:], pool.v_exp[:] = 110, 111
+    table = np.full((n, 2), -1, np.int32)
+    table[some] = rng.permutation(2 * len(some)).reshape(-1, 2)
+    cu, pos = np.arange(0, per * n + 1, per, dtype=np.int32), np.full(n, PAGE - 1, np.int32)
+    row = hkv * 128 * 4
+    bufs, new = [], []
+    for _ in range(2):
+        x = rng.standard_normal((per * len(some), hkv, 128)).astype(np.float32)
+        b = DeviceBuffer(per * n * row)
+        for j, i in enumerate(some):
+            b.upload(x[per * j:per * (j + 1)], per * i * row)
+        bufs.append(b)
+        new.append(x)
+    dev = upload_pool(pool)
+    print("store of", n, "sequences,", hkv, "heads", flush=True)
+    Kernels().store_kv_paged(dev, 0, *bufs, ints(cu), ints(pos), ints(table), n, 2, per * n)
+    synchronize()
+    ref.store(pool, 0, *new, np.arange(0, per * len(some) + 1, per), pos[some], table[some])
+    assert_pool(dev, pool)
