@@ -137,10 +137,16 @@ int dequant_q8_launch(const void* src, float* dst, size_t rows, hipStream_t stre
 }
 
 int fill_u8_launch(void* dst, uint8_t value, size_t bytes, hipStream_t stream) {
-    if (bytes == 0) return BRASA_OK;
-    hipLaunchKernelGGL(fill_u8_kernel, dim3(blocks_for(bytes)), dim3(kTpb), 0, stream,
-                       static_cast<uint8_t*>(dst), value, bytes);
-    return check_launch("fill_u8");
+    // (a launch of 2^32 threads or more runs fewer, without an error)
+    constexpr size_t kMost = (size_t)1 << 31;
+    for (size_t at = 0; at < bytes; at += kMost) {
+        const size_t n = bytes - at < kMost ? bytes - at : kMost;
+        hipLaunchKernelGGL(fill_u8_kernel, dim3(blocks_for(n)), dim3(kTpb), 0, stream,
+                           static_cast<uint8_t*>(dst) + at, value, n);
+        const int st = check_launch("fill_u8");
+        if (st != BRASA_OK) return st;
+    }
+    return BRASA_OK;
 }
 
 int fill_normal_launch(float* out, size_t n, uint64_t seed, float scale, hipStream_t stream) {

@@ -63,3 +63,14 @@ def test_store_of_most_workgroups():
     synchronize()
     ref.store(pool, 0, *new, np.arange(0, per * len(some) + 1, per), pos[some], table[some])
     assert_pool(dev, pool)
+
+
+def test_fill_past_4_gib():
+    """Clearing a pool or a workspace of more than 2^32 bytes writes all of it."""
+    b = DeviceBuffer((1 << 32) + 300)
+    at = [0, 511, 512, (1 << 31) - 1, 1 << 31, (1 << 32) - 1, 1 << 32, b.nbytes - 1]
+    for value in (0x5A, 0x11):
+        print("fill", value, flush=True)
+        b.fill(value)
+        synchronize()
+        assert [int(b.download(np.uint8, 1, i)[0]) for i in at] == [value] * len(at)
