@@ -138,8 +138,10 @@ store_paged_kernel(StoreArgs a) {
 //
 // o[i, h] = sum_j p_j v_j / sum_j p_j over the lk[i] keys of sequence i, p_j = exp(q . k_j / sqrt(128)).
 //
-// Bound: HBM, 256 bytes of codes per (key, KV head), where a launch has a few pages for every wave; the
-// chain lengths -> page ids -> codes -> merge where it has not. The pages of all sequences stand in
+// Bound: where a launch has a few pages for every wave, the loads of its 256 bytes of codes per (key, KV
+// head): 5.0 TB/s, of 6.05 that the f16 decode of a ragged batch reads at. The vector units are 23 % busy
+// then and the matrix cores 6 %; waves wait for data 35 % and to issue 45 % of their time. Else the
+// chain lengths -> page ids -> codes -> merge. The pages of all sequences stand in
 // one line, and workgroup w of a head takes the w-th equal run of them, so every CU reads the same
 // number whatever the lengths, which only the device knows. A run's pieces of one sequence are its
 // segments; a segment that is not the whole sequence leaves (m, l, sums) in the workspace, and
@@ -158,14 +160,16 @@ store_paged_kernel(StoreArgs a) {
 // conversion, so neither K nor V goes through LDS. The blocks' scales are exponents: K's is
 // folded into the exponential's argument, V's multiplies the page's sum.
 //
-// Measured at 32 heads over 8: one sequence of 257 keys 8.0 us, 4096 12.0, 16384 15.4 (a layer of
-// many, 2.2 TB/s), 32768 23.5 (2.9); 64 sequences of 300 to 16000 110 us (5.0 TB/s, an ordinary copy
-// 4.7); 200 of 300 to 1000 63 us (3.8). Where the 15 us at 16384 go: 2 until a wave's first page is asked
-// for, 7 for the codes (32 workgroups of 8 pages a head), 1.5 for the waves' sums, parts and arrivals,
-// 4 for the last workgroup's merge, whose one CU has 64 KB of parts to fetch. Two workgroups per CU, 256
-// registers a wave: with 256 or 1024 workgroups in place of 512 the batch takes 137 and 143 us, with
-// eight waves in each 138 (of 128 then). The parts' loads, (m, l) first and 16 ahead, took 52 us to
-// 18; the columns of halves 18.1 to 16.8.
+// Measured at 32 heads over 8: one sequence of 257 keys 8.0 us, 4096 13.1, 16384 15.5 (a layer of
+// many, 2.2 TB/s), 32768 23.3 (2.9); 64 sequences of 300 to 16000 111 us (5.0 TB/s); 200 of 300 to 1000
+// 63 us (3.8). A group of 16 heads reads its pages once for each 8: 128 heads over 8 take 23.0 us at
+// 16384 and 186 us for the batch (64 over 8: 17.9 and 115). Where the 15 us at 16384 go: 2 until a wave's
+// first page is asked for, 7 for the codes (32 workgroups of 8 pages a head), 1.5 for the waves' sums, parts
+// and arrivals, 4 for the last workgroup's merge, whose one CU has 64 KB of parts to fetch. Two workgroups
+// per CU, 256 registers a wave: with 256 or 1024 workgroups in place of 512 the batch takes 123 and 120
+// us in place of 111, with 256 of eight waves 116 (which take 32768 keys in 21.5 us, 16384 in 15.4). Runs
+// of 12 or 16 pages in place of kMinPages = 8 take 16384 keys in 16.5 and 18.7 us, 4096 in 15.1 and 17.9,
+// 32768 in 25.3 and 21.8.
 constexpr int kWaves = 4;
 constexpr int kDecThreads = 64 * kWaves;
 constexpr int kMaxCols = 8;      // query heads of a workgroup

@@ -1935,9 +1935,11 @@ prefill_merge_kernel(PrefillArgs a) {
 // prompts first (the y-th in descending tile number), so that the launch ends with light ones.
 //
 // Bound, for long prompts: the matrix cores, busy 58 % of the cycles at a clock that falls to 1.46 GHz in a
-// profiled run (15876 rows in seven prompts, 32 heads over 8: 715 to 743 us, 1.0 PFLOP/s; a large f16
-// matrix product reaches 1.2 to 1.3); LDS bank conflicts are below 1 % of the CUs' cycles. Chats: the
-// longest prompt's chain of stages (twelve prompts of 2030 rows 21 us, 58 MB). Tried and not faster: 64
+// profiled run (15876 rows in seven prompts, 32 heads over 8: 713 to 775 us on several cards, 0.95 to 1.03
+// PFLOP/s; a large f16 matrix product reaches 1.2 to 1.3); LDS bank conflicts are below 1 % of the CUs'
+// cycles. P in two halves throughout (F16_PF32): 984 us. Chats: the longest prompt's chain (twelve prompts
+// of 2030 rows 21 us, 58 MB; by time stamps of the 501-row prompt's last tile: 1.4 us to find the tile,
+// 3.5 to Q and the first stages' copies, 16 stages of 1.0, 1.4 for the result). Tried and not faster: 64
 // queries a wave (half the LDS reads; 768 us against 737), the same with S and P V of neighbouring
 // stages interleaved (its accumulators leave the vector registers), one barrier a stage (751),
 // raised wave priority around the products (no difference).
@@ -2013,10 +2015,12 @@ __device__ __forceinline__ PrefillArgs prompt_args(const PackedArgs& p, const Pa
 }
 
 // The first query tiles of a prompt carry P in f32 accuracy (two halves) in F16 precision too: rows
-// below 128, or the first eighth of a long prompt. Over few keys outputs are largest, so much of a
-// result's error (f16's rounding of P beside that of Q and of the result) is theirs, and their few
-// stages cost little: prompts of 100 / 600 / 8000 rows err by 1.29 / 1.43 / 1.44 times the result's own
-// rounding, 1.44 / 1.55 / 1.60 without (1.29 / 1.33 / 1.35 with two halves throughout, a third slower).
+// below 128, or the first eighth of a long prompt. The aim is an error of at most 1.5 times the rounding
+// of the result to f16. Over few keys outputs are largest, so much of a result's error (f16's rounding
+// of P beside that of Q and of the result) is theirs, and their few stages cost little: prompts of 100 /
+// 600 / 8000 rows err by 1.29 / 1.43 / 1.44 times that rounding (up to 1.46 over all cases), 1.44 / 1.55 /
+// 1.60 without (1.29 / 1.33 / 1.35 with two halves throughout, a third slower). For f16 rows: the split
+// kernels, which serve f32 rows, keep one half in F16 precision as in the single-sequence calls.
 __device__ __forceinline__ bool full_p(int row, int len) { return row < max(len / 8, 128); }
 
 template <int HW, bool PS>
@@ -2524,9 +2528,14 @@ template <int KV, int HW, bool QS, bool PS, bool OF32>
 int launch_packed_split(const PackedArgs& p, hipStream_t stream) {
     constexpr int TPW = 32 * 4 / HW;
     // Four key groups of two column blocks where workgroups of four blocks leave CUs idle: half as many
-    // serial stages, twice the workgroups (f32 rows: prompts of 130, 257, 1 and 600 rows, 16 heads over
-    // 8, 34.6 -> 29.3 us; one of 501, 32 over 8, 30.6 -> 25.9; not with 272 workgroups, 37.2 and 43.0,
-    // nor on short prompts, ten of 50 rows 8.9 and 9.6).
+    // serial stages, twice the workgroups. Four groups against two, f32 rows, us, by workgroups of four
+    // blocks. One prompt: 32 / 40 / 64 workgroups (400 / 600 / 1000 rows, 8 heads over 8) 20.4 and 25.1,
+    // 26.2 and 32.8, 36.6 and 48.8; 128 (1000 rows, 16 over 8) 38.9 and 49.3; 152 / 176 / 200 / 256 (600 to
+    // 1000 rows, 32 over 8) 30.5 and 34.4, 34.0 and 38.5, 40.8 and 42.9, 51.2 and 50.7. Prompts of
+    // equal lengths lose from about 160 on, having no longest one that sets the time (two of 300 rows 24.8
+    // and 22.8, three of 200 24.5 and 19.3); uneven ones gain (20, 20 and 500 rows, 152 workgroups: 24.9
+    // and 30.3). By rows a prompt, four prompts of 60 / 80 / 100 / 120 rows: 9.7 and 10.5, 12.5 and 11.5,
+    // 14.2 and 13.7, 14.2 and 15.2 (16 over 8); ten of 50 rows 16.2 and 10.9 (32 over 8).
     if (packed_tiles(p, TPW) * (p.a.hq / HW) <= 192 && p.a.tokens / 100 >= p.n) {
         constexpr int H2 = HW < 2 ? HW : 2;
         return launch_tiles(p, packed_split_kernel<KV, H2, QS, PS, OF32, 2>, H2, 32 * 2 / H2, 512,

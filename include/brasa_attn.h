@@ -366,8 +366,12 @@ int brasa_prefill_trace_read(unsigned long long* dst, size_t n);
  * reference, which prefills one sequence per call, lib.rs:1185-1248). q: [tokens, hq, 128] f32;
  * k, v: [tokens, hkv, 128] rows of the type shape.kv (BRASA_KV_F32 or BRASA_KV_F16; a prompt's own
  * rows are not read back from an 8-bit cache: BRASA_ERR_UNSUPPORTED for q8_0); o: [tokens, hq, 128],
- * f16 for BRASA_PREFILL_F16 / _F16_PF32, f32 for _F32, with brasa_flash_attention_with's numerics
- * (softmax and sums in f32). cu: DEVICE array of n + 1 row numbers, 0 <= cu[0] <= ... <= cu[n] <=
+ * f16 for BRASA_PREFILL_F16 / _F16_PF32, f32 for _F32. Softmax and sums are in f32. F16 rounds q /
+ * sqrt(128) and the weights to f16, but on f16 rows keeps the weights of a prompt's first rows in two
+ * halves (22 bits): 128 rows, or an eighth of a prompt of more than 1024 (up to a query tile more).
+ * F16_PF32 keeps all weights in two halves, F32 q / sqrt(128) too. The bits of a row depend on the length
+ * of its prompt and on the call's tokens, n and heads (they choose the kernel, and with it the order
+ * of the sums), not on timing. cu: DEVICE array of n + 1 row numbers, 0 <= cu[0] <= ... <= cu[n] <=
  * tokens: prompt i holds rows cu[i] .. cu[i + 1], none where the two are equal, and its row t attends
  * to its rows up to t. Rows before cu[0] and from cu[n] on are neither read for another row's
  * result nor written. The lengths are read on the device: a captured graph may be replayed with other
@@ -416,10 +420,12 @@ typedef struct brasa_kv_pool {
 size_t brasa_kv_pool_bytes(size_t layers, size_t pages, size_t hkv, size_t dim);
 
 /*
- * The tables, lengths and counts of the calls below are DEVICE arrays of int32, so a step whose
- * sequences grow, fork or end replays one captured graph. table: [n, width] page ids, row i the
- * pages of sequence i in order (position p in entry p / 64), -1 where it has none. Ids out of
- * [0, pages) are never followed. n up to 65536, n * width up to 2^30.
+ * The tables, lengths and counts of the calls below are DEVICE arrays of int32, so a captured graph of
+ * these calls may be replayed while its sequences grow, fork or end. (The rotary calls,
+ * brasa_rope_neox and brasa_qk_norm_rope_store, take one position per call from the host: rotate the
+ * q and k of such a graph by positions read on the device, or launch them outside of it.)
+ * table: [n, width] page ids, row i the pages of sequence i in order (position p in entry p / 64), -1
+ * where it has none. Ids out of [0, pages) are never followed. n up to 65536, n * width up to 2^30.
  */
 
 /*
