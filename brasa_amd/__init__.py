@@ -7,16 +7,16 @@ plumbing the harnesses need.
 """
 from ._lib import BrasaError, LIB_PATH, build
 from .kernels import (DECODE_CHUNK, GQA_GROUPS, KV_ALIGN, AttnShape, Kernels, KvType, OutDType,
-                      PrefillPrecision, RopeTable, decode_batch_partials_len, decode_partials_len, gqa_supported,
-                      rope_table)
+                      PrefillPrecision, RopeAxes, RopeTable, decode_batch_partials_len, decode_partials_len,
+                      gqa_supported, rope_table)
 from .kvcache import KvCache, kv_cache_bytes, kv_cache_len, kv_capacity, kv_offset
-from .kvpool import (KV_PAGE, KvPool, decode_paged_workspace_len, kv_pages_workspace_len,
+from .kvpool import (KV_PAGE, KvPool, attention_paged_workspace_len, decode_paged_workspace_len, kv_pages_workspace_len,
                      kv_pool_bytes)
 
 __all__ = [
     "AttnShape", "BrasaError", "DECODE_CHUNK", "GQA_GROUPS", "KV_ALIGN", "Kernels", "KvType",
-    "LIB_PATH", "OutDType", "PrefillPrecision", "RopeTable", "build", "decode_batch_partials_len", "decode_partials_len",
+    "LIB_PATH", "OutDType", "PrefillPrecision", "RopeAxes", "RopeTable", "build", "decode_batch_partials_len", "decode_partials_len",
     "gqa_supported", "rope_table", "KvCache", "kv_cache_bytes", "kv_cache_len", "kv_capacity",
-    "kv_offset", "KV_PAGE", "KvPool", "decode_paged_workspace_len", "kv_pages_workspace_len",
+    "kv_offset", "KV_PAGE", "KvPool", "attention_paged_workspace_len", "decode_paged_workspace_len", "kv_pages_workspace_len",
     "kv_pool_bytes",
 ]

@@ -31,6 +31,12 @@ class RopeTableC(ctypes.Structure):
     _fields_ = [("cos", VP), ("sin", VP), ("dim", SZ), ("max_pos", SZ)]
 
 
+class RopeAxesC(ctypes.Structure):
+    """``brasa_rope_axes_map``."""
+
+    _fields_ = [("axes", SZ), ("of", ctypes.c_uint8 * 128)]
+
+
 class KvPoolC(ctypes.Structure):
     """``brasa_kv_pool``."""
 
@@ -67,6 +73,14 @@ SYMBOLS = {
     "brasa_kv_pages_workspace_len": (SZ, [SZ, SZ, SZ]),
     "brasa_kv_pages_reserve": (INT, [KvPoolC, VP, VP, VP, VP, VP, VP, VP, SZ, SZ, VP, SZ, VP]),
     "brasa_kv_pages_compact": (INT, [KvPoolC, VP, VP, VP, VP, VP, SZ, SZ, VP, SZ, VP]),
+    "brasa_rope_axes": (INT, [VP, RopeTableC, RopeAxesC, VP, SZ, SZ, SZ, VP]),
+    "brasa_qk_norm_rope_store_paged": (INT, [KvPoolC, SZ, VP, VP, VP, VP, VP, ctypes.c_float, RopeTableC, RopeAxesC,
+                                             VP, VP, VP, VP, SZ, SZ, SZ, SZ, VP]),
+    "brasa_kv_rows": (INT, [VP, VP, VP, SZ, SZ, SZ, SZ, VP, VP, VP, VP, VP, VP]),
+    "brasa_kv_pages_shared": (INT, [VP, VP, VP, SZ, SZ, SZ, SZ, VP, VP]),
+    "brasa_attention_paged_workspace_len": (SZ, [SZ, SZ, SZ, SZ, SZ]),
+    "brasa_attention_paged_plan": (INT, [VP, VP, VP, VP, SZ, SZ, SZ, SZ, SZ, SZ, VP, SZ, VP]),
+    "brasa_attention_paged": (INT, [VP, KvPoolC, SZ, VP, SZ, SZ, SZ, VP, SZ, VP, INT, SZ, VP]),
     "brasa_rope_table": (INT, [ctypes.c_double, SZ, SZ, VP, VP]),
     "brasa_rms_norm": (INT, [VP, VP, VP, SZ, SZ, ctypes.c_float, VP]),
     "brasa_rope_neox": (INT, [VP, RopeTableC, SZ, SZ, SZ, SZ, VP]),

@@ -56,6 +56,23 @@ int kv_pages_reserve_launch(const PoolArgs& pool, const int* add, const int* tab
 int kv_pages_compact_launch(const PoolArgs& pool, const int* table, const int* ref, int* table_out,
                             int* ref_out, int* live, int n, int width, void* ws, hipStream_t stream);
 
+int kv_rows_launch(const int* add, const int* len, const int* table, int* cu, int* lk, int* seq, int* pos,
+                   int* slot, int n, int width, int pages, int tokens, hipStream_t stream);
+int kv_pages_shared_launch(const int* table, const int* len, const int* group, int groups, int* prefix, int n,
+                           int width, int pages, hipStream_t stream);
+int rope_axes_launch(float* x, const float* cos_t, const float* sin_t, int max_pos,
+                     const brasa_rope_axes_map& map, const int* pos, int tokens, int heads, int dim,
+                     hipStream_t stream);
+int norm_rope_paged_launch(const PoolArgs& pool, float* q, float* k, const float* v, const float* qn,
+                           const float* kn, float eps, const float* cos_t, const float* sin_t, int max_pos,
+                           const brasa_rope_axes_map& map, const int* rope_pos, const int* cu, const int* pos,
+                           const int* table, int n, int width, int tokens, int hq, hipStream_t stream);
+size_t attend_workspace_len(int n, int groups, int tokens, int hq, int hkv);
+int attend_plan_launch(const int* cu, const int* pos, const int* group, const int* prefix, int groups, int n,
+                       int width, int tokens, int hq, int hkv, void* ws, hipStream_t stream);
+int attend_launch(const float* q, const PoolArgs& pool, const int* table, int width, int n, int tokens,
+                  void* ws, size_t ws_len, void* o, int o_f16, int hq, hipStream_t stream);
+
 namespace {
 thread_local char g_err[512] = "";
 }
@@ -468,6 +485,146 @@ int brasa_kv_pages_compact(brasa_kv_pool pool, const int32_t* table, const int32
         return set_error(BRASA_ERR_ARG, "kv_pages_compact: null pointer");
     return kv_pages_compact_launch(p, table, ref, table_out, ref_out, live, (int)n, (int)width, workspace,
                                    as_stream(stream));
+}
+
+// The axes of `half` pairs and the table they index.
+static int axes_check(const char* what, const brasa_rope_axes_map& m, const brasa_rope_table_view& table, size_t dim) {
+    if (dim != table.dim) return set_error(BRASA_ERR_SHAPE, "RoPE table dimension");
+    if (dim == 0 || dim % 2 != 0 || dim / 2 > sizeof(m.of))
+        return set_error(BRASA_ERR_SHAPE, "%s: head_dim %zu", what, dim);
+    if (m.axes == 0 || m.axes > BRASA_ROPE_AXES) return set_error(BRASA_ERR_SHAPE, "%s: %zu axes", what, m.axes);
+    for (size_t i = 0; i < dim / 2; ++i)
+        if (m.of[i] >= m.axes) return set_error(BRASA_ERR_ARG, "%s: pair %zu has axis %d of %zu", what, i, m.of[i], m.axes);
+    if (table.max_pos > kMaxPositions) return set_error(BRASA_ERR_SHAPE, "%s: RoPE table too large", what);
+    return BRASA_OK;
+}
+
+int brasa_rope_axes(float* x, brasa_rope_table_view table, brasa_rope_axes_map axes, const int32_t* pos,
+                    size_t tokens, size_t heads, size_t dim, void* stream) {
+    g_err[0] = 0;
+    const char* what = "rope_axes";
+    const int st = axes_check(what, axes, table, dim);
+    if (st != BRASA_OK) return st;
+    if (heads > kMaxHeads || tokens > kMaxPositions) return set_error(BRASA_ERR_SHAPE, "%s: shape too large", what);
+    if (tokens == 0 || heads == 0) return BRASA_OK;
+    if (!x || !pos || (table.max_pos && (!table.cos || !table.sin)))
+        return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if ((uintptr_t)x % 4) return set_error(BRASA_ERR_ARG, "%s: x must be 4-byte aligned", what);
+    return rope_axes_launch(x, table.cos, table.sin, (int)table.max_pos, axes, pos, (int)tokens, (int)heads, (int)dim,
+                            as_stream(stream));
+}
+
+int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, float* k, const float* v,
+                                   const float* q_norm, const float* k_norm, float eps,
+                                   brasa_rope_table_view table, brasa_rope_axes_map axes,
+                                   const int32_t* rope_pos, const int32_t* cu, const int32_t* pos,
+                                   const int32_t* pages, size_t n, size_t width, size_t tokens, size_t hq,
+                                   void* stream) {
+    g_err[0] = 0;
+    const char* what = "qk_norm_rope_store_paged";
+    PoolArgs p;
+    int st = pool_check(what, pool, layer, &p);
+    if (st == BRASA_OK) st = table_check(what, n, width);
+    if (st == BRASA_OK) st = axes_check(what, axes, table, kDim);
+    if (st != BRASA_OK) return st;
+    if (hq > kMaxHeads || tokens > kMaxPositions / (hq + 2 * pool.hkv))
+        return set_error(BRASA_ERR_SHAPE, "%s: shape too large", what);
+    if (table.max_pos == 0) return set_error(BRASA_ERR_SHAPE, "%s: an empty RoPE table", what);
+    if (n == 0 || tokens == 0) return BRASA_OK;
+    if ((hq && (!q || !q_norm)) || !k || !v || !k_norm || !table.cos || !table.sin || !rope_pos || !cu || !pos ||
+        (width && !pages))
+        return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16)
+        return set_error(BRASA_ERR_ARG, "%s: the rows must be 16-byte aligned", what);
+    return norm_rope_paged_launch(p, q, k, v, q_norm, k_norm, eps, table.cos, table.sin, (int)table.max_pos, axes,
+                                  rope_pos, cu, pos, pages, (int)n, (int)width, (int)tokens, (int)hq,
+                                  as_stream(stream));
+}
+
+int brasa_kv_rows(const int32_t* add, const int32_t* len, const int32_t* table, size_t n, size_t width,
+                  size_t pages, size_t tokens, int32_t* cu, int32_t* lk, int32_t* seq, int32_t* pos,
+                  int32_t* slot, void* stream) {
+    g_err[0] = 0;
+    const char* what = "kv_rows";
+    const int st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    if (pages == 0 || pages > kMaxPages) return set_error(BRASA_ERR_SHAPE, "%s: %zu pages", what, pages);
+    if (tokens > kMaxPositions) return set_error(BRASA_ERR_SHAPE, "%s: %zu rows", what, tokens);
+    if (n == 0) return set_error(BRASA_ERR_SHAPE, "%s: no sequences", what);
+    if (!add || !len || (slot && width && !table)) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if (lk == len || cu == add) return set_error(BRASA_ERR_ARG, "%s: lk and cu must be arrays of their own", what);
+    return kv_rows_launch(add, len, table, cu, lk, seq, pos, slot, (int)n, (int)width, (int)pages, (int)tokens,
+                          as_stream(stream));
+}
+
+int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_t* group, size_t groups,
+                          size_t n, size_t width, size_t pages, int32_t* prefix, void* stream) {
+    g_err[0] = 0;
+    const char* what = "kv_pages_shared";
+    const int st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    if (pages == 0 || pages > kMaxPages) return set_error(BRASA_ERR_SHAPE, "%s: %zu pages", what, pages);
+    if (groups > kMaxSeqs) return set_error(BRASA_ERR_SHAPE, "%s: %zu groups", what, groups);
+    if (groups == 0) return BRASA_OK;
+    if (!group || !prefix || (n && (!len || (width && !table)))) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    return kv_pages_shared_launch(table, len, group, (int)groups, prefix, (int)n, (int)width, (int)pages,
+                                  as_stream(stream));
+}
+
+// Sizes that the plan and the calls on it check alike.
+static int attend_check(const char* what, size_t n, size_t groups, size_t width, size_t tokens, size_t hq, size_t hkv) {
+    const int st = table_check(what, n, width);
+    if (st != BRASA_OK) return st;
+    if (hkv == 0 || hq == 0 || hq > kMaxHeads || hq % hkv != 0)
+        return set_error(BRASA_ERR_SHAPE, "hq must be a multiple of hkv, at most %zu", kMaxHeads);
+    if (groups > kMaxSeqs || tokens > ((size_t)1 << 29) / hq)
+        return set_error(BRASA_ERR_SHAPE, "%s: shape too large", what);
+    return BRASA_OK;
+}
+
+size_t brasa_attention_paged_workspace_len(size_t n, size_t groups, size_t tokens, size_t hq, size_t hkv) {
+    g_err[0] = 0;
+    if (attend_check("attention_paged_workspace_len", n, groups, 1, tokens, hq, hkv) != BRASA_OK) return 0;
+    return attend_workspace_len((int)n, (int)groups, (int)tokens, (int)hq, (int)hkv);
+}
+
+int brasa_attention_paged_plan(const int32_t* cu, const int32_t* pos, const int32_t* group,
+                               const int32_t* prefix, size_t groups, size_t n, size_t width, size_t tokens,
+                               size_t hq, size_t hkv, void* workspace, size_t workspace_len, void* stream) {
+    g_err[0] = 0;
+    const char* what = "attention_paged_plan";
+    const int st = attend_check(what, n, groups, width, tokens, hq, hkv);
+    if (st != BRASA_OK) return st;
+    const size_t need = attend_workspace_len((int)n, (int)groups, (int)tokens, (int)hq, (int)hkv);
+    if (workspace_len < need)
+        return set_error(BRASA_ERR_SCRATCH, "%s: workspace too small (%zu < %zu bytes)", what, workspace_len, need);
+    if (!workspace || (n && (!cu || !pos)) || (groups && (!group || !prefix)))
+        return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if ((uintptr_t)workspace % 256) return set_error(BRASA_ERR_ARG, "%s: the workspace must be 256-byte aligned", what);
+    return attend_plan_launch(cu, pos, group, prefix, (int)groups, (int)n, (int)width, (int)tokens, (int)hq, (int)hkv,
+                              workspace, as_stream(stream));
+}
+
+int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, const int32_t* table, size_t width,
+                          size_t n, size_t tokens, void* workspace, size_t workspace_len, void* o, int o_dtype,
+                          size_t hq, void* stream) {
+    g_err[0] = 0;
+    const char* what = "attention_paged";
+    if (o_dtype != BRASA_OUT_F32 && o_dtype != BRASA_OUT_F16)
+        return set_error(BRASA_ERR_ARG, "%s: invalid output dtype %d", what, o_dtype);
+    PoolArgs p;
+    int st = pool_check(what, pool, layer, &p);
+    if (st == BRASA_OK) st = attend_check(what, n, 0, width, tokens, hq, pool.hkv);
+    if (st != BRASA_OK) return st;
+    const size_t need = attend_workspace_len((int)n, 0, (int)tokens, (int)hq, p.hkv);
+    if (workspace_len < need)
+        return set_error(BRASA_ERR_SCRATCH, "%s: workspace too small (%zu < %zu bytes)", what, workspace_len, need);
+    if (n == 0 || tokens == 0) return BRASA_OK;
+    if (!q || (!table && width) || !workspace || !o) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    if ((uintptr_t)workspace % 256 || ((uintptr_t)q | (uintptr_t)o) % 16)
+        return set_error(BRASA_ERR_ARG, "%s: q and o must be 16-byte, the workspace 256-byte aligned", what);
+    return attend_launch(q, p, table, (int)width, (int)n, (int)tokens, workspace, workspace_len, o,
+                         o_dtype == BRASA_OUT_F16, (int)hq, as_stream(stream));
 }
 
 int brasa_rope_table(double theta, size_t dim, size_t max_pos, float* cos_out, float* sin_out) {

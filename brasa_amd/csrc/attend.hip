@@ -1,0 +1,943 @@
+// Attention of new rows, one or many for each sequence, over the paged 8-bit cache, with the pages that
+// a group of sequences shares read and multiplied once for all of the group's rows.
+//
+// o[t, h] = sum_j p_j v_j / sum_j p_j over the positions j <= the row's own, p_j = exp(q . k_j / sqrt(128)).
+// The sums over two sets of positions join as (m, l, acc) pairs: with m = max(m1, m2), l = l1 2^(m1 - m)
+// + l2 2^(m2 - m), and acc alike. So a row's positions may be cut anywhere, and the rows of several
+// sequences may stand together in one product where they read the same pages.
+//
+// A column is a (row, query head) of a KV head; a tile is up to 128 columns over a run of pages of one
+// table row. A group's rows (of sequences with fewer than 128 columns: more fill tiles of their own)
+// make prefix tiles over the shared pages, and each sequence's rows tiles over its other pages. All
+// tiles of a KV head stand in one line by their cost, and workgroup w takes the w-th equal run of
+// it, so that every CU has the same work whatever the lengths, which only the device knows. The plan
+// kernel lays the line out once a step, every layer's launch walks it; a tile that a run's border
+// cuts, or whose sequence has a prefix tile, leaves (m, l, acc) in the workspace and a second
+// launch joins them in order, so the result does not depend on timing.
+#include <climits>
+
+#include "paged.hpp"
+
+namespace brasa {
+namespace {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kCols = 32;                    // columns of a wave
+constexpr int kTileCols = kCols * kWaves;    // of a tile
+constexpr int kSlots = 512;                  // workgroups of a launch: two per CU
+constexpr int kMergeCols = 16;               // columns of a merge entry
+constexpr int kPad = kDim + 4;               // floats of a column in LDS: stores of 16 bytes spread over the banks
+
+// Cost of a page by the waves that share its tile's columns: one, two or four column groups.
+__host__ __device__ constexpr int page_cost(int groups) { return groups == 1 ? 2 : groups == 2 ? 3 : 4; }
+constexpr int kMinRun = 8 * page_cost(1);  // least cost of a run: two pages for each wave
+
+struct Tile {
+    int seq;          // table row whose pages it reads
+    int row0;         // own tile: the sequence's first packed row; prefix tile: offset in the row list
+    int col0, cols;   // its columns among the sequence's, or the group's
+    int b0, b1;       // pages
+    int pos0;         // own tile: position of the sequence's first new row
+    int kind;         // kPrefix, kDirect, kBad
+    long long start;  // in the line
+    int cost;         // of a page
+    int base, parts;  // partials: columns base + part * cols + column; parts of it
+    int run0;         // run of its first part
+    int ptile, pcol;  // prefix tile and column in the group where its first column continues; -1: none
+};
+static_assert(sizeof(Tile) == 64, "a tile is one line");
+enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4 };
+
+// Where the plan and the partials stand in the workspace.
+struct Layout {
+    int runs;
+    size_t run_tile, tiles, merges, seqs, first, group, rows, ml, acc, bytes;
+    long long cap;  // columns of partials, for each KV head
+    int max_tiles, max_merges;
+};
+
+struct Header {
+    int magic, n, tokens, width, hq, hkv, runs, tiles, merges;
+    long long size, total;  // of a run, of the line
+    Layout at;
+};
+constexpr int kMagic = 0x61747031;
+
+// A sequence and a group as the plan sees them.
+struct PlanSeq {
+    int c0, rows;  // its packed rows
+    int pos;       // of the first; -1: there is no page for it
+    int group;     // whose prefix it may share; -1: none
+    int scol;      // columns of such sequences before it
+};
+struct PlanGroup {
+    int s0, s1;      // its sequences
+    int lead, many;  // the first of those that may share its prefix, and how many
+};
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+Layout layout(int n, int groups, int tokens, int hq, int hkv) {
+    Layout l;
+    const long long g = hq / hkv, cols = (long long)tokens * g, seqs = std::min(n, tokens);
+    // columns of sequences that may share: each has fewer than a tile's
+    const long long shared = groups ? std::min(cols, seqs * (kTileCols - 1)) : 0;
+    l.runs = std::max(kSlots / hkv, 1);
+    l.max_tiles = (int)(seqs + cols / kTileCols + (groups ? std::min((long long)groups, seqs) + shared / kTileCols : 0));
+    // entries: all shared columns, and eight for each tile that a run's border cuts
+    l.max_merges = (int)(shared / kMergeCols + (groups ? seqs : 0) + (long long)l.runs * (kTileCols / kMergeCols));
+    // shared columns once in each of the two tiles, and for each border a tile's columns once or twice
+    l.cap = 2 * shared + 2LL * l.runs * std::min((long long)kTileCols, cols);
+    size_t at = up256(sizeof(Header));
+    auto take = [&](size_t bytes) {
+        const size_t a = at;
+        at += up256(bytes);
+        return a;
+    };
+    l.run_tile = take(4 * (size_t)l.runs);
+    l.tiles = take(sizeof(Tile) * (size_t)l.max_tiles);
+    l.merges = take(4 * (size_t)l.max_merges);
+    l.seqs = take(sizeof(PlanSeq) * (size_t)n);
+    l.first = take(4 * ((size_t)groups + n + 1));
+    l.group = take(sizeof(PlanGroup) * (size_t)groups);
+    l.rows = take(groups ? 4 * (size_t)tokens : 0);
+    l.ml = take(8 * (size_t)l.cap * hkv);
+    l.acc = take(4 * kDim * (size_t)l.cap * hkv);
+    l.bytes = at;
+    return l;
+}
+
+// ---- the plan -----------------------------------------------------------------------------------
+//
+// One workgroup: sequences, then groups and sequences again (how many tiles each has), then the tiles, a
+// thread for each of them. Bound: the latency of that chain of loads and scans, once a step.
+struct PlanArgs {
+    const int* cu;
+    const int* pos;
+    const int* group;
+    const int* prefix;
+    Header* head;
+    int* run_tile;
+    Tile* tile;
+    int* merge;
+    PlanSeq* seq;
+    int* first;  // [groups + n + 1]: first tile of each group's prefix, then of each sequence
+    PlanGroup* grp;
+    int* rows;  // packed rows of the sequences that may share, in order
+    int n, groups, width, tokens, hq, hkv, per_row, runs;
+    Layout at;
+};
+
+__device__ __forceinline__ void st_l2(int* p, int x) {
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// exclusive sum over the workgroup of values up to 2^62; s: kScanWaves of LDS
+__device__ __forceinline__ long long block_scan64(long long x, long long* s, long long& sum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    long long incl = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const long long y = __shfl_up(incl, d);
+        if (lane >= d) incl += y;
+    }
+    __syncthreads();  // s is free
+    if (lane == 63) s[wave] = incl;
+    __syncthreads();
+    long long before = 0;
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) {
+        const long long y = s[w];
+        if (w < wave) before += y;
+        sum += y;
+    }
+    return before + incl - x;
+}
+// inclusive maximum over the workgroup and `before`; `all`: of the whole workgroup
+__device__ __forceinline__ int block_max(int x, int before, int* s, int& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    x = max(x, before);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x = max(x, y);
+    }
+    __syncthreads();  // s is free
+    if (lane == 63) s[wave] = x;
+    __syncthreads();
+    all = before;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) {
+        const int y = s[w];
+        if (w < wave) x = max(x, y);
+        all = max(all, y);
+    }
+    return x;
+}
+// x / d for 0 <= x < 2^52, d > 0, with inv = 1.0 / d
+__device__ __forceinline__ long long div_by(long long x, long long d, double inv) {
+    long long q = (long long)((double)x * inv);
+    q -= q * d > x;
+    q += (q + 1) * d <= x;
+    return q;
+}
+__device__ __forceinline__ int col_groups(int cols) { return cols <= kCols ? 1 : cols <= 2 * kCols ? 2 : 4; }
+
+__global__ void __launch_bounds__(kScanThreads)
+attend_plan_kernel(PlanArgs a) {
+    __shared__ long long s_scan[kScanWaves];
+    __shared__ int s_scan32[kScanWaves];
+    __shared__ int s_merges;
+    const int tid = threadIdx.x;
+    if (tid == 0) s_merges = 0;
+    const int per_row = a.per_row;
+
+    // ---- groups: runs of sequences, in order and apart ------------------------------------------
+    for (int g0 = 0, before = 0; g0 < a.groups; g0 += kScanThreads) {
+        const int g = g0 + tid;
+        int all;
+        const int s0 = block_max(g < a.groups ? min(max(a.group[g], 0), a.n) : 0, before, s_scan32, all);
+        const int s1 = max(s0, g < a.groups ? min(max(a.group[g + 1], 0), a.n) : 0);
+        before = all;
+        if (g < a.groups) {
+            st_l2(&a.grp[g].s0, s0);
+            st_l2(&a.grp[g].s1, s1);
+            st_l2(&a.grp[g].lead, a.n);
+            st_l2(&a.grp[g].many, 0);
+        }
+    }
+    if (a.groups) stores_barrier();
+    auto prefix_pages = [&](int g) { return min(max(a.prefix[g], 0) / kPage, a.width); };
+
+    // ---- sequences: their rows, in order and apart, and who may share a prefix --------------------
+    int scols = 0;
+    for (int i0 = 0, before = 0; i0 < a.n; i0 += kScanThreads) {
+        const int i = i0 + tid;
+        int all;
+        const int c0 = block_max(i < a.n ? min(max(a.cu[i], 0), a.tokens) : 0, before, s_scan32, all);
+        before = all;
+        PlanSeq s;
+        s.c0 = c0;
+        s.rows = i < a.n ? max(min(max(a.cu[i + 1], 0), a.tokens) - c0, 0) : 0;
+        s.pos = i < a.n ? a.pos[i] : -1;
+        if (s.pos >= a.width * kPage) s.pos = -1;
+        s.group = -1;
+        int cols = 0;
+        // (whose rows all stand behind the prefix, and do not fill a tile)
+        if (a.groups && s.rows > 0 && s.rows < kTileCols && s.rows * per_row < kTileCols) {
+            int lo = 0, hi = a.groups;  // the last group that starts at or before i
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (ld_l2(&a.grp[mid].s0) <= i) lo = mid;
+                else hi = mid;
+            }
+            if (ld_l2(&a.grp[lo].s0) <= i && i < ld_l2(&a.grp[lo].s1)) {
+                const int pages = prefix_pages(lo);
+                if (pages > 0 && s.pos >= pages * kPage) {
+                    s.group = lo;
+                    cols = s.rows * per_row;
+                    atomicMin(&a.grp[lo].lead, i);
+                    atomicAdd(&a.grp[lo].many, 1);
+                }
+            }
+        }
+        if (a.groups) {
+            int sum;
+            s.scol = scols + block_scan(cols, s_scan32, sum);
+            scols += sum;
+            // (the rows of one that turns out to be alone in its group are listed, and not used)
+            for (int r = 0; cols && r < s.rows; ++r) a.rows[s.scol / per_row + r] = s.c0 + r;
+        }
+        if (i < a.n) {
+            st_l2(&a.seq[i].c0, s.c0);
+            st_l2(&a.seq[i].rows, s.rows);
+            st_l2(&a.seq[i].pos, s.pos);
+            st_l2(&a.seq[i].group, s.group);
+            st_l2(&a.seq[i].scol, s.scol);
+        }
+    }
+    stores_barrier();
+    auto load_seq = [&](int i) {
+        PlanSeq s = {ld_l2(&a.seq[i].c0), ld_l2(&a.seq[i].rows), ld_l2(&a.seq[i].pos), ld_l2(&a.seq[i].group), 0};
+        if (s.group >= 0) {
+            if (ld_l2(&a.grp[s.group].many) < 2) s.group = -1;
+            else s.scol = ld_l2(&a.seq[i].scol);
+        }
+        return s;
+    };
+    // columns of a group's sharing sequences, and how many there are before them in the list
+    auto group_cols = [&](int g, int& col0) {
+        if (ld_l2(&a.grp[g].many) < 2) return 0;
+        const int s0 = ld_l2(&a.grp[g].s0), s1 = ld_l2(&a.grp[g].s1);
+        col0 = ld_l2(&a.seq[s0].scol);
+        return (s1 < a.n ? ld_l2(&a.seq[s1].scol) : scols) - col0;
+    };
+
+    // ---- how many tiles each has ------------------------------------------------------------------
+    int ntiles = 0;
+    const int entries = a.groups + a.n;
+    for (int e0 = 0; e0 < entries; e0 += kScanThreads) {
+        const int e = e0 + tid;
+        int tiles = 0, col0;
+        if (e < a.groups) tiles = (group_cols(e, col0) + kTileCols - 1) / kTileCols;
+        else if (e < entries) tiles = (int)(((long long)ld_l2(&a.seq[e - a.groups].rows) * per_row + kTileCols - 1) / kTileCols);
+        int sum;
+        const int at = ntiles + block_scan(tiles, s_scan32, sum);
+        ntiles += sum;
+        if (e < entries) st_l2(a.first + e, at);
+    }
+    if (tid == 0) st_l2(a.first + entries, ntiles);
+    stores_barrier();
+
+    auto make_tile = [&](int at) {
+        int lo = 0, hi = entries;  // the last group or sequence that starts at or before `at`: one with tiles
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (ld_l2(a.first + mid) <= at) lo = mid;
+            else hi = mid;
+        }
+        Tile t;
+        t.col0 = (at - ld_l2(a.first + lo)) * kTileCols;
+        t.ptile = t.pcol = -1;
+        if (lo < a.groups) {
+            int col0;
+            const int cols = group_cols(lo, col0);
+            t.kind = kPrefix;
+            t.seq = ld_l2(&a.grp[lo].lead);
+            t.row0 = col0 / per_row;
+            t.cols = min(cols - t.col0, kTileCols);
+            t.b0 = 0;
+            t.b1 = prefix_pages(lo);
+            t.pos0 = 0;
+        } else {
+            const int i = lo - a.groups;
+            const PlanSeq s = load_seq(i);
+            t.kind = s.pos < 0 ? kBad : 0;
+            t.seq = i;
+            t.row0 = s.c0;
+            t.cols = (int)min((long long)s.rows * per_row - t.col0, (long long)kTileCols);
+            t.b0 = s.group >= 0 ? prefix_pages(s.group) : 0;
+            // (a sequence without a place gets one page, not read, whose tile writes NaN)
+            const int last = (t.col0 + t.cols - 1) / per_row;
+            t.b1 = s.pos < 0 ? 1 : min((int)(((long long)s.pos + last) / kPage) + 1, a.width);
+            t.pos0 = s.pos;
+            if (s.group >= 0) {
+                int gcol0 = 0;
+                group_cols(s.group, gcol0);
+                t.ptile = ld_l2(a.first + s.group) + (s.scol - gcol0) / kTileCols;
+                t.pcol = (s.scol - gcol0) % kTileCols;
+            }
+        }
+        t.cost = page_cost(col_groups(t.cols));
+        return t;
+    };
+
+    // ---- the line's length, and that of a run -----------------------------------------------------
+    long long mine = 0, total;
+    Tile t = {};
+    for (int i = tid; i < ntiles; i += kScanThreads) {
+        t = make_tile(i);
+        mine += (long long)(t.b1 - t.b0) * t.cost;
+    }
+    block_scan64(mine, s_scan, total);
+    const long long size = max((total + a.runs - 1) / a.runs, (long long)kMinRun);
+    const double inv = 1.0 / (double)size;
+
+    // ---- the tiles --------------------------------------------------------------------------------
+    long long line = 0, cols = 0;
+    for (int t0 = 0; t0 < ntiles; t0 += kScanThreads) {
+        const int at = t0 + tid;
+        const bool on = at < ntiles;
+        if (on && ntiles > kScanThreads) t = make_tile(at);  // (else it is at hand)
+        const long long len = on ? (long long)(t.b1 - t.b0) * t.cost : 0;
+        long long sum;
+        t.start = line + block_scan64(len, s_scan, sum);
+        line += sum;
+        t.run0 = (int)div_by(t.start, size, inv);
+        const int last = on ? (int)div_by(t.start + len - 1, size, inv) : 0;
+        t.parts = last - t.run0 + 1;
+        if (!(t.kind & kPrefix) && t.ptile < 0 && t.parts == 1) t.kind |= kDirect;
+        const long long part_cols = on && !(t.kind & kDirect) ? (long long)t.cols * t.parts : 0;
+        t.base = (int)(cols + block_scan64(part_cols, s_scan, sum));
+        cols += sum;
+        if (!on) continue;
+        a.tile[at] = t;
+        for (int w = t.run0 + (t.start > t.run0 * size); w <= last; ++w) a.run_tile[w] = at;
+        if (!(t.kind & (kPrefix | kDirect))) {
+            const int many = (t.cols + kMergeCols - 1) / kMergeCols;
+            const int e = atomicAdd(&s_merges, many);
+            for (int j = 0; j < many; ++j) a.merge[e + j] = at * (kTileCols / kMergeCols) + j;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        Header h;
+        h.magic = kMagic;
+        h.n = a.n;
+        h.tokens = a.tokens;
+        h.width = a.width;
+        h.hq = a.hq;
+        h.hkv = a.hkv;
+        h.runs = a.runs;
+        h.tiles = ntiles;
+        h.merges = s_merges;
+        h.size = size;
+        h.total = line;
+        h.at = a.at;
+        *a.head = h;
+    }
+}
+
+// ---- tiles --------------------------------------------------------------------------------------
+//
+// A wave holds 32 columns and takes 32 keys (half a page) at a time, all of it in registers: K's codes
+// are converted exactly (an e4m3 value is an f16 value) from the loaded pieces into the A operand of
+// S^T = K Q^T on 32x32x16 f16 MFMAs, once with the hi and once with the lo halves of q (22 bits
+// together). S^T's layout is the B operand of O^T += V^T P^T, P in hi and lo halves again; V's operand
+// needs eight keys of one dim in a lane, which byte permutes pair up from four dims of each key
+// before the conversion. The waves of a tile take a column group each, or where it has fewer than four
+// groups share its pages; those waves' sums are joined through LDS.
+struct AttendArgs {
+    const uint8_t* ws;
+    size_t ws_len;
+    const float* q;
+    PoolArgs p;  // of one layer
+    const int* table;
+    void* o;
+    int n, width, tokens, hq, per_row, o_f16;
+};
+// The workspace's header and the parts it names.
+struct Plan {
+    Header head;
+    const int* run_tile;
+    const Tile* tile;
+    const int* merge;
+    const int* rows;
+    float* ml;
+    float* acc;
+    bool fits;  // it is a plan of this call's sizes
+};
+__device__ __forceinline__ Plan load_plan(const AttendArgs& a) {
+    Plan p;
+    p.head = *reinterpret_cast<const Header*>(a.ws);
+    const Header& h = p.head;
+    p.fits = h.magic == kMagic && h.n == a.n && h.tokens == a.tokens && h.width == a.width && h.hq == a.hq &&
+             h.hkv == a.p.hkv && h.at.bytes <= a.ws_len;
+    p.run_tile = reinterpret_cast<const int*>(a.ws + h.at.run_tile);
+    p.tile = reinterpret_cast<const Tile*>(a.ws + h.at.tiles);
+    p.merge = reinterpret_cast<const int*>(a.ws + h.at.merges);
+    p.rows = reinterpret_cast<const int*>(a.ws + h.at.rows);
+    p.ml = reinterpret_cast<float*>(const_cast<uint8_t*>(a.ws) + h.at.ml);
+    p.acc = reinterpret_cast<float*>(const_cast<uint8_t*>(a.ws) + h.at.acc);
+    return p;
+}
+
+__device__ __forceinline__ f32x16 mfma32(half8v a, half8v b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// e4m3 codes 0, 1 (2, 3) of a word -> f16 values, exact
+__device__ __forceinline__ half2v f16_of_lo(uint32_t w) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+}
+__device__ __forceinline__ half2v f16_of_hi(uint32_t w) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+}
+__device__ __forceinline__ half8v join(half2v a, half2v b, half2v c, half2v d) {
+    return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// x and y as f16 halves hi + lo (up to 2^-22 of each)
+__device__ __forceinline__ void split(float x, float y, half2v& hi, half2v& lo) {
+    hi = half2v{(_Float16)x, (_Float16)y};
+    lo = half2v{(_Float16)(x - (float)hi.x), (_Float16)(y - (float)hi.y)};
+}
+// 0x80 in the places of a word's NaN codes
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// over the two lanes c, c + 32 of a column
+__device__ __forceinline__ float max_h(float x) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_h(float x) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+// weight of a part whose largest score is m in a sum whose largest is top (no key: m = -inf)
+__device__ __forceinline__ float part_weight(float m, float top) {
+    return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+}
+__device__ __forceinline__ void write_o(const AttendArgs& a, size_t at, f32x4 x, float l) {
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = x[e] / l;
+    if (a.o_f16) {
+        u32x2 w = {f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + at) = w;
+    } else {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + at) = y;
+    }
+}
+
+// V^T P^T of 32 keys added to acc. v[4 q + r]: four codes (dims 4 i .. + 4 of lane i) of key 8 q + 4 h + r.
+__device__ __forceinline__ void add_pv(const uint32_t (&v)[16], const half8v (&hi)[2], const half8v (&lo)[2],
+                                       f32x16 (&acc)[4]) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {  // dims 4 i + 2 t2, 4 i + 2 t2 + 1
+            const uint32_t by = 2 * t2, sel = by | (4 + by) << 8 | (by + 1) << 16 | (5 + by) << 24;
+            half2v x0[4], x1[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t w = __builtin_amdgcn_perm(v[8 * st + 2 * e + 1], v[8 * st + 2 * e], sel);
+                x0[e] = f16_of_lo(w);
+                x1[e] = f16_of_hi(w);
+            }
+            const half8v v0 = join(x0[0], x0[1], x0[2], x0[3]), v1 = join(x1[0], x1[1], x1[2], x1[3]);
+            acc[2 * t2] = mfma32(v0, hi[st], acc[2 * t2]);
+            acc[2 * t2 + 1] = mfma32(v1, hi[st], acc[2 * t2 + 1]);
+            acc[2 * t2] = mfma32(v0, lo[st], acc[2 * t2]);
+            acc[2 * t2 + 1] = mfma32(v1, lo[st], acc[2 * t2 + 1]);
+        }
+}
+
+__global__ void __launch_bounds__(kThreads, 2)
+attend_kernel(AttendArgs a) {
+    __shared__ __attribute__((aligned(16))) float s_acc[kWaves][kCols][kPad];
+    __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
+
+    const Plan plan = load_plan(a);
+    if (!plan.fits) return;
+    const Header& head = plan.head;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv;
+    const long long lo = run * head.size, end = min(lo + head.size, head.total);
+    if (lo >= end) return;
+
+    for (int ti = plan.run_tile[run]; ti < head.tiles; ++ti) {
+        const Tile t = plan.tile[ti];
+        if (t.start >= end) break;
+        // ---- this run's pages of the tile ------------------------------------------------------------
+        const int len = (t.b1 - t.b0) * t.cost;
+        const int from = (int)max(lo - t.start, 0LL), to = (int)min(end - t.start, (long long)len);
+        const int p0 = t.b0 + (from + t.cost - 1) / t.cost;
+        const int p1 = to == len ? t.b1 : t.b0 + (to + t.cost - 1) / t.cost;
+        const bool prefix = t.kind & kPrefix, nowhere = t.kind & kBad;
+        // the wave's column group, and which of the pages are its
+        const int groups = t.cols <= kCols ? 1 : t.cols <= 2 * kCols ? 2 : 4;
+        const int cg = wave & (groups - 1), phase = wave / groups, step = kWaves / groups;
+        const int cols = min(t.cols - kCols * cg, kCols);  // of this wave (none: at most 0)
+        const int* ids = a.table + (size_t)t.seq * a.width;
+
+        // ---- Q: hi and lo halves of q / sqrt(128) * log2 e, each column's exponent taken out -----------
+        const int col = t.col0 + min(kCols * cg + c, t.cols - 1);  // (lanes past the last column repeat it)
+        const int local = col / a.per_row;
+        const int row = prefix ? plan.rows[t.row0 + local] : t.row0 + local;
+        const int head_of = kh * a.per_row + col - local * a.per_row;
+        const int limit = prefix ? INT_MAX : nowhere ? -1 : t.pos0 + local;  // the last position it sees
+        half8v qh[8], ql[8];
+        int qx;
+        {
+            // step s holds dims 32 (s / 2) + 16 h + 8 (s % 2) .. + 8, as K's 16-byte loads do
+            const float* qrow = a.q + ((size_t)row * a.hq + head_of) * kDim + 16 * h;
+            const float scale = 0.08838834764831845f * kLog2e;
+            float x[8][8];
+            float qmax = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(qrow + 32 * (s >> 1) + 8 * (s & 1) + 4 * e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[s][4 * e + j] = as_f32(y[j] * scale);
+                        qmax = fmaxf(qmax, fabsf(x[s][4 * e + j]));
+                    }
+                }
+            qmax = max_h(qmax);
+            qx = (int)(__float_as_uint(qmax) >> 23) - 127 - 8;  // the row's largest to [2^8, 2^9)
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                half2v u[4], w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split(ldexpf(x[s][2 * j], -qx), ldexpf(x[s][2 * j + 1], -qx), u[j], w[j]);
+                qh[s] = join(u[0], u[1], u[2], u[3]);
+                ql[s] = join(w[0], w[1], w[2], w[3]);
+            }
+        }
+        // the least and the largest position that a column of this wave sees
+        int lim0 = limit, lim1 = limit;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            lim0 = min(lim0, __shfl_xor(lim0, d));
+            lim1 = max(lim1, __shfl_xor(lim1, d));
+        }
+        lim0 = __builtin_amdgcn_readfirstlane(lim0);
+        lim1 = __builtin_amdgcn_readfirstlane(lim1);
+
+        float m_used = -INFINITY, lsum = 0.0f;
+        f32x16 acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
+        int vref = 0;     // acc stands in units of 2^(vref - 127); 0: nothing yet
+        bool bad = nowhere;
+
+        u32x4 kw[4];      // key 32 half + c, dims 32 i + 16 h .. + 16
+        uint32_t vw[16];  // key 32 half + 8 q + 4 h + r at 4 q + r, dims 4 c .. + 4
+        auto load_k = [&](size_t tile, int half) {
+            const uint8_t* p = a.p.k + tile * kTileBytes8 + (32 * half + c) * kDim + 16 * h;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(p + 32 * i);
+        };
+        auto load_v = [&](size_t tile, int half) {
+            const uint8_t* p = a.p.v + tile * kTileBytes8 + (32 * half + 4 * h) * kDim + 4 * c;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                vw[i] = *reinterpret_cast<const uint32_t*>(p + (8 * (i >> 2) + (i & 3)) * kDim);
+        };
+        // a page that is not there reads page 0 in its place
+        auto tile_of = [&](int id, bool& there) {
+            there = id >= 0 && id < a.p.pages;
+            return (size_t)(there ? id : 0) * a.p.hkv + kh;
+        };
+
+        const int first = p0 + phase;
+        if (!nowhere && cols > 0 && first < p1) {
+            int page = first, half = 0;
+            bool there, there_next = true;
+            size_t tile = tile_of(ids[page], there), tile_next = tile;
+            load_k(tile, 0);
+            load_v(tile, 0);
+            int kx = a.p.kx[tile], vx = a.p.vx[tile], kx_next = kx, vx_next = vx;
+            while (true) {
+                const int k0 = page * kPage + 32 * half;
+                // where the next half page is
+                const int page_next = half ? page + step : page;
+                const bool more = page_next < p1;
+                if (half && more) {
+                    tile_next = tile_of(ids[page_next], there_next);
+                    kx_next = a.p.kx[tile_next];
+                    vx_next = a.p.vx[tile_next];
+                }
+                // ---- scores: key k0 + 8 q + 4 h + r of column c, in units of log2 and of 2^(qx + kx - 127)
+                f32x16 s;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[j] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t w0 = kw[i >> 1][2 * (i & 1)], w1 = kw[i >> 1][2 * (i & 1) + 1];
+                    const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
+                    s = mfma32(ka, qh[i], s);
+                    s = mfma32(ka, ql[i], s);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (more) load_k(tile_next, half ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+                // (past the clamp every score is 0, or so far from the next that one key takes all)
+                const float sc = ldexpf(1.0f, min(max(qx + kx - 127, -126), 127));
+                if (!there && limit >= page * kPage) lsum = NAN;
+                const bool edge = k0 + 31 > lim0;  // some column does not see all of these keys
+                bool odd = false;                  // V holds NaN codes among them
+                if (edge) {
+                    uint32_t nans = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                        if (key > limit) s[i] = -INFINITY;
+                        if (key > lim1) vw[i] = 0;  // the codes behind the last key may be anything
+                        nans |= nan_codes(vw[i]);
+                    }
+                    odd = __builtin_amdgcn_ballot_w64(nans != 0);
+                }
+                float top = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+                top = max_h(top) * sc;
+                // a reference point that moves only when the maximum has grown by 2^8: p stays below
+                // 2^15 with the bias of 2^7 that keeps the lo halves of small p out of f16's subnormals
+                const bool grow = top > m_used + 8.0f;
+                if (__builtin_amdgcn_ballot_w64(grow)) {
+                    const float alpha = grow ? __builtin_amdgcn_exp2f(m_used - top) : 1.0f;
+                    if (grow) m_used = top;
+                    lsum *= alpha;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i] *= alpha;
+                }
+                // a column that has seen no key yet: its scores are all -inf, and p 0
+                const float mb = m_used == -INFINITY ? 0.0f : 7.0f - m_used;
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sc, mb));
+                    lsum += p[i];
+                }
+                // V's scale: acc's unit grows with it, and p shrinks where it is smaller
+                if (vx > vref) {
+                    if (vref) {
+                        const float f = ldexpf(1.0f, vref - vx);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[i] *= f;
+                    }
+                    vref = vx;
+                } else if (vx < vref) {
+                    const float f = ldexpf(1.0f, max(vx - vref, -126));
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[i] *= f;
+                }
+                half8v ph[2], pl[2];
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    half2v u[4], w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], u[e], w[e]);
+                    ph[st] = join(u[0], u[1], u[2], u[3]);
+                    pl[st] = join(w[0], w[1], w[2], w[3]);
+                }
+                if (odd) {
+                    // NaN values that some columns see and others do not: 0 in the product, and a second
+                    // one of ones in their places with the columns that see them
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        f32x16 count;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) count[j] = 0.0f;
+#pragma unroll
+                        for (int st = 0; st < 2; ++st) {
+                            half8v there, see;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int key = k0 + 8 * (2 * st + (j >> 2)) + 4 * h + (j & 3);
+                                there[j] = nan_codes(vw[8 * st + j]) >> 8 * d & 0x80u ? (_Float16)1.0f : (_Float16)0.0f;
+                                see[j] = key <= limit ? (_Float16)1.0f : (_Float16)0.0f;
+                            }
+                            count = mfma32(there, see, count);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (count[j] > 0.0f) acc[d][j] = NAN;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) vw[i] &= ~((nan_codes(vw[i]) >> 7) * 0xffu);
+                }
+                add_pv(vw, ph, pl, acc);
+                __builtin_amdgcn_sched_barrier(0);
+                if (!more) break;
+                load_v(tile_next, half ^ 1);
+                page = page_next;
+                half ^= 1;
+                there = there_next;
+                tile = tile_next;
+                kx = kx_next;
+                vx = vx_next;
+            }
+        }
+        // (a row past the table's width has no page)
+        if (bad || (!prefix && limit >= a.width * kPage)) lsum = NAN;
+        lsum = sum_h(lsum);
+        const float unit = ldexpf(1.0f, vref - 127);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= unit;
+
+        // ---- out: to o, or to the parts --------------------------------------------------------------
+        const bool direct = t.kind & kDirect;
+        const size_t part = (size_t)kh * head.at.cap + t.base + (size_t)(run - t.run0) * t.cols;
+        if (step == 1) {
+            if (c < cols) {
+                // the lane holds dims 4 (8 q + 4 h + r) + t of its column
+                const size_t at = direct ? ((size_t)row * a.hq + head_of) * kDim : (part + kCols * cg + c) * kDim;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const f32x4 x = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+                    const size_t d = at + 4 * (8 * (i >> 2) + 4 * h + (i & 3));
+                    if (direct) write_o(a, d, x, lsum);
+                    else *reinterpret_cast<f32x4*>(plan.acc + d) = x;
+                }
+                if (!direct && h == 0)
+                    *reinterpret_cast<f32x2*>(plan.ml + 2 * (part + kCols * cg + c)) = f32x2{m_used, lsum};
+            }
+            continue;
+        }
+        __syncthreads();  // the LDS is free
+        if (c < cols) {
+            if (h == 0) {
+                s_m[wave][c] = m_used;
+                s_l[wave][c] = lsum;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                *reinterpret_cast<f32x4*>(&s_acc[wave][c][4 * (8 * (i >> 2) + 4 * h + (i & 3))]) =
+                    f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < t.cols * (kDim / 4); i += kThreads) {
+            const int tc = i / (kDim / 4), d = 4 * (i % (kDim / 4));
+            const int w0 = tc / kCols, cc = tc % kCols;  // waves w0, w0 + groups, ... hold the column
+            float m = s_m[w0][cc];
+            for (int w = w0 + groups; w < kWaves; w += groups) m = fmaxf(m, s_m[w][cc]);
+            float l = 0.0f;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = w0; w < kWaves; w += groups) {
+                // a wave without a key has m = -inf, l = 0 (or NaN for a page that is not there)
+                const float f = part_weight(s_m[w][cc], m);
+                l += s_m[w][cc] == -INFINITY ? s_l[w][cc] : s_l[w][cc] * f;
+                const f32x4 y = *reinterpret_cast<const f32x4*>(&s_acc[w][cc][d]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
+            }
+            if (direct) {
+                const int col = t.col0 + tc, local = col / a.per_row;
+                const size_t at = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
+                write_o(a, at * kDim + d, x, l);
+            } else {
+                *reinterpret_cast<f32x4*>(plan.acc + (part + tc) * kDim + d) = x;
+                if (d == 0) *reinterpret_cast<f32x2*>(plan.ml + 2 * (part + tc)) = f32x2{m, l};
+            }
+        }
+    }
+}
+
+// ---- parts into rows ----------------------------------------------------------------------------
+//
+// A wave per column: its parts are those of its own tile and of the prefix tile that holds its
+// column. The halves of the wave take every other part, 16 bytes of its sums a lane.
+__global__ void __launch_bounds__(kThreads)
+attend_merge_kernel(AttendArgs a) {
+    const Plan plan = load_plan(a);
+    const Header& head = plan.head;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kh = blockIdx.x % a.p.hkv, e0 = blockIdx.x / a.p.hkv, es = gridDim.x / a.p.hkv;
+    if (!plan.fits) {  // of another step's sizes, or none: no row is left looking like a result
+        const size_t all = (size_t)a.tokens * a.hq * kDim;
+        for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (size_t)gridDim.x * kThreads) {
+            if (a.o_f16) static_cast<uint16_t*>(a.o)[i] = 0x7e00;
+            else static_cast<float*>(a.o)[i] = NAN;
+        }
+        return;
+    }
+    for (int e = e0; e < head.merges; e += es) {
+        const int entry = plan.merge[e];
+        const Tile t = plan.tile[entry / (kTileCols / kMergeCols)];
+        const int first = entry % (kTileCols / kMergeCols) * kMergeCols;
+        for (int c = first + wave; c < min(first + kMergeCols, t.cols); c += kWaves) {
+            int pparts = 0, pcols = 0, pbase = 0;
+            if (t.ptile >= 0) {
+                const int pc = t.pcol + c;
+                const Tile& p = plan.tile[t.ptile + pc / kTileCols];
+                pparts = p.parts;
+                pcols = p.cols;
+                pbase = p.base + pc % kTileCols;
+            }
+            const int parts = pparts + t.parts;
+            auto at = [&](int i) {
+                return (size_t)kh * head.at.cap + (i < pparts ? pbase + i * pcols : t.base + (i - pparts) * t.cols + c);
+            };
+            float m = -INFINITY, l = 0.0f;
+            for (int i = lane; i < parts; i += 64) m = fmaxf(m, plan.ml[2 * at(i)]);
+#pragma unroll
+            for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i0 = 0; i0 < parts; i0 += 64) {
+                const int mine = min(i0 + lane, parts - 1);
+                const f32x2 ml = *reinterpret_cast<const f32x2*>(plan.ml + 2 * at(mine));
+                const float w = i0 + lane < parts ? part_weight(ml[0], m) : 0.0f;
+                if (i0 + lane < parts) l += ml[0] == -INFINITY ? ml[1] : ml[1] * w;
+                const int many = min(parts - i0, 64);
+                for (int i = 0; i < many; i += 16) {
+                    f32x4 y[8];
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int k = i + 2 * j + (lane >> 5);
+                        y[j] = *reinterpret_cast<const f32x4*>(plan.acc + at(i0 + min(k, many - 1)) * kDim + 4 * (lane & 31));
+                        f[j] = __shfl(w, min(k, 63));
+                        if (k >= many) f[j] = 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) x[d] = f[j] == 0.0f ? x[d] : fmaf(y[j][d], f[j], x[d]);
+                }
+            }
+#pragma unroll
+            for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) x[d] = sum_h(x[d]);
+            const int col = t.col0 + c, local = col / a.per_row;
+            const size_t o = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
+            if (lane < 32) write_o(a, o * kDim + 4 * lane, x, l);
+        }
+    }
+}
+
+}  // namespace
+
+size_t attend_workspace_len(int n, int groups, int tokens, int hq, int hkv) {
+    return layout(n, groups, tokens, hq, hkv).bytes;
+}
+
+int attend_plan_launch(const int* cu, const int* pos, const int* group, const int* prefix, int groups, int n,
+                       int width, int tokens, int hq, int hkv, void* ws, hipStream_t stream) {
+    const Layout l = layout(n, groups, tokens, hq, hkv);
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    PlanArgs a = {};
+    a.cu = cu;
+    a.pos = pos;
+    a.group = group;
+    a.prefix = prefix;
+    a.head = reinterpret_cast<Header*>(w);
+    a.run_tile = reinterpret_cast<int*>(w + l.run_tile);
+    a.tile = reinterpret_cast<Tile*>(w + l.tiles);
+    a.merge = reinterpret_cast<int*>(w + l.merges);
+    a.seq = reinterpret_cast<PlanSeq*>(w + l.seqs);
+    a.first = reinterpret_cast<int*>(w + l.first);
+    a.grp = reinterpret_cast<PlanGroup*>(w + l.group);
+    a.rows = reinterpret_cast<int*>(w + l.rows);
+    a.n = n;
+    a.groups = groups;
+    a.width = width;
+    a.tokens = tokens;
+    a.hq = hq;
+    a.hkv = hkv;
+    a.per_row = hq / hkv;
+    a.runs = l.runs;
+    a.at = l;
+    hipLaunchKernelGGL(attend_plan_kernel, dim3(1), dim3(kScanThreads), 0, stream, a);
+    return check_launch("attend_plan_kernel");
+}
+
+int attend_launch(const float* q, const PoolArgs& pool, const int* table, int width, int n, int tokens,
+                  void* ws, size_t ws_len, void* o, int o_f16, int hq, hipStream_t stream) {
+    AttendArgs a = {};
+    a.ws = static_cast<const uint8_t*>(ws);
+    a.ws_len = ws_len;
+    a.q = q;
+    a.p = pool;
+    a.table = table;
+    a.o = o;
+    a.n = n;
+    a.width = width;
+    a.tokens = tokens;
+    a.hq = hq;
+    a.per_row = hq / pool.hkv;
+    a.o_f16 = o_f16;
+    const Layout l = layout(n, n, tokens, hq, pool.hkv);  // (the most entries: the plan's may have fewer groups)
+    hipLaunchKernelGGL(attend_kernel, dim3((unsigned)(l.runs * pool.hkv)), dim3(kThreads), 0, stream, a);
+    const int st = check_launch("attend_kernel");
+    if (st != BRASA_OK) return st;
+    // a workgroup for each entry of a KV head, up to four per CU
+    const int wgs = std::max(std::min(l.max_merges, 1024 / pool.hkv), 1);
+    hipLaunchKernelGGL(attend_merge_kernel, dim3((unsigned)(wgs * pool.hkv)), dim3(kThreads), 0, stream, a);
+    return check_launch("attend_merge_kernel");
+}
+
+}  // namespace brasa

@@ -24,59 +24,23 @@ struct StoreArgs {
     PoolArgs p;  // of one layer
     const float* k;
     const float* v;
-    const int* cu;
-    const int* pos;
-    const int* table;
-    int n, width, tokens;
+    NewRows rows;
     int item0;  // first item of the launch
 };
-
-// the blocks that sequence i's new rows touch: [first, first + count)
-__device__ __forceinline__ int touched_blocks(const StoreArgs& a, int i, int& c0, int& c1, int& pos) {
-    c0 = min(max(a.cu[i], 0), a.tokens);
-    c1 = min(max(a.cu[i + 1], c0), a.tokens);
-    pos = a.pos[i];
-    // (a negative position, or one past what the table can hold, has no block)
-    if (c1 == c0 || pos < 0 || pos >= a.width * kPage) return 0;
-    return min((pos + (c1 - c0) - 1) / kPage, a.width - 1) - pos / kPage + 1;
-}
 
 __global__ void __launch_bounds__(kStoreThreads)
 store_paged_kernel(StoreArgs a) {
     const int lane = threadIdx.x & 63;
-    const int item = a.item0 + blockIdx.x / a.p.hkv, kh = blockIdx.x % a.p.hkv;
+    const int kh = blockIdx.x % a.p.hkv;
     const bool is_v = blockIdx.y;
-
-    // the sequence and block of this item: every wave walks the sequences' block counts, 64 at a
-    // time
-    int seq = -1, before = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 64) {
-        int c0, c1, pos, nb = 0;
-        if (i0 + lane < a.n) nb = touched_blocks(a, i0 + lane, c0, c1, pos);
-        const int incl = wave_scan(nb) + before;
-        const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > item);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            seq = i0 + l;
-            before = __shfl(incl - nb, l);
-            break;
-        }
-        before = __shfl(incl, 63);
-    }
-    if (seq < 0) return;  // the grid's bound is loose
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    int c0, c1, pos;
-    touched_blocks(a, seq, c0, c1, pos);
-    const int block = pos / kPage + item - before;
-    const int page = a.table[(size_t)seq * a.width + block];
-    if (page < 0 || page >= a.p.pages) return;
+    TouchedBlock t;
+    if (!touched_block(a.rows, a.item0 + blockIdx.x / a.p.hkv, a.p.pages, t)) return;
     // slots [s0, s1) of the block are new, [0, s0) hold earlier rows
-    const int s0 = max(pos - block * kPage, 0);
-    const int s1 = min(pos + (c1 - c0) - block * kPage, kPage);
-    const size_t tile = (size_t)page * a.p.hkv + kh;
+    const int s0 = t.s0, s1 = t.s1;
+    const size_t tile = (size_t)t.page * a.p.hkv + kh;
     uint8_t* codes = (is_v ? a.p.v : a.p.k) + tile * kTileBytes8;
     uint8_t* scale = (is_v ? a.p.vx : a.p.kx) + tile;
-    const int row0 = c0 + block * kPage - pos;  // the packed row of slot 0
+    const int row0 = t.row0;  // the packed row of slot 0
     const float* src = (is_v ? a.v : a.k) + kh * kDim + 4 * (threadIdx.x & 31);
 
     const int old = s0 > 0 ? *scale : 0;
@@ -105,23 +69,7 @@ store_paged_kernel(StoreArgs a) {
     for (int w = 0; w < kStoreThreads / 64; ++w) amax = fmaxf(amax, s_max[w]);
     const int ex = max(e4m3_scale(amax), old);
 
-    if (s0 > 0 && ex > old) {
-        // the earlier rows, rounded to the larger scale (exact but where they leave e4m3's normal
-        // range)
-        for (int i = threadIdx.x; i < s0 * (kDim / 4); i += kStoreThreads) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
-            const uint32_t c = *w;
-            float y[4];
-            y[0] = __builtin_amdgcn_cvt_f32_fp8(c, 0);
-            y[1] = __builtin_amdgcn_cvt_f32_fp8(c, 1);
-            y[2] = __builtin_amdgcn_cvt_f32_fp8(c, 2);
-            y[3] = __builtin_amdgcn_cvt_f32_fp8(c, 3);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)  // (a NaN code keeps its sign too)
-                if ((c >> 8 * e & 0x7fu) == 0x7fu) y[e] = __uint_as_float(0x7fc00000u | (c >> 8 * e << 24 & 0x80000000u));
-            *w = e4m3_quad(y, old - ex);
-        }
-    }
+    if (s0 > 0 && ex > old) rescale_rows<kStoreThreads>(codes, s0, old - ex);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int s = 8 * j + (threadIdx.x >> 5);
@@ -715,10 +663,8 @@ int decode_runs(int hkv, int chunks) { return std::max(kSlots / (hkv * chunks), 
 int store_paged_launch(const PoolArgs& pool, const float* k, const float* v, const int* cu,
                        const int* pos, const int* table, int n, int width, int tokens,
                        hipStream_t stream) {
-    StoreArgs a{pool, k, v, cu, pos, table, n, width, tokens, 0};
-    // blocks touched: a sequence of r rows touches (r - 1) / 64 + 2 at most
-    const long long m = std::min(n, tokens);
-    const long long items = (tokens - m) / kPage + 2 * m;
+    StoreArgs a{pool, k, v, {cu, pos, table, n, width, tokens}, 0};
+    const long long items = most_blocks(n, tokens);
     // A launch of 2^32 threads or more runs fewer, without an error: at most 2^31 in each.
     const long long most = (1LL << 31) / kStoreThreads / pool.hkv;
     for (long long i = 0; i < items; i += most) {

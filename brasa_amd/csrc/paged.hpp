@@ -26,6 +26,101 @@ __device__ __forceinline__ int wave_scan(int x) {
     return x;
 }
 
+// ---- workgroup scans of 1024 threads ------------------------------------------------------------
+constexpr int kScanThreads = 1024;
+constexpr int kScanWaves = kScanThreads / 64;
+
+// exclusive sum over the workgroup's threads; `sum` is the total. s: kScanWaves ints of LDS, free
+// again after the next barrier.
+__device__ __forceinline__ int across_waves(int mine, int* s, int& sum) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __syncthreads();  // s is free
+    if (lane == 0) s[wave] = mine;
+    __syncthreads();
+    static_assert(kScanWaves == 16, "a row of 16 lanes scans the waves");
+    int w = s[lane & 15];
+    w += __builtin_amdgcn_update_dpp(0, w, 0x111, 0xF, 0xF, true);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x112, 0xF, 0xF, true);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x114, 0xF, 0xF, true);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x118, 0xF, 0xF, true);
+    sum = __builtin_amdgcn_readlane(w, 15);
+    return __builtin_amdgcn_readlane(w, wave) - mine;
+}
+__device__ __forceinline__ int block_scan(int x, int* s, int& sum) {
+    const int incl = wave_scan(x);
+    return across_waves(__builtin_amdgcn_readlane(incl, 63), s, sum) + incl - x;
+}
+// Workgroup barrier after which the workgroup's earlier global stores and atomics have reached the L2,
+// where its later atomics and device-scope loads see them.
+__device__ __forceinline__ void stores_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+__device__ __forceinline__ int ld_l2(const int* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- new rows -----------------------------------------------------------------------------------
+// Packed new rows and where they go: sequence i's rows cu[i] .. cu[i + 1] to positions pos[i], ...
+struct NewRows {
+    const int* cu;
+    const int* pos;
+    const int* table;
+    int n, width, tokens;
+};
+
+// the blocks that sequence i's new rows touch: [pos / kPage, + count)
+__device__ __forceinline__ int touched_blocks(const NewRows& a, int i, int& c0, int& c1, int& pos) {
+    c0 = min(max(a.cu[i], 0), a.tokens);
+    c1 = min(max(a.cu[i + 1], c0), a.tokens);
+    pos = a.pos[i];
+    // (a negative position, or one past what the table can hold, has no block)
+    if (c1 == c0 || pos < 0 || pos >= a.width * kPage) return 0;
+    return min((pos + (c1 - c0) - 1) / kPage, a.width - 1) - pos / kPage + 1;
+}
+
+// The item-th block of all that new rows touch: its page, its slots [s0, s1) that are new, and the
+// packed row of its slot 0. Every wave walks the sequences' block counts, 64 at a time. False: there
+// is no such block, or it has no page.
+struct TouchedBlock {
+    int page, s0, s1, row0;
+};
+__device__ __forceinline__ bool touched_block(const NewRows& a, int item, int pages, TouchedBlock& t) {
+    const int lane = threadIdx.x & 63;
+    int seq = -1, before = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 64) {
+        int c0, c1, pos, nb = 0;
+        if (i0 + lane < a.n) nb = touched_blocks(a, i0 + lane, c0, c1, pos);
+        const int incl = wave_scan(nb) + before;
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > item);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            seq = i0 + l;
+            before = __shfl(incl - nb, l);
+            break;
+        }
+        before = __shfl(incl, 63);
+    }
+    if (seq < 0) return false;  // the grid's bound is loose
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    int c0, c1, pos;
+    touched_blocks(a, seq, c0, c1, pos);
+    const int block = pos / kPage + item - before;
+    t.page = a.table[(size_t)seq * a.width + block];
+    if (t.page < 0 || t.page >= pages) return false;
+    t.s0 = max(pos - block * kPage, 0);
+    t.s1 = min(pos + (c1 - c0) - block * kPage, kPage);
+    t.row0 = c0 + block * kPage - pos;
+    return true;
+}
+
+// Blocks that new rows can touch: a sequence of r rows touches (r - 1) / 64 + 2 at most.
+inline long long most_blocks(int n, int tokens) {
+    const long long m = std::min(n, tokens);
+    return (tokens - m) / kPage + 2 * m;
+}
+
 // ---- e4m3 -----------------------------------------------------------------------------------
 // The scale byte of a block by its largest finite magnitude: the least x >= 0 with
 // amax <= 448 * 2^(x - 127). 448 = 1.75 * 2^8, so amax = m 2^a (1 <= m < 2) takes a - 8, and one
@@ -50,6 +145,25 @@ __device__ __forceinline__ uint32_t e4m3_quad(const float (&x)[4], int shift) {
         if (!(fabsf(x[e]) < INFINITY))
             c = (c & ~(0xffu << 8 * e)) | (0x7fu | (__float_as_uint(x[e]) >> 24 & 0x80u)) << 8 * e;
     return c;
+}
+
+// The codes of a block's slots [0, s0), rounded to a scale 2^-shift as large (exact but where they leave
+// e4m3's normal range), by a workgroup of THREADS.
+template <int THREADS>
+__device__ __forceinline__ void rescale_rows(uint8_t* codes, int s0, int shift) {
+    for (int i = threadIdx.x; i < s0 * (kDim / 4); i += THREADS) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
+        const uint32_t c = *w;
+        float y[4];
+        y[0] = __builtin_amdgcn_cvt_f32_fp8(c, 0);
+        y[1] = __builtin_amdgcn_cvt_f32_fp8(c, 1);
+        y[2] = __builtin_amdgcn_cvt_f32_fp8(c, 2);
+        y[3] = __builtin_amdgcn_cvt_f32_fp8(c, 3);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // (a NaN code keeps its sign too)
+            if ((c >> 8 * e & 0x7fu) == 0x7fu) y[e] = __uint_as_float(0x7fc00000u | (c >> 8 * e << 24 & 0x80000000u));
+        *w = e4m3_quad(y, shift);
+    }
 }
 
 }  // namespace brasa

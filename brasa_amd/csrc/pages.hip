@@ -15,46 +15,15 @@
 namespace brasa {
 namespace {
 
-constexpr int kPagesThreads = 1024;
-constexpr int kPagesWaves = kPagesThreads / 64;
+constexpr int kPagesThreads = kScanThreads;
+constexpr int kPagesWaves = kScanWaves;
 
-// exclusive sum over the workgroup's threads; `sum` is the total. s: kPagesWaves ints of LDS, free
-// again after the next barrier.
-__device__ __forceinline__ int across_waves(int mine, int* s, int& sum) {
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    __syncthreads();  // s is free
-    if (lane == 0) s[wave] = mine;
-    __syncthreads();
-    static_assert(kPagesWaves == 16, "a row of 16 lanes scans the waves");
-    int w = s[lane & 15];
-    w += __builtin_amdgcn_update_dpp(0, w, 0x111, 0xF, 0xF, true);
-    w += __builtin_amdgcn_update_dpp(0, w, 0x112, 0xF, 0xF, true);
-    w += __builtin_amdgcn_update_dpp(0, w, 0x114, 0xF, 0xF, true);
-    w += __builtin_amdgcn_update_dpp(0, w, 0x118, 0xF, 0xF, true);
-    sum = __builtin_amdgcn_readlane(w, 15);
-    return __builtin_amdgcn_readlane(w, wave) - mine;
-}
-__device__ __forceinline__ int block_scan(int x, int* s, int& sum) {
-    const int incl = wave_scan(x);
-    return across_waves(__builtin_amdgcn_readlane(incl, 63), s, sum) + incl - x;
-}
-// the same for truth values
+// exclusive rank of the threads for which `on` holds
 __device__ __forceinline__ int block_rank(bool on, int* s, int& sum) {
     const unsigned long long b = __builtin_amdgcn_ballot_w64(on);
     const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
     return across_waves(__builtin_popcountll(b), s, sum) + before;
 }
-// Workgroup barrier after which the workgroup's earlier global stores and atomics have reached the L2,
-// where its later atomics and device-scope loads see them.
-__device__ __forceinline__ void stores_barrier() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
-__device__ __forceinline__ int ld_l2(const int* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // dst = src by `threads` threads, this one the tid-th, eight loads in flight
 __device__ __forceinline__ void copy_ints(int* dst, const int* src, long long n, int tid, int threads) {
     if (dst == src) return;

@@ -1,0 +1,349 @@
+// Rotary positions read on the device, with one to four axes: alone on rows of any even head_dim, and
+// fused with the per-head norms of q and k and the paged 8-bit cache's writer.
+//
+// Pair i of a row, (x_i, x_{i + dim / 2}), belongs to axis a(i) and turns by the angle of that axis'
+// position p = pos[a(i)][t]: y_i = x_i c - x_{i + dim / 2} s, y_{i + dim / 2} = x_{i + dim / 2} c + x_i s,
+// with c and s the table's entries (p, i). One axis is rope_neox, bit for bit.
+//
+// Bound: HBM, 8 bytes a value in and out.
+#include "paged.hpp"
+
+namespace brasa {
+namespace {
+
+// Two bits for each pair: its axis.
+struct AxisMap {
+    uint32_t w[8];
+    int axes;
+};
+
+struct RopeArgs {
+    float* x;
+    const float* cos_t;
+    const float* sin_t;
+    const int* pos;  // [axes][tokens]
+    AxisMap map;
+    int tokens, heads, half, max_pos;  // tokens: of the whole call
+    int count;         // tokens of the launch
+    int units, spans;  // V-pair units of a row; kSpan-head spans of a token
+};
+
+// A row is left as it is where a position is negative, and becomes NaN where one is past the table.
+enum RowKind { kTurn, kLeave, kNone };
+__device__ __forceinline__ RowKind row_kind(const int* pos, int axes, int tokens, int t, int max_pos) {
+    bool leave = false, none = false;
+    for (int a = 0; a < axes; ++a) {
+        const int p = pos[(size_t)a * tokens + t];
+        leave |= p < 0;
+        none |= p >= max_pos;
+    }
+    return leave ? kLeave : none ? kNone : kTurn;
+}
+
+// A thread turns V neighbouring pairs of up to kSpan heads of a token, whose angles it loads once.
+constexpr int kSpan = 4;
+constexpr int kRopeThreads = 256;
+template <int V>
+__global__ void __launch_bounds__(kRopeThreads)
+rope_axes_kernel(RopeArgs a) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const long long idx = (long long)blockIdx.x * kRopeThreads + threadIdx.x;
+    const int unit = (int)(idx % a.units);
+    const long long ts = idx / a.units;
+    const int t = (int)(ts / a.spans), h0 = (int)(ts % a.spans) * kSpan;
+    if (t >= a.count) return;
+    const int i0 = unit * V;
+    const RowKind kind = row_kind(a.pos, a.map.axes, a.tokens, t, a.max_pos);
+    if (kind == kLeave) return;
+    float c[V], s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int i = i0 + v, axis = a.map.w[i >> 4] >> 2 * (i & 15) & 3;
+        const size_t at = (size_t)(kind == kTurn ? a.pos[(size_t)axis * a.tokens + t] : 0) * a.half + i;
+        c[v] = kind == kTurn ? a.cos_t[at] : NAN;
+        s[v] = kind == kTurn ? a.sin_t[at] : NAN;
+    }
+    float* x = a.x + ((size_t)t * a.heads + h0) * (2 * a.half) + i0;
+    const int heads = min(a.heads - h0, kSpan);
+    vec p[kSpan], q[kSpan];
+#pragma unroll
+    for (int j = 0; j < kSpan; ++j)
+        if (j < heads) {
+            p[j] = *reinterpret_cast<const vec*>(x + (size_t)j * 2 * a.half);
+            q[j] = *reinterpret_cast<const vec*>(x + (size_t)j * 2 * a.half + a.half);
+        }
+#pragma unroll
+    for (int j = 0; j < kSpan; ++j)
+        if (j < heads) {
+            vec y, z;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                y[v] = p[j][v] * c[v] - q[j][v] * s[v];
+                z[v] = q[j][v] * c[v] + p[j][v] * s[v];
+            }
+            *reinterpret_cast<vec*>(x + (size_t)j * 2 * a.half) = y;
+            *reinterpret_cast<vec*>(x + (size_t)j * 2 * a.half + a.half) = z;
+        }
+}
+
+// ---- norm, rotation and the paged writer --------------------------------------------------------
+//
+// A workgroup takes the new rows of one (block, KV head) of K or V, a row per wave and instruction, all
+// of them in registers (lane l holds values l and l + 64, a rotary pair and rms_norm's order of sums, so
+// the bits are those of rms_norm, rope_axes and store_kv_paged in sequence); the workgroups behind
+// them take rows of q.
+constexpr int kWriteWaves = 4;
+constexpr int kWriteThreads = 64 * kWriteWaves;
+constexpr int kTileRows = kPage / kWriteWaves;  // rows of a block that a wave takes
+
+struct WriteArgs {
+    PoolArgs p;  // of one layer
+    float* q;
+    float* k;
+    const float* v;
+    const float* qn;
+    const float* kn;
+    const float* cos_t;
+    const float* sin_t;
+    const int* rope_pos;  // [axes][tokens]
+    AxisMap map;
+    NewRows rows;
+    float eps;
+    int hq, max_pos;
+    long long item0;    // first block of the launch
+    long long q0;       // and first row of q
+    unsigned tiles;     // workgroups that write the cache
+};
+
+__device__ __forceinline__ float wave_sum(float p) {
+    p = row16_sum(p);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(p), __float_as_int(p), false, false);
+    p = __int_as_float(a[0]) + __int_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(p), __float_as_int(p), false, false);
+    return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+
+// This lane's angle for row t (NaN where a position is outside the table).
+__device__ __forceinline__ void angle_of(const WriteArgs& a, int t, int lane, float& c, float& s) {
+    bool there = true;
+    int mine = 0;
+    const int axis = a.map.w[lane >> 4] >> 2 * (lane & 15) & 3;
+    for (int i = 0; i < a.map.axes; ++i) {
+        const int p = a.rope_pos[(size_t)i * a.rows.tokens + t];
+        there &= p >= 0 && p < a.max_pos;
+        if (i == axis) mine = p;
+    }
+    const size_t at = (size_t)(there ? mine : 0) * (kDim / 2) + lane;
+    c = there ? a.cos_t[at] : NAN;
+    s = there ? a.sin_t[at] : NAN;
+}
+__device__ __forceinline__ void norm_turn(float& x0, float& x1, float w0, float w1, float c, float s, float eps) {
+    float p = 0.0f;
+    p += x0 * x0;
+    p += x1 * x1;
+    const float scale = 1.0f / sqrtf(wave_sum(p) / (float)kDim + eps);
+    const float a0 = (x0 * scale) * w0, b0 = (x1 * scale) * w1;
+    x0 = a0 * c - b0 * s;
+    x1 = b0 * c + a0 * s;
+}
+
+template <int RPW>  // rows of q for each wave
+__global__ void __launch_bounds__(kWriteThreads)
+norm_rope_paged_kernel(WriteArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (blockIdx.x >= a.tiles) {
+        // ---- q ------------------------------------------------------------------------------------
+        const int first = min(max(a.rows.cu[0], 0), a.rows.tokens);
+        const int last = min(max(a.rows.cu[a.rows.n], first), a.rows.tokens);
+        const long long r0 = a.q0 + ((long long)(blockIdx.x - a.tiles) * kWriteWaves + wave) * RPW;
+        float x0[RPW], x1[RPW], c[RPW], s[RPW];
+        const float w0 = a.qn[lane], w1 = a.qn[lane + 64];
+        bool on[RPW];
+#pragma unroll
+        for (int j = 0; j < RPW; ++j) {
+            const long long t = (r0 + j) / a.hq;
+            on[j] = t >= first && t < last;
+            if (!on[j]) continue;
+            const float* row = a.q + (size_t)(r0 + j) * kDim;
+            x0[j] = row[lane];
+            x1[j] = row[lane + 64];
+            angle_of(a, (int)t, lane, c[j], s[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < RPW; ++j) {
+            if (!on[j]) continue;
+            norm_turn(x0[j], x1[j], w0, w1, c[j], s[j], a.eps);
+            float* row = a.q + (size_t)(r0 + j) * kDim;
+            row[lane] = x0[j];
+            row[lane + 64] = x1[j];
+        }
+        return;
+    }
+    // ---- a block of K or V --------------------------------------------------------------------------
+    const int kh = blockIdx.x / 2 % a.p.hkv;
+    const bool is_v = blockIdx.x & 1;
+    TouchedBlock t;
+    if (!touched_block(a.rows, (int)(a.item0 + blockIdx.x / 2 / a.p.hkv), a.p.pages, t)) return;
+    const int s0 = t.s0, s1 = t.s1;
+    const size_t tile = (size_t)t.page * a.p.hkv + kh;
+    uint8_t* codes = (is_v ? a.p.v : a.p.k) + tile * kTileBytes8;
+    uint8_t* scale = (is_v ? a.p.vx : a.p.kx) + tile;
+    const int old = s0 > 0 ? *scale : 0;
+    const float* src = is_v ? a.v : a.k;
+    auto row_at = [&](int s) { return ((size_t)(t.row0 + s) * a.p.hkv + kh) * kDim + lane; };
+    float x0[kTileRows], x1[kTileRows];
+    float amax = 0.0f;
+    auto take = [&](float y0, float y1) {  // NaN and inf take no part in the scale
+        const float m0 = fabsf(y0), m1 = fabsf(y1);
+        amax = fmaxf(amax, fmaxf(m0 < INFINITY ? m0 : 0.0f, m1 < INFINITY ? m1 : 0.0f));
+    };
+#pragma unroll
+    for (int j = 0; j < kTileRows; ++j) {
+        const int s = kWriteWaves * j + wave;
+        x0[j] = x1[j] = 0.0f;
+        if (s >= s0 && s < s1) {
+            x0[j] = src[row_at(s)];
+            x1[j] = src[row_at(s) + 64];
+        }
+    }
+    if (!is_v) {
+        const float w0 = a.kn[lane], w1 = a.kn[lane + 64];
+        float c[kTileRows], sn[kTileRows];
+#pragma unroll
+        for (int j = 0; j < kTileRows; ++j) {
+            const int s = kWriteWaves * j + wave;
+            if (s >= s0 && s < s1) angle_of(a, t.row0 + s, lane, c[j], sn[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kTileRows; ++j) {
+            const int s = kWriteWaves * j + wave;
+            if (s < s0 || s >= s1) continue;
+            norm_turn(x0[j], x1[j], w0, w1, c[j], sn[j], a.eps);
+            a.k[row_at(s)] = x0[j];
+            a.k[row_at(s) + 64] = x1[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kTileRows; ++j) take(x0[j], x1[j]);
+    __shared__ float s_max[kWriteWaves];
+    __shared__ __attribute__((aligned(16))) uint8_t s_codes[kTileBytes8];
+#pragma unroll
+    for (int d = 32; d; d /= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if (lane == 0) s_max[wave] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWriteWaves; ++w) amax = fmaxf(amax, s_max[w]);
+    const int ex = max(e4m3_scale(amax), old);
+    if (s0 > 0 && ex > old) rescale_rows<kWriteThreads>(codes, s0, old - ex);
+    // through LDS, so that the codes leave as whole pieces of 16 bytes
+#pragma unroll
+    for (int j = 0; j < kTileRows; j += 2) {
+        const int s = kWriteWaves * j + wave;
+        if (s + kWriteWaves < s0 || s >= s1) continue;
+        const float y[4] = {x0[j], x1[j], x0[j + 1], x1[j + 1]};
+        const uint32_t w = e4m3_quad(y, 127 - ex);
+        uint8_t* to = s_codes + s * kDim + lane;
+        to[0] = (uint8_t)w;
+        to[64] = (uint8_t)(w >> 8);
+        to[kWriteWaves * kDim] = (uint8_t)(w >> 16);
+        to[kWriteWaves * kDim + 64] = (uint8_t)(w >> 24);
+    }
+    __syncthreads();
+    for (int i = s0 * (kDim / 16) + (int)threadIdx.x; i < s1 * (kDim / 16); i += kWriteThreads)
+        reinterpret_cast<u32x4*>(codes)[i] = reinterpret_cast<const u32x4*>(s_codes)[i];
+    // (every thread that needed the old scale has read it before the barriers above)
+    if (threadIdx.x == 0) *scale = (uint8_t)ex;
+}
+
+AxisMap pack_axes(const brasa_rope_axes_map& m, int half) {
+    AxisMap out = {};
+    out.axes = (int)m.axes;
+    for (int i = 0; i < half; ++i) out.w[i >> 4] |= (uint32_t)m.of[i] << 2 * (i & 15);
+    return out;
+}
+
+template <int V>
+int launch_rope(RopeArgs a, hipStream_t stream) {
+    a.units = a.half / V;
+    a.spans = (a.heads + kSpan - 1) / kSpan;
+    // A launch of 2^32 threads or more runs fewer, without an error: whole tokens of at most 2^31 in each.
+    const long long per_token = (long long)a.units * a.spans;
+    const int most = (int)std::min((1LL << 31) / per_token - 1, (long long)a.tokens);
+    const int tokens = a.tokens;
+    for (int t0 = 0; t0 < tokens; t0 += most) {
+        RopeArgs b = a;
+        const int count = std::min(tokens - t0, most);
+        b.x = a.x + (size_t)t0 * a.heads * 2 * a.half;
+        b.pos = a.pos + t0;
+        b.count = count;
+        const long long threads = per_token * count;
+        hipLaunchKernelGGL(rope_axes_kernel<V>, dim3((unsigned)((threads + kRopeThreads - 1) / kRopeThreads)),
+                           dim3(kRopeThreads), 0, stream, b);
+        const int st = check_launch("rope_axes_kernel");
+        if (st != BRASA_OK) return st;
+    }
+    return BRASA_OK;
+}
+
+}  // namespace
+
+int rope_axes_launch(float* x, const float* cos_t, const float* sin_t, int max_pos,
+                     const brasa_rope_axes_map& map, const int* pos, int tokens, int heads, int dim,
+                     hipStream_t stream) {
+    RopeArgs a = {};
+    a.x = x;
+    a.cos_t = cos_t;
+    a.sin_t = sin_t;
+    a.pos = pos;
+    a.map = pack_axes(map, dim / 2);
+    a.tokens = tokens;
+    a.heads = heads;
+    a.half = dim / 2;
+    a.max_pos = max_pos;
+    if (a.half % 4 == 0 && (uintptr_t)x % 16 == 0) return launch_rope<4>(a, stream);
+    return launch_rope<1>(a, stream);
+}
+
+int norm_rope_paged_launch(const PoolArgs& pool, float* q, float* k, const float* v, const float* qn,
+                           const float* kn, float eps, const float* cos_t, const float* sin_t, int max_pos,
+                           const brasa_rope_axes_map& map, const int* rope_pos, const int* cu, const int* pos,
+                           const int* table, int n, int width, int tokens, int hq, hipStream_t stream) {
+    WriteArgs a = {};
+    a.p = pool;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.qn = qn;
+    a.kn = kn;
+    a.cos_t = cos_t;
+    a.sin_t = sin_t;
+    a.rope_pos = rope_pos;
+    a.map = pack_axes(map, kDim / 2);
+    a.rows = {cu, pos, table, n, width, tokens};
+    a.eps = eps;
+    a.hq = hq;
+    a.max_pos = max_pos;
+    const long long items = width ? most_blocks(n, tokens) : 0;
+    const long long q_rows = (long long)tokens * hq;
+    // one row of q per wave while every row can have a wave at once, else four, whose loads travel together
+    const int rpw = q_rows <= 256 * 32 ? 1 : 4;
+    // A launch of 2^32 threads or more runs fewer, without an error: at most 2^30 of each kind in each.
+    const long long most = (1LL << 30) / kWriteThreads / (2 * pool.hkv), most_q = (1LL << 30) / 64 * rpw;
+    for (long long i = 0, r = 0; i < items || r < q_rows; i += most, r += most_q) {
+        a.item0 = i;
+        a.q0 = r;
+        a.tiles = (unsigned)(std::min(std::max(items - i, 0LL), most) * 2 * pool.hkv);
+        const long long rows = std::min(std::max(q_rows - r, 0LL), most_q);
+        const unsigned more = (unsigned)((rows + kWriteWaves * rpw - 1) / (kWriteWaves * rpw));
+        if (rpw == 1)
+            hipLaunchKernelGGL(norm_rope_paged_kernel<1>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
+        else
+            hipLaunchKernelGGL(norm_rope_paged_kernel<4>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
+        const int st = check_launch("norm_rope_paged_kernel");
+        if (st != BRASA_OK) return st;
+    }
+    return BRASA_OK;
+}
+
+}  // namespace brasa

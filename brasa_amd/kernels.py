@@ -13,10 +13,11 @@ Buffers are ``DeviceBuffer`` objects or raw device addresses (ints); a view at a
 """
 from __future__ import annotations
 
+import ctypes
 import enum
 from dataclasses import dataclass
 
-from ._lib import AttnShapeC, RopeTableC, check, lib
+from ._lib import AttnShapeC, BrasaError, RopeAxesC, RopeTableC, check, lib
 from .device import DeviceBuffer, Stream
 
 DECODE_CHUNK = 128
@@ -39,7 +40,6 @@ class KvType(enum.IntEnum):
     def bytes(self, n: int) -> int:
         if self is KvType.Q8_0:
             if n % KV_Q8_DIM:
-                from ._lib import RopeTableC, BrasaError
                 raise BrasaError(1, f"KV Q8: rows of {KV_Q8_DIM} values")
             return n // KV_Q8_DIM * KV_Q8_ROW
         return n * self.block_bytes() // 32
@@ -137,12 +137,58 @@ class RopeTable:
         self.sin.upload(sin)
         self.dim, self.max_pos = dim, max_pos
 
+    @classmethod
+    def view(cls, cos, sin, dim: int, max_pos: int) -> "RopeTable":
+        """A table over the caller's device arrays [max_pos, dim / 2] f32."""
+        t = cls.__new__(cls)
+        t.cos, t.sin, t.dim, t.max_pos = cos, sin, dim, max_pos
+        return t
+
     def c(self) -> RopeTableC:
-        return RopeTableC(self.cos.ptr, self.sin.ptr, self.dim, self.max_pos)
+        return RopeTableC(_ptr(self.cos), _ptr(self.sin), self.dim, self.max_pos)
 
     def free(self) -> None:
         self.cos.free()
         self.sin.free()
+
+
+class RopeAxes:
+    """The axis of each rotary pair (``brasa_rope_axes_map``; no reference counterpart): ``sections``
+    pairs for each axis, one run after another, or in turn while an axis has pairs left."""
+
+    def __init__(self, sections, interleaved: bool = False):
+        left = [int(x) for x in sections]
+        if min(left, default=-1) < 0:
+            raise BrasaError(1, f"rotary sections {list(sections)}")
+        if not interleaved:
+            of = [a for a, x in enumerate(left) for _ in range(x)]
+        else:
+            of = []
+            while any(left):
+                for a in range(len(left)):
+                    if left[a]:
+                        of.append(a)
+                        left[a] -= 1
+        self._set(of, len(left))
+
+    @classmethod
+    def of_pairs(cls, of, axes: int | None = None) -> "RopeAxes":
+        """Pair i has axis ``of[i]``."""
+        of = [int(x) for x in of]
+        m = cls.__new__(cls)
+        m._set(of, max(of, default=0) + 1 if axes is None else axes)
+        return m
+
+    def _set(self, of, axes: int):
+        if len(of) > 128 or any(not 0 <= a < 256 for a in of):
+            raise BrasaError(1, f"rotary axes of {len(of)} pairs")
+        self.axes, self.pairs = axes, len(of)
+        self._c = RopeAxesC(axes, (ctypes.c_uint8 * 128)(*of))
+
+    def c(self, dim: int) -> RopeAxesC:
+        if 2 * self.pairs != dim:
+            raise BrasaError(1, f"rotary axes of {self.pairs} pairs for head_dim {dim}")
+        return self._c
 
 
 class Kernels:
@@ -194,7 +240,6 @@ class Kernels:
                                partials_len: int | None = None) -> None:
         """Ragged batched decode: sequence i has query q[i], caches ks[i] / vs[i] and lks[i]
         keys; one launch for all of them (the reference decodes one sequence per call)."""
-        import ctypes
         n = len(lks)
         assert len(ks) == n and len(vs) == n
         karr = (ctypes.c_void_p * max(n, 1))(*[_ptr(x) for x in ks])
@@ -213,6 +258,13 @@ class Kernels:
     def rope_neox(self, x, table: RopeTable, tokens: int, heads: int, dim: int, pos0: int,
                   stream=None) -> None:
         check(lib().brasa_rope_neox(_ptr(x), table.c(), tokens, heads, dim, pos0,
+                                    _stream(stream or self.stream)))
+
+    def rope_axes(self, x, table: RopeTable, axes: RopeAxes, pos, tokens: int, heads: int, dim: int,
+                  stream=None) -> None:
+        """``rope_neox`` at device positions ``pos`` [axes, tokens] int32 (no reference counterpart):
+        pair i turns with its axis' position; a row with a negative one is left as it is."""
+        check(lib().brasa_rope_axes(_ptr(x), table.c(), axes.c(dim), _ptr(pos), tokens, heads, dim,
                                     _stream(stream or self.stream)))
 
     def qk_norm_rope_store(self, kv: KvType, qkv, norms, eps: float, table: RopeTable, dst,
@@ -275,6 +327,42 @@ class Kernels:
                                                  _ptr(lk), n, _ptr(workspace), workspace_len,
                                                  _ptr(o), int(out), hq,
                                                  _stream(stream or self.stream)))
+
+    def qk_norm_rope_store_paged(self, pool, layer: int, qkv, norms, eps: float, table: RopeTable, axes: RopeAxes,
+                                 rope_pos, cu, pos, pages, n: int, width: int, tokens: int, hq: int,
+                                 stream=None) -> None:
+        """``rms_norm`` of q's and k's heads, ``rope_axes`` and ``store_kv_paged`` in one launch: ``qkv = (q,
+        k, v)``, ``norms = (qn, kn)``, ``pages`` the table of the paged calls."""
+        q, k, v = qkv
+        qn, kn = norms
+        check(lib().brasa_qk_norm_rope_store_paged(
+            pool.c(), layer, _ptr(q), _ptr(k), _ptr(v), _ptr(qn), _ptr(kn), eps, table.c(), axes.c(pool.dim),
+            _ptr(rope_pos), _ptr(cu), _ptr(pos), _ptr(pages), n, width, tokens, hq, _stream(stream or self.stream)))
+
+    def kv_rows(self, add, lens, table, n: int, width: int, pages: int, tokens: int, cu=None, lk=None, seq=None,
+                pos=None, slot=None, stream=None) -> None:
+        """A step's maps from its requests' lengths: ``cu`` and ``lk`` of the sequences, sequence, position
+        and slot of each packed row (outputs that are None are left out)."""
+        check(lib().brasa_kv_rows(_ptr(add), _ptr(lens), _ptr(table), n, width, pages, tokens, _ptr(cu), _ptr(lk),
+                                  _ptr(seq), _ptr(pos), _ptr(slot), _stream(stream or self.stream)))
+
+    def kv_pages_shared(self, table, lens, group, groups: int, n: int, width: int, pages: int, prefix,
+                        stream=None) -> None:
+        check(lib().brasa_kv_pages_shared(_ptr(table), _ptr(lens), _ptr(group), groups, n, width, pages, _ptr(prefix),
+                                          _stream(stream or self.stream)))
+
+    def attention_paged_plan(self, cu, pos, group, prefix, groups: int, n: int, width: int, tokens: int, hq: int,
+                             hkv: int, workspace, workspace_len: int, stream=None) -> None:
+        """The work of a step's ``attention_paged`` calls, laid out on the device into ``workspace``."""
+        check(lib().brasa_attention_paged_plan(_ptr(cu), _ptr(pos), _ptr(group), _ptr(prefix), groups, n, width,
+                                               tokens, hq, hkv, _ptr(workspace), workspace_len,
+                                               _stream(stream or self.stream)))
+
+    def attention_paged(self, q, pool, layer: int, table, n: int, width: int, tokens: int, workspace,
+                        workspace_len: int, o, hq: int, out: OutDType = OutDType.F32, stream=None) -> None:
+        """Attention of a step's new rows over the paged cache, on the plan in ``workspace``."""
+        check(lib().brasa_attention_paged(_ptr(q), pool.c(), layer, _ptr(table), width, n, tokens, _ptr(workspace),
+                                          workspace_len, _ptr(o), int(out), hq, _stream(stream or self.stream)))
 
     def kv_pages_fork(self, parent, table, lens, ref, table_out, lens_out, ref_out, n: int,
                       width: int, pages: int, stream=None) -> None:

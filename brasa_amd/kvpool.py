@@ -28,6 +28,11 @@ def kv_pages_workspace_len(pages: int, n: int, width: int) -> int:
     return int(lib().brasa_kv_pages_workspace_len(pages, n, width))
 
 
+def attention_paged_workspace_len(n: int, groups: int, tokens: int, hq: int, hkv: int) -> int:
+    """Bytes of workspace of ``attention_paged_plan`` and the ``attention_paged`` calls on it."""
+    return int(lib().brasa_attention_paged_workspace_len(n, groups, tokens, hq, hkv))
+
+
 class KvPool:
     """Codes and scale bytes of ``pages`` pages in each of ``layers`` layers."""
 

@@ -305,6 +305,28 @@ int brasa_qk_norm_rope_store(int kv, float* q, float* k, const float* v, const f
                              void* k_dst, void* v_dst, brasa_attn_shape shape, void* stream);
 
 /*
+ * Rotary positions with several axes (time, height and width of images and video; one axis for text), read on
+ * the device. Pair i of a head, (x[i], x[i + dim / 2]), turns with axis of[i] < axes: of[i] is 0 throughout for
+ * plain text, one run for each axis where a model cuts its pairs into sections, the axes in turn where it
+ * interleaves them. 1 to 4 axes, dim up to 256.
+ */
+#define BRASA_ROPE_AXES 4
+typedef struct brasa_rope_axes_map {
+    size_t axes;
+    uint8_t of[128];
+} brasa_rope_axes_map;
+
+/*
+ * RoPE-NeoX in place on x [tokens, heads, dim] (f32), with the positions pos [axes, tokens] (device int32): y[i]
+ * = x[i] c - x[i + dim / 2] s, y[i + dim / 2] = x[i + dim / 2] c + x[i] s, where c and s are table entry (pos[of[i]][t], i).
+ * A row with a negative position in any axis is left as it is (the rows behind a step's last, brasa_kv_rows);
+ * one with a position past the table becomes NaN. With one axis the bits are brasa_rope_neox's at those
+ * positions. dim == table.dim, even, 16-byte aligned rows are fastest but not required.
+ */
+int brasa_rope_axes(float* x, brasa_rope_table_view table, brasa_rope_axes_map axes, const int32_t* pos,
+                    size_t tokens, size_t heads, size_t dim, void* stream);
+
+/*
  * No counterpart in the reference. Returns the library's per-stream state to its initial
  * condition: the stream -> counter slot assignments (decode and prefill split merges) and the
  * ownership of the fixed prefill workspace. Call it only while no call of this library is in
@@ -421,9 +443,9 @@ size_t brasa_kv_pool_bytes(size_t layers, size_t pages, size_t hkv, size_t dim);
 
 /*
  * The tables, lengths and counts of the calls below are DEVICE arrays of int32, so a captured graph of
- * these calls may be replayed while its sequences grow, fork or end. (The rotary calls,
- * brasa_rope_neox and brasa_qk_norm_rope_store, take one position per call from the host: rotate the
- * q and k of such a graph by positions read on the device, or launch them outside of it.)
+ * these calls may be replayed while its sequences grow, fork or end. (brasa_rope_neox and
+ * brasa_qk_norm_rope_store take one position per call from the host; brasa_rope_axes and
+ * brasa_qk_norm_rope_store_paged read theirs on the device.)
  * table: [n, width] page ids, row i the pages of sequence i in order (position p in entry p / 64), -1
  * where it has none. Ids out of [0, pages) are never followed. n up to 65536, n * width up to 2^30.
  */
@@ -463,6 +485,74 @@ int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t laye
                                  const int32_t* table, size_t width, const int32_t* lk, size_t n,
                                  void* workspace, size_t workspace_len, void* o, int o_dtype,
                                  size_t hq, void* stream);
+
+/*
+ * brasa_rms_norm of the heads of q and k, brasa_rope_axes and brasa_store_kv_paged in one launch, with their bits: q
+ * [tokens, hq, 128] and k [tokens, hkv, 128] (f32, in place) are normalised with q_norm / k_norm [128] and eps
+ * and turned by rope_pos [axes, tokens]; k (turned) and v (as given) go into the pages as in
+ * brasa_store_kv_paged. Rows of q from cu[0] to cu[n], and rows of k whose position has a page; the others
+ * are left as they are. (A rotary position outside the table, a negative one too, gives NaN here.) Requires
+ * table.dim == 128; rows of q, k and v 16-byte aligned.
+ */
+int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, float* k, const float* v,
+                                   const float* q_norm, const float* k_norm, float eps,
+                                   brasa_rope_table_view table, brasa_rope_axes_map axes,
+                                   const int32_t* rope_pos, const int32_t* cu, const int32_t* pos,
+                                   const int32_t* pages, size_t n, size_t width, size_t tokens, size_t hq,
+                                   void* stream);
+
+/*
+ * The maps of a step's packed rows from its requests' lengths: sequence i holds len[i] positions and adds add[i]
+ * (none where add[i] <= 0 or len[i] < 0). cu [n + 1]: its rows are cu[i] .. cu[i + 1]; lk [n]: its length after the step;
+ * and for each row t < tokens its sequence seq[t], position pos[t] and slot[t] = page * 64 + position % 64 of
+ * its page in the table, -1 where that is not there. Rows behind the last sequence's get -1 in all three; rows past
+ * `tokens` are cut off (cu and lk too). table as above (`pages`: the pool's). Any output may be NULL; lk must not
+ * be len, nor cu add.
+ */
+int brasa_kv_rows(const int32_t* add, const int32_t* len, const int32_t* table, size_t n, size_t width,
+                  size_t pages, size_t tokens, int32_t* cu, int32_t* lk, int32_t* seq, int32_t* pos,
+                  int32_t* slot, void* stream);
+
+/*
+ * The positions that groups of sequences share: group g is sequences group[g] .. group[g + 1] (device, [groups + 1]),
+ * and prefix[g] = 64 times the number of leading pages that all of its sequences with len[i] > 0 name alike and fill
+ * (64 positions of each page at least; as forks of one sequence or requests behind one system prompt do); 0
+ * for a group with fewer than two such sequences. Bounds of group outside [0, n] or out of order are clamped.
+ */
+int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_t* group, size_t groups,
+                          size_t n, size_t width, size_t pages, int32_t* prefix, void* stream);
+
+/*
+ * Attention of new rows over the paged cache, theirs included (store them first): row t of sequence i (cu[i] <= t <
+ * cu[i + 1], at position pos[i] + t - cu[i]) over positions 0 .. its own in `layer`. One row for each sequence (a decode
+ * step), a few (drafts under verification) or many (a prompt, or a chunk of one behind what is cached) take the
+ * same call. q: [tokens, hq, 128] f32, o: [tokens, hq, 128] in o_dtype, sums in f32; q and the weights are contracted as two
+ * f16 halves (22 bits). Any hq a multiple of hkv.
+ *
+ * The plan of a step is laid out on the device by brasa_attention_paged_plan, once for all layers:
+ * sequences group[g] .. group[g + 1] (as in brasa_kv_pages_shared) are taken to name the same pages in their first
+ * prefix[g] positions (rounded down to whole pages; not checked: they may be brasa_kv_pages_shared's or a server's
+ * own), and those pages are read and multiplied once for all rows of the group, but for sequences with too
+ * many rows to gain from it or with positions below the prefix. groups == 0: none are shared. The calls that
+ * follow take the plan's workspace and its n, width, tokens, hq and hkv; one whose sizes are not the plan's, or
+ * without a plan, fills o with NaN.
+ *
+ * Rows outside all sequences are left as they were in o. A sequence with a negative pos, one past the table, or a
+ * page id out of range among the pages a row sees gives NaN in those rows. Codes behind a row's own
+ * position never reach it, whatever they hold. Values of cu and group out of order are raised to the largest before
+ * them. The result bits depend on the lengths of all sequences, not on timing.
+ *
+ * workspace: brasa_attention_paged_workspace_len bytes, 256-byte aligned, any contents: the plan, then the partial
+ * sums of one call at a time. Calls that may run at the same time need workspaces (and plans) of their own. q and o
+ * 16-byte aligned; tokens * hq up to 2^29.
+ */
+size_t brasa_attention_paged_workspace_len(size_t n, size_t groups, size_t tokens, size_t hq, size_t hkv);
+int brasa_attention_paged_plan(const int32_t* cu, const int32_t* pos, const int32_t* group,
+                               const int32_t* prefix, size_t groups, size_t n, size_t width, size_t tokens,
+                               size_t hq, size_t hkv, void* workspace, size_t workspace_len, void* stream);
+int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, const int32_t* table, size_t width,
+                          size_t n, size_t tokens, void* workspace, size_t workspace_len, void* o, int o_dtype,
+                          size_t hq, void* stream);
 
 /*
  * Forks and frees: row i of table_out / len_out becomes row parent[i] of table / len (a beam
