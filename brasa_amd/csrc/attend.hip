@@ -6,14 +6,14 @@
 // + l2 2^(m2 - m), and acc alike. So a row's positions may be cut anywhere, and the rows of several
 // sequences may stand together in one product where they read the same pages.
 //
-// A column is a (row, query head) of a KV head; a tile is up to 128 columns over a run of pages of one
-// table row. A group's rows (of sequences with fewer than 128 columns: more fill tiles of their own)
+// A column is a (row, query head) of a KV head; a tile is up to 32 columns over a run of pages of one table
+// row, the work of one wave. The rows of a group's sequences that have too few for a tile of their own
 // make prefix tiles over the shared pages, and each sequence's rows tiles over its other pages. All
-// tiles of a KV head stand in one line by their cost, and workgroup w takes the w-th equal run of
-// it, so that every CU has the same work whatever the lengths, which only the device knows. The plan
-// kernel lays the line out once a step, every layer's launch walks it; a tile that a run's border
-// cuts, or whose sequence has a prefix tile, leaves (m, l, acc) in the workspace and a second
-// launch joins them in order, so the result does not depend on timing.
+// tiles of a KV head stand in one line by their pages, and wave w takes the w-th equal run of it, so
+// that every CU has the same work whatever the lengths, which only the device knows. The plan kernel
+// lays the line out once a step, every layer's launch walks it; a tile that a run's border cuts, or
+// whose sequence has a prefix tile, leaves (m, l, acc) in the workspace and a second launch joins them
+// in order, so the result does not depend on timing.
 #include <climits>
 
 #include "paged.hpp"
@@ -27,15 +27,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kCols = 32;                    // columns of a wave
-constexpr int kTileCols = kCols * kWaves;    // of a tile
-constexpr int kSlots = 512;                  // workgroups of a launch: two per CU
-constexpr int kMergeCols = 16;               // columns of a merge entry
-constexpr int kPad = kDim + 4;               // floats of a column in LDS: stores of 16 bytes spread over the banks
-
-// Cost of a page by the waves that share its tile's columns: one, two or four column groups.
-__host__ __device__ constexpr int page_cost(int groups) { return groups == 1 ? 2 : groups == 2 ? 3 : 4; }
-constexpr int kMinRun = 8 * page_cost(1);  // least cost of a run: two pages for each wave
+constexpr int kCols = 32;     // columns of a tile
+constexpr int kRuns = 2048;   // waves of a launch: two per SIMD
+constexpr int kOver = 2;      // pages whose time a tile costs beside its own
+constexpr int kMinRun = 4;    // least length of a run
+constexpr int kFewParts = 8;  // parts of a column that one wave joins
 
 struct Tile {
     int seq;          // table row whose pages it reads
@@ -44,11 +40,11 @@ struct Tile {
     int b0, b1;       // pages
     int pos0;         // own tile: position of the sequence's first new row
     int kind;         // kPrefix, kDirect, kBad
-    long long start;  // in the line
-    int cost;         // of a page
+    long long start;  // of its pages in the line
     int base, parts;  // partials: columns base + part * cols + column; parts of it
     int run0;         // run of its first part
-    int ptile, pcol;  // prefix tile and column in the group where its first column continues; -1: none
+    int ptile, pcol;  // prefix tile and its column where the tile's first column continues; -1: none
+    int unused;
 };
 static_assert(sizeof(Tile) == 64, "a tile is one line");
 enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4 };
@@ -86,13 +82,13 @@ Layout layout(int n, int groups, int tokens, int hq, int hkv) {
     Layout l;
     const long long g = hq / hkv, cols = (long long)tokens * g, seqs = std::min(n, tokens);
     // columns of sequences that may share: each has fewer than a tile's
-    const long long shared = groups ? std::min(cols, seqs * (kTileCols - 1)) : 0;
-    l.runs = std::max(kSlots / hkv, 1);
-    l.max_tiles = (int)(seqs + cols / kTileCols + (groups ? std::min((long long)groups, seqs) + shared / kTileCols : 0));
-    // entries: all shared columns, and eight for each tile that a run's border cuts
-    l.max_merges = (int)(shared / kMergeCols + (groups ? seqs : 0) + (long long)l.runs * (kTileCols / kMergeCols));
+    const long long shared = groups ? std::min(cols, seqs * (kCols - 1)) : 0;
+    l.runs = std::max(kRuns / hkv, kWaves);
+    l.max_tiles = (int)(seqs + cols / kCols + (groups ? std::min((long long)groups, seqs) + shared / kCols : 0));
+    // all shared columns, and those of the tiles that a run's border cuts
+    l.max_merges = (int)(shared + (long long)l.runs * std::min((long long)kCols, cols));
     // shared columns once in each of the two tiles, and for each border a tile's columns once or twice
-    l.cap = 2 * shared + 2LL * l.runs * std::min((long long)kTileCols, cols);
+    l.cap = 2 * shared + 2LL * l.runs * std::min((long long)kCols, cols);
     size_t at = up256(sizeof(Header));
     auto take = [&](size_t bytes) {
         const size_t a = at;
@@ -186,8 +182,6 @@ __device__ __forceinline__ long long div_by(long long x, long long d, double inv
     q += (q + 1) * d <= x;
     return q;
 }
-__device__ __forceinline__ int col_groups(int cols) { return cols <= kCols ? 1 : cols <= 2 * kCols ? 2 : 4; }
-
 __global__ void __launch_bounds__(kScanThreads)
 attend_plan_kernel(PlanArgs a) {
     __shared__ long long s_scan[kScanWaves];
@@ -229,7 +223,7 @@ attend_plan_kernel(PlanArgs a) {
         s.group = -1;
         int cols = 0;
         // (whose rows all stand behind the prefix, and do not fill a tile)
-        if (a.groups && s.rows > 0 && s.rows < kTileCols && s.rows * per_row < kTileCols) {
+        if (a.groups && s.rows > 0 && s.rows < kCols && s.rows * per_row < kCols) {
             int lo = 0, hi = a.groups;  // the last group that starts at or before i
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
@@ -284,8 +278,8 @@ attend_plan_kernel(PlanArgs a) {
     for (int e0 = 0; e0 < entries; e0 += kScanThreads) {
         const int e = e0 + tid;
         int tiles = 0, col0;
-        if (e < a.groups) tiles = (group_cols(e, col0) + kTileCols - 1) / kTileCols;
-        else if (e < entries) tiles = (int)(((long long)ld_l2(&a.seq[e - a.groups].rows) * per_row + kTileCols - 1) / kTileCols);
+        if (e < a.groups) tiles = (group_cols(e, col0) + kCols - 1) / kCols;
+        else if (e < entries) tiles = (int)(((long long)ld_l2(&a.seq[e - a.groups].rows) * per_row + kCols - 1) / kCols);
         int sum;
         const int at = ntiles + block_scan(tiles, s_scan32, sum);
         ntiles += sum;
@@ -302,7 +296,7 @@ attend_plan_kernel(PlanArgs a) {
             else hi = mid;
         }
         Tile t;
-        t.col0 = (at - ld_l2(a.first + lo)) * kTileCols;
+        t.col0 = (at - ld_l2(a.first + lo)) * kCols;
         t.ptile = t.pcol = -1;
         if (lo < a.groups) {
             int col0;
@@ -310,7 +304,7 @@ attend_plan_kernel(PlanArgs a) {
             t.kind = kPrefix;
             t.seq = ld_l2(&a.grp[lo].lead);
             t.row0 = col0 / per_row;
-            t.cols = min(cols - t.col0, kTileCols);
+            t.cols = min(cols - t.col0, kCols);
             t.b0 = 0;
             t.b1 = prefix_pages(lo);
             t.pos0 = 0;
@@ -320,7 +314,7 @@ attend_plan_kernel(PlanArgs a) {
             t.kind = s.pos < 0 ? kBad : 0;
             t.seq = i;
             t.row0 = s.c0;
-            t.cols = (int)min((long long)s.rows * per_row - t.col0, (long long)kTileCols);
+            t.cols = (int)min((long long)s.rows * per_row - t.col0, (long long)kCols);
             t.b0 = s.group >= 0 ? prefix_pages(s.group) : 0;
             // (a sequence without a place gets one page, not read, whose tile writes NaN)
             const int last = (t.col0 + t.cols - 1) / per_row;
@@ -329,11 +323,11 @@ attend_plan_kernel(PlanArgs a) {
             if (s.group >= 0) {
                 int gcol0 = 0;
                 group_cols(s.group, gcol0);
-                t.ptile = ld_l2(a.first + s.group) + (s.scol - gcol0) / kTileCols;
-                t.pcol = (s.scol - gcol0) % kTileCols;
+                t.ptile = ld_l2(a.first + s.group) + (s.scol - gcol0) / kCols;
+                t.pcol = (s.scol - gcol0) % kCols;
             }
         }
-        t.cost = page_cost(col_groups(t.cols));
+        t.unused = 0;
         return t;
     };
 
@@ -342,7 +336,7 @@ attend_plan_kernel(PlanArgs a) {
     Tile t = {};
     for (int i = tid; i < ntiles; i += kScanThreads) {
         t = make_tile(i);
-        mine += (long long)(t.b1 - t.b0) * t.cost;
+        mine += kOver + t.b1 - t.b0;
     }
     block_scan64(mine, s_scan, total);
     const long long size = max((total + a.runs - 1) / a.runs, (long long)kMinRun);
@@ -354,9 +348,9 @@ attend_plan_kernel(PlanArgs a) {
         const int at = t0 + tid;
         const bool on = at < ntiles;
         if (on && ntiles > kScanThreads) t = make_tile(at);  // (else it is at hand)
-        const long long len = on ? (long long)(t.b1 - t.b0) * t.cost : 0;
+        const long long len = on ? t.b1 - t.b0 : 0;
         long long sum;
-        t.start = line + block_scan64(len, s_scan, sum);
+        t.start = line + block_scan64(on ? len + kOver : 0, s_scan, sum) + kOver;
         line += sum;
         t.run0 = (int)div_by(t.start, size, inv);
         const int last = on ? (int)div_by(t.start + len - 1, size, inv) : 0;
@@ -367,11 +361,14 @@ attend_plan_kernel(PlanArgs a) {
         cols += sum;
         if (!on) continue;
         a.tile[at] = t;
-        for (int w = t.run0 + (t.start > t.run0 * size); w <= last; ++w) a.run_tile[w] = at;
+        // the runs that start in it, or in the pages' worth before it
+        for (int w = (int)div_by(t.start - kOver + size - 1, size, inv); w <= last; ++w) a.run_tile[w] = at;
         if (!(t.kind & (kPrefix | kDirect))) {
-            const int many = (t.cols + kMergeCols - 1) / kMergeCols;
+            int parts = t.parts;
+            if (t.ptile >= 0) parts += (int)div_by(t.b0, size, inv) + 1;  // (about: the prefix tile's)
+            const int each = parts > kFewParts ? 1 : kWaves, many = (t.cols + each - 1) / each;
             const int e = atomicAdd(&s_merges, many);
-            for (int j = 0; j < many; ++j) a.merge[e + j] = at * (kTileCols / kMergeCols) + j;
+            for (int j = 0; j < many; ++j) a.merge[e + j] = (at * kCols + j * each) * 2 + (each == 1);
         }
     }
     __syncthreads();
@@ -400,8 +397,7 @@ attend_plan_kernel(PlanArgs a) {
 // S^T = K Q^T on 32x32x16 f16 MFMAs, once with the hi and once with the lo halves of q (22 bits
 // together). S^T's layout is the B operand of O^T += V^T P^T, P in hi and lo halves again; V's operand
 // needs eight keys of one dim in a lane, which byte permutes pair up from four dims of each key
-// before the conversion. The waves of a tile take a column group each, or where it has fewer than four
-// groups share its pages; those waves' sums are joined through LDS.
+// before the conversion. No wave waits for another.
 struct AttendArgs {
     const uint8_t* ws;
     size_t ws_len;
@@ -411,6 +407,17 @@ struct AttendArgs {
     void* o;
     int n, width, tokens, hq, per_row, o_f16;
 };
+// Memory that no kernel of the launch writes, read through the scalar cache: uniform values that arrive
+// without a place among the vector loads in flight.
+template <typename T>
+using Scalar = const __attribute__((address_space(4))) T*;
+template <typename T>
+__device__ __forceinline__ Scalar<T> scalar(const T* p) { return (Scalar<T>)(uintptr_t)p; }
+// the byte at p + i (its aligned word is read)
+__device__ __forceinline__ int scalar_byte(const uint8_t* p, size_t i) {
+    const uintptr_t at = (uintptr_t)(p + i);
+    return (int)(*(Scalar<uint32_t>)(at & ~(uintptr_t)3) >> 8 * (at & 3) & 0xffu);
+}
 // The workspace's header and the parts it names.
 struct Plan {
     Header head;
@@ -437,6 +444,16 @@ __device__ __forceinline__ Plan load_plan(const AttendArgs& a) {
     return p;
 }
 
+__device__ __forceinline__ Tile load_tile(const Tile* p) {
+    union {
+        Tile t;
+        uint32_t w[sizeof(Tile) / 4];
+    } u;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Tile) / 4); ++i) u.w[i] = ((Scalar<uint32_t>)(uintptr_t)p)[i];
+    return u.t;
+}
+
 __device__ __forceinline__ f32x16 mfma32(half8v a, half8v b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
@@ -453,7 +470,9 @@ __device__ __forceinline__ half8v join(half2v a, half2v b, half2v c, half2v d) {
 // x and y as f16 halves hi + lo (up to 2^-22 of each)
 __device__ __forceinline__ void split(float x, float y, half2v& hi, half2v& lo) {
     hi = half2v{(_Float16)x, (_Float16)y};
-    lo = half2v{(_Float16)(x - (float)hi.x), (_Float16)(y - (float)hi.y)};
+    // (kept as one register: the remainders are then mixed FMAs of it, not conversions made again)
+    asm volatile("" : "+v"(hi));
+    lo = half2v{(_Float16)fmaf((float)hi.x, -1.0f, x), (_Float16)fmaf((float)hi.y, -1.0f, y)};
 }
 // 0x80 in the places of a word's NaN codes
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
@@ -470,10 +489,11 @@ __device__ __forceinline__ float sum_h(float x) {
 __device__ __forceinline__ float part_weight(float m, float top) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 }
-__device__ __forceinline__ void write_o(const AttendArgs& a, size_t at, f32x4 x, float l) {
+// x times 1 / l, in o's type
+__device__ __forceinline__ void write_o(const AttendArgs& a, size_t at, f32x4 x, float inv) {
     f32x4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = x[e] / l;
+    for (int e = 0; e < 4; ++e) y[e] = x[e] * inv;
     if (a.o_f16) {
         u32x2 w = {f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
         *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + at) = w;
@@ -507,8 +527,7 @@ __device__ __forceinline__ void add_pv(const uint32_t (&v)[16], const half8v (&h
 
 __global__ void __launch_bounds__(kThreads, 2)
 attend_kernel(AttendArgs a) {
-    __shared__ __attribute__((aligned(16))) float s_acc[kWaves][kCols][kPad];
-    __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
+    __shared__ __attribute__((aligned(16))) int s_nan[kWaves][kDim];  // first key with a NaN value, for each dim
 
     const Plan plan = load_plan(a);
     if (!plan.fits) return;
@@ -516,27 +535,21 @@ attend_kernel(AttendArgs a) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
-    const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv;
+    const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv * kWaves + wave;
     const long long lo = run * head.size, end = min(lo + head.size, head.total);
-    if (lo >= end) return;
+    if (run >= head.runs || lo >= end) return;
 
-    for (int ti = plan.run_tile[run]; ti < head.tiles; ++ti) {
-        const Tile t = plan.tile[ti];
+    for (int ti = scalar(plan.run_tile)[run]; ti < head.tiles; ++ti) {
+        const Tile t = load_tile(plan.tile + ti);
         if (t.start >= end) break;
         // ---- this run's pages of the tile ------------------------------------------------------------
-        const int len = (t.b1 - t.b0) * t.cost;
-        const int from = (int)max(lo - t.start, 0LL), to = (int)min(end - t.start, (long long)len);
-        const int p0 = t.b0 + (from + t.cost - 1) / t.cost;
-        const int p1 = to == len ? t.b1 : t.b0 + (to + t.cost - 1) / t.cost;
+        const int p0 = t.b0 + (int)max(lo - t.start, 0LL), p1 = min(t.b0 + (int)min(end - t.start, (long long)INT_MAX / 2), t.b1);
+        if (p0 >= p1) continue;  // (its pages are the next run's)
         const bool prefix = t.kind & kPrefix, nowhere = t.kind & kBad;
-        // the wave's column group, and which of the pages are its
-        const int groups = t.cols <= kCols ? 1 : t.cols <= 2 * kCols ? 2 : 4;
-        const int cg = wave & (groups - 1), phase = wave / groups, step = kWaves / groups;
-        const int cols = min(t.cols - kCols * cg, kCols);  // of this wave (none: at most 0)
-        const int* ids = a.table + (size_t)t.seq * a.width;
+        const Scalar<int> ids = scalar(a.table + (size_t)t.seq * a.width);
 
         // ---- Q: hi and lo halves of q / sqrt(128) * log2 e, each column's exponent taken out -----------
-        const int col = t.col0 + min(kCols * cg + c, t.cols - 1);  // (lanes past the last column repeat it)
+        const int col = t.col0 + min(c, t.cols - 1);  // (lanes past the last column repeat it)
         const int local = col / a.per_row;
         const int row = prefix ? plan.rows[t.row0 + local] : t.row0 + local;
         const int head_of = kh * a.per_row + col - local * a.per_row;
@@ -587,7 +600,7 @@ attend_kernel(AttendArgs a) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-        int vref = 0;     // acc stands in units of 2^(vref - 127); 0: nothing yet
+        int vref = 0;     // acc stands in units of 2^(vref - 127)
         bool bad = nowhere;
 
         u32x4 kw[4];      // key 32 half + c, dims 32 i + 16 h .. + 16
@@ -609,23 +622,25 @@ attend_kernel(AttendArgs a) {
             return (size_t)(there ? id : 0) * a.p.hkv + kh;
         };
 
-        const int first = p0 + phase;
-        if (!nowhere && cols > 0 && first < p1) {
-            int page = first, half = 0;
+        if (!nowhere) {
+            int page = p0, half = 0;
             bool there, there_next = true;
             size_t tile = tile_of(ids[page], there), tile_next = tile;
             load_k(tile, 0);
             load_v(tile, 0);
-            int kx = a.p.kx[tile], vx = a.p.vx[tile], kx_next = kx, vx_next = vx;
+            int kx = scalar_byte(a.p.kx, tile), vx = scalar_byte(a.p.vx, tile), kx_next = kx, vx_next = vx;
+            vref = vx;
+            int id = page + 1 < p1 ? ids[page + 1] : 0;  // of the page after this one
             while (true) {
                 const int k0 = page * kPage + 32 * half;
                 // where the next half page is
-                const int page_next = half ? page + step : page;
+                const int page_next = half ? page + 1 : page;
                 const bool more = page_next < p1;
                 if (half && more) {
-                    tile_next = tile_of(ids[page_next], there_next);
-                    kx_next = a.p.kx[tile_next];
-                    vx_next = a.p.vx[tile_next];
+                    tile_next = tile_of(id, there_next);
+                    kx_next = scalar_byte(a.p.kx, tile_next);
+                    vx_next = scalar_byte(a.p.vx, tile_next);
+                    id = page_next + 1 < p1 ? ids[page_next + 1] : 0;
                 }
                 // ---- scores: key k0 + 8 q + 4 h + r of column c, in units of log2 and of 2^(qx + kx - 127)
                 f32x16 s;
@@ -643,7 +658,7 @@ attend_kernel(AttendArgs a) {
                 __builtin_amdgcn_sched_barrier(0);
                 // (past the clamp every score is 0, or so far from the next that one key takes all)
                 const float sc = ldexpf(1.0f, min(max(qx + kx - 127, -126), 127));
-                if (!there && limit >= page * kPage) lsum = NAN;
+                if (!there) lsum = limit >= page * kPage ? NAN : lsum;
                 const bool edge = k0 + 31 > lim0;  // some column does not see all of these keys
                 bool odd = false;                  // V holds NaN codes among them
                 if (edge) {
@@ -671,24 +686,27 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[i] *= alpha;
                 }
-                // a column that has seen no key yet: its scores are all -inf, and p 0
-                const float mb = m_used == -INFINITY ? 0.0f : 7.0f - m_used;
-                float p[16];
+                // V's scale: acc's unit grows with it, and where it is smaller p shrinks, through its exponent
+                int less = 0;
+                if (vx > vref) {
+                    const float f = ldexpf(1.0f, vref - vx);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i] *= f;
+                    vref = vx;
+                } else {
+                    less = min(vref - vx, 100);
+                }
+                // (a column that has seen no key yet: its scores are all -inf, and p 0)
+                const float mb = m_used == -INFINITY ? 0.0f : 7.0f - (float)less - m_used;
+                float p[16], psum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sc, mb));
-                    lsum += p[i];
+                    psum += p[i];
                 }
-                // V's scale: acc's unit grows with it, and p shrinks where it is smaller
-                if (vx > vref) {
-                    if (vref) {
-                        const float f = ldexpf(1.0f, vref - vx);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[i] *= f;
-                    }
-                    vref = vx;
-                } else if (vx < vref) {
-                    const float f = ldexpf(1.0f, max(vx - vref, -126));
+                lsum = fmaf(psum, ldexpf(1.0f, less), lsum);
+                if (vref - vx > 100) {
+                    const float f = ldexpf(1.0f, max(vx - vref + 100, -126));
 #pragma unroll
                     for (int i = 0; i < 16; ++i) p[i] *= f;
                 }
@@ -702,31 +720,27 @@ attend_kernel(AttendArgs a) {
                     pl[st] = join(w[0], w[1], w[2], w[3]);
                 }
                 if (odd) {
-                    // NaN values that some columns see and others do not: 0 in the product, and a second
-                    // one of ones in their places with the columns that see them
+                    // NaN values that some columns see and others do not: 0 in the product, and NaN for the
+                    // columns at or past the first such key of the dim
+                    int low[4] = {INT_MAX, INT_MAX, INT_MAX, INT_MAX};
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        f32x16 count;
+                    for (int i = 15; i >= 0; --i) {
+                        const uint32_t w = nan_codes(vw[i]);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) count[j] = 0.0f;
-#pragma unroll
-                        for (int st = 0; st < 2; ++st) {
-                            half8v there, see;
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int key = k0 + 8 * (2 * st + (j >> 2)) + 4 * h + (j & 3);
-                                there[j] = nan_codes(vw[8 * st + j]) >> 8 * d & 0x80u ? (_Float16)1.0f : (_Float16)0.0f;
-                                see[j] = key <= limit ? (_Float16)1.0f : (_Float16)0.0f;
-                            }
-                            count = mfma32(there, see, count);
-                        }
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (count[j] > 0.0f) acc[d][j] = NAN;
-                        __builtin_amdgcn_sched_barrier(0);
+                        for (int d = 0; d < 4; ++d)
+                            if (w >> 8 * d & 0x80u) low[d] = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                        vw[i] &= ~((w >> 7) * 0xffu);
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) vw[i] &= ~((nan_codes(vw[i]) >> 7) * 0xffu);
+                    for (int d = 0; d < 4; ++d) {
+                        const auto b = __builtin_amdgcn_permlane32_swap(low[d], low[d], false, false);
+                        s_nan[wave][4 * c + d] = min((int)b[0], (int)b[1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+                            if (s_nan[wave][4 * (8 * (i >> 2) + 4 * h + (i & 3)) + d] <= limit) acc[d][i] = NAN;
                 }
                 add_pv(vw, ph, pl, acc);
                 __builtin_amdgcn_sched_barrier(0);
@@ -747,73 +761,36 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] *= unit;
 
-        // ---- out: to o, or to the parts --------------------------------------------------------------
-        const bool direct = t.kind & kDirect;
-        const size_t part = (size_t)kh * head.at.cap + t.base + (size_t)(run - t.run0) * t.cols;
-        if (step == 1) {
-            if (c < cols) {
-                // the lane holds dims 4 (8 q + 4 h + r) + t of its column
-                const size_t at = direct ? ((size_t)row * a.hq + head_of) * kDim : (part + kCols * cg + c) * kDim;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const f32x4 x = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-                    const size_t d = at + 4 * (8 * (i >> 2) + 4 * h + (i & 3));
-                    if (direct) write_o(a, d, x, lsum);
-                    else *reinterpret_cast<f32x4*>(plan.acc + d) = x;
-                }
-                if (!direct && h == 0)
-                    *reinterpret_cast<f32x2*>(plan.ml + 2 * (part + kCols * cg + c)) = f32x2{m_used, lsum};
-            }
-            continue;
-        }
-        __syncthreads();  // the LDS is free
-        if (c < cols) {
-            if (h == 0) {
-                s_m[wave][c] = m_used;
-                s_l[wave][c] = lsum;
-            }
+        // ---- out: to o, or to the parts. The lane holds dims 4 (8 q + 4 h + r) + t of its column ----------
+        if (c >= t.cols) continue;
+        if (t.kind & kDirect) {
+            const int local = col / a.per_row;  // (a prefix tile is never direct)
+            const size_t at = ((size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row) * kDim;
+            const float inv = 1.0f / lsum;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                *reinterpret_cast<f32x4*>(&s_acc[wave][c][4 * (8 * (i >> 2) + 4 * h + (i & 3))]) =
-                    f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < t.cols * (kDim / 4); i += kThreads) {
-            const int tc = i / (kDim / 4), d = 4 * (i % (kDim / 4));
-            const int w0 = tc / kCols, cc = tc % kCols;  // waves w0, w0 + groups, ... hold the column
-            float m = s_m[w0][cc];
-            for (int w = w0 + groups; w < kWaves; w += groups) m = fmaxf(m, s_m[w][cc]);
-            float l = 0.0f;
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int w = w0; w < kWaves; w += groups) {
-                // a wave without a key has m = -inf, l = 0 (or NaN for a page that is not there)
-                const float f = part_weight(s_m[w][cc], m);
-                l += s_m[w][cc] == -INFINITY ? s_l[w][cc] : s_l[w][cc] * f;
-                const f32x4 y = *reinterpret_cast<const f32x4*>(&s_acc[w][cc][d]);
+                write_o(a, at + 4 * (8 * (i >> 2) + 4 * h + (i & 3)), f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]}, inv);
+        } else {
+            const size_t part = (size_t)kh * head.at.cap + t.base + (size_t)(run - t.run0) * t.cols + c;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
-            }
-            if (direct) {
-                const int col = t.col0 + tc, local = col / a.per_row;
-                const size_t at = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
-                write_o(a, at * kDim + d, x, l);
-            } else {
-                *reinterpret_cast<f32x4*>(plan.acc + (part + tc) * kDim + d) = x;
-                if (d == 0) *reinterpret_cast<f32x2*>(plan.ml + 2 * (part + tc)) = f32x2{m, l};
-            }
+            for (int i = 0; i < 16; ++i)
+                *reinterpret_cast<f32x4*>(plan.acc + part * kDim + 4 * (8 * (i >> 2) + 4 * h + (i & 3))) =
+                    f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+            if (h == 0) *reinterpret_cast<f32x2*>(plan.ml + 2 * part) = f32x2{m_used, lsum};
         }
     }
 }
 
 // ---- parts into rows ----------------------------------------------------------------------------
 //
-// A wave per column: its parts are those of its own tile and of the prefix tile that holds its
-// column. The halves of the wave take every other part, 16 bytes of its sums a lane.
+// A wave per column, or a workgroup where it has many parts: those of its own tile and of the prefix
+// tile that holds its column. The halves of a wave take parts in turn, 16 bytes of their sums a lane.
 __global__ void __launch_bounds__(kThreads)
 attend_merge_kernel(AttendArgs a) {
+    __shared__ __attribute__((aligned(16))) float s_x[kWaves][kDim];
     const Plan plan = load_plan(a);
     const Header& head = plan.head;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.x % a.p.hkv, e0 = blockIdx.x / a.p.hkv, es = gridDim.x / a.p.hkv;
     if (!plan.fits) {  // of another step's sizes, or none: no row is left looking like a result
@@ -825,43 +802,45 @@ attend_merge_kernel(AttendArgs a) {
         return;
     }
     for (int e = e0; e < head.merges; e += es) {
-        const int entry = plan.merge[e];
-        const Tile t = plan.tile[entry / (kTileCols / kMergeCols)];
-        const int first = entry % (kTileCols / kMergeCols) * kMergeCols;
-        for (int c = first + wave; c < min(first + kMergeCols, t.cols); c += kWaves) {
+        const int entry = scalar(plan.merge)[e];
+        const bool together = entry & 1;  // all four waves on one column
+        const Tile t = load_tile(plan.tile + entry / (2 * kCols));
+        const int c = entry / 2 % kCols + (together ? 0 : wave);
+        const int first = 2 * (together ? wave : 0) + h, step = together ? 2 * kWaves : 2;
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+        if (c < t.cols) {
             int pparts = 0, pcols = 0, pbase = 0;
             if (t.ptile >= 0) {
-                const int pc = t.pcol + c;
-                const Tile& p = plan.tile[t.ptile + pc / kTileCols];
+                const Tile p = load_tile(plan.tile + t.ptile + (t.pcol + c) / kCols);
                 pparts = p.parts;
                 pcols = p.cols;
-                pbase = p.base + pc % kTileCols;
+                pbase = p.base + (t.pcol + c) % kCols;
             }
             const int parts = pparts + t.parts;
             auto at = [&](int i) {
                 return (size_t)kh * head.at.cap + (i < pparts ? pbase + i * pcols : t.base + (i - pparts) * t.cols + c);
             };
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY;
             for (int i = lane; i < parts; i += 64) m = fmaxf(m, plan.ml[2 * at(i)]);
 #pragma unroll
             for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int i0 = 0; i0 < parts; i0 += 64) {
-                const int mine = min(i0 + lane, parts - 1);
-                const f32x2 ml = *reinterpret_cast<const f32x2*>(plan.ml + 2 * at(mine));
+                const f32x2 ml = *reinterpret_cast<const f32x2*>(plan.ml + 2 * at(min(i0 + lane, parts - 1)));
                 const float w = i0 + lane < parts ? part_weight(ml[0], m) : 0.0f;
                 if (i0 + lane < parts) l += ml[0] == -INFINITY ? ml[1] : ml[1] * w;
                 const int many = min(parts - i0, 64);
-                for (int i = 0; i < many; i += 16) {
+                for (int i = 0; i < many; i += 8 * step) {
                     f32x4 y[8];
                     float f[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int k = i + 2 * j + (lane >> 5);
+                        const int k = i + step * j + first;
                         y[j] = *reinterpret_cast<const f32x4*>(plan.acc + at(i0 + min(k, many - 1)) * kDim + 4 * (lane & 31));
                         f[j] = __shfl(w, min(k, 63));
                         if (k >= many) f[j] = 0.0f;
                     }
+                    // (a part without a key holds zeros, or NaN where its weight's sum does)
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -872,9 +851,22 @@ attend_merge_kernel(AttendArgs a) {
             for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
 #pragma unroll
             for (int d = 0; d < 4; ++d) x[d] = sum_h(x[d]);
+        }
+        if (together) {
+            if (lane < 32) *reinterpret_cast<f32x4*>(&s_x[wave][4 * lane]) = x;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(&s_x[w][4 * (lane & 31)]);
+                if (w == 0) x = y;
+                else x += y;
+            }
+            __syncthreads();  // the LDS is free for the next entry
+        }
+        if (c < t.cols && lane < 32 && (!together || wave == 0)) {
             const int col = t.col0 + c, local = col / a.per_row;
             const size_t o = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
-            if (lane < 32) write_o(a, o * kDim + 4 * lane, x, l);
+            write_o(a, o * kDim + 4 * lane, x, 1.0f / l);
         }
     }
 }
@@ -931,11 +923,12 @@ int attend_launch(const float* q, const PoolArgs& pool, const int* table, int wi
     a.per_row = hq / pool.hkv;
     a.o_f16 = o_f16;
     const Layout l = layout(n, n, tokens, hq, pool.hkv);  // (the most entries: the plan's may have fewer groups)
-    hipLaunchKernelGGL(attend_kernel, dim3((unsigned)(l.runs * pool.hkv)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(attend_kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0,
+                       stream, a);
     const int st = check_launch("attend_kernel");
     if (st != BRASA_OK) return st;
-    // a workgroup for each entry of a KV head, up to four per CU
-    const int wgs = std::max(std::min(l.max_merges, 1024 / pool.hkv), 1);
+    // a workgroup for each entry of a KV head, up to eight per CU
+    const int wgs = std::max(std::min(l.max_merges, 2048 / pool.hkv), 1);
     hipLaunchKernelGGL(attend_merge_kernel, dim3((unsigned)(wgs * pool.hkv)), dim3(kThreads), 0, stream, a);
     return check_launch("attend_merge_kernel");
 }
