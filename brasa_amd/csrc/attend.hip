@@ -407,17 +407,6 @@ struct AttendArgs {
     void* o;
     int n, width, tokens, hq, per_row, o_f16;
 };
-// Memory that no kernel of the launch writes, read through the scalar cache: uniform values that arrive
-// without a place among the vector loads in flight.
-template <typename T>
-using Scalar = const __attribute__((address_space(4))) T*;
-template <typename T>
-__device__ __forceinline__ Scalar<T> scalar(const T* p) { return (Scalar<T>)(uintptr_t)p; }
-// the byte at p + i (its aligned word is read)
-__device__ __forceinline__ int scalar_byte(const uint8_t* p, size_t i) {
-    const uintptr_t at = (uintptr_t)(p + i);
-    return (int)(*(Scalar<uint32_t>)(at & ~(uintptr_t)3) >> 8 * (at & 3) & 0xffu);
-}
 // The workspace's header and the parts it names.
 struct Plan {
     Header head;

@@ -111,7 +111,7 @@ struct WriteArgs {
     float eps;
     int hq, max_pos;
     long long item0;    // first block of the launch
-    long long q0;       // and first row of q
+    int t0, spans;      // first token of q; workgroups of a token
     unsigned tiles;     // workgroups that write the cache
 };
 
@@ -124,18 +124,20 @@ __device__ __forceinline__ float wave_sum(float p) {
 }
 
 // This lane's angle for row t (NaN where a position is outside the table).
-__device__ __forceinline__ void angle_of(const WriteArgs& a, int t, int lane, float& c, float& s) {
+__device__ __forceinline__ void angle_of(const WriteArgs& a, int t, int lane, int axis, float& c, float& s) {
     bool there = true;
     int mine = 0;
-    const int axis = a.map.w[lane >> 4] >> 2 * (lane & 15) & 3;
-    for (int i = 0; i < a.map.axes; ++i) {
-        const int p = a.rope_pos[(size_t)i * a.rows.tokens + t];
-        there &= p >= 0 && p < a.max_pos;
-        if (i == axis) mine = p;
-    }
+#pragma unroll
+    for (int i = 0; i < BRASA_ROPE_AXES; ++i)
+        if (i < a.map.axes) {
+            const int p = scalar(a.rope_pos)[(size_t)i * a.rows.tokens + t];
+            there &= p >= 0 && p < a.max_pos;
+            mine = i == axis ? p : mine;
+        }
     const size_t at = (size_t)(there ? mine : 0) * (kDim / 2) + lane;
-    c = there ? a.cos_t[at] : NAN;
-    s = there ? a.sin_t[at] : NAN;
+    c = a.cos_t[at];
+    s = a.sin_t[at];
+    if (!there) c = s = NAN;
 }
 __device__ __forceinline__ void norm_turn(float& x0, float& x1, float w0, float w1, float c, float s, float eps) {
     float p = 0.0f;
@@ -147,36 +149,36 @@ __device__ __forceinline__ void norm_turn(float& x0, float& x1, float w0, float 
     x1 = b0 * c + a0 * s;
 }
 
-template <int RPW>  // rows of q for each wave
-__global__ void __launch_bounds__(kWriteThreads)
+template <int RPW>  // rows of q for each wave, of one token
+__global__ void __launch_bounds__(kWriteThreads, 5)
 norm_rope_paged_kernel(WriteArgs a) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int axis = a.map.w[lane >> 4] >> 2 * (lane & 15) & 3;
     if (blockIdx.x >= a.tiles) {
-        // ---- q ------------------------------------------------------------------------------------
-        const int first = min(max(a.rows.cu[0], 0), a.rows.tokens);
-        const int last = min(max(a.rows.cu[a.rows.n], first), a.rows.tokens);
-        const long long r0 = a.q0 + ((long long)(blockIdx.x - a.tiles) * kWriteWaves + wave) * RPW;
-        float x0[RPW], x1[RPW], c[RPW], s[RPW];
-        const float w0 = a.qn[lane], w1 = a.qn[lane + 64];
-        bool on[RPW];
+        // ---- q: heads h0 .. of token t --------------------------------------------------------------
+        const int first = min(max(scalar(a.rows.cu)[0], 0), a.rows.tokens);
+        const int last = min(max(scalar(a.rows.cu)[a.rows.n], first), a.rows.tokens);
+        const unsigned unit = blockIdx.x - a.tiles;
+        const int t = a.t0 + (int)(unit / a.spans), h0 = ((int)(unit % a.spans) * kWriteWaves + wave) * RPW;
+        if (t < first || t >= last || h0 >= a.hq) return;
+        float* q = a.q + ((size_t)t * a.hq + h0) * kDim + lane;
+        float x0[RPW], x1[RPW], c, s;
+        const int rows = min(a.hq - h0, RPW);
 #pragma unroll
         for (int j = 0; j < RPW; ++j) {
-            const long long t = (r0 + j) / a.hq;
-            on[j] = t >= first && t < last;
-            if (!on[j]) continue;
-            const float* row = a.q + (size_t)(r0 + j) * kDim;
-            x0[j] = row[lane];
-            x1[j] = row[lane + 64];
-            angle_of(a, (int)t, lane, c[j], s[j]);
+            const int r = min(j, rows - 1);
+            x0[j] = q[r * kDim];
+            x1[j] = q[r * kDim + 64];
         }
+        angle_of(a, t, lane, axis, c, s);
+        const float w0 = a.qn[lane], w1 = a.qn[lane + 64];
 #pragma unroll
         for (int j = 0; j < RPW; ++j) {
-            if (!on[j]) continue;
-            norm_turn(x0[j], x1[j], w0, w1, c[j], s[j], a.eps);
-            float* row = a.q + (size_t)(r0 + j) * kDim;
-            row[lane] = x0[j];
-            row[lane + 64] = x1[j];
+            if (j >= rows) break;
+            norm_turn(x0[j], x1[j], w0, w1, c, s, a.eps);
+            q[j * kDim] = x0[j];
+            q[j * kDim + 64] = x1[j];
         }
         return;
     }
@@ -190,8 +192,11 @@ norm_rope_paged_kernel(WriteArgs a) {
     uint8_t* codes = (is_v ? a.p.v : a.p.k) + tile * kTileBytes8;
     uint8_t* scale = (is_v ? a.p.vx : a.p.kx) + tile;
     const int old = s0 > 0 ? *scale : 0;
-    const float* src = is_v ? a.v : a.k;
-    auto row_at = [&](int s) { return ((size_t)(t.row0 + s) * a.p.hkv + kh) * kDim + lane; };
+    // this block's rows (slot 0's may lie before the first): 32-bit offsets from there
+    const ptrdiff_t row0 = ((ptrdiff_t)t.row0 * a.p.hkv + kh) * kDim;
+    const float* src = (is_v ? a.v : a.k) + row0;
+    float* dst = a.k + row0;
+    auto row_at = [&](int s) { return s * a.p.hkv * kDim + lane; };
     float x0[kTileRows], x1[kTileRows];
     float amax = 0.0f;
     auto take = [&](float y0, float y1) {  // NaN and inf take no part in the scale
@@ -209,19 +214,24 @@ norm_rope_paged_kernel(WriteArgs a) {
     }
     if (!is_v) {
         const float w0 = a.kn[lane], w1 = a.kn[lane + 64];
-        float c[kTileRows], sn[kTileRows];
+        constexpr int kAhead = 4;  // rows whose angles are on their way together
 #pragma unroll
-        for (int j = 0; j < kTileRows; ++j) {
-            const int s = kWriteWaves * j + wave;
-            if (s >= s0 && s < s1) angle_of(a, t.row0 + s, lane, c[j], sn[j]);
-        }
+        for (int j0 = 0; j0 < kTileRows; j0 += kAhead) {
+            if (kWriteWaves * (j0 + kAhead) <= s0 || kWriteWaves * j0 >= s1) continue;
+            float c[kAhead], sn[kAhead];
 #pragma unroll
-        for (int j = 0; j < kTileRows; ++j) {
-            const int s = kWriteWaves * j + wave;
-            if (s < s0 || s >= s1) continue;
-            norm_turn(x0[j], x1[j], w0, w1, c[j], sn[j], a.eps);
-            a.k[row_at(s)] = x0[j];
-            a.k[row_at(s) + 64] = x1[j];
+            for (int j = 0; j < kAhead; ++j) {
+                const int s = min(max(kWriteWaves * (j0 + j) + wave, s0), s1 - 1);
+                angle_of(a, t.row0 + s, lane, axis, c[j], sn[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int s = kWriteWaves * (j0 + j) + wave;
+                if (s < s0 || s >= s1) continue;
+                norm_turn(x0[j0 + j], x1[j0 + j], w0, w1, c[j], sn[j], a.eps);
+                dst[row_at(s)] = x0[j0 + j];
+                dst[row_at(s) + 64] = x1[j0 + j];
+            }
         }
     }
 #pragma unroll
@@ -325,21 +335,23 @@ int norm_rope_paged_launch(const PoolArgs& pool, float* q, float* k, const float
     a.hq = hq;
     a.max_pos = max_pos;
     const long long items = width ? most_blocks(n, tokens) : 0;
-    const long long q_rows = (long long)tokens * hq;
-    // one row of q per wave while every row can have a wave at once, else four, whose loads travel together
-    const int rpw = q_rows <= 256 * 32 ? 1 : 4;
+    // one row of q per wave while every row can have a wave at once, else eight of a token, whose loads
+    // travel together
+    const int rpw = (long long)tokens * hq <= 256 * 32 ? 1 : 8;
+    a.spans = (hq + kWriteWaves * rpw - 1) / (kWriteWaves * rpw);
     // A launch of 2^32 threads or more runs fewer, without an error: at most 2^30 of each kind in each.
-    const long long most = (1LL << 30) / kWriteThreads / (2 * pool.hkv), most_q = (1LL << 30) / 64 * rpw;
-    for (long long i = 0, r = 0; i < items || r < q_rows; i += most, r += most_q) {
+    const long long most = (1LL << 30) / kWriteThreads / (2 * pool.hkv);
+    const long long most_q = a.spans ? (1LL << 30) / kWriteThreads / a.spans : tokens;
+    for (long long i = 0, t = 0; i < items || t < tokens; i += most, t += most_q) {
         a.item0 = i;
-        a.q0 = r;
+        a.t0 = (int)t;
         a.tiles = (unsigned)(std::min(std::max(items - i, 0LL), most) * 2 * pool.hkv);
-        const long long rows = std::min(std::max(q_rows - r, 0LL), most_q);
-        const unsigned more = (unsigned)((rows + kWriteWaves * rpw - 1) / (kWriteWaves * rpw));
+        const unsigned more = (unsigned)(std::min(std::max(tokens - t, 0LL), most_q) * a.spans);
+        if (a.tiles + more == 0) break;
         if (rpw == 1)
             hipLaunchKernelGGL(norm_rope_paged_kernel<1>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
         else
-            hipLaunchKernelGGL(norm_rope_paged_kernel<4>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
+            hipLaunchKernelGGL(norm_rope_paged_kernel<8>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
         const int st = check_launch("norm_rope_paged_kernel");
         if (st != BRASA_OK) return st;
     }
