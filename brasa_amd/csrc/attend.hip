@@ -31,7 +31,8 @@ constexpr int kCols = 32;     // columns of a tile
 constexpr int kRuns = 2048;   // waves of a launch: two per SIMD
 constexpr int kOver = 2;      // pages whose time a tile costs beside its own
 constexpr int kMinRun = 4;    // least length of a run
-constexpr int kFewParts = 8;  // parts of a column that one wave joins
+constexpr int kFewParts = 8;  // parts of a column that half a wave joins
+constexpr int kMergeCols = 2 * kWaves;  // columns of such an entry
 
 struct Tile {
     int seq;          // table row whose pages it reads
@@ -50,17 +51,19 @@ static_assert(sizeof(Tile) == 64, "a tile is one line");
 enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4 };
 
 // Where the plan and the partials stand in the workspace.
-struct Layout {
-    int runs;
-    size_t run_tile, tiles, merges, seqs, first, group, rows, ml, acc, bytes;
+struct Places {
+    size_t run_tile, tiles, merges, rows, ml, acc, bytes;
     long long cap;  // columns of partials, for each KV head
-    int max_tiles, max_merges;
+};
+struct Layout : Places {
+    size_t seqs, first, group;  // the plan's own lists
+    int runs, max_tiles, max_merges;
 };
 
 struct Header {
     int magic, n, tokens, width, hq, hkv, runs, tiles, merges;
     long long size, total;  // of a run, of the line
-    Layout at;
+    Places at;
 };
 constexpr int kMagic = 0x61747031;
 
@@ -126,12 +129,9 @@ struct PlanArgs {
     PlanGroup* grp;
     int* rows;  // packed rows of the sequences that may share, in order
     int n, groups, width, tokens, hq, hkv, per_row, runs;
-    Layout at;
+    Places at;
 };
 
-__device__ __forceinline__ void st_l2(int* p, int x) {
-    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 // exclusive sum over the workgroup of values up to 2^62; s: kScanWaves of LDS
 __device__ __forceinline__ long long block_scan64(long long x, long long* s, long long& sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -182,8 +182,24 @@ __device__ __forceinline__ long long div_by(long long x, long long d, double inv
     q += (q + 1) * d <= x;
     return q;
 }
+// IN_LDS: the lists of sequences and groups fit the LDS (up to kPlanLds of each); else they stand in the
+// workspace, and every look at one costs a trip to the L2 (64 sequences in one group 21 us in place of 12).
+constexpr int kPlanLds = 1024;
+template <bool IN_LDS>
 __global__ void __launch_bounds__(kScanThreads)
 attend_plan_kernel(PlanArgs a) {
+    __shared__ PlanSeq s_seq[IN_LDS ? kPlanLds : 1];
+    __shared__ PlanGroup s_grp[IN_LDS ? kPlanLds : 1];
+    __shared__ int s_first[IN_LDS ? 2 * kPlanLds + 1 : 1];
+    PlanSeq* const seqs = IN_LDS ? s_seq : a.seq;
+    PlanGroup* const grps = IN_LDS ? s_grp : a.grp;
+    int* const firsts = IN_LDS ? s_first : a.first;
+    // (within the workgroup, but past its L1 where they stand in the workspace)
+    auto ld_l2 = [](const int* p) { return IN_LDS ? *p : brasa::ld_l2(p); };
+    auto st_l2 = [](int* p, int x) {
+        if (IN_LDS) *p = x;
+        else __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
     __shared__ long long s_scan[kScanWaves];
     __shared__ int s_scan32[kScanWaves];
     __shared__ int s_merges;
@@ -199,10 +215,10 @@ attend_plan_kernel(PlanArgs a) {
         const int s1 = max(s0, g < a.groups ? min(max(a.group[g + 1], 0), a.n) : 0);
         before = all;
         if (g < a.groups) {
-            st_l2(&a.grp[g].s0, s0);
-            st_l2(&a.grp[g].s1, s1);
-            st_l2(&a.grp[g].lead, a.n);
-            st_l2(&a.grp[g].many, 0);
+            st_l2(&grps[g].s0, s0);
+            st_l2(&grps[g].s1, s1);
+            st_l2(&grps[g].lead, a.n);
+            st_l2(&grps[g].many, 0);
         }
     }
     if (a.groups) stores_barrier();
@@ -227,16 +243,16 @@ attend_plan_kernel(PlanArgs a) {
             int lo = 0, hi = a.groups;  // the last group that starts at or before i
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (ld_l2(&a.grp[mid].s0) <= i) lo = mid;
+                if (ld_l2(&grps[mid].s0) <= i) lo = mid;
                 else hi = mid;
             }
-            if (ld_l2(&a.grp[lo].s0) <= i && i < ld_l2(&a.grp[lo].s1)) {
+            if (ld_l2(&grps[lo].s0) <= i && i < ld_l2(&grps[lo].s1)) {
                 const int pages = prefix_pages(lo);
                 if (pages > 0 && s.pos >= pages * kPage) {
                     s.group = lo;
                     cols = s.rows * per_row;
-                    atomicMin(&a.grp[lo].lead, i);
-                    atomicAdd(&a.grp[lo].many, 1);
+                    atomicMin(&grps[lo].lead, i);
+                    atomicAdd(&grps[lo].many, 1);
                 }
             }
         }
@@ -248,28 +264,28 @@ attend_plan_kernel(PlanArgs a) {
             for (int r = 0; cols && r < s.rows; ++r) a.rows[s.scol / per_row + r] = s.c0 + r;
         }
         if (i < a.n) {
-            st_l2(&a.seq[i].c0, s.c0);
-            st_l2(&a.seq[i].rows, s.rows);
-            st_l2(&a.seq[i].pos, s.pos);
-            st_l2(&a.seq[i].group, s.group);
-            st_l2(&a.seq[i].scol, s.scol);
+            st_l2(&seqs[i].c0, s.c0);
+            st_l2(&seqs[i].rows, s.rows);
+            st_l2(&seqs[i].pos, s.pos);
+            st_l2(&seqs[i].group, s.group);
+            st_l2(&seqs[i].scol, s.scol);
         }
     }
     stores_barrier();
     auto load_seq = [&](int i) {
-        PlanSeq s = {ld_l2(&a.seq[i].c0), ld_l2(&a.seq[i].rows), ld_l2(&a.seq[i].pos), ld_l2(&a.seq[i].group), 0};
+        PlanSeq s = {ld_l2(&seqs[i].c0), ld_l2(&seqs[i].rows), ld_l2(&seqs[i].pos), ld_l2(&seqs[i].group), 0};
         if (s.group >= 0) {
-            if (ld_l2(&a.grp[s.group].many) < 2) s.group = -1;
-            else s.scol = ld_l2(&a.seq[i].scol);
+            if (ld_l2(&grps[s.group].many) < 2) s.group = -1;
+            else s.scol = ld_l2(&seqs[i].scol);
         }
         return s;
     };
     // columns of a group's sharing sequences, and how many there are before them in the list
     auto group_cols = [&](int g, int& col0) {
-        if (ld_l2(&a.grp[g].many) < 2) return 0;
-        const int s0 = ld_l2(&a.grp[g].s0), s1 = ld_l2(&a.grp[g].s1);
-        col0 = ld_l2(&a.seq[s0].scol);
-        return (s1 < a.n ? ld_l2(&a.seq[s1].scol) : scols) - col0;
+        if (ld_l2(&grps[g].many) < 2) return 0;
+        const int s0 = ld_l2(&grps[g].s0), s1 = ld_l2(&grps[g].s1);
+        col0 = ld_l2(&seqs[s0].scol);
+        return (s1 < a.n ? ld_l2(&seqs[s1].scol) : scols) - col0;
     };
 
     // ---- how many tiles each has ------------------------------------------------------------------
@@ -279,30 +295,30 @@ attend_plan_kernel(PlanArgs a) {
         const int e = e0 + tid;
         int tiles = 0, col0;
         if (e < a.groups) tiles = (group_cols(e, col0) + kCols - 1) / kCols;
-        else if (e < entries) tiles = (int)(((long long)ld_l2(&a.seq[e - a.groups].rows) * per_row + kCols - 1) / kCols);
+        else if (e < entries) tiles = (int)(((long long)ld_l2(&seqs[e - a.groups].rows) * per_row + kCols - 1) / kCols);
         int sum;
         const int at = ntiles + block_scan(tiles, s_scan32, sum);
         ntiles += sum;
-        if (e < entries) st_l2(a.first + e, at);
+        if (e < entries) st_l2(firsts + e, at);
     }
-    if (tid == 0) st_l2(a.first + entries, ntiles);
+    if (tid == 0) st_l2(firsts + entries, ntiles);
     stores_barrier();
 
     auto make_tile = [&](int at) {
         int lo = 0, hi = entries;  // the last group or sequence that starts at or before `at`: one with tiles
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (ld_l2(a.first + mid) <= at) lo = mid;
+            if (ld_l2(firsts + mid) <= at) lo = mid;
             else hi = mid;
         }
         Tile t;
-        t.col0 = (at - ld_l2(a.first + lo)) * kCols;
+        t.col0 = (at - ld_l2(firsts + lo)) * kCols;
         t.ptile = t.pcol = -1;
         if (lo < a.groups) {
             int col0;
             const int cols = group_cols(lo, col0);
             t.kind = kPrefix;
-            t.seq = ld_l2(&a.grp[lo].lead);
+            t.seq = ld_l2(&grps[lo].lead);
             t.row0 = col0 / per_row;
             t.cols = min(cols - t.col0, kCols);
             t.b0 = 0;
@@ -323,7 +339,7 @@ attend_plan_kernel(PlanArgs a) {
             if (s.group >= 0) {
                 int gcol0 = 0;
                 group_cols(s.group, gcol0);
-                t.ptile = ld_l2(a.first + s.group) + (s.scol - gcol0) / kCols;
+                t.ptile = ld_l2(firsts + s.group) + (s.scol - gcol0) / kCols;
                 t.pcol = (s.scol - gcol0) % kCols;
             }
         }
@@ -366,27 +382,32 @@ attend_plan_kernel(PlanArgs a) {
         if (!(t.kind & (kPrefix | kDirect))) {
             int parts = t.parts;
             if (t.ptile >= 0) parts += (int)div_by(t.b0, size, inv) + 1;  // (about: the prefix tile's)
-            const int each = parts > kFewParts ? 1 : kWaves, many = (t.cols + each - 1) / each;
+            const int each = parts > kFewParts ? 1 : kMergeCols, many = (t.cols + each - 1) / each;
             const int e = atomicAdd(&s_merges, many);
             for (int j = 0; j < many; ++j) a.merge[e + j] = (at * kCols + j * each) * 2 + (each == 1);
         }
     }
     __syncthreads();
     if (tid == 0) {
-        Header h;
-        h.magic = kMagic;
-        h.n = a.n;
-        h.tokens = a.tokens;
-        h.width = a.width;
-        h.hq = a.hq;
-        h.hkv = a.hkv;
-        h.runs = a.runs;
-        h.tiles = ntiles;
-        h.merges = s_merges;
-        h.size = size;
-        h.total = line;
-        h.at = a.at;
-        *a.head = h;
+        a.head->magic = kMagic;
+        a.head->n = a.n;
+        a.head->tokens = a.tokens;
+        a.head->width = a.width;
+        a.head->hq = a.hq;
+        a.head->hkv = a.hkv;
+        a.head->runs = a.runs;
+        a.head->tiles = ntiles;
+        a.head->merges = s_merges;
+        a.head->size = size;
+        a.head->total = line;
+        a.head->at.run_tile = a.at.run_tile;
+        a.head->at.tiles = a.at.tiles;
+        a.head->at.merges = a.at.merges;
+        a.head->at.rows = a.at.rows;
+        a.head->at.ml = a.at.ml;
+        a.head->at.acc = a.at.acc;
+        a.head->at.bytes = a.at.bytes;
+        a.head->at.cap = a.at.cap;
     }
 }
 
@@ -772,8 +793,9 @@ attend_kernel(AttendArgs a) {
 
 // ---- parts into rows ----------------------------------------------------------------------------
 //
-// A wave per column, or a workgroup where it has many parts: those of its own tile and of the prefix
-// tile that holds its column. The halves of a wave take parts in turn, 16 bytes of their sums a lane.
+// Half a wave per column, 16 bytes of its sums a lane and all parts' loads in flight together, or a workgroup
+// where there are many: those of the column's own tile and of the prefix tile that holds it. Bound: the
+// chain entry -> tile -> parts -> o, and for prompts the parts' bytes.
 __global__ void __launch_bounds__(kThreads)
 attend_merge_kernel(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) float s_x[kWaves][kDim];
@@ -792,24 +814,57 @@ attend_merge_kernel(AttendArgs a) {
     }
     for (int e = e0; e < head.merges; e += es) {
         const int entry = scalar(plan.merge)[e];
-        const bool together = entry & 1;  // all four waves on one column
+        const bool together = entry & 1;  // the whole workgroup on one column
         const Tile t = load_tile(plan.tile + entry / (2 * kCols));
-        const int c = entry / 2 % kCols + (together ? 0 : wave);
-        const int first = 2 * (together ? wave : 0) + h, step = together ? 2 * kWaves : 2;
+        const int c = entry / 2 % kCols + (together ? 0 : 2 * wave + h);
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
         float l = 0.0f;
-        if (c < t.cols) {
-            int pparts = 0, pcols = 0, pbase = 0;
-            if (t.ptile >= 0) {
-                const Tile p = load_tile(plan.tile + t.ptile + (t.pcol + c) / kCols);
-                pparts = p.parts;
-                pcols = p.cols;
-                pbase = p.base + (t.pcol + c) % kCols;
+        int pparts = 0, pcols = 0, pbase = 0;
+        if (t.ptile >= 0) {
+            const Tile* p = plan.tile + t.ptile + (t.pcol + c) / kCols;  // (two halves may have two)
+            if (c < t.cols) {
+                pparts = p->parts;
+                pcols = p->cols;
+                pbase = p->base + (t.pcol + c) % kCols;
             }
-            const int parts = pparts + t.parts;
-            auto at = [&](int i) {
-                return (size_t)kh * head.at.cap + (i < pparts ? pbase + i * pcols : t.base + (i - pparts) * t.cols + c);
-            };
+        }
+        const int parts = pparts + t.parts;
+        auto at = [&](int i) {
+            return (size_t)kh * head.at.cap + (i < pparts ? pbase + i * pcols : t.base + (i - pparts) * t.cols + c);
+        };
+        if (!together) {
+            // (the count of a shared column's parts was an estimate when the entry was made)
+            if (c < t.cols) {
+                float m = -INFINITY;
+                for (int i0 = 0; i0 < parts; i0 += kFewParts) {
+                    f32x4 y[kFewParts];
+                    f32x2 ml[kFewParts];
+#pragma unroll
+                    for (int j = 0; j < kFewParts; ++j) {
+                        const size_t p = at(min(i0 + j, parts - 1));
+                        ml[j] = *reinterpret_cast<const f32x2*>(plan.ml + 2 * p);
+                        y[j] = *reinterpret_cast<const f32x4*>(plan.acc + p * kDim + 4 * (lane & 31));
+                    }
+                    float top = m;
+#pragma unroll
+                    for (int j = 0; j < kFewParts; ++j) top = fmaxf(top, ml[j][0]);
+                    const float before = part_weight(m, top);
+                    l *= before;
+                    x *= before;
+                    m = top;
+#pragma unroll
+                    for (int j = 0; j < kFewParts; ++j) {
+                        if (i0 + j >= parts) break;
+                        // (a part without a key holds zeros, and a sum that is 0 or NaN)
+                        const float f = part_weight(ml[j][0], m);
+                        l = fmaf(ml[j][1], f, l);
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) x[d] = fmaf(y[j][d], f, x[d]);
+                    }
+                }
+            }
+        } else {
+            const int first = 2 * wave + h, step = 2 * kWaves;
             float m = -INFINITY;
             for (int i = lane; i < parts; i += 64) m = fmaxf(m, plan.ml[2 * at(i)]);
 #pragma unroll
@@ -817,7 +872,7 @@ attend_merge_kernel(AttendArgs a) {
             for (int i0 = 0; i0 < parts; i0 += 64) {
                 const f32x2 ml = *reinterpret_cast<const f32x2*>(plan.ml + 2 * at(min(i0 + lane, parts - 1)));
                 const float w = i0 + lane < parts ? part_weight(ml[0], m) : 0.0f;
-                if (i0 + lane < parts) l += ml[0] == -INFINITY ? ml[1] : ml[1] * w;
+                l = fmaf(ml[1], w, l);
                 const int many = min(parts - i0, 64);
                 for (int i = 0; i < many; i += 8 * step) {
                     f32x4 y[8];
@@ -829,19 +884,16 @@ attend_merge_kernel(AttendArgs a) {
                         f[j] = __shfl(w, min(k, 63));
                         if (k >= many) f[j] = 0.0f;
                     }
-                    // (a part without a key holds zeros, or NaN where its weight's sum does)
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) x[d] = f[j] == 0.0f ? x[d] : fmaf(y[j][d], f[j], x[d]);
+                        for (int d = 0; d < 4; ++d) x[d] = fmaf(y[j][d], f[j], x[d]);
                 }
             }
 #pragma unroll
             for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
 #pragma unroll
             for (int d = 0; d < 4; ++d) x[d] = sum_h(x[d]);
-        }
-        if (together) {
             if (lane < 32) *reinterpret_cast<f32x4*>(&s_x[wave][4 * lane]) = x;
             __syncthreads();
 #pragma unroll
@@ -852,10 +904,10 @@ attend_merge_kernel(AttendArgs a) {
             }
             __syncthreads();  // the LDS is free for the next entry
         }
-        if (c < t.cols && lane < 32 && (!together || wave == 0)) {
+        if (c < t.cols && (!together || (wave == 0 && h == 0))) {
             const int col = t.col0 + c, local = col / a.per_row;
             const size_t o = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
-            write_o(a, o * kDim + 4 * lane, x, 1.0f / l);
+            write_o(a, o * kDim + 4 * (lane & 31), x, 1.0f / l);
         }
     }
 }
@@ -892,7 +944,8 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
     a.per_row = hq / hkv;
     a.runs = l.runs;
     a.at = l;
-    hipLaunchKernelGGL(attend_plan_kernel, dim3(1), dim3(kScanThreads), 0, stream, a);
+    auto kernel = n <= kPlanLds && groups <= kPlanLds ? attend_plan_kernel<true> : attend_plan_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kScanThreads), 0, stream, a);
     return check_launch("attend_plan_kernel");
 }
 
