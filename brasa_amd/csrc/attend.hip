@@ -15,6 +15,7 @@
 // whose sequence has a prefix tile, leaves (m, l, acc) in the workspace and a second launch joins them
 // in order, so the result does not depend on timing.
 #include <climits>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -24,6 +25,7 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
@@ -513,6 +515,7 @@ __device__ __forceinline__ void write_o(const AttendArgs& a, size_t at, f32x4 x,
 }
 
 // V^T P^T of 32 keys added to acc. v[4 q + r]: four codes (dims 4 i .. + 4 of lane i) of key 8 q + 4 h + r.
+template <bool EXACT>
 __device__ __forceinline__ void add_pv(const uint32_t (&v)[16], const half8v (&hi)[2], const half8v (&lo)[2],
                                        f32x16 (&acc)[4]) {
 #pragma unroll
@@ -530,11 +533,47 @@ __device__ __forceinline__ void add_pv(const uint32_t (&v)[16], const half8v (&h
             const half8v v0 = join(x0[0], x0[1], x0[2], x0[3]), v1 = join(x1[0], x1[1], x1[2], x1[3]);
             acc[2 * t2] = mfma32(v0, hi[st], acc[2 * t2]);
             acc[2 * t2 + 1] = mfma32(v1, hi[st], acc[2 * t2 + 1]);
-            acc[2 * t2] = mfma32(v0, lo[st], acc[2 * t2]);
-            acc[2 * t2 + 1] = mfma32(v1, lo[st], acc[2 * t2 + 1]);
+            if constexpr (EXACT) {
+                acc[2 * t2] = mfma32(v0, lo[st], acc[2 * t2]);
+                acc[2 * t2 + 1] = mfma32(v1, lo[st], acc[2 * t2 + 1]);
+            }
         }
 }
 
+// Q of a wave's columns as the B operands of S^T = K Q^T: f16 values, and what they leave over, as f16 values
+// too (EXACT: 22 bits together) or as e4m3 codes of 2^11 times it (15 bits, at half the matrix cores' time,
+// and K's codes are the other operand as they are).
+template <bool EXACT>
+struct QueryOps {
+    half8v hi[8];
+    half8v lo[EXACT ? 8 : 1];
+    i32x8 lo8[EXACT ? 1 : 2];
+};
+constexpr int kLoScale = 127 - 11;  // 2^-11 as an exponent byte
+template <bool EXACT>
+__device__ __forceinline__ f32x16 scores(const u32x4 (&kw)[4], const QueryOps<EXACT>& q) {
+    f32x16 s;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = 0.0f;
+    if constexpr (!EXACT) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const u32x4 a = kw[2 * i], b = kw[2 * i + 1];
+            const i32x8 k = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q.lo8[i], s, 0, 0, 0, 127, 0, kLoScale);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t w0 = kw[i >> 1][2 * (i & 1)], w1 = kw[i >> 1][2 * (i & 1) + 1];
+        const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
+        s = mfma32(ka, q.hi[i], s);
+        if constexpr (EXACT) s = mfma32(ka, q.lo[i], s);
+    }
+    return s;
+}
+
+template <bool EXACT>
 __global__ void __launch_bounds__(kThreads, 2)
 attend_kernel(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) int s_nan[kWaves][kDim];  // first key with a NaN value, for each dim
@@ -564,7 +603,7 @@ attend_kernel(AttendArgs a) {
         const int row = prefix ? plan.rows[t.row0 + local] : t.row0 + local;
         const int head_of = kh * a.per_row + col - local * a.per_row;
         const int limit = prefix ? INT_MAX : nowhere ? -1 : t.pos0 + local;  // the last position it sees
-        half8v qh[8], ql[8];
+        QueryOps<EXACT> q;
         int qx;
         {
             // step s holds dims 32 (s / 2) + 16 h + 8 (s % 2) .. + 8, as K's 16-byte loads do
@@ -588,10 +627,25 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 half2v u[4], w[4];
+                float rest[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) split(ldexpf(x[s][2 * j], -qx), ldexpf(x[s][2 * j + 1], -qx), u[j], w[j]);
-                qh[s] = join(u[0], u[1], u[2], u[3]);
-                ql[s] = join(w[0], w[1], w[2], w[3]);
+                for (int j = 0; j < 4; ++j) {
+                    const float y0 = ldexpf(x[s][2 * j], -qx), y1 = ldexpf(x[s][2 * j + 1], -qx);
+                    split(y0, y1, u[j], w[j]);
+                    rest[2 * j] = ldexpf(y0 - (float)u[j].x, 11);
+                    rest[2 * j + 1] = ldexpf(y1 - (float)u[j].y, 11);
+                }
+                q.hi[s] = join(u[0], u[1], u[2], u[3]);
+                if constexpr (EXACT) {
+                    q.lo[s] = join(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        int word = __builtin_amdgcn_cvt_pk_fp8_f32(rest[4 * j], rest[4 * j + 1], 0, false);
+                        word = __builtin_amdgcn_cvt_pk_fp8_f32(rest[4 * j + 2], rest[4 * j + 3], word, true);
+                        q.lo8[s >> 2][2 * (s & 3) + j] = word;
+                    }
+                }
             }
         }
         // the least and the largest position that a column of this wave sees
@@ -633,7 +687,7 @@ attend_kernel(AttendArgs a) {
         };
 
         if (!nowhere) {
-            int page = p0, half = 0;
+            int page = p0;
             bool there, there_next = true;
             size_t tile = tile_of(ids[page], there), tile_next = tile;
             load_k(tile, 0);
@@ -641,37 +695,21 @@ attend_kernel(AttendArgs a) {
             int kx = scalar_byte(a.p.kx, tile), vx = scalar_byte(a.p.vx, tile), kx_next = kx, vx_next = vx;
             vref = vx;
             int id = page + 1 < p1 ? ids[page + 1] : 0;  // of the page after this one
-            while (true) {
+            // the scores of the half page at hand: of key k0 + 8 q + 4 h + r and column c, in units of
+            // log2 and of 2^(qx + kx - 127)
+            f32x16 s = scores(kw, q);
+            load_k(tile, 1);
+
+            // One half page: its weights, the scores of the next, and its share of the sums. The next page's K
+            // (or this one's second half) takes the registers of the K just used, V later V's.
+            auto half_page = [&](auto HALF, bool more) {
+                constexpr int half = HALF;
                 const int k0 = page * kPage + 32 * half;
-                // where the next half page is
-                const int page_next = half ? page + 1 : page;
-                const bool more = page_next < p1;
-                if (half && more) {
-                    tile_next = tile_of(id, there_next);
-                    kx_next = scalar_byte(a.p.kx, tile_next);
-                    vx_next = scalar_byte(a.p.vx, tile_next);
-                    id = page_next + 1 < p1 ? ids[page_next + 1] : 0;
-                }
-                // ---- scores: key k0 + 8 q + 4 h + r of column c, in units of log2 and of 2^(qx + kx - 127)
-                f32x16 s;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) s[j] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t w0 = kw[i >> 1][2 * (i & 1)], w1 = kw[i >> 1][2 * (i & 1) + 1];
-                    const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
-                    s = mfma32(ka, qh[i], s);
-                    s = mfma32(ka, ql[i], s);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                if (more) load_k(tile_next, half ^ 1);
-                __builtin_amdgcn_sched_barrier(0);
                 // (past the clamp every score is 0, or so far from the next that one key takes all)
                 const float sc = ldexpf(1.0f, min(max(qx + kx - 127, -126), 127));
                 if (!there) lsum = limit >= page * kPage ? NAN : lsum;
-                const bool edge = k0 + 31 > lim0;  // some column does not see all of these keys
-                bool odd = false;                  // V holds NaN codes among them
-                if (edge) {
+                bool odd = false;  // V holds NaN codes that not all columns see
+                if (k0 + 31 > lim0) {  // some column does not see all of these keys
                     uint32_t nans = 0;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -687,7 +725,7 @@ attend_kernel(AttendArgs a) {
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
                 top = max_h(top) * sc;
                 // a reference point that moves only when the maximum has grown by 2^8: p stays below
-                // 2^15 with the bias of 2^7 that keeps the lo halves of small p out of f16's subnormals
+                // 2^15 with the bias of 2^7 that keeps small p out of f16's subnormals
                 const bool grow = top > m_used + 8.0f;
                 if (__builtin_amdgcn_ballot_w64(grow)) {
                     const float alpha = grow ? __builtin_amdgcn_exp2f(m_used - top) : 1.0f;
@@ -696,39 +734,55 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[i] *= alpha;
                 }
-                // V's scale: acc's unit grows with it, and where it is smaller p shrinks, through its exponent
-                int less = 0;
+                // V's scale: acc's unit grows with it, and where it is smaller p shrinks, through its
+                // exponent (by 2^100 at most: p is 0 in f16 from 2^40 on)
                 if (vx > vref) {
                     const float f = ldexpf(1.0f, vref - vx);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[i] *= f;
                     vref = vx;
-                } else {
-                    less = min(vref - vx, 100);
                 }
+                const int less = min(vref - vx, 100);
                 // (a column that has seen no key yet: its scores are all -inf, and p 0)
                 const float mb = m_used == -INFINITY ? 0.0f : 7.0f - (float)less - m_used;
+                __builtin_amdgcn_sched_barrier(0);
+                f32x16 next;
+                if constexpr (!EXACT) next = scores(kw, q);
                 float p[16], psum = 0.0f;
+                half8v ph[2], pl[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sc, mb));
                     psum += p[i];
                 }
-                lsum = fmaf(psum, ldexpf(1.0f, less), lsum);
-                if (vref - vx > 100) {
-                    const float f = ldexpf(1.0f, max(vx - vref + 100, -126));
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) p[i] *= f;
-                }
-                half8v ph[2], pl[2];
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     half2v u[4], w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) split(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], u[e], w[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (EXACT) split(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], u[e], w[e]);
+                        else u[e] = half2v{(_Float16)p[8 * st + 2 * e], (_Float16)p[8 * st + 2 * e + 1]};
+                    }
                     ph[st] = join(u[0], u[1], u[2], u[3]);
-                    pl[st] = join(w[0], w[1], w[2], w[3]);
+                    if constexpr (EXACT) pl[st] = join(w[0], w[1], w[2], w[3]);
                 }
+                // (here, among the products, not sunk behind the branch below)
+                asm volatile("" : "+v"(ph[0]), "+v"(ph[1]), "+v"(psum));
+                lsum = fmaf(psum, ldexpf(1.0f, less), lsum);
+                if constexpr (!EXACT) {
+                    // the products first ask for no conversion; then one after each seven vector instructions
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 14, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x402, 10, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (!EXACT && more) load_k(tile_next, half);
+                __builtin_amdgcn_sched_barrier(0);
                 if (odd) {
                     // NaN values that some columns see and others do not: 0 in the product, and NaN for the
                     // columns at or past the first such key of the dim
@@ -752,12 +806,31 @@ attend_kernel(AttendArgs a) {
                         for (int d = 0; d < 4; ++d)
                             if (s_nan[wave][4 * (8 * (i >> 2) + 4 * h + (i & 3)) + d] <= limit) acc[d][i] = NAN;
                 }
-                add_pv(vw, ph, pl, acc);
+                add_pv<EXACT>(vw, ph, pl, acc);
                 __builtin_amdgcn_sched_barrier(0);
+                if (half == 0) load_v(tile, 1);
+                else if (more) load_v(tile_next, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (EXACT) {
+                    next = scores(kw, q);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (more) load_k(tile_next, half);
+                }
+                s = next;
+            };
+            while (true) {
+                const bool more = page + 1 < p1;
+                if (more) {
+                    tile_next = tile_of(id, there_next);
+                    kx_next = scalar_byte(a.p.kx, tile_next);
+                    vx_next = scalar_byte(a.p.vx, tile_next);
+                    id = page + 2 < p1 ? ids[page + 2] : 0;
+                }
+                half_page(std::integral_constant<int, 0>{}, more);
+                // (behind the last page the next scores are of the keys at hand again, and not used)
+                half_page(std::integral_constant<int, 1>{}, more);
                 if (!more) break;
-                load_v(tile_next, half ^ 1);
-                page = page_next;
-                half ^= 1;
+                ++page;
                 there = there_next;
                 tile = tile_next;
                 kx = kx_next;
@@ -965,7 +1038,8 @@ int attend_launch(const float* q, const PoolArgs& pool, const int* table, int wi
     a.per_row = hq / pool.hkv;
     a.o_f16 = o_f16;
     const Layout l = layout(n, n, tokens, hq, pool.hkv);  // (the most entries: the plan's may have fewer groups)
-    hipLaunchKernelGGL(attend_kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0,
+    auto kernel = o_f16 ? attend_kernel<false> : attend_kernel<true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0,
                        stream, a);
     const int st = check_launch("attend_kernel");
     if (st != BRASA_OK) return st;

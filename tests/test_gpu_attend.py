@@ -5,7 +5,10 @@ row's largest sum of |q k| / sqrt(128): q / sqrt(128) * log2 e in two f16 halves
 (2 * 2^-24), 128 + 2 roundings of f32 sums, exp2 and its argument; a weight in two halves adds 2^-22 and a few
 roundings; numerator and denominator both carry it. Sums over keys in f32: a lane adds every second key of its
 wave's pages, so at most lk / 2 additions in a chain, and 300 for the parts and their joining. A weight below f16's
-normal range errs by 2^-32 of the largest one, times |v| of its key. An f16 result adds 2^-11 of itself.
+normal range errs by 2^-32 of the largest one, times |v| of its key. An f16 result adds 2^-11 of itself, and its call
+keeps less of q and the weights: q's f16 value errs by 2^-11 of it, and the e4m3 code of what is left by 2^-4 of
+that, or by half the least code, 2^-10 / 2^11 where the row's largest |q| is at least 2^8: 2^-15 of each q, and 2^-29
+of the largest times the key's sum of |k|; a weight errs by 2^-11 of itself.
 """
 import numpy as np
 import pytest
@@ -97,7 +100,12 @@ class Step:
             lk = self.held[i] + int(b - a)
             k, v = ref.rows_of(self.pool, self.layer, self.table[i, :-(-lk // PAGE)], lk)
             o, av, top = step_ref.attend(self.q[a:b], k, v, self.held[i])
-            tol = av * (2 * (top * (2.0 ** -22 + 136 * 2.0 ** -24) + 2.0 ** -22 + 8 * 2.0 ** -24)
+            e_q, e_p, rest = 2.0 ** -22, 2.0 ** -22, 0.0
+            if self.out == OutDType.F16:
+                e_q, e_p = 2.0 ** -15, 2.0 ** -11
+                most = np.abs(np.nan_to_num(k)).sum(-1).max(0).repeat(self.hq // self.hkv)[None, :, None]
+                rest = 2.0 ** -29 * np.abs(np.nan_to_num(self.q[a:b])).max(-1, keepdims=True) * most / np.sqrt(DIM)
+            tol = av * (2 * (top * (e_q + 136 * 2.0 ** -24) + rest + e_p + 8 * 2.0 ** -24)
                         + (lk / 2 + 300) * 2.0 ** -24) + 1e-37
             tol += 2.0 ** -32 * np.abs(np.nan_to_num(v)).sum(0).repeat(self.hq // self.hkv, 0)
             if self.out == OutDType.F16:
@@ -146,15 +154,24 @@ def test_head_counts(hq, hkv):
     _run(("heads", hq, hkv), new=[1, 2, 1], held=[130, 70, 200], groups=[(3, 64)], hq=hq, hkv=hkv, seed=hq)
 
 
+@pytest.mark.parametrize("new,held,groups", [
+    ([1], [0], []), ([1], [256], []), ([65], [0], []), ([33, 1, 70], [100, 2000, 63], []), ([1] * 6, [100, 300, 63, 64, 1000, 130], [(3, 64), (3, 64)]),
+    ([2] * 5, [4200, 4100, 4097, 4300, 4500], [(5, 4096)])], ids=str)
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (4, 4), (16, 1), (128, 1)])
+def test_f16_results(new, held, groups, hq, hkv):
+    _run(("f16", new[:5], groups, hq, hkv), new=new, held=held, groups=groups, hq=hq, hkv=hkv, out=OutDType.F16, seed=len(new) + hq)
+
+
 @pytest.mark.parametrize("out", list(OutDType))
 def test_f16_and_layers(out):
     _run(("layer", out), new=[1, 50, 1, 200], held=[500, 448, 449, 20], groups=[(3, 448)], hq=16, hkv=4, layers=3, layer=1, out=out)
 
 
-def test_scales_far_apart():
+@pytest.mark.parametrize("exps,q_scale,out", [((60, 200), 1.0, OutDType.F32), ((0, 3), 1e-3, OutDType.F32), ((100, 140), 1e-30, OutDType.F32),
+                                              ((127, 135), 3.0, OutDType.F32), ((105, 121), 1e-2, OutDType.F16), ((110, 114), 50.0, OutDType.F16)])
+def test_scales_far_apart(exps, q_scale, out):
     """V's scale jumps between pages, and the scores are large or tiny."""
-    for exps, q_scale in (((60, 200), 1.0), ((0, 3), 1e-3), ((100, 140), 1e-30), ((127, 135), 3.0)):
-        _run(("scales", exps, q_scale), new=[1, 40, 3], held=[700, 64, 200], groups=[(3, 64)], exps=exps, q_scale=q_scale, seed=5)
+    _run(("scales", exps, q_scale), new=[1, 40, 3], held=[700, 64, 200], groups=[(3, 64)], exps=exps, q_scale=q_scale, out=out, seed=5)
 
 
 def test_first_keys_small():
@@ -183,9 +200,10 @@ def test_many_sequences():
     s.check()
 
 
-def test_values_that_are_not_finite():
+@pytest.mark.parametrize("out", list(OutDType))
+def test_values_that_are_not_finite(out):
     """NaN keys and values reach the rows that see them, in their places, and no others."""
-    s = Step(new=[50, 1, 1, 9], held=[70, 200, 130, 128], groups=[(4, 64)], hq=8, hkv=2, seed=8)
+    s = Step(new=[50, 1, 1, 9], held=[70, 200, 130, 128], groups=[(4, 64)], hq=8, hkv=2, out=out, seed=8)
     s.pool.v[0, s.table[0, 1], 1, 20, 5] = 127    # position 84, below some of sequence 0's rows only
     s.pool.v[0, s.table[0, 1], 0, 55, :] = 255    # position 119, its last row's own
     s.pool.k[0, s.table[1, 3], 0, 3, 7] = 127     # position 195: sequence 1 sees it
