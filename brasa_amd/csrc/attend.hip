@@ -514,30 +514,45 @@ __device__ __forceinline__ void write_o(const AttendArgs& a, size_t at, f32x4 x,
     }
 }
 
-// V^T P^T of 32 keys added to acc. v[4 q + r]: four codes (dims 4 i .. + 4 of lane i) of key 8 q + 4 h + r.
+// Keeps what is written before it before what is written after: the products below stand among the vector
+// instructions that run beside them.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// V^T's operands of 16 keys and dims 4 i + 2 t2 (x), 4 i + 2 t2 + 1 (y) of lane i. v[4 q + r]: four codes (dims 4 i .. + 4)
+// of key 8 q + 4 h + r.
+struct ValueOps {
+    half8v x, y;
+};
+__device__ __forceinline__ ValueOps value_ops(const uint32_t (&v)[16], int st, int t2) {
+    const uint32_t by = 2 * t2, sel = by | (4 + by) << 8 | (by + 1) << 16 | (5 + by) << 24;
+    half2v x[4], y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t w = __builtin_amdgcn_perm(v[8 * st + 2 * e + 1], v[8 * st + 2 * e], sel);
+        x[e] = f16_of_lo(w);
+        y[e] = f16_of_hi(w);
+    }
+    return ValueOps{join(x[0], x[1], x[2], x[3]), join(y[0], y[1], y[2], y[3])};
+}
+// V^T P^T of 32 keys added to acc: the operands of each product are made while the one before it runs.
 template <bool EXACT>
 __device__ __forceinline__ void add_pv(const uint32_t (&v)[16], const half8v (&hi)[2], const half8v (&lo)[2],
                                        f32x16 (&acc)[4]) {
+    ValueOps now = value_ops(v, 0, 0);
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {  // dims 4 i + 2 t2, 4 i + 2 t2 + 1
-            const uint32_t by = 2 * t2, sel = by | (4 + by) << 8 | (by + 1) << 16 | (5 + by) << 24;
-            half2v x0[4], x1[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = __builtin_amdgcn_perm(v[8 * st + 2 * e + 1], v[8 * st + 2 * e], sel);
-                x0[e] = f16_of_lo(w);
-                x1[e] = f16_of_hi(w);
-            }
-            const half8v v0 = join(x0[0], x0[1], x0[2], x0[3]), v1 = join(x1[0], x1[1], x1[2], x1[3]);
-            acc[2 * t2] = mfma32(v0, hi[st], acc[2 * t2]);
-            acc[2 * t2 + 1] = mfma32(v1, hi[st], acc[2 * t2 + 1]);
-            if constexpr (EXACT) {
-                acc[2 * t2] = mfma32(v0, lo[st], acc[2 * t2]);
-                acc[2 * t2 + 1] = mfma32(v1, lo[st], acc[2 * t2 + 1]);
-            }
-        }
+    for (int g = 0; g < 4; ++g) {
+        const int st = g >> 1, t2 = g & 1;
+        acc[2 * t2] = mfma32(now.x, hi[st], acc[2 * t2]);
+        if constexpr (EXACT) acc[2 * t2] = mfma32(now.x, lo[st], acc[2 * t2]);
+        in_order();
+        ValueOps next;
+        if (g < 3) next = value_ops(v, (g + 1) >> 1, (g + 1) & 1);
+        in_order();
+        acc[2 * t2 + 1] = mfma32(now.y, hi[st], acc[2 * t2 + 1]);
+        if constexpr (EXACT) acc[2 * t2 + 1] = mfma32(now.y, lo[st], acc[2 * t2 + 1]);
+        in_order();
+        if (g < 3) now = next;
+    }
 }
 
 // Q of a wave's columns as the B operands of S^T = K Q^T: f16 values, and what they leave over, as f16 values
@@ -550,25 +565,40 @@ struct QueryOps {
     i32x8 lo8[EXACT ? 1 : 2];
 };
 constexpr int kLoScale = 127 - 11;  // 2^-11 as an exponent byte
-template <bool EXACT>
-__device__ __forceinline__ f32x16 scores(const u32x4 (&kw)[4], const QueryOps<EXACT>& q) {
+__device__ __forceinline__ half8v key_op(const u32x4 (&kw)[4], int i) {
+    const uint32_t w0 = kw[i >> 1][2 * (i & 1)], w1 = kw[i >> 1][2 * (i & 1) + 1];
+    return join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
+}
+// S^T of 32 keys, and beside it `work(0)` .. `work(9)`, vector instructions that do not depend on it.
+template <bool EXACT, typename W>
+__device__ __forceinline__ f32x16 scores(const u32x4 (&kw)[4], const QueryOps<EXACT>& q, W work) {
     f32x16 s;
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = 0.0f;
+    half8v now, next;
     if constexpr (!EXACT) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const u32x4 a = kw[2 * i], b = kw[2 * i + 1];
             const i32x8 k = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
             s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q.lo8[i], s, 0, 0, 0, 127, 0, kLoScale);
+            in_order();
+            if (i == 1) now = key_op(kw, 0);
+            work(i);
+            in_order();
         }
+    } else {
+        now = key_op(kw, 0);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t w0 = kw[i >> 1][2 * (i & 1)], w1 = kw[i >> 1][2 * (i & 1) + 1];
-        const half8v ka = join(f16_of_lo(w0), f16_of_hi(w0), f16_of_lo(w1), f16_of_hi(w1));
-        s = mfma32(ka, q.hi[i], s);
-        if constexpr (EXACT) s = mfma32(ka, q.lo[i], s);
+        s = mfma32(now, q.hi[i], s);
+        if constexpr (EXACT) s = mfma32(now, q.lo[i], s);
+        in_order();
+        if (i < 7) next = key_op(kw, i + 1);
+        work(i + 2);
+        in_order();
+        now = next;
     }
     return s;
 }
@@ -669,27 +699,28 @@ attend_kernel(AttendArgs a) {
 
         u32x4 kw[4];      // key 32 half + c, dims 32 i + 16 h .. + 16
         uint32_t vw[16];  // key 32 half + 8 q + 4 h + r at 4 q + r, dims 4 c .. + 4
-        auto load_k = [&](size_t tile, int half) {
-            const uint8_t* p = a.p.k + tile * kTileBytes8 + (32 * half + c) * kDim + 16 * h;
+        const uint32_t k_at = c * kDim + 16 * h, v_at = 4 * h * kDim + 4 * c;  // of this lane, from a half page on
+        auto load_k = [&](uint32_t tile, int half) {
+            const uint8_t* p = a.p.k + (size_t)tile * kTileBytes8 + 32 * half * kDim;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(p + 32 * i);
+            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(p + k_at + 32 * i);
         };
-        auto load_v = [&](size_t tile, int half) {
-            const uint8_t* p = a.p.v + tile * kTileBytes8 + (32 * half + 4 * h) * kDim + 4 * c;
+        auto load_v = [&](uint32_t tile, int half) {
+            const uint8_t* p = a.p.v + (size_t)tile * kTileBytes8 + 32 * half * kDim;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                vw[i] = *reinterpret_cast<const uint32_t*>(p + (8 * (i >> 2) + (i & 3)) * kDim);
+                vw[i] = *reinterpret_cast<const uint32_t*>(p + v_at + (8 * (i >> 2) + (i & 3)) * kDim);
         };
         // a page that is not there reads page 0 in its place
         auto tile_of = [&](int id, bool& there) {
             there = id >= 0 && id < a.p.pages;
-            return (size_t)(there ? id : 0) * a.p.hkv + kh;
+            return (uint32_t)(there ? id : 0) * a.p.hkv + kh;  // (a layer has at most 2^31 of them)
         };
 
         if (!nowhere) {
             int page = p0;
             bool there, there_next = true;
-            size_t tile = tile_of(ids[page], there), tile_next = tile;
+            uint32_t tile = tile_of(ids[page], there), tile_next = tile;
             load_k(tile, 0);
             load_v(tile, 0);
             int kx = scalar_byte(a.p.kx, tile), vx = scalar_byte(a.p.vx, tile), kx_next = kx, vx_next = vx;
@@ -697,7 +728,7 @@ attend_kernel(AttendArgs a) {
             int id = page + 1 < p1 ? ids[page + 1] : 0;  // of the page after this one
             // the scores of the half page at hand: of key k0 + 8 q + 4 h + r and column c, in units of
             // log2 and of 2^(qx + kx - 127)
-            f32x16 s = scores(kw, q);
+            f32x16 s = scores(kw, q, [](int) {});
             load_k(tile, 1);
 
             // One half page: its weights, the scores of the next, and its share of the sums. The next page's K
@@ -745,44 +776,51 @@ attend_kernel(AttendArgs a) {
                 const int less = min(vref - vx, 100);
                 // (a column that has seen no key yet: its scores are all -inf, and p 0)
                 const float mb = m_used == -INFINITY ? 0.0f : 7.0f - (float)less - m_used;
-                __builtin_amdgcn_sched_barrier(0);
+                in_order();
                 f32x16 next;
-                if constexpr (!EXACT) next = scores(kw, q);
                 float p[16], psum = 0.0f;
                 half8v ph[2], pl[2];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                auto weigh = [&](int i) {
                     p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sc, mb));
-                    psum += p[i];
-                }
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    half2v u[4], w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if constexpr (EXACT) split(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], u[e], w[e]);
-                        else u[e] = half2v{(_Float16)p[8 * st + 2 * e], (_Float16)p[8 * st + 2 * e + 1]};
+                };
+                auto pack = [&](int i) {  // weights 2 i, 2 i + 1
+                    half2v u, w;
+                    if constexpr (EXACT) {
+                        split(p[2 * i], p[2 * i + 1], u, w);
+                        pl[i >> 2][2 * (i & 3)] = w.x;
+                        pl[i >> 2][2 * (i & 3) + 1] = w.y;
+                    } else {
+                        u = half2v{(_Float16)p[2 * i], (_Float16)p[2 * i + 1]};
                     }
-                    ph[st] = join(u[0], u[1], u[2], u[3]);
-                    if constexpr (EXACT) pl[st] = join(w[0], w[1], w[2], w[3]);
+                    ph[i >> 2][2 * (i & 3)] = u.x;
+                    ph[i >> 2][2 * (i & 3) + 1] = u.y;
+                    psum += p[2 * i];
+                    psum += p[2 * i + 1];
+                };
+                if constexpr (EXACT) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) weigh(i);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pack(i);
+                } else {
+                    next = scores(kw, q, [&](int i) {
+                        if (i < 2) {
+                            weigh(4 * i);
+                            weigh(4 * i + 1);
+                            weigh(4 * i + 2);
+                            weigh(4 * i + 3);
+                        } else {
+                            weigh(6 + i);
+                            pack(i - 2);
+                        }
+                    });
                 }
                 // (here, among the products, not sunk behind the branch below)
                 asm volatile("" : "+v"(ph[0]), "+v"(ph[1]), "+v"(psum));
                 lsum = fmaf(psum, ldexpf(1.0f, less), lsum);
-                if constexpr (!EXACT) {
-                    // the products first ask for no conversion; then one after each seven vector instructions
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x402, 14, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        __builtin_amdgcn_sched_group_barrier(0x402, 10, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                in_order();
                 if (!EXACT && more) load_k(tile_next, half);
-                __builtin_amdgcn_sched_barrier(0);
+                in_order();
                 if (odd) {
                     // NaN values that some columns see and others do not: 0 in the product, and NaN for the
                     // columns at or past the first such key of the dim
@@ -807,13 +845,13 @@ attend_kernel(AttendArgs a) {
                             if (s_nan[wave][4 * (8 * (i >> 2) + 4 * h + (i & 3)) + d] <= limit) acc[d][i] = NAN;
                 }
                 add_pv<EXACT>(vw, ph, pl, acc);
-                __builtin_amdgcn_sched_barrier(0);
+                in_order();
                 if (half == 0) load_v(tile, 1);
                 else if (more) load_v(tile_next, 0);
-                __builtin_amdgcn_sched_barrier(0);
+                in_order();
                 if constexpr (EXACT) {
-                    next = scores(kw, q);
-                    __builtin_amdgcn_sched_barrier(0);
+                    next = scores(kw, q, [](int) {});
+                    in_order();
                     if (more) load_k(tile_next, half);
                 }
                 s = next;
