@@ -422,7 +422,7 @@ attend_plan_kernel(PlanArgs a) {
 // needs eight keys of one dim in a lane, which byte permutes pair up from four dims of each key
 // before the conversion. No wave waits for another.
 struct AttendArgs {
-    const uint8_t* ws;
+    uint8_t* ws;
     size_t ws_len;
     const float* q;
     PoolArgs p;  // of one layer
@@ -451,8 +451,8 @@ __device__ __forceinline__ Plan load_plan(const AttendArgs& a) {
     p.tile = reinterpret_cast<const Tile*>(a.ws + h.at.tiles);
     p.merge = reinterpret_cast<const int*>(a.ws + h.at.merges);
     p.rows = reinterpret_cast<const int*>(a.ws + h.at.rows);
-    p.ml = reinterpret_cast<float*>(const_cast<uint8_t*>(a.ws) + h.at.ml);
-    p.acc = reinterpret_cast<float*>(const_cast<uint8_t*>(a.ws) + h.at.acc);
+    p.ml = reinterpret_cast<float*>(a.ws + h.at.ml);
+    p.acc = reinterpret_cast<float*>(a.ws + h.at.acc);
     return p;
 }
 
@@ -502,15 +502,16 @@ __device__ __forceinline__ float part_weight(float m, float top) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 }
 // x times 1 / l, in o's type
-__device__ __forceinline__ void write_o(const AttendArgs& a, size_t at, f32x4 x, float inv) {
+template <bool F16>
+__device__ __forceinline__ void write_o(void* o, size_t at, f32x4 x, float inv) {
     f32x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = x[e] * inv;
-    if (a.o_f16) {
+    if (F16) {
         u32x2 w = {f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + at) = w;
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(o) + at) = w;
     } else {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + at) = y;
+        *reinterpret_cast<f32x4*>(static_cast<float*>(o) + at) = y;
     }
 }
 
@@ -608,36 +609,53 @@ __global__ void __launch_bounds__(kThreads, 2)
 attend_kernel(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) int s_nan[kWaves][kDim];  // first key with a NaN value, for each dim
 
-    const Plan plan = load_plan(a);
-    if (!plan.fits) return;
-    const Header& head = plan.head;
+    if (!load_plan(a).fits) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv * kWaves + wave;
-    const long long lo = run * head.size, end = min(lo + head.size, head.total);
-    if (run >= head.runs || lo >= end) return;
+    // The arguments and the header are read again where they are needed: held in scalar registers over
+    // the loop they would crowd out its own.
+    auto args = [] { return (Scalar<AttendArgs>)again(__builtin_amdgcn_kernarg_segment_ptr()); };
+    auto header = [&] { return (Scalar<Header>)(uintptr_t)args()->ws; };
+    if (run >= header()->runs || run * header()->size >= header()->total) return;
 
-    for (int ti = scalar(plan.run_tile)[run]; ti < head.tiles; ++ti) {
-        const Tile t = load_tile(plan.tile + ti);
-        if (t.start >= end) break;
+    for (int ti = *(Scalar<int>)(uintptr_t)(args()->ws + header()->at.run_tile + 4 * (size_t)run); ti < header()->tiles; ++ti) {
         // ---- this run's pages of the tile ------------------------------------------------------------
-        const int p0 = t.b0 + (int)max(lo - t.start, 0LL), p1 = min(t.b0 + (int)min(end - t.start, (long long)INT_MAX / 2), t.b1);
-        if (p0 >= p1) continue;  // (its pages are the next run's)
-        const bool prefix = t.kind & kPrefix, nowhere = t.kind & kBad;
-        const Scalar<int> ids = scalar(a.table + (size_t)t.seq * a.width);
+        int p0, p1, row0, col0, cols, pos0, kind;
+        Scalar<int> ids;
+        {
+            const auto g = args();
+            const auto hd = header();
+            const Tile t = load_tile(reinterpret_cast<const Tile*>(g->ws + hd->at.tiles) + ti);
+            const long long lo = run * hd->size, end = min(lo + hd->size, (long long)hd->total);
+            if (t.start >= end) break;
+            p0 = t.b0 + (int)max(lo - t.start, 0LL);
+            p1 = min(t.b0 + (int)min(end - t.start, (long long)INT_MAX / 2), t.b1);
+            if (p0 >= p1) continue;  // (its pages are the next run's)
+            ids = scalar(g->table + (size_t)t.seq * g->width);
+            row0 = t.row0;
+            col0 = t.col0;
+            cols = t.cols;
+            pos0 = t.pos0;
+            kind = t.kind;
+        }
+        const bool nowhere = kind & kBad;
 
-        // ---- Q: hi and lo halves of q / sqrt(128) * log2 e, each column's exponent taken out -----------
-        const int col = t.col0 + min(c, t.cols - 1);  // (lanes past the last column repeat it)
-        const int local = col / a.per_row;
-        const int row = prefix ? plan.rows[t.row0 + local] : t.row0 + local;
-        const int head_of = kh * a.per_row + col - local * a.per_row;
-        const int limit = prefix ? INT_MAX : nowhere ? -1 : t.pos0 + local;  // the last position it sees
+        // ---- Q: hi and lo parts of q / sqrt(128) * log2 e, each column's exponent taken out ------------
+        int limit;  // the last position this lane's column sees
         QueryOps<EXACT> q;
         int qx;
         {
+            const auto g = args();
+            const int col = col0 + min(c, cols - 1);  // (lanes past the last column repeat it)
+            const int local = col / g->per_row;
+            int row = row0 + local;
+            if (kind & kPrefix) row = reinterpret_cast<const int*>(g->ws + header()->at.rows)[row];
+            const int head_of = kh * g->per_row + col - local * g->per_row;
+            limit = kind & kPrefix ? INT_MAX : nowhere ? -1 : pos0 + local;
             // step s holds dims 32 (s / 2) + 16 h + 8 (s % 2) .. + 8, as K's 16-byte loads do
-            const float* qrow = a.q + ((size_t)row * a.hq + head_of) * kDim + 16 * h;
+            const float* qrow = g->q + ((size_t)row * g->hq + head_of) * kDim + 16 * h;
             const float scale = 0.08838834764831845f * kLog2e;
             float x[8][8];
             float qmax = 0.0f;
@@ -695,7 +713,6 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
         int vref = 0;     // acc stands in units of 2^(vref - 127)
-        bool bad = nowhere;
 
         u32x4 kw[4];      // key 32 half + c, dims 32 i + 16 h .. + 16
         uint32_t vw[16];  // key 32 half + 8 q + 4 h + r at 4 q + r, dims 4 c .. + 4
@@ -741,12 +758,14 @@ attend_kernel(AttendArgs a) {
                 if (!there) lsum = limit >= page * kPage ? NAN : lsum;
                 bool odd = false;  // V holds NaN codes that not all columns see
                 if (k0 + 31 > lim0) {  // some column does not see all of these keys
+                    // (keys counted from k0 + 4 h, so that they are constants)
+                    const int last = limit - k0 - 4 * h, last1 = lim1 - k0 - 4 * h;
                     uint32_t nans = 0;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int key = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
-                        if (key > limit) s[i] = -INFINITY;
-                        if (key > lim1) vw[i] = 0;  // the codes behind the last key may be anything
+                        const int key = 8 * (i >> 2) + (i & 3);
+                        if (key > last) s[i] = -INFINITY;
+                        if (key > last1) vw[i] = 0;  // the codes behind the last key may be anything
                         nans |= nan_codes(vw[i]);
                     }
                     odd = __builtin_amdgcn_ballot_w64(nans != 0);
@@ -824,25 +843,30 @@ attend_kernel(AttendArgs a) {
                 if (odd) {
                     // NaN values that some columns see and others do not: 0 in the product, and NaN for the
                     // columns at or past the first such key of the dim
-                    int low[4] = {INT_MAX, INT_MAX, INT_MAX, INT_MAX};
+                    int low[4] = {64, 64, 64, 64};  // (no key)
 #pragma unroll
                     for (int i = 15; i >= 0; --i) {
                         const uint32_t w = nan_codes(vw[i]);
 #pragma unroll
                         for (int d = 0; d < 4; ++d)
-                            if (w >> 8 * d & 0x80u) low[d] = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                            if (w >> 8 * d & 0x80u) low[d] = 8 * (i >> 2) + (i & 3);
                         vw[i] &= ~((w >> 7) * 0xffu);
+                        in_order();
                     }
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        const auto b = __builtin_amdgcn_permlane32_swap(low[d], low[d], false, false);
+                        const int key = low[d] + 4 * h;
+                        const auto b = __builtin_amdgcn_permlane32_swap(key, key, false, false);
                         s_nan[wave][4 * c + d] = min((int)b[0], (int)b[1]);
                     }
+                    const int last = min(limit - k0, 31);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
+                    for (int i = 0; i < 16; ++i) {
 #pragma unroll
                         for (int d = 0; d < 4; ++d)
-                            if (s_nan[wave][4 * (8 * (i >> 2) + 4 * h + (i & 3)) + d] <= limit) acc[d][i] = NAN;
+                            if (s_nan[wave][4 * (8 * (i >> 2) + 4 * h + (i & 3)) + d] <= last) acc[d][i] = NAN;
+                        in_order();
+                    }
                 }
                 add_pv<EXACT>(vw, ph, pl, acc);
                 in_order();
@@ -876,28 +900,31 @@ attend_kernel(AttendArgs a) {
             }
         }
         // (a row past the table's width has no page)
-        if (bad || (!prefix && limit >= a.width * kPage)) lsum = NAN;
+        const auto g = args();
+        if (nowhere || (!(kind & kPrefix) && limit >= g->width * kPage)) lsum = NAN;
         lsum = sum_h(lsum);
         const float unit = ldexpf(1.0f, vref - 127);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] *= unit;
 
         // ---- out: to o, or to the parts. The lane holds dims 4 (8 q + 4 h + r) + t of its column ----------
-        if (c >= t.cols) continue;
-        if (t.kind & kDirect) {
-            const int local = col / a.per_row;  // (a prefix tile is never direct)
-            const size_t at = ((size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row) * kDim;
+        if (c >= cols) continue;
+        if (kind & kDirect) {
+            const int col = col0 + c, local = col / g->per_row;  // (a prefix tile is never direct)
+            const size_t at = ((size_t)(row0 + local) * g->hq + kh * g->per_row + col - local * g->per_row) * kDim;
             const float inv = 1.0f / lsum;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                write_o(a, at + 4 * (8 * (i >> 2) + 4 * h + (i & 3)), f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]}, inv);
+                write_o<!EXACT>(g->o, at + 4 * (8 * (i >> 2) + 4 * h + (i & 3)), f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]}, inv);
         } else {
-            const size_t part = (size_t)kh * head.at.cap + t.base + (size_t)(run - t.run0) * t.cols + c;
+            const auto hd = header();
+            const auto t = (Scalar<Tile>)(uintptr_t)(g->ws + hd->at.tiles) + ti;
+            const size_t part = (size_t)kh * hd->at.cap + t->base + (size_t)(run - t->run0) * cols + c;
+            float* to = reinterpret_cast<float*>(g->ws + hd->at.acc) + part * kDim + 16 * h;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                *reinterpret_cast<f32x4*>(plan.acc + part * kDim + 4 * (8 * (i >> 2) + 4 * h + (i & 3))) =
-                    f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-            if (h == 0) *reinterpret_cast<f32x2*>(plan.ml + 2 * part) = f32x2{m_used, lsum};
+                *reinterpret_cast<f32x4*>(to + 4 * (8 * (i >> 2) + (i & 3))) = f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+            if (h == 0) *reinterpret_cast<f32x2*>(reinterpret_cast<float*>(g->ws + hd->at.ml) + 2 * part) = f32x2{m_used, lsum};
         }
     }
 }
@@ -1018,7 +1045,8 @@ attend_merge_kernel(AttendArgs a) {
         if (c < t.cols && (!together || (wave == 0 && h == 0))) {
             const int col = t.col0 + c, local = col / a.per_row;
             const size_t o = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
-            write_o(a, o * kDim + 4 * (lane & 31), x, 1.0f / l);
+            if (a.o_f16) write_o<true>(a.o, o * kDim + 4 * (lane & 31), x, 1.0f / l);
+            else write_o<false>(a.o, o * kDim + 4 * (lane & 31), x, 1.0f / l);
         }
     }
 }
@@ -1063,7 +1091,7 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
 int attend_launch(const float* q, const PoolArgs& pool, const int* table, int width, int n, int tokens,
                   void* ws, size_t ws_len, void* o, int o_f16, int hq, hipStream_t stream) {
     AttendArgs a = {};
-    a.ws = static_cast<const uint8_t*>(ws);
+    a.ws = static_cast<uint8_t*>(ws);
     a.ws_len = ws_len;
     a.q = q;
     a.p = pool;

@@ -33,6 +33,13 @@ template <typename T>
 using Scalar = const __attribute__((address_space(4))) T*;
 template <typename T>
 __device__ __forceinline__ Scalar<T> scalar(const T* p) { return (Scalar<T>)(uintptr_t)p; }
+// The same pointer, which the compiler does not know to be the same: what is read through it is read again.
+template <typename T>
+__device__ __forceinline__ uintptr_t again(T p) {
+    uintptr_t x = (uintptr_t)p;
+    asm volatile("" : "+s"(x));
+    return x;
+}
 // the byte at p + i (its aligned word is read)
 __device__ __forceinline__ int scalar_byte(const uint8_t* p, size_t i) {
     const uintptr_t at = (uintptr_t)(p + i);
