@@ -739,18 +739,18 @@ attend_kernel(AttendArgs a) {
             bool there, there_next = true;
             uint32_t tile = tile_of(ids[page], there), tile_next = tile;
             load_k(tile, 0);
-            load_v(tile, 0);
             int kx = scalar_byte(a.p.kx, tile), vx = scalar_byte(a.p.vx, tile), kx_next = kx, vx_next = vx;
             vref = vx;
-            int id = page + 1 < p1 ? ids[page + 1] : 0;  // of the page after this one
+            int id = ids[min(page + 1, p1 - 1)];  // of the page after this one
             // the scores of the half page at hand: of key k0 + 8 q + 4 h + r and column c, in units of
             // log2 and of 2^(qx + kx - 127)
             f32x16 s = scores(kw, q, [](int) {});
             load_k(tile, 1);
+            load_v(tile, 0);  // (behind K, as in the loop: the waits for K then leave it on its way)
 
             // One half page: its weights, the scores of the next, and its share of the sums. The next page's K
             // (or this one's second half) takes the registers of the K just used, V later V's.
-            auto half_page = [&](auto HALF, bool more) {
+            auto half_page = [&](auto HALF) {
                 constexpr int half = HALF;
                 const int k0 = page * kPage + 32 * half;
                 // (past the clamp every score is 0, or so far from the next that one key takes all)
@@ -838,7 +838,7 @@ attend_kernel(AttendArgs a) {
                 asm volatile("" : "+v"(ph[0]), "+v"(ph[1]), "+v"(psum));
                 lsum = fmaf(psum, ldexpf(1.0f, less), lsum);
                 in_order();
-                if (!EXACT && more) load_k(tile_next, half);
+                if constexpr (!EXACT) load_k(tile_next, half);
                 in_order();
                 if (odd) {
                     // NaN values that some columns see and others do not: 0 in the product, and NaN for the
@@ -870,27 +870,25 @@ attend_kernel(AttendArgs a) {
                 }
                 add_pv<EXACT>(vw, ph, pl, acc);
                 in_order();
-                if (half == 0) load_v(tile, 1);
-                else if (more) load_v(tile_next, 0);
+                load_v(half ? tile_next : tile, half ^ 1);
                 in_order();
                 if constexpr (EXACT) {
                     next = scores(kw, q, [](int) {});
                     in_order();
-                    if (more) load_k(tile_next, half);
+                    load_k(tile_next, half);
                 }
                 s = next;
             };
             while (true) {
+                // (behind the last page comes the same again, and is not used: a load that might not be on its
+                // way would have every wait behind it wait for all of them)
                 const bool more = page + 1 < p1;
-                if (more) {
-                    tile_next = tile_of(id, there_next);
-                    kx_next = scalar_byte(a.p.kx, tile_next);
-                    vx_next = scalar_byte(a.p.vx, tile_next);
-                    id = page + 2 < p1 ? ids[page + 2] : 0;
-                }
-                half_page(std::integral_constant<int, 0>{}, more);
-                // (behind the last page the next scores are of the keys at hand again, and not used)
-                half_page(std::integral_constant<int, 1>{}, more);
+                if (more) tile_next = tile_of(id, there_next);
+                kx_next = scalar_byte(a.p.kx, tile_next);
+                vx_next = scalar_byte(a.p.vx, tile_next);
+                id = ids[min(page + 2, p1 - 1)];
+                half_page(std::integral_constant<int, 0>{});
+                half_page(std::integral_constant<int, 1>{});
                 if (!more) break;
                 ++page;
                 there = there_next;
