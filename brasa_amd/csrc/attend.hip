@@ -415,12 +415,15 @@ attend_plan_kernel(PlanArgs a) {
 
 // ---- tiles --------------------------------------------------------------------------------------
 //
-// A wave holds 32 columns and takes 32 keys (half a page) at a time, all of it in registers: K's codes
-// are converted exactly (an e4m3 value is an f16 value) from the loaded pieces into the A operand of
-// S^T = K Q^T on 32x32x16 f16 MFMAs, once with the hi and once with the lo halves of q (22 bits
-// together). S^T's layout is the B operand of O^T += V^T P^T, P in hi and lo halves again; V's operand
-// needs eight keys of one dim in a lane, which byte permutes pair up from four dims of each key
-// before the conversion. No wave waits for another.
+// A wave holds 32 columns and takes 32 keys (half a page) at a time, on its own: no wave waits for another.
+// K's and V's codes are copied into the wave's LDS, one half page ahead, in pieces of 16 bytes (a vector
+// memory instruction costs a CU about 20 cycles whatever its width, and V by 4 bytes a lane, as its
+// operand wants them, took 16 for a half page: 410 of 560 us of a pass were loads). Rows are swizzled:
+// 16-byte piece c of row r stands in place c ^ (r & 7), so that rows are read and transposed without
+// bank conflicts. K's codes are converted exactly (an e4m3 value is an f16 value) into the A operand of
+// S^T = K Q^T on 32x32x16 f16 MFMAs. S^T's layout is the B operand of O^T += V^T P^T: lane (c, h) holds
+// keys 16 st + 8 (j / 4) + 4 h + j % 4 of column c, j < 8, and V's rows stand in LDS in that order, so that
+// ds_read_b64_tr_b8 gives a lane eight keys of one dim at once.
 struct AttendArgs {
     uint8_t* ws;
     size_t ws_len;
@@ -519,40 +522,60 @@ __device__ __forceinline__ void write_o(void* o, size_t at, f32x4 x, float inv) 
 // instructions that run beside them.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// V^T's operands of 16 keys and dims 4 i + 2 t2 (x), 4 i + 2 t2 + 1 (y) of lane i. v[4 q + r]: four codes (dims 4 i .. + 4)
-// of key 8 q + 4 h + r.
-struct ValueOps {
-    half8v x, y;
-};
-__device__ __forceinline__ ValueOps value_ops(const uint32_t (&v)[16], int st, int t2) {
-    const uint32_t by = 2 * t2, sel = by | (4 + by) << 8 | (by + 1) << 16 | (5 + by) << 24;
-    half2v x[4], y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t w = __builtin_amdgcn_perm(v[8 * st + 2 * e + 1], v[8 * st + 2 * e], sel);
-        x[e] = f16_of_lo(w);
-        y[e] = f16_of_hi(w);
-    }
-    return ValueOps{join(x[0], x[1], x[2], x[3]), join(y[0], y[1], y[2], y[3])};
+// Half a page's codes from p on (this lane's share of it) into the LDS at `to`, whole: K's row r to row r.
+__device__ __forceinline__ void copy_keys(const uint8_t* p, uint32_t to) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "global_load_lds_dwordx4 %1, off offset:1024\n\t"
+        "global_load_lds_dwordx4 %1, off offset:2048\n\t"
+        "global_load_lds_dwordx4 %1, off offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(p), "s"(to)
+        : "memory");
 }
-// V^T P^T of 32 keys added to acc: the operands of each product are made while the one before it runs.
+// V's row of key 16 st + 8 (j / 4) + 4 h + j % 4 to row 16 st + 8 h + j (an instruction's offset counts in
+// memory and in LDS; the second half's 512 bytes in memory are 1024 in LDS).
+__device__ __forceinline__ void copy_values(const uint8_t* p, uint32_t to) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "global_load_lds_dwordx4 %1, off offset:2048\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off offset:512\n\t"
+        "global_load_lds_dwordx4 %1, off offset:2560\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(p), "s"(to), "s"(to + 512)
+        : "memory");
+}
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+// eight codes of one dim -> f16 values
+__device__ __forceinline__ half8v value_op(i32x2 w) {
+    return join(f16_of_lo(w.x), f16_of_hi(w.x), f16_of_lo(w.y), f16_of_hi(w.y));
+}
+// V^T P^T of 32 keys added to acc (rows 32 t .. + 32 of V^T in acc[t]): the operand of each product is made while
+// the one before it runs.
 template <bool EXACT>
-__device__ __forceinline__ void add_pv(const uint32_t (&v)[16], const half8v (&hi)[2], const half8v (&lo)[2],
+__device__ __forceinline__ void add_pv(const i32x2 (&v)[2][4], const half8v (&hi)[2], const half8v (&lo)[2],
                                        f32x16 (&acc)[4]) {
-    ValueOps now = value_ops(v, 0, 0);
+    half8v now = value_op(v[0][0]);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int st = g >> 1, t2 = g & 1;
-        acc[2 * t2] = mfma32(now.x, hi[st], acc[2 * t2]);
-        if constexpr (EXACT) acc[2 * t2] = mfma32(now.x, lo[st], acc[2 * t2]);
+    for (int i = 0; i < 8; ++i) {
+        const int st = i >> 2, t = i & 3;
+        acc[t] = mfma32(now, hi[st], acc[t]);
+        if constexpr (EXACT) acc[t] = mfma32(now, lo[st], acc[t]);
         in_order();
-        ValueOps next;
-        if (g < 3) next = value_ops(v, (g + 1) >> 1, (g + 1) & 1);
+        if (i < 7) now = value_op(v[(i + 1) >> 2][(i + 1) & 3]);
         in_order();
-        acc[2 * t2 + 1] = mfma32(now.y, hi[st], acc[2 * t2 + 1]);
-        if constexpr (EXACT) acc[2 * t2 + 1] = mfma32(now.y, lo[st], acc[2 * t2 + 1]);
-        in_order();
-        if (g < 3) now = next;
     }
 }
 
@@ -604,11 +627,54 @@ __device__ __forceinline__ f32x16 scores(const u32x4 (&kw)[4], const QueryOps<EX
     return s;
 }
 
+// A half page that not all columns see whole: V's rows behind the last key that any sees become zeros in
+// LDS (whatever stands there), and NaN values that some columns see and others do not become 0 there and
+// NaN in the sums of the columns that see them. `last1`, `last`: the last key that any column, and this
+// lane's, sees, from the half page's first on. Rare: one or two half pages of a sequence.
+__device__ __forceinline__ uint64_t hidden_rows(uint8_t* v, int* first, int last1) {
+    const int lane = threadIdx.x & 63;
+    // two lanes a row, four pieces of 16 bytes each
+    const int row = lane >> 1, j = row & 7;
+    const int key = 16 * (row >> 4) + 8 * (j >> 2) + 4 * (row >> 3 & 1) + (j & 3);
+    u32x4* at = reinterpret_cast<u32x4*>(v + row * kDim + 64 * (lane & 1));
+    first[lane] = first[lane + 64] = 64;  // (no key)
+    uint32_t nans = 0;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+        u32x4 w = at[i];
+        if (key > last1) w = u32x4{0, 0, 0, 0};
+        const int dim = 16 * ((4 * (lane & 1) + i) ^ j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t n = nan_codes(w[e]);
+            nans |= n;
+#pragma unroll 1
+            for (int b = 0; n && b < 4; ++b)
+                if (n >> 8 * b & 0x80u) atomicMin(&first[dim + 4 * e + b], key);
+            w[e] &= ~((n >> 7) * 0xffu);
+        }
+        at[i] = w;
+    }
+    return __builtin_amdgcn_ballot_w64(nans != 0);
+}
+__device__ __forceinline__ void hide_values(uint8_t* v, int* first, int last1, int last, f32x16 (&acc)[4]) {
+    if (!hidden_rows(v, first, last1)) return;
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (first[32 * (i >> 2) + 8 * (i & 3) + 4 * h + r] <= min(last, 63)) acc[i >> 2][4 * (i & 3) + r] = NAN;
+        in_order();
+    }
+}
+
 template <bool EXACT>
 __global__ void __launch_bounds__(kThreads, 2)
 attend_kernel(AttendArgs a) {
+    constexpr int kHalf = 32 * kDim;  // codes of half a page
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[kWaves][2][kHalf], s_v[kWaves][2][kHalf];
     __shared__ __attribute__((aligned(16))) int s_nan[kWaves][kDim];  // first key with a NaN value, for each dim
-
     if (!load_plan(a).fits) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -714,19 +780,30 @@ attend_kernel(AttendArgs a) {
             for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
         int vref = 0;     // acc stands in units of 2^(vref - 127)
 
-        u32x4 kw[4];      // key 32 half + c, dims 32 i + 16 h .. + 16
-        uint32_t vw[16];  // key 32 half + 8 q + 4 h + r at 4 q + r, dims 4 c .. + 4
-        const uint32_t k_at = c * kDim + 16 * h, v_at = 4 * h * kDim + 4 * c;  // of this lane, from a half page on
+        // this lane's share of a half page's copies, and where it reads them
+        const uint32_t j8 = lane >> 3, piece = ((lane & 7) ^ j8) * 16;
+        const uint32_t k_from = j8 * kDim + piece, v_from = 1024 * (j8 >> 2) + kDim * (j8 & 3) + piece;
+        const uint32_t k_at = c * kDim + ((h ^ (c & 7)) * 16), jv = (lane & 15) >> 1;
+        const uint32_t v_at = (8 * h + jv) * kDim + 8 * (lane & 1) + ((((lane >> 4) & 1) ^ jv) * 16);
+        const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_k[wave]));
+        const uint32_t v_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_v[wave]));
         auto load_k = [&](uint32_t tile, int half) {
-            const uint8_t* p = a.p.k + (size_t)tile * kTileBytes8 + 32 * half * kDim;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(p + k_at + 32 * i);
+            copy_keys(a.p.k + (size_t)tile * kTileBytes8 + half * kHalf + k_from, k_lds + half * kHalf);
         };
         auto load_v = [&](uint32_t tile, int half) {
-            const uint8_t* p = a.p.v + (size_t)tile * kTileBytes8 + 32 * half * kDim;
+            copy_values(a.p.v + (size_t)tile * kTileBytes8 + half * kHalf + v_from, v_lds + half * kHalf);
+        };
+        u32x4 kw[4];    // key c, dims 32 i + 16 h .. + 16
+        i32x2 vw[2][4]; // keys 16 st + 8 (j / 4) + 4 h + j % 4 of dim 32 t + c at [st][t]
+        auto read_k = [&](int half) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                vw[i] = *reinterpret_cast<const uint32_t*>(p + v_at + (8 * (i >> 2) + (i & 3)) * kDim);
+            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(&s_k[wave][half][k_at ^ 32 * i]);
+        };
+        auto read_v = [&](int half) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                vw[i >> 2][i & 3] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2*)&s_v[wave][half][2048 * (i >> 2) + (v_at ^ 32 * (i & 3))]);
         };
         // a page that is not there reads page 0 in its place
         auto tile_of = [&](int id, bool& there) {
@@ -739,36 +816,46 @@ attend_kernel(AttendArgs a) {
             bool there, there_next = true;
             uint32_t tile = tile_of(ids[page], there), tile_next = tile;
             load_k(tile, 0);
+            load_k(tile, 1);
+            load_v(tile, 0);
             int kx = scalar_byte(a.p.kx, tile), vx = scalar_byte(a.p.vx, tile), kx_next = kx, vx_next = vx;
             vref = vx;
             int id = ids[min(page + 1, p1 - 1)];  // of the page after this one
             // the scores of the half page at hand: of key k0 + 8 q + 4 h + r and column c, in units of
             // log2 and of 2^(qx + kx - 127)
+            wait_vmcnt<8>();
+            read_k(0);
             f32x16 s = scores(kw, q, [](int) {});
-            load_k(tile, 1);
-            load_v(tile, 0);  // (behind K, as in the loop: the waits for K then leave it on its way)
 
-            // One half page: its weights, the scores of the next, and its share of the sums. The next page's K
-            // (or this one's second half) takes the registers of the K just used, V later V's.
-            auto half_page = [&](auto HALF) {
+            // One half page: its weights, the scores of the next, and its share of the sums. K of the half
+            // after the next and V of the next go on their way first: into the places of what has been used.
+            auto half_page = [&](auto HALF, bool more) {
                 constexpr int half = HALF;
                 const int k0 = page * kPage + 32 * half;
+                if (half == 0) {
+                    if (more) load_k(tile_next, 0);
+                    load_v(tile, 1);
+                    if (more) wait_vmcnt<8>();
+                    else wait_vmcnt<4>();
+                } else if (more) {
+                    load_k(tile_next, 1);
+                    load_v(tile_next, 0);
+                    wait_vmcnt<8>();
+                } else {
+                    wait_vmcnt<0>();
+                }
+                // (behind the last page K is an earlier one's, and its scores are not used)
+                read_k(half ^ 1);
                 // (past the clamp every score is 0, or so far from the next that one key takes all)
                 const float sc = ldexpf(1.0f, min(max(qx + kx - 127, -126), 127));
                 if (!there) lsum = limit >= page * kPage ? NAN : lsum;
-                bool odd = false;  // V holds NaN codes that not all columns see
                 if (k0 + 31 > lim0) {  // some column does not see all of these keys
                     // (keys counted from k0 + 4 h, so that they are constants)
-                    const int last = limit - k0 - 4 * h, last1 = lim1 - k0 - 4 * h;
-                    uint32_t nans = 0;
+                    const int last = limit - k0 - 4 * h;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = 8 * (i >> 2) + (i & 3);
-                        if (key > last) s[i] = -INFINITY;
-                        if (key > last1) vw[i] = 0;  // the codes behind the last key may be anything
-                        nans |= nan_codes(vw[i]);
-                    }
-                    odd = __builtin_amdgcn_ballot_w64(nans != 0);
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (i >> 2) + (i & 3) > last) s[i] = -INFINITY;
+                    hide_values(s_v[wave][half], s_nan[wave], lim1 - k0, limit - k0, acc);
                 }
                 float top = s[0];
 #pragma unroll
@@ -816,79 +903,41 @@ attend_kernel(AttendArgs a) {
                     psum += p[2 * i];
                     psum += p[2 * i + 1];
                 };
-                if constexpr (EXACT) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) weigh(i);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) pack(i);
-                } else {
-                    next = scores(kw, q, [&](int i) {
-                        if (i < 2) {
+                read_v(half);
+                next = scores(kw, q, [&](int i) {
+                    if (i < 2) {
+                        if constexpr (!EXACT) {
                             weigh(4 * i);
                             weigh(4 * i + 1);
                             weigh(4 * i + 2);
                             weigh(4 * i + 3);
-                        } else {
-                            weigh(6 + i);
-                            pack(i - 2);
                         }
-                    });
-                }
+                    } else if constexpr (EXACT) {
+                        weigh(2 * i - 4);
+                        weigh(2 * i - 3);
+                        pack(i - 2);
+                    } else {
+                        weigh(6 + i);
+                        pack(i - 2);
+                    }
+                });
                 // (here, among the products, not sunk behind the branch below)
                 asm volatile("" : "+v"(ph[0]), "+v"(ph[1]), "+v"(psum));
                 lsum = fmaf(psum, ldexpf(1.0f, less), lsum);
                 in_order();
-                if constexpr (!EXACT) load_k(tile_next, half);
-                in_order();
-                if (odd) {
-                    // NaN values that some columns see and others do not: 0 in the product, and NaN for the
-                    // columns at or past the first such key of the dim
-                    int low[4] = {64, 64, 64, 64};  // (no key)
-#pragma unroll
-                    for (int i = 15; i >= 0; --i) {
-                        const uint32_t w = nan_codes(vw[i]);
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            if (w >> 8 * d & 0x80u) low[d] = 8 * (i >> 2) + (i & 3);
-                        vw[i] &= ~((w >> 7) * 0xffu);
-                        in_order();
-                    }
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        const int key = low[d] + 4 * h;
-                        const auto b = __builtin_amdgcn_permlane32_swap(key, key, false, false);
-                        s_nan[wave][4 * c + d] = min((int)b[0], (int)b[1]);
-                    }
-                    const int last = min(limit - k0, 31);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            if (s_nan[wave][4 * (8 * (i >> 2) + 4 * h + (i & 3)) + d] <= last) acc[d][i] = NAN;
-                        in_order();
-                    }
-                }
                 add_pv<EXACT>(vw, ph, pl, acc);
-                in_order();
-                load_v(half ? tile_next : tile, half ^ 1);
-                in_order();
-                if constexpr (EXACT) {
-                    next = scores(kw, q, [](int) {});
-                    in_order();
-                    load_k(tile_next, half);
-                }
                 s = next;
             };
             while (true) {
-                // (behind the last page comes the same again, and is not used: a load that might not be on its
-                // way would have every wait behind it wait for all of them)
                 const bool more = page + 1 < p1;
-                if (more) tile_next = tile_of(id, there_next);
-                kx_next = scalar_byte(a.p.kx, tile_next);
-                vx_next = scalar_byte(a.p.vx, tile_next);
-                id = ids[min(page + 2, p1 - 1)];
-                half_page(std::integral_constant<int, 0>{});
-                half_page(std::integral_constant<int, 1>{});
+                if (more) {
+                    tile_next = tile_of(id, there_next);
+                    kx_next = scalar_byte(a.p.kx, tile_next);
+                    vx_next = scalar_byte(a.p.vx, tile_next);
+                    id = ids[min(page + 2, p1 - 1)];
+                }
+                half_page(std::integral_constant<int, 0>{}, more);
+                half_page(std::integral_constant<int, 1>{}, more);
                 if (!more) break;
                 ++page;
                 there = there_next;
@@ -905,23 +954,29 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] *= unit;
 
-        // ---- out: to o, or to the parts. The lane holds dims 4 (8 q + 4 h + r) + t of its column ----------
+        // ---- out: to o, or to the parts. The lane holds dims 32 t + 8 q + 4 h + r of its column -------------
         if (c >= cols) continue;
         if (kind & kDirect) {
             const int col = col0 + c, local = col / g->per_row;  // (a prefix tile is never direct)
             const size_t at = ((size_t)(row0 + local) * g->hq + kh * g->per_row + col - local * g->per_row) * kDim;
             const float inv = 1.0f / lsum;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                write_o<!EXACT>(g->o, at + 4 * (8 * (i >> 2) + 4 * h + (i & 3)), f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]}, inv);
+            for (int i = 0; i < 16; ++i) {
+                const f32x16& x = acc[i >> 2];
+                const int r = 4 * (i & 3);
+                write_o<!EXACT>(g->o, at + 32 * (i >> 2) + 2 * r + 4 * h, f32x4{x[r], x[r + 1], x[r + 2], x[r + 3]}, inv);
+            }
         } else {
             const auto hd = header();
             const auto t = (Scalar<Tile>)(uintptr_t)(g->ws + hd->at.tiles) + ti;
             const size_t part = (size_t)kh * hd->at.cap + t->base + (size_t)(run - t->run0) * cols + c;
-            float* to = reinterpret_cast<float*>(g->ws + hd->at.acc) + part * kDim + 16 * h;
+            float* to = reinterpret_cast<float*>(g->ws + hd->at.acc) + part * kDim + 4 * h;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                *reinterpret_cast<f32x4*>(to + 4 * (8 * (i >> 2) + (i & 3))) = f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+            for (int i = 0; i < 16; ++i) {
+                const f32x16& x = acc[i >> 2];
+                const int r = 4 * (i & 3);
+                *reinterpret_cast<f32x4*>(to + 32 * (i >> 2) + 2 * r) = f32x4{x[r], x[r + 1], x[r + 2], x[r + 3]};
+            }
             if (h == 0) *reinterpret_cast<f32x2*>(reinterpret_cast<float*>(g->ws + hd->at.ml) + 2 * part) = f32x2{m_used, lsum};
         }
     }
