@@ -47,17 +47,18 @@ struct Tile {
     int base, parts;  // partials: columns base + part * cols + column; parts of it
     int run0;         // run of its first part
     int ptile, pcol;  // prefix tile and its column where the tile's first column continues; -1: none
-    int unused;
+    int index;        // its own
 };
 static_assert(sizeof(Tile) == 64, "a tile is one line");
 enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4 };
 
 // Where the plan and the partials stand in the workspace.
 struct Places {
-    size_t run_tile, tiles, merges, rows, ml, acc, bytes;
+    size_t merges, rows, ml, acc, bytes;
     long long cap;  // columns of partials, for each KV head
 };
 struct Layout : Places {
+    size_t starts, tiles;       // where hq and hkv alone say
     size_t seqs, first, group;  // the plan's own lists
     int runs, max_tiles, max_merges;
 };
@@ -100,7 +101,7 @@ Layout layout(int n, int groups, int tokens, int hq, int hkv) {
         at += up256(bytes);
         return a;
     };
-    l.run_tile = take(4 * (size_t)l.runs);
+    l.starts = take(sizeof(Tile) * (size_t)l.runs);
     l.tiles = take(sizeof(Tile) * (size_t)l.max_tiles);
     l.merges = take(4 * (size_t)l.max_merges);
     l.seqs = take(sizeof(PlanSeq) * (size_t)n);
@@ -123,7 +124,7 @@ struct PlanArgs {
     const int* group;
     const int* prefix;
     Header* head;
-    int* run_tile;
+    Tile* start;  // [runs]: the tile where each run starts
     Tile* tile;
     int* merge;
     PlanSeq* seq;
@@ -345,7 +346,7 @@ attend_plan_kernel(PlanArgs a) {
                 t.pcol = (s.scol - gcol0) % kCols;
             }
         }
-        t.unused = 0;
+        t.index = at;
         return t;
     };
 
@@ -380,7 +381,7 @@ attend_plan_kernel(PlanArgs a) {
         if (!on) continue;
         a.tile[at] = t;
         // the runs that start in it, or in the pages' worth before it
-        for (int w = (int)div_by(t.start - kOver + size - 1, size, inv); w <= last; ++w) a.run_tile[w] = at;
+        for (int w = (int)div_by(t.start - kOver + size - 1, size, inv); w <= last; ++w) a.start[w] = t;
         if (!(t.kind & (kPrefix | kDirect))) {
             int parts = t.parts;
             if (t.ptile >= 0) parts += (int)div_by(t.b0, size, inv) + 1;  // (about: the prefix tile's)
@@ -402,8 +403,6 @@ attend_plan_kernel(PlanArgs a) {
         a.head->merges = s_merges;
         a.head->size = size;
         a.head->total = line;
-        a.head->at.run_tile = a.at.run_tile;
-        a.head->at.tiles = a.at.tiles;
         a.head->at.merges = a.at.merges;
         a.head->at.rows = a.at.rows;
         a.head->at.ml = a.at.ml;
@@ -426,6 +425,8 @@ attend_plan_kernel(PlanArgs a) {
 // ds_read_b64_tr_b8 gives a lane eight keys of one dim at once.
 struct AttendArgs {
     uint8_t* ws;
+    const Tile* start;  // in it
+    const Tile* tile;
     size_t ws_len;
     const float* q;
     PoolArgs p;  // of one layer
@@ -436,8 +437,6 @@ struct AttendArgs {
 // The workspace's header and the parts it names.
 struct Plan {
     Header head;
-    const int* run_tile;
-    const Tile* tile;
     const int* merge;
     const int* rows;
     float* ml;
@@ -450,8 +449,6 @@ __device__ __forceinline__ Plan load_plan(const AttendArgs& a) {
     const Header& h = p.head;
     p.fits = h.magic == kMagic && h.n == a.n && h.tokens == a.tokens && h.width == a.width && h.hq == a.hq &&
              h.hkv == a.p.hkv && h.at.bytes <= a.ws_len;
-    p.run_tile = reinterpret_cast<const int*>(a.ws + h.at.run_tile);
-    p.tile = reinterpret_cast<const Tile*>(a.ws + h.at.tiles);
     p.merge = reinterpret_cast<const int*>(a.ws + h.at.merges);
     p.rows = reinterpret_cast<const int*>(a.ws + h.at.rows);
     p.ml = reinterpret_cast<float*>(a.ws + h.at.ml);
@@ -675,7 +672,6 @@ attend_kernel(AttendArgs a) {
     constexpr int kHalf = 32 * kDim;  // codes of half a page
     __shared__ __attribute__((aligned(16))) uint8_t s_k[kWaves][2][kHalf], s_v[kWaves][2][kHalf];
     __shared__ __attribute__((aligned(16))) int s_nan[kWaves][kDim];  // first key with a NaN value, for each dim
-    if (!load_plan(a).fits) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
@@ -684,29 +680,63 @@ attend_kernel(AttendArgs a) {
     // the loop they would crowd out its own.
     auto args = [] { return (Scalar<AttendArgs>)again(__builtin_amdgcn_kernarg_segment_ptr()); };
     auto header = [&] { return (Scalar<Header>)(uintptr_t)args()->ws; };
-    if (run >= header()->runs || run * header()->size >= header()->total) return;
+    // (a run's first tile comes with the header, before it is known to be one)
+    Tile t = load_tile(a.start + min(run, max(kRuns / a.p.hkv, kWaves) - 1));
+    {
+        const Plan plan = load_plan(a);
+        if (!plan.fits || run >= plan.head.runs || run * plan.head.size >= plan.head.total) return;
+    }
 
-    for (int ti = *(Scalar<int>)(uintptr_t)(args()->ws + header()->at.run_tile + 4 * (size_t)run); ti < header()->tiles; ++ti) {
+    while (true) {
         // ---- this run's pages of the tile ------------------------------------------------------------
+        const int ti = t.index;
         int p0, p1, row0, col0, cols, pos0, kind;
-        Scalar<int> ids;
+        const int* ids;
         {
             const auto g = args();
             const auto hd = header();
-            const Tile t = load_tile(reinterpret_cast<const Tile*>(g->ws + hd->at.tiles) + ti);
             const long long lo = run * hd->size, end = min(lo + hd->size, (long long)hd->total);
             if (t.start >= end) break;
             p0 = t.b0 + (int)max(lo - t.start, 0LL);
             p1 = min(t.b0 + (int)min(end - t.start, (long long)INT_MAX / 2), t.b1);
-            if (p0 >= p1) continue;  // (its pages are the next run's)
-            ids = scalar(g->table + (size_t)t.seq * g->width);
+            ids = g->table + (size_t)t.seq * g->width;
             row0 = t.row0;
             col0 = t.col0;
             cols = t.cols;
             pos0 = t.pos0;
             kind = t.kind;
         }
+        if (p0 < p1) {
         const bool nowhere = kind & kBad;
+
+        // this lane's share of a half page's copies, and where it reads them
+        const uint32_t j8 = lane >> 3, piece = ((lane & 7) ^ j8) * 16;
+        const uint32_t k_from = j8 * kDim + piece, v_from = 1024 * (j8 >> 2) + kDim * (j8 & 3) + piece;
+        const uint32_t k_at = c * kDim + ((h ^ (c & 7)) * 16), jv = (lane & 15) >> 1;
+        const uint32_t v_at = (8 * h + jv) * kDim + 8 * (lane & 1) + ((((lane >> 4) & 1) ^ jv) * 16);
+        const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_k[wave]));
+        const uint32_t v_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_v[wave]));
+        auto load_k = [&](uint32_t tile, int half) {
+            copy_keys(a.p.k + (size_t)tile * kTileBytes8 + half * kHalf + k_from, k_lds + half * kHalf);
+        };
+        auto load_v = [&](uint32_t tile, int half) {
+            copy_values(a.p.v + (size_t)tile * kTileBytes8 + half * kHalf + v_from, v_lds + half * kHalf);
+        };
+        // Pages 64 at a time, a lane each: their tiles (page 0's in the place of one that is not there), which
+        // are there, and their scale bytes. (Through the scalar cache they would have every LDS read wait
+        // for them: both count in one counter, and scalar loads return in any order.)
+        uint32_t tile_of_lane, kx_of_lane, vx_of_lane;
+        uint64_t are_there;
+        auto look_up = [&](int id) {  // of this lane's page
+            const bool there = id >= 0 && id < a.p.pages;
+            tile_of_lane = (uint32_t)(there ? id : 0) * a.p.hkv + kh;  // (a layer has at most 2^31 of them)
+            are_there = __builtin_amdgcn_ballot_w64(there);
+            kx_of_lane = a.p.kx[tile_of_lane];
+            vx_of_lane = a.p.vx[tile_of_lane];
+        };
+        int looked_up = p0;  // the first of the 64
+        const int first_id = nowhere ? 0 : ids[min(p0 + lane, p1 - 1)];  // (one without a place: page 0, not used)
+        uint32_t tile;
 
         // ---- Q: hi and lo parts of q / sqrt(128) * log2 e, each column's exponent taken out ------------
         int limit;  // the last position this lane's column sees
@@ -720,21 +750,32 @@ attend_kernel(AttendArgs a) {
             if (kind & kPrefix) row = reinterpret_cast<const int*>(g->ws + header()->at.rows)[row];
             const int head_of = kh * g->per_row + col - local * g->per_row;
             limit = kind & kPrefix ? INT_MAX : nowhere ? -1 : pos0 + local;
-            // step s holds dims 32 (s / 2) + 16 h + 8 (s % 2) .. + 8, as K's 16-byte loads do
+            // step s holds dims 32 (s / 2) + 16 h + 8 (s % 2) .. + 8, as K's 16-byte pieces do
             const float* qrow = g->q + ((size_t)row * g->hq + head_of) * kDim + 16 * h;
+            f32x4 raw[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                raw[i] = *reinterpret_cast<const f32x4*>(qrow + 32 * (i >> 2) + 8 * ((i >> 1) & 1) + 4 * (i & 1));
+            // Q here, then the first page's copies on their way, then the work on Q under them. (The compiler
+            // does not count the copies: a wait for an earlier load would be one for them too.)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(raw[i]));
+            in_order();
+            look_up(first_id);
+            tile = __builtin_amdgcn_readlane(tile_of_lane, 0);
+            load_k(tile, 0);
+            load_k(tile, 1);
+            load_v(tile, 0);
+            in_order();
             const float scale = 0.08838834764831845f * kLog2e;
             float x[8][8];
             float qmax = 0.0f;
 #pragma unroll
             for (int s = 0; s < 8; ++s)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(qrow + 32 * (s >> 1) + 8 * (s & 1) + 4 * e);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        x[s][4 * e + j] = as_f32(y[j] * scale);
-                        qmax = fmaxf(qmax, fabsf(x[s][4 * e + j]));
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    x[s][j] = as_f32(raw[2 * s + (j >> 2)][j & 3] * scale);
+                    qmax = fmaxf(qmax, fabsf(x[s][j]));
                 }
             qmax = max_h(qmax);
             qx = (int)(__float_as_uint(qmax) >> 23) - 127 - 8;  // the row's largest to [2^8, 2^9)
@@ -761,6 +802,8 @@ attend_kernel(AttendArgs a) {
                     }
                 }
             }
+            in_order();
+            asm volatile("" : "+v"(kx_of_lane), "+v"(vx_of_lane));
         }
         // the least and the largest position that a column of this wave sees
         int lim0 = limit, lim1 = limit;
@@ -780,19 +823,6 @@ attend_kernel(AttendArgs a) {
             for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
         int vref = 0;     // acc stands in units of 2^(vref - 127)
 
-        // this lane's share of a half page's copies, and where it reads them
-        const uint32_t j8 = lane >> 3, piece = ((lane & 7) ^ j8) * 16;
-        const uint32_t k_from = j8 * kDim + piece, v_from = 1024 * (j8 >> 2) + kDim * (j8 & 3) + piece;
-        const uint32_t k_at = c * kDim + ((h ^ (c & 7)) * 16), jv = (lane & 15) >> 1;
-        const uint32_t v_at = (8 * h + jv) * kDim + 8 * (lane & 1) + ((((lane >> 4) & 1) ^ jv) * 16);
-        const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_k[wave]));
-        const uint32_t v_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_v[wave]));
-        auto load_k = [&](uint32_t tile, int half) {
-            copy_keys(a.p.k + (size_t)tile * kTileBytes8 + half * kHalf + k_from, k_lds + half * kHalf);
-        };
-        auto load_v = [&](uint32_t tile, int half) {
-            copy_values(a.p.v + (size_t)tile * kTileBytes8 + half * kHalf + v_from, v_lds + half * kHalf);
-        };
         u32x4 kw[4];    // key c, dims 32 i + 16 h .. + 16
         i32x2 vw[2][4]; // keys 16 st + 8 (j / 4) + 4 h + j % 4 of dim 32 t + c at [st][t]
         auto read_k = [&](int half) {
@@ -805,22 +835,12 @@ attend_kernel(AttendArgs a) {
                 vw[i >> 2][i & 3] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                     (__attribute__((address_space(3))) i32x2*)&s_v[wave][half][2048 * (i >> 2) + (v_at ^ 32 * (i & 3))]);
         };
-        // a page that is not there reads page 0 in its place
-        auto tile_of = [&](int id, bool& there) {
-            there = id >= 0 && id < a.p.pages;
-            return (uint32_t)(there ? id : 0) * a.p.hkv + kh;  // (a layer has at most 2^31 of them)
-        };
-
         if (!nowhere) {
             int page = p0;
-            bool there, there_next = true;
-            uint32_t tile = tile_of(ids[page], there), tile_next = tile;
-            load_k(tile, 0);
-            load_k(tile, 1);
-            load_v(tile, 0);
-            int kx = scalar_byte(a.p.kx, tile), vx = scalar_byte(a.p.vx, tile), kx_next = kx, vx_next = vx;
+            uint32_t tile_next = tile;
+            int kx = __builtin_amdgcn_readlane(kx_of_lane, 0), vx = __builtin_amdgcn_readlane(vx_of_lane, 0);
+            bool there = are_there & 1;
             vref = vx;
-            int id = ids[min(page + 1, p1 - 1)];  // of the page after this one
             // the scores of the half page at hand: of key k0 + 8 q + 4 h + r and column c, in units of
             // log2 and of 2^(qx + kx - 127)
             wait_vmcnt<8>();
@@ -857,14 +877,14 @@ attend_kernel(AttendArgs a) {
                         if (8 * (i >> 2) + (i & 3) > last) s[i] = -INFINITY;
                     hide_values(s_v[wave][half], s_nan[wave], lim1 - k0, limit - k0, acc);
                 }
-                float top = s[0];
+                float top = fmaxf(fmaxf(s[12], s[13]), fmaxf(s[14], s[15]));
 #pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-                top = max_h(top) * sc;
+                for (int i = 0; i < 12; i += 3) top = fmaxf(top, fmaxf(fmaxf(s[i], s[i + 1]), s[i + 2]));
                 // a reference point that moves only when the maximum has grown by 2^8: p stays below
                 // 2^15 with the bias of 2^7 that keeps small p out of f16's subnormals
-                const bool grow = top > m_used + 8.0f;
-                if (__builtin_amdgcn_ballot_w64(grow)) {
+                if (__builtin_amdgcn_ballot_w64(top * sc > m_used + 8.0f)) {
+                    top = max_h(top) * sc;
+                    const bool grow = top > m_used + 8.0f;
                     const float alpha = grow ? __builtin_amdgcn_exp2f(m_used - top) : 1.0f;
                     if (grow) m_used = top;
                     lsum *= alpha;
@@ -931,20 +951,24 @@ attend_kernel(AttendArgs a) {
             while (true) {
                 const bool more = page + 1 < p1;
                 if (more) {
-                    tile_next = tile_of(id, there_next);
-                    kx_next = scalar_byte(a.p.kx, tile_next);
-                    vx_next = scalar_byte(a.p.vx, tile_next);
-                    id = ids[min(page + 2, p1 - 1)];
+                    if (page + 1 - looked_up == 64) {
+                        looked_up += 64;
+                        look_up(ids[min(looked_up + lane, p1 - 1)]);
+                        asm volatile("" : "+v"(kx_of_lane), "+v"(vx_of_lane));  // (waited for here, not on every page)
+                    }
+                    tile_next = __builtin_amdgcn_readlane(tile_of_lane, page + 1 - looked_up);
                 }
                 half_page(std::integral_constant<int, 0>{}, more);
                 half_page(std::integral_constant<int, 1>{}, more);
                 if (!more) break;
                 ++page;
-                there = there_next;
                 tile = tile_next;
-                kx = kx_next;
-                vx = vx_next;
+                kx = __builtin_amdgcn_readlane(kx_of_lane, page - looked_up);
+                vx = __builtin_amdgcn_readlane(vx_of_lane, page - looked_up);
+                there = are_there >> (page - looked_up) & 1;
             }
+        } else {
+            wait_vmcnt<0>();  // (no copy outlives the workgroup)
         }
         // (a row past the table's width has no page)
         const auto g = args();
@@ -955,8 +979,8 @@ attend_kernel(AttendArgs a) {
         for (int i = 0; i < 4; ++i) acc[i] *= unit;
 
         // ---- out: to o, or to the parts. The lane holds dims 32 t + 8 q + 4 h + r of its column -------------
-        if (c >= cols) continue;
-        if (kind & kDirect) {
+        if (c >= cols) {
+        } else if (kind & kDirect) {
             const int col = col0 + c, local = col / g->per_row;  // (a prefix tile is never direct)
             const size_t at = ((size_t)(row0 + local) * g->hq + kh * g->per_row + col - local * g->per_row) * kDim;
             const float inv = 1.0f / lsum;
@@ -968,8 +992,8 @@ attend_kernel(AttendArgs a) {
             }
         } else {
             const auto hd = header();
-            const auto t = (Scalar<Tile>)(uintptr_t)(g->ws + hd->at.tiles) + ti;
-            const size_t part = (size_t)kh * hd->at.cap + t->base + (size_t)(run - t->run0) * cols + c;
+            const auto own = (Scalar<Tile>)(uintptr_t)g->tile + ti;
+            const size_t part = (size_t)kh * hd->at.cap + own->base + (size_t)(run - own->run0) * cols + c;
             float* to = reinterpret_cast<float*>(g->ws + hd->at.acc) + part * kDim + 4 * h;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -979,6 +1003,9 @@ attend_kernel(AttendArgs a) {
             }
             if (h == 0) *reinterpret_cast<f32x2*>(reinterpret_cast<float*>(g->ws + hd->at.ml) + 2 * part) = f32x2{m_used, lsum};
         }
+        }
+        if (ti + 1 >= header()->tiles) break;
+        t = load_tile(reinterpret_cast<const Tile*>((uintptr_t)args()->tile) + ti + 1);
     }
 }
 
@@ -1006,13 +1033,13 @@ attend_merge_kernel(AttendArgs a) {
     for (int e = e0; e < head.merges; e += es) {
         const int entry = scalar(plan.merge)[e];
         const bool together = entry & 1;  // the whole workgroup on one column
-        const Tile t = load_tile(plan.tile + entry / (2 * kCols));
+        const Tile t = load_tile(a.tile + entry / (2 * kCols));
         const int c = entry / 2 % kCols + (together ? 0 : 2 * wave + h);
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
         float l = 0.0f;
         int pparts = 0, pcols = 0, pbase = 0;
         if (t.ptile >= 0) {
-            const Tile* p = plan.tile + t.ptile + (t.pcol + c) / kCols;  // (two halves may have two)
+            const Tile* p = a.tile + t.ptile + (t.pcol + c) / kCols;  // (two halves may have two)
             if (c < t.cols) {
                 pparts = p->parts;
                 pcols = p->cols;
@@ -1120,7 +1147,7 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
     a.group = group;
     a.prefix = prefix;
     a.head = reinterpret_cast<Header*>(w);
-    a.run_tile = reinterpret_cast<int*>(w + l.run_tile);
+    a.start = reinterpret_cast<Tile*>(w + l.starts);
     a.tile = reinterpret_cast<Tile*>(w + l.tiles);
     a.merge = reinterpret_cast<int*>(w + l.merges);
     a.seq = reinterpret_cast<PlanSeq*>(w + l.seqs);
@@ -1143,9 +1170,12 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
 
 int attend_launch(const float* q, const PoolArgs& pool, const int* table, int width, int n, int tokens,
                   void* ws, size_t ws_len, void* o, int o_f16, int hq, hipStream_t stream) {
+    const Layout l = layout(n, n, tokens, hq, pool.hkv);  // (the most entries: the plan's may have fewer groups)
     AttendArgs a = {};
     a.ws = static_cast<uint8_t*>(ws);
     a.ws_len = ws_len;
+    a.start = reinterpret_cast<const Tile*>(a.ws + l.starts);
+    a.tile = reinterpret_cast<const Tile*>(a.ws + l.tiles);
     a.q = q;
     a.p = pool;
     a.table = table;
@@ -1156,7 +1186,6 @@ int attend_launch(const float* q, const PoolArgs& pool, const int* table, int wi
     a.hq = hq;
     a.per_row = hq / pool.hkv;
     a.o_f16 = o_f16;
-    const Layout l = layout(n, n, tokens, hq, pool.hkv);  // (the most entries: the plan's may have fewer groups)
     auto kernel = o_f16 ? attend_kernel<false> : attend_kernel<true>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0,
                        stream, a);
