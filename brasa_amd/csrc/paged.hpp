@@ -40,12 +40,6 @@ __device__ __forceinline__ uintptr_t again(T p) {
     asm volatile("" : "+s"(x));
     return x;
 }
-// the byte at p + i (its aligned word is read)
-__device__ __forceinline__ int scalar_byte(const uint8_t* p, size_t i) {
-    const uintptr_t at = (uintptr_t)(p + i);
-    return (int)(*(Scalar<uint32_t>)(at & ~(uintptr_t)3) >> 8 * (at & 3) & 0xffu);
-}
-
 // ---- workgroup scans of 1024 threads ------------------------------------------------------------
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / 64;
