@@ -38,8 +38,6 @@ constexpr int kOver = 4;
 // with runs of 2 and 13.0 with 4, four rows over 16K positions 17.0 + 5.9 us with 2 and 15.8 + 4.8 with 4.
 constexpr int kShortLine = 64;
 __device__ __forceinline__ long long least_run(long long total) { return total <= kShortLine ? 2 : 4; }
-constexpr int kFewParts = 8;  // parts of a column that half a wave joins
-constexpr int kMergeCols = 2 * kWaves;  // columns of such an entry
 
 struct Tile {
     int seq;          // table row whose pages it reads
@@ -56,6 +54,18 @@ struct Tile {
 };
 static_assert(sizeof(Tile) == 64, "a tile is one line");
 enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4 };
+
+// Columns whose parts a workgroup of the merge joins: `many` of one tile, which continue in one prefix tile or in none.
+struct Join {
+    int base, parts, cols;     // own parts: columns base + part * cols + column
+    int pbase, pparts, pcols;  // the prefix tile's
+    int row0, col0, many;      // columns from col0 on of the sequence whose first packed row is row0
+    int lanes;                 // of a column: 32, 64 or all
+    int unused0, unused1;
+};
+static_assert(sizeof(Join) % 16 == 0, "read in wide pieces");
+// Half a wave has eight parts on their way at once: it takes two turns before more of them pay.
+__host__ __device__ constexpr int join_lanes(int parts) { return parts <= 8 ? 32 : parts <= 32 ? 64 : kThreads; }
 
 // Where the plan and the partials stand in the workspace.
 struct Places {
@@ -85,6 +95,7 @@ struct PlanSeq {
 struct PlanGroup {
     int s0, s1;      // its sequences
     int lead, many;  // the first of those that may share its prefix, and how many
+    int pages;       // of its prefix
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -108,7 +119,7 @@ Layout layout(int n, int groups, int tokens, int hq, int hkv) {
     };
     l.starts = take(sizeof(Tile) * (size_t)l.runs);
     l.tiles = take(sizeof(Tile) * (size_t)l.max_tiles);
-    l.merges = take(4 * (size_t)l.max_merges);
+    l.merges = take(sizeof(Join) * (size_t)l.max_merges);
     l.seqs = take(sizeof(PlanSeq) * (size_t)n);
     l.first = take(4 * ((size_t)groups + n + 1));
     l.group = take(sizeof(PlanGroup) * (size_t)groups);
@@ -131,7 +142,7 @@ struct PlanArgs {
     Header* head;
     Tile* start;  // [runs]: the tile where each run starts
     Tile* tile;
-    int* merge;
+    Join* merge;
     PlanSeq* seq;
     int* first;  // [groups + n + 1]: first tile of each group's prefix, then of each sequence
     PlanGroup* grp;
@@ -140,7 +151,8 @@ struct PlanArgs {
     Places at;
 };
 
-// exclusive sum over the workgroup of values up to 2^62; s: kScanWaves of LDS
+// exclusive sum over a workgroup of W waves of values up to 2^62; s: W of LDS
+template <int W>
 __device__ __forceinline__ long long block_scan64(long long x, long long* s, long long& sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     long long incl = x;
@@ -155,7 +167,7 @@ __device__ __forceinline__ long long block_scan64(long long x, long long* s, lon
     long long before = 0;
     sum = 0;
 #pragma unroll
-    for (int w = 0; w < kScanWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
         const long long y = s[w];
         if (w < wave) before += y;
         sum += y;
@@ -163,6 +175,7 @@ __device__ __forceinline__ long long block_scan64(long long x, long long* s, lon
     return before + incl - x;
 }
 // inclusive maximum over the workgroup and `before`; `all`: of the whole workgroup
+template <int W>
 __device__ __forceinline__ int block_max(int x, int before, int* s, int& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     x = max(x, before);
@@ -176,12 +189,21 @@ __device__ __forceinline__ int block_max(int x, int before, int* s, int& all) {
     __syncthreads();
     all = before;
 #pragma unroll
-    for (int w = 0; w < kScanWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
         const int y = s[w];
         if (w < wave) x = max(x, y);
         all = max(all, y);
     }
     return x;
+}
+__device__ __forceinline__ Tile read_lane(const Tile& t, int lane) {
+    union {
+        Tile t;
+        uint32_t w[sizeof(Tile) / 4];
+    } u = {t};
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Tile) / 4); ++i) u.w[i] = __builtin_amdgcn_readlane(u.w[i], lane);
+    return u.t;
 }
 // x / d for 0 <= x < 2^52, d > 0, with inv = 1.0 / d
 __device__ __forceinline__ long long div_by(long long x, long long d, double inv) {
@@ -192,13 +214,15 @@ __device__ __forceinline__ long long div_by(long long x, long long d, double inv
 }
 // IN_LDS: the lists of sequences and groups fit the LDS (up to kPlanLds of each); else they stand in the
 // workspace, and every look at one costs a trip to the L2 (64 sequences in one group 21 us in place of 12).
-constexpr int kPlanLds = 1024;
-template <bool IN_LDS>
-__global__ void __launch_bounds__(kScanThreads)
+// Up to kPlanFew sequences and tiles take as many threads, whose scans wait for four waves only.
+constexpr int kPlanLds = 1024, kPlanFew = 256;
+template <bool IN_LDS, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 attend_plan_kernel(PlanArgs a) {
-    __shared__ PlanSeq s_seq[IN_LDS ? kPlanLds : 1];
-    __shared__ PlanGroup s_grp[IN_LDS ? kPlanLds : 1];
-    __shared__ int s_first[IN_LDS ? 2 * kPlanLds + 1 : 1];
+    constexpr int kInLds = !IN_LDS ? 1 : std::min(THREADS, kPlanLds), W = THREADS / 64;
+    __shared__ PlanSeq s_seq[kInLds];
+    __shared__ PlanGroup s_grp[kInLds];
+    __shared__ int s_first[2 * kInLds + 1];
     PlanSeq* const seqs = IN_LDS ? s_seq : a.seq;
     PlanGroup* const grps = IN_LDS ? s_grp : a.grp;
     int* const firsts = IN_LDS ? s_first : a.first;
@@ -208,41 +232,56 @@ attend_plan_kernel(PlanArgs a) {
         if (IN_LDS) *p = x;
         else __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
-    __shared__ long long s_scan[kScanWaves];
-    __shared__ int s_scan32[kScanWaves];
+    __shared__ long long s_scan[W];
+    __shared__ int s_scan32[W];
     __shared__ int s_merges;
+    __shared__ int s_parts[THREADS], s_cols[THREADS], s_base[THREADS];  // of the tiles, where there is one a thread
     const int tid = threadIdx.x;
     if (tid == 0) s_merges = 0;
     const int per_row = a.per_row;
+    // (the first of each list at once: what follows then waits for one trip to memory, not for three)
+    struct In {
+        int cu0, cu1, pos;
+    };
+    struct InGroup {
+        int s0, s1, prefix;
+    };
+    auto load_in = [&](int i) { return i < a.n ? In{a.cu[i], a.cu[i + 1], a.pos[i]} : In{0, 0, -1}; };
+    auto load_group = [&](int g) { return g < a.groups ? InGroup{a.group[g], a.group[g + 1], a.prefix[g]} : InGroup{0, 0, 0}; };
+    const In in0 = load_in(tid);
+    const InGroup group0 = load_group(tid);
 
     // ---- groups: runs of sequences, in order and apart ------------------------------------------
-    for (int g0 = 0, before = 0; g0 < a.groups; g0 += kScanThreads) {
+    for (int g0 = 0, before = 0; g0 < a.groups; g0 += THREADS) {
         const int g = g0 + tid;
         int all;
-        const int s0 = block_max(g < a.groups ? min(max(a.group[g], 0), a.n) : 0, before, s_scan32, all);
-        const int s1 = max(s0, g < a.groups ? min(max(a.group[g + 1], 0), a.n) : 0);
+        const InGroup in = g0 ? load_group(g) : group0;
+        const int s0 = block_max<W>(min(max(in.s0, 0), a.n), before, s_scan32, all);
+        const int s1 = max(s0, min(max(in.s1, 0), a.n));
         before = all;
         if (g < a.groups) {
             st_l2(&grps[g].s0, s0);
             st_l2(&grps[g].s1, s1);
             st_l2(&grps[g].lead, a.n);
             st_l2(&grps[g].many, 0);
+            st_l2(&grps[g].pages, min(max(in.prefix, 0) / kPage, a.width));
         }
     }
     if (a.groups) stores_barrier();
-    auto prefix_pages = [&](int g) { return min(max(a.prefix[g], 0) / kPage, a.width); };
+    auto prefix_pages = [&](int g) { return ld_l2(&grps[g].pages); };
 
     // ---- sequences: their rows, in order and apart, and who may share a prefix --------------------
     int scols = 0;
-    for (int i0 = 0, before = 0; i0 < a.n; i0 += kScanThreads) {
+    for (int i0 = 0, before = 0; i0 < a.n; i0 += THREADS) {
         const int i = i0 + tid;
         int all;
-        const int c0 = block_max(i < a.n ? min(max(a.cu[i], 0), a.tokens) : 0, before, s_scan32, all);
+        const In in = i0 ? load_in(i) : in0;
+        const int c0 = block_max<W>(min(max(in.cu0, 0), a.tokens), before, s_scan32, all);
         before = all;
         PlanSeq s;
         s.c0 = c0;
-        s.rows = i < a.n ? max(min(max(a.cu[i + 1], 0), a.tokens) - c0, 0) : 0;
-        s.pos = i < a.n ? a.pos[i] : -1;
+        s.rows = max(min(max(in.cu1, 0), a.tokens) - c0, 0);
+        s.pos = in.pos;
         if (s.pos >= a.width * kPage) s.pos = -1;
         s.group = -1;
         int cols = 0;
@@ -266,7 +305,7 @@ attend_plan_kernel(PlanArgs a) {
         }
         if (a.groups) {
             int sum;
-            s.scol = scols + block_scan(cols, s_scan32, sum);
+            s.scol = scols + block_scan<W>(cols, s_scan32, sum);
             scols += sum;
             // (the rows of one that turns out to be alone in its group are listed, and not used)
             for (int r = 0; cols && r < s.rows; ++r) a.rows[s.scol / per_row + r] = s.c0 + r;
@@ -299,13 +338,13 @@ attend_plan_kernel(PlanArgs a) {
     // ---- how many tiles each has ------------------------------------------------------------------
     int ntiles = 0;
     const int entries = a.groups + a.n;
-    for (int e0 = 0; e0 < entries; e0 += kScanThreads) {
+    for (int e0 = 0; e0 < entries; e0 += THREADS) {
         const int e = e0 + tid;
         int tiles = 0, col0;
         if (e < a.groups) tiles = (group_cols(e, col0) + kCols - 1) / kCols;
         else if (e < entries) tiles = (int)(((long long)ld_l2(&seqs[e - a.groups].rows) * per_row + kCols - 1) / kCols);
         int sum;
-        const int at = ntiles + block_scan(tiles, s_scan32, sum);
+        const int at = ntiles + block_scan<W>(tiles, s_scan32, sum);
         ntiles += sum;
         if (e < entries) st_l2(firsts + e, at);
     }
@@ -358,41 +397,80 @@ attend_plan_kernel(PlanArgs a) {
     // ---- the line's length, and that of a run -----------------------------------------------------
     long long mine = 0, total;
     Tile t = {};
-    for (int i = tid; i < ntiles; i += kScanThreads) {
+    for (int i = tid; i < ntiles; i += THREADS) {
         t = make_tile(i);
         mine += kOver + t.b1 - t.b0;
     }
-    block_scan64(mine, s_scan, total);
+    block_scan64<W>(mine, s_scan, total);
     const long long size = max((total + a.runs - 1) / a.runs, least_run(total));
     const double inv = 1.0 / (double)size;
 
     // ---- the tiles --------------------------------------------------------------------------------
     long long line = 0, cols = 0;
-    for (int t0 = 0; t0 < ntiles; t0 += kScanThreads) {
+    for (int t0 = 0; t0 < ntiles; t0 += THREADS) {
         const int at = t0 + tid;
         const bool on = at < ntiles;
-        if (on && ntiles > kScanThreads) t = make_tile(at);  // (else it is at hand)
+        if (on && ntiles > THREADS) t = make_tile(at);  // (else it is at hand)
         const long long len = on ? t.b1 - t.b0 : 0;
         long long sum;
-        t.start = line + block_scan64(on ? len + kOver : 0, s_scan, sum) + kOver;
+        t.start = line + block_scan64<W>(on ? len + kOver : 0, s_scan, sum) + kOver;
         line += sum;
         t.run0 = (int)div_by(t.start, size, inv);
         const int last = on ? (int)div_by(t.start + len - 1, size, inv) : 0;
         t.parts = last - t.run0 + 1;
         if (!(t.kind & kPrefix) && t.ptile < 0 && t.parts == 1) t.kind |= kDirect;
         const long long part_cols = on && !(t.kind & kDirect) ? (long long)t.cols * t.parts : 0;
-        t.base = (int)(cols + block_scan64(part_cols, s_scan, sum));
+        t.base = (int)(cols + block_scan64<W>(part_cols, s_scan, sum));
         cols += sum;
-        if (!on) continue;
-        a.tile[at] = t;
-        // the runs that start in it, or in the pages' worth before it
-        for (int w = (int)div_by(t.start - kOver + size - 1, size, inv); w <= last; ++w) a.start[w] = t;
-        if (!(t.kind & (kPrefix | kDirect))) {
-            int parts = t.parts;
-            if (t.ptile >= 0) parts += (int)div_by(t.b0, size, inv) + 1;  // (about: the prefix tile's)
-            const int each = parts > kFewParts ? 1 : kMergeCols, many = (t.cols + each - 1) / each;
-            const int e = atomicAdd(&s_merges, many);
-            for (int j = 0; j < many; ++j) a.merge[e + j] = (at * kCols + j * each) * 2 + (each == 1);
+        if (on) {
+            a.tile[at] = t;
+            s_parts[tid] = t.parts;
+            s_cols[tid] = t.cols;
+            s_base[tid] = t.base;
+        }
+        // the runs that start in it, or in the pages' worth before it; a wave together where they are many
+        int w = on ? (int)div_by(t.start - kOver + size - 1, size, inv) : 1;
+        for (uint64_t many = __builtin_amdgcn_ballot_w64(last - w >= 4); many; many &= many - 1) {
+            const int from = __builtin_ctzll(many), w1 = __builtin_amdgcn_readlane(last, from);
+            const Tile u = read_lane(t, from);
+            for (int k = __builtin_amdgcn_readlane(w, from) + (tid & 63); k <= w1; k += 64) a.start[k] = u;
+        }
+        if (last - w < 4)
+            for (; w <= last; ++w) a.start[w] = t;
+    }
+    if (ntiles > THREADS) stores_barrier();
+    else __syncthreads();
+
+    // ---- the columns to join ----------------------------------------------------------------------
+    for (int at = tid; at < ntiles; at += THREADS) {
+        if (ntiles > THREADS) t = a.tile[at];
+        if (t.kind & (kPrefix | kDirect)) continue;
+        const int border = t.ptile >= 0 ? min(kCols - t.pcol, t.cols) : t.cols;  // (the rest in the next prefix tile)
+        for (int c0 = 0; c0 < t.cols; c0 = border) {
+            const int c1 = c0 < border ? border : t.cols;
+            Join j = {};
+            j.parts = t.parts;
+            j.cols = t.cols;
+            j.base = t.base + c0;
+            if (t.ptile >= 0) {
+                const int pt = t.ptile + (c0 > 0);
+                j.pparts = ntiles > THREADS ? brasa::ld_l2(&a.tile[pt].parts) : s_parts[pt];
+                j.pcols = ntiles > THREADS ? brasa::ld_l2(&a.tile[pt].cols) : s_cols[pt];
+                j.pbase = (ntiles > THREADS ? brasa::ld_l2(&a.tile[pt].base) : s_base[pt]) + (c0 > 0 ? 0 : t.pcol);
+            }
+            j.row0 = t.row0;
+            j.col0 = t.col0 + c0;
+            j.lanes = join_lanes(j.parts + j.pparts);
+            const int each = kThreads / j.lanes;
+            int to = atomicAdd(&s_merges, (c1 - c0 + each - 1) / each);
+            for (int c = c0; c < c1; c += each) {
+                j.many = min(c1 - c, each);
+                a.merge[to++] = j;
+                j.base += each;
+                j.pbase += each;
+                j.col0 += each;
+            }
+            if (c1 == t.cols) break;
         }
     }
     __syncthreads();
@@ -442,7 +520,7 @@ struct AttendArgs {
 // The workspace's header and the parts it names.
 struct Plan {
     Header head;
-    const int* merge;
+    const Join* merge;
     const int* rows;
     float* ml;
     float* acc;
@@ -454,20 +532,21 @@ __device__ __forceinline__ Plan load_plan(const AttendArgs& a) {
     const Header& h = p.head;
     p.fits = h.magic == kMagic && h.n == a.n && h.tokens == a.tokens && h.width == a.width && h.hq == a.hq &&
              h.hkv == a.p.hkv && h.at.bytes <= a.ws_len;
-    p.merge = reinterpret_cast<const int*>(a.ws + h.at.merges);
+    p.merge = reinterpret_cast<const Join*>(a.ws + h.at.merges);
     p.rows = reinterpret_cast<const int*>(a.ws + h.at.rows);
     p.ml = reinterpret_cast<float*>(a.ws + h.at.ml);
     p.acc = reinterpret_cast<float*>(a.ws + h.at.acc);
     return p;
 }
 
-__device__ __forceinline__ Tile load_tile(const Tile* p) {
+template <typename T>
+__device__ __forceinline__ T load_line(const T* p) {
     union {
-        Tile t;
-        uint32_t w[sizeof(Tile) / 4];
+        T t;
+        uint32_t w[sizeof(T) / 4];
     } u;
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(Tile) / 4); ++i) u.w[i] = ((Scalar<uint32_t>)(uintptr_t)p)[i];
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) u.w[i] = ((Scalar<uint32_t>)(uintptr_t)p)[i];
     return u.t;
 }
 
@@ -686,7 +765,7 @@ attend_kernel(AttendArgs a) {
     auto args = [] { return (Scalar<AttendArgs>)again(__builtin_amdgcn_kernarg_segment_ptr()); };
     auto header = [&] { return (Scalar<Header>)(uintptr_t)args()->ws; };
     // (a run's first tile comes with the header, before it is known to be one)
-    Tile t = load_tile(a.start + min(run, max(kRuns / a.p.hkv, kWaves) - 1));
+    Tile t = load_line(a.start + min(run, max(kRuns / a.p.hkv, kWaves) - 1));
     {
         const Plan plan = load_plan(a);
         if (!plan.fits || run >= plan.head.runs || run * plan.head.size >= plan.head.total) return;
@@ -1010,21 +1089,22 @@ attend_kernel(AttendArgs a) {
         }
         }
         if (ti + 1 >= header()->tiles) break;
-        t = load_tile(reinterpret_cast<const Tile*>((uintptr_t)args()->tile) + ti + 1);
+        t = load_line(reinterpret_cast<const Tile*>((uintptr_t)args()->tile) + ti + 1);
     }
 }
 
 // ---- parts into rows ----------------------------------------------------------------------------
 //
-// Half a wave per column, 16 bytes of its sums a lane and all parts' loads in flight together, or a workgroup
-// where there are many: those of the column's own tile and of the prefix tile that holds it. Bound: the
-// chain entry -> tile -> parts -> o, and for prompts the parts' bytes.
+// Half a wave per column, a wave or a workgroup, by the number of its parts: each half wave joins every second,
+// or every eighth, 16 bytes of their sums a lane and eight parts on their way at once, and then the halves
+// theirs. Bound: the chain header -> unit -> parts -> o, and for prompts the parts' bytes.
 __global__ void __launch_bounds__(kThreads)
 attend_merge_kernel(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) float s_x[kWaves][kDim];
+    __shared__ f32x2 s_ml[kWaves];
     const Plan plan = load_plan(a);
     const Header& head = plan.head;
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int lane = threadIdx.x & 63, h = lane >> 5, d = 4 * (lane & 31);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.x % a.p.hkv, e0 = blockIdx.x / a.p.hkv, es = gridDim.x / a.p.hkv;
     if (!plan.fits) {  // of another step's sizes, or none: no row is left looking like a result
@@ -1035,103 +1115,74 @@ attend_merge_kernel(AttendArgs a) {
         }
         return;
     }
+    const float* ml = plan.ml + 2 * (size_t)kh * head.at.cap;
+    const float* sums = plan.acc + (size_t)kh * head.at.cap * kDim + d;
     for (int e = e0; e < head.merges; e += es) {
-        const int entry = scalar(plan.merge)[e];
-        const bool together = entry & 1;  // the whole workgroup on one column
-        const Tile t = load_tile(a.tile + entry / (2 * kCols));
-        const int c = entry / 2 % kCols + (together ? 0 : 2 * wave + h);
+        const Join j = load_line(plan.merge + e);
+        // this half wave's column, and its first part
+        const int half = 2 * wave + h, step = j.lanes / 32;
+        const int c = j.lanes == 32 ? half : j.lanes == 64 ? wave : 0, first = half & (step - 1);
+        const int parts = c < j.many ? j.pparts + j.parts : 0;
+        float m = -INFINITY, l = 0.0f;
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        float l = 0.0f;
-        int pparts = 0, pcols = 0, pbase = 0;
-        if (t.ptile >= 0) {
-            const Tile* p = a.tile + t.ptile + (t.pcol + c) / kCols;  // (two halves may have two)
-            if (c < t.cols) {
-                pparts = p->parts;
-                pcols = p->cols;
-                pbase = p->base + (t.pcol + c) % kCols;
+        for (int i0 = first; i0 < parts; i0 += 8 * step) {
+            f32x4 y[8];
+            f32x2 w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = min(i0 + k * step, parts - 1);
+                const int p = c + (i < j.pparts ? j.pbase + i * j.pcols : j.base + (i - j.pparts) * j.cols);
+                w[k] = *reinterpret_cast<const f32x2*>(ml + 2 * (size_t)p);
+                y[k] = *reinterpret_cast<const f32x4*>(sums + (size_t)p * kDim);
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, w[k][0]);
+            const float before = part_weight(m, top);
+            l *= before;
+            x *= before;
+            m = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (i0 + k * step >= parts) break;
+                // (a part without a key holds zeros, and a sum that is 0 or NaN)
+                const float f = part_weight(w[k][0], m);
+                l = fmaf(w[k][1], f, l);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(y[k][r], f, x[r]);
             }
         }
-        const int parts = pparts + t.parts;
-        auto at = [&](int i) {
-            return (size_t)kh * head.at.cap + (i < pparts ? pbase + i * pcols : t.base + (i - pparts) * t.cols + c);
-        };
-        if (!together) {
-            // (the count of a shared column's parts was an estimate when the entry was made)
-            if (c < t.cols) {
-                float m = -INFINITY;
-                for (int i0 = 0; i0 < parts; i0 += kFewParts) {
-                    f32x4 y[kFewParts];
-                    f32x2 ml[kFewParts];
+        if (j.lanes > 32) {
+            const float top = max_h(m), f = part_weight(m, top);
+            l = sum_h(l * f);
 #pragma unroll
-                    for (int j = 0; j < kFewParts; ++j) {
-                        const size_t p = at(min(i0 + j, parts - 1));
-                        ml[j] = *reinterpret_cast<const f32x2*>(plan.ml + 2 * p);
-                        y[j] = *reinterpret_cast<const f32x4*>(plan.acc + p * kDim + 4 * (lane & 31));
-                    }
-                    float top = m;
-#pragma unroll
-                    for (int j = 0; j < kFewParts; ++j) top = fmaxf(top, ml[j][0]);
-                    const float before = part_weight(m, top);
-                    l *= before;
-                    x *= before;
-                    m = top;
-#pragma unroll
-                    for (int j = 0; j < kFewParts; ++j) {
-                        if (i0 + j >= parts) break;
-                        // (a part without a key holds zeros, and a sum that is 0 or NaN)
-                        const float f = part_weight(ml[j][0], m);
-                        l = fmaf(ml[j][1], f, l);
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) x[d] = fmaf(y[j][d], f, x[d]);
-                    }
-                }
-            }
-        } else {
-            const int first = 2 * wave + h, step = 2 * kWaves;
-            float m = -INFINITY;
-            for (int i = lane; i < parts; i += 64) m = fmaxf(m, plan.ml[2 * at(i)]);
-#pragma unroll
-            for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-            for (int i0 = 0; i0 < parts; i0 += 64) {
-                const f32x2 ml = *reinterpret_cast<const f32x2*>(plan.ml + 2 * at(min(i0 + lane, parts - 1)));
-                const float w = i0 + lane < parts ? part_weight(ml[0], m) : 0.0f;
-                l = fmaf(ml[1], w, l);
-                const int many = min(parts - i0, 64);
-                for (int i = 0; i < many; i += 8 * step) {
-                    f32x4 y[8];
-                    float f[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int k = i + step * j + first;
-                        y[j] = *reinterpret_cast<const f32x4*>(plan.acc + at(i0 + min(k, many - 1)) * kDim + 4 * (lane & 31));
-                        f[j] = __shfl(w, min(k, 63));
-                        if (k >= many) f[j] = 0.0f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) x[d] = fmaf(y[j][d], f[j], x[d]);
-                }
-            }
-#pragma unroll
-            for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
-#pragma unroll
-            for (int d = 0; d < 4; ++d) x[d] = sum_h(x[d]);
-            if (lane < 32) *reinterpret_cast<f32x4*>(&s_x[wave][4 * lane]) = x;
+            for (int r = 0; r < 4; ++r) x[r] = sum_h(x[r] * f);
+            m = top;
+        }
+        if (j.lanes > 64) {
+            if (h == 0) *reinterpret_cast<f32x4*>(&s_x[wave][d]) = x;
+            if (lane == 0) s_ml[wave] = f32x2{m, l};
             __syncthreads();
+            m = s_ml[0][0];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_ml[w][0]);
+            l = 0.0f;
+            x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                const f32x4 y = *reinterpret_cast<const f32x4*>(&s_x[w][4 * (lane & 31)]);
-                if (w == 0) x = y;
-                else x += y;
+                const float f = part_weight(s_ml[w][0], m);
+                l = fmaf(s_ml[w][1], f, l);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(&s_x[w][d]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], f, x[r]);
             }
-            __syncthreads();  // the LDS is free for the next entry
+            __syncthreads();  // the LDS is free for the next unit
         }
-        if (c < t.cols && (!together || (wave == 0 && h == 0))) {
-            const int col = t.col0 + c, local = col / a.per_row;
-            const size_t o = (size_t)(t.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row;
-            if (a.o_f16) write_o<true>(a.o, o * kDim + 4 * (lane & 31), x, 1.0f / l);
-            else write_o<false>(a.o, o * kDim + 4 * (lane & 31), x, 1.0f / l);
+        if (c < j.many && first == 0) {
+            const int col = j.col0 + c, local = col / a.per_row;
+            const size_t o = ((size_t)(j.row0 + local) * a.hq + kh * a.per_row + col - local * a.per_row) * kDim + d;
+            if (a.o_f16) write_o<true>(a.o, o, x, 1.0f / l);
+            else write_o<false>(a.o, o, x, 1.0f / l);
         }
     }
 }
@@ -1154,7 +1205,7 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
     a.head = reinterpret_cast<Header*>(w);
     a.start = reinterpret_cast<Tile*>(w + l.starts);
     a.tile = reinterpret_cast<Tile*>(w + l.tiles);
-    a.merge = reinterpret_cast<int*>(w + l.merges);
+    a.merge = reinterpret_cast<Join*>(w + l.merges);
     a.seq = reinterpret_cast<PlanSeq*>(w + l.seqs);
     a.first = reinterpret_cast<int*>(w + l.first);
     a.grp = reinterpret_cast<PlanGroup*>(w + l.group);
@@ -1168,8 +1219,11 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
     a.per_row = hq / hkv;
     a.runs = l.runs;
     a.at = l;
-    auto kernel = n <= kPlanLds && groups <= kPlanLds ? attend_plan_kernel<true> : attend_plan_kernel<false>;
-    hipLaunchKernelGGL(kernel, dim3(1), dim3(kScanThreads), 0, stream, a);
+    const bool few = n <= kPlanFew && groups <= kPlanFew && l.max_tiles <= kPlanFew;
+    auto kernel = few                                       ? attend_plan_kernel<true, kPlanFew>
+                  : n <= kPlanLds && groups <= kPlanLds ? attend_plan_kernel<true, kScanThreads>
+                                                        : attend_plan_kernel<false, kScanThreads>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(few ? kPlanFew : kScanThreads), 0, stream, a);
     return check_launch("attend_plan_kernel");
 }
 

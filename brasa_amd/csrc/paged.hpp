@@ -44,26 +44,28 @@ __device__ __forceinline__ uintptr_t again(T p) {
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / 64;
 
-// exclusive sum over the workgroup's threads; `sum` is the total. s: kScanWaves ints of LDS, free
+// exclusive sum over the threads of a workgroup of W waves; `sum` is the total. s: W ints of LDS, free
 // again after the next barrier.
+template <int W = kScanWaves>
 __device__ __forceinline__ int across_waves(int mine, int* s, int& sum) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __syncthreads();  // s is free
     if (lane == 0) s[wave] = mine;
     __syncthreads();
-    static_assert(kScanWaves == 16, "a row of 16 lanes scans the waves");
-    int w = s[lane & 15];
+    static_assert(W <= 16, "a row of 16 lanes scans the waves");
+    int w = s[lane & (W - 1)];
     w += __builtin_amdgcn_update_dpp(0, w, 0x111, 0xF, 0xF, true);
-    w += __builtin_amdgcn_update_dpp(0, w, 0x112, 0xF, 0xF, true);
-    w += __builtin_amdgcn_update_dpp(0, w, 0x114, 0xF, 0xF, true);
-    w += __builtin_amdgcn_update_dpp(0, w, 0x118, 0xF, 0xF, true);
-    sum = __builtin_amdgcn_readlane(w, 15);
+    if (W > 2) w += __builtin_amdgcn_update_dpp(0, w, 0x112, 0xF, 0xF, true);
+    if (W > 4) w += __builtin_amdgcn_update_dpp(0, w, 0x114, 0xF, 0xF, true);
+    if (W > 8) w += __builtin_amdgcn_update_dpp(0, w, 0x118, 0xF, 0xF, true);
+    sum = __builtin_amdgcn_readlane(w, W - 1);
     return __builtin_amdgcn_readlane(w, wave) - mine;
 }
+template <int W = kScanWaves>
 __device__ __forceinline__ int block_scan(int x, int* s, int& sum) {
     const int incl = wave_scan(x);
-    return across_waves(__builtin_amdgcn_readlane(incl, 63), s, sum) + incl - x;
+    return across_waves<W>(__builtin_amdgcn_readlane(incl, 63), s, sum) + incl - x;
 }
 // Workgroup barrier after which the workgroup's earlier global stores and atomics have reached the L2,
 // where its later atomics and device-scope loads see them.
