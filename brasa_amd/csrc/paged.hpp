@@ -104,24 +104,24 @@ struct TouchedBlock {
 };
 __device__ __forceinline__ bool touched_block(const NewRows& a, int item, int pages, TouchedBlock& t) {
     const int lane = threadIdx.x & 63;
-    int seq = -1, before = 0;
+    int seq = -1, before = 0, c0 = 0, c1 = 0, pos = 0;
     for (int i0 = 0; i0 < a.n; i0 += 64) {
-        int c0, c1, pos, nb = 0;
+        int nb = 0;
         if (i0 + lane < a.n) nb = touched_blocks(a, i0 + lane, c0, c1, pos);
         const int incl = wave_scan(nb) + before;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > item);
         if (past) {
             const int l = __builtin_ctzll(past);
             seq = i0 + l;
-            before = __shfl(incl - nb, l);
+            before = __builtin_amdgcn_readlane(incl - nb, l);
+            c0 = __builtin_amdgcn_readlane(c0, l);
+            c1 = __builtin_amdgcn_readlane(c1, l);
+            pos = __builtin_amdgcn_readlane(pos, l);
             break;
         }
-        before = __shfl(incl, 63);
+        before = __builtin_amdgcn_readlane(incl, 63);
     }
     if (seq < 0) return false;  // the grid's bound is loose
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    int c0, c1, pos;
-    touched_blocks(a, seq, c0, c1, pos);
     const int block = pos / kPage + item - before;
     t.page = a.table[(size_t)seq * a.width + block];
     if (t.page < 0 || t.page >= pages) return false;

@@ -112,8 +112,10 @@ struct SharedArgs {
     int n, width, pages;
 };
 
-// A workgroup per group: the first row with positions leads; the others' entries are compared with
-// its, a wave per row, 256 entries at a time, up to the least difference found so far.
+// A workgroup per group: the first row with positions leads; the others' entries are compared with its, four
+// rows a wave, 256 entries at a time, up to the least difference found so far. Bound: the chain group ->
+// lengths -> entries.
+constexpr int kRowsAtOnce = 4;
 __global__ void __launch_bounds__(kScanThreads)
 kv_pages_shared_kernel(SharedArgs a) {
     __shared__ int s_lead, s_live, s_run;
@@ -145,23 +147,33 @@ kv_pages_shared_kernel(SharedArgs a) {
     live = s_live;
     if (live > 1) {
         const int* want = a.table + (size_t)lead * a.width;
-        for (int i = r0 + wave; i < r1; i += kScanWaves) {
-            if (a.len[i] <= 0) continue;
-            const int* row = a.table + (size_t)i * a.width;
+        for (int i0 = r0 + wave; i0 < r1; i0 += kRowsAtOnce * kScanWaves) {
+            int len[kRowsAtOnce];
+            const int* row[kRowsAtOnce];
+#pragma unroll
+            for (int r = 0; r < kRowsAtOnce; ++r) {
+                const int i = min(i0 + r * kScanWaves, r1 - 1);  // (the last once more is no other answer)
+                len[r] = a.len[i];
+                row[r] = a.table + (size_t)i * a.width;
+            }
             // (another wave's lower bound is only a shorter way: the least of all is the same)
             for (int c0 = 0; c0 < *(volatile int*)&s_run; c0 += 256) {
-                int x[4], y[4];
+                int x[4], y[kRowsAtOnce][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int c = min(c0 + 64 * j + lane, a.width - 1);
                     x[j] = want[c];
-                    y[j] = row[c];
+#pragma unroll
+                    for (int r = 0; r < kRowsAtOnce; ++r) y[r][j] = row[r][c];
                 }
                 int at = a.width;
 #pragma unroll
                 for (int j = 3; j >= 0; --j) {
-                    const unsigned long long other = __builtin_amdgcn_ballot_w64(x[j] != y[j] || x[j] < 0 || x[j] >= a.pages);
-                    if (other) at = c0 + 64 * j + __builtin_ctzll(other);
+                    bool other = x[j] < 0 || x[j] >= a.pages;
+#pragma unroll
+                    for (int r = 0; r < kRowsAtOnce; ++r) other |= len[r] > 0 && x[j] != y[r][j];
+                    const uint64_t others = __builtin_amdgcn_ballot_w64(other);
+                    if (others) at = c0 + 64 * j + __builtin_ctzll(others);
                 }
                 if (at < a.width) {
                     if (lane == 0) atomicMin(&s_run, at);
