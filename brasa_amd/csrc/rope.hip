@@ -47,12 +47,11 @@ template <int V>
 __global__ void __launch_bounds__(kRopeThreads)
 rope_axes_kernel(RopeArgs a) {
     typedef float vec __attribute__((ext_vector_type(V)));
-    const long long idx = (long long)blockIdx.x * kRopeThreads + threadIdx.x;
-    const int unit = (int)(idx % a.units);
-    const long long ts = idx / a.units;
-    const int t = (int)(ts / a.spans), h0 = (int)(ts % a.spans) * kSpan;
+    const uint32_t idx = blockIdx.x * kRopeThreads + threadIdx.x;  // (a launch has at most 2^31 of them)
+    const uint32_t ts = idx / (uint32_t)a.units;
+    const int t = (int)(ts / (uint32_t)a.spans), h0 = (int)(ts % (uint32_t)a.spans) * kSpan;
     if (t >= a.count) return;
-    const int i0 = unit * V;
+    const int i0 = (int)(idx % (uint32_t)a.units) * V;
     const RowKind kind = row_kind(a.pos, a.map.axes, a.tokens, t, a.max_pos);
     if (kind == kLeave) return;
     float c[V], s[V];
