@@ -41,7 +41,7 @@ __device__ __forceinline__ long long least_run(long long total) { return total <
 
 struct Tile {
     int seq;          // table row whose pages it reads
-    int row0;         // own tile: the sequence's first packed row; prefix tile: offset in the row list
+    int row0;         // own tile: the sequence's first packed row; prefix tile: the group's first, or offset in the row list
     int col0, cols;   // its columns among the sequence's, or the group's
     int b0, b1;       // pages
     int pos0;         // own tile: position of the sequence's first new row
@@ -53,7 +53,8 @@ struct Tile {
     int index;        // its own
 };
 static_assert(sizeof(Tile) == 64, "a tile is one line");
-enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4 };
+// kInRow: a prefix tile whose group's sharing rows are all packed behind each other (a load less before Q's)
+enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4, kInRow = 8 };
 
 // Columns whose parts a workgroup of the merge joins: `many` of one tile, which continue in one prefix tile or in none.
 struct Join {
@@ -69,11 +70,11 @@ __host__ __device__ constexpr int join_lanes(int parts) { return parts <= 8 ? 32
 
 // Where the plan and the partials stand in the workspace.
 struct Places {
-    size_t merges, rows, ml, acc, bytes;
+    size_t tiles, rows, ml, acc, bytes;
     long long cap;  // columns of partials, for each KV head
 };
 struct Layout : Places {
-    size_t starts, tiles;       // where hq and hkv alone say
+    size_t starts, merges;      // where hkv alone says
     size_t seqs, first, group;  // the plan's own lists
     int runs, max_tiles, max_merges;
 };
@@ -96,9 +97,13 @@ struct PlanGroup {
     int s0, s1;      // its sequences
     int lead, many;  // the first of those that may share its prefix, and how many
     int pages;       // of its prefix
+    int end;         // packed row behind theirs
 };
 
-size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+__host__ __device__ constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+constexpr size_t kStarts = up256(sizeof(Header));
+__host__ __device__ constexpr size_t merges_at(int runs) { return kStarts + up256(sizeof(Tile) * (size_t)runs); }
 
 Layout layout(int n, int groups, int tokens, int hq, int hkv) {
     Layout l;
@@ -117,9 +122,9 @@ Layout layout(int n, int groups, int tokens, int hq, int hkv) {
         at += up256(bytes);
         return a;
     };
-    l.starts = take(sizeof(Tile) * (size_t)l.runs);
-    l.tiles = take(sizeof(Tile) * (size_t)l.max_tiles);
+    l.starts = take(sizeof(Tile) * (size_t)l.runs);  // (at kStarts)
     l.merges = take(sizeof(Join) * (size_t)l.max_merges);
+    l.tiles = take(sizeof(Tile) * (size_t)l.max_tiles);
     l.seqs = take(sizeof(PlanSeq) * (size_t)n);
     l.first = take(4 * ((size_t)groups + n + 1));
     l.group = take(sizeof(PlanGroup) * (size_t)groups);
@@ -135,10 +140,6 @@ Layout layout(int n, int groups, int tokens, int hq, int hkv) {
 // One workgroup: sequences, then groups and sequences again (how many tiles each has), then the tiles, a
 // thread for each of them. Bound: the latency of that chain of loads and scans, once a step.
 struct PlanArgs {
-    const int* cu;
-    const int* pos;
-    const int* group;
-    const int* prefix;
     Header* head;
     Tile* start;  // [runs]: the tile where each run starts
     Tile* tile;
@@ -218,7 +219,7 @@ __device__ __forceinline__ long long div_by(long long x, long long d, double inv
 constexpr int kPlanLds = 1024, kPlanFew = 256;
 template <bool IN_LDS, int THREADS>
 __global__ void __launch_bounds__(THREADS)
-attend_plan_kernel(PlanArgs a) {
+attend_plan_kernel(const int* cu, const int* pos, const int* group, const int* prefix, int n, int groups, PlanArgs a) {
     constexpr int kInLds = !IN_LDS ? 1 : std::min(THREADS, kPlanLds), W = THREADS / 64;
     __shared__ PlanSeq s_seq[kInLds];
     __shared__ PlanGroup s_grp[kInLds];
@@ -246,8 +247,8 @@ attend_plan_kernel(PlanArgs a) {
     struct InGroup {
         int s0, s1, prefix;
     };
-    auto load_in = [&](int i) { return i < a.n ? In{a.cu[i], a.cu[i + 1], a.pos[i]} : In{0, 0, -1}; };
-    auto load_group = [&](int g) { return g < a.groups ? InGroup{a.group[g], a.group[g + 1], a.prefix[g]} : InGroup{0, 0, 0}; };
+    auto load_in = [&](int i) { return i < n ? In{cu[i], cu[i + 1], pos[i]} : In{0, 0, -1}; };
+    auto load_group = [&](int g) { return g < groups ? InGroup{group[g], group[g + 1], prefix[g]} : InGroup{0, 0, 0}; };
     const In in0 = load_in(tid);
     const InGroup group0 = load_group(tid);
 
@@ -264,6 +265,7 @@ attend_plan_kernel(PlanArgs a) {
             st_l2(&grps[g].s1, s1);
             st_l2(&grps[g].lead, a.n);
             st_l2(&grps[g].many, 0);
+            st_l2(&grps[g].end, 0);
             st_l2(&grps[g].pages, min(max(in.prefix, 0) / kPage, a.width));
         }
     }
@@ -300,6 +302,7 @@ attend_plan_kernel(PlanArgs a) {
                     cols = s.rows * per_row;
                     atomicMin(&grps[lo].lead, i);
                     atomicAdd(&grps[lo].many, 1);
+                    atomicMax(&grps[lo].end, c0 + s.rows);
                 }
             }
         }
@@ -366,7 +369,13 @@ attend_plan_kernel(PlanArgs a) {
             const int cols = group_cols(lo, col0);
             t.kind = kPrefix;
             t.seq = ld_l2(&grps[lo].lead);
-            t.row0 = col0 / per_row;
+            const int r0 = ld_l2(&seqs[t.seq].c0);
+            if ((ld_l2(&grps[lo].end) - r0) * (long long)per_row == cols) {
+                t.kind |= kInRow;
+                t.row0 = r0;
+            } else {
+                t.row0 = col0 / per_row;
+            }
             t.cols = min(cols - t.col0, kCols);
             t.b0 = 0;
             t.b1 = prefix_pages(lo);
@@ -486,7 +495,7 @@ attend_plan_kernel(PlanArgs a) {
         a.head->merges = s_merges;
         a.head->size = size;
         a.head->total = line;
-        a.head->at.merges = a.at.merges;
+        a.head->at.tiles = a.at.tiles;
         a.head->at.rows = a.at.rows;
         a.head->at.ml = a.at.ml;
         a.head->at.acc = a.at.acc;
@@ -506,10 +515,11 @@ attend_plan_kernel(PlanArgs a) {
 // S^T = K Q^T on 32x32x16 f16 MFMAs. S^T's layout is the B operand of O^T += V^T P^T: lane (c, h) holds
 // keys 16 st + 8 (j / 4) + 4 h + j % 4 of column c, j < 8, and V's rows stand in LDS in that order, so that
 // ds_read_b64_tr_b8 gives a lane eight keys of one dim at once.
+//
+// ws, hkv and runs are kernel arguments of their own, before the others: such ones are in scalar registers when a
+// wave starts, and the header and the run's tile need not wait for the rest (0.3 us).
 struct AttendArgs {
     uint8_t* ws;
-    const Tile* start;  // in it
-    const Tile* tile;
     size_t ws_len;
     const float* q;
     PoolArgs p;  // of one layer
@@ -517,23 +527,24 @@ struct AttendArgs {
     void* o;
     int n, width, tokens, hq, per_row, o_f16;
 };
+struct AttendCall {  // the kernels' arguments as they stand in memory
+    uint8_t* ws;
+    int hkv, runs;
+    AttendArgs a;
+};
 // The workspace's header and the parts it names.
 struct Plan {
     Header head;
-    const Join* merge;
-    const int* rows;
     float* ml;
     float* acc;
     bool fits;  // it is a plan of this call's sizes
 };
-__device__ __forceinline__ Plan load_plan(const AttendArgs& a) {
+__device__ __forceinline__ Plan load_plan(const uint8_t* ws, const AttendArgs& a) {
     Plan p;
-    p.head = *reinterpret_cast<const Header*>(a.ws);
+    p.head = *reinterpret_cast<const Header*>(ws);
     const Header& h = p.head;
     p.fits = h.magic == kMagic && h.n == a.n && h.tokens == a.tokens && h.width == a.width && h.hq == a.hq &&
              h.hkv == a.p.hkv && h.at.bytes <= a.ws_len;
-    p.merge = reinterpret_cast<const Join*>(a.ws + h.at.merges);
-    p.rows = reinterpret_cast<const int*>(a.ws + h.at.rows);
     p.ml = reinterpret_cast<float*>(a.ws + h.at.ml);
     p.acc = reinterpret_cast<float*>(a.ws + h.at.acc);
     return p;
@@ -614,6 +625,19 @@ __device__ __forceinline__ void copy_keys(const uint8_t* p, uint32_t to) {
         "global_load_lds_dwordx4 %1, off offset:1024\n\t"
         "global_load_lds_dwordx4 %1, off offset:2048\n\t"
         "global_load_lds_dwordx4 %1, off offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(p), "s"(to)
+        : "memory");
+}
+// 16 bytes a lane from p into the LDS at `to`, one lane's behind another's.
+__device__ __forceinline__ void copy_rows(const float* p, uint32_t to) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
         : "v"(p), "s"(to)
@@ -752,29 +776,31 @@ __device__ __forceinline__ void hide_values(uint8_t* v, int* first, int last1, i
 
 template <bool EXACT>
 __global__ void __launch_bounds__(kThreads, 2)
-attend_kernel(AttendArgs a) {
+attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
     constexpr int kHalf = 32 * kDim;  // codes of half a page
-    __shared__ __attribute__((aligned(16))) uint8_t s_k[kWaves][2][kHalf], s_v[kWaves][2][kHalf];
+    // a wave's: V's two halves, K's; before them Q's rows and behind them the result's, 512 bytes a column
+    __shared__ __attribute__((aligned(16))) uint8_t s_kv[kWaves][4 * kHalf];
+    static_assert(4 * kHalf == kCols * 4 * kDim, "32 columns of f32");
     __shared__ __attribute__((aligned(16))) int s_nan[kWaves][kDim];  // first key with a NaN value, for each dim
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
-    const int kh = blockIdx.x % a.p.hkv, run = blockIdx.x / a.p.hkv * kWaves + wave;
+    const int kh = blockIdx.x % hkv, run = blockIdx.x / hkv * kWaves + wave;
     // The arguments and the header are read again where they are needed: held in scalar registers over
     // the loop they would crowd out its own.
-    auto args = [] { return (Scalar<AttendArgs>)again(__builtin_amdgcn_kernarg_segment_ptr()); };
+    auto args = [] { return (Scalar<AttendArgs>)(again(__builtin_amdgcn_kernarg_segment_ptr()) + offsetof(AttendCall, a)); };
     auto header = [&] { return (Scalar<Header>)(uintptr_t)args()->ws; };
     // (a run's first tile comes with the header, before it is known to be one)
-    Tile t = load_line(a.start + min(run, max(kRuns / a.p.hkv, kWaves) - 1));
+    Tile t = load_line(reinterpret_cast<const Tile*>(ws + kStarts) + min(run, runs - 1));
     {
-        const Plan plan = load_plan(a);
+        const Plan plan = load_plan(ws, a);
         if (!plan.fits || run >= plan.head.runs || run * plan.head.size >= plan.head.total) return;
     }
 
     while (true) {
         // ---- this run's pages of the tile ------------------------------------------------------------
         const int ti = t.index;
-        int p0, p1, row0, col0, cols, pos0, kind;
+        int p0, p1, row0, col0, cols, pos0, kind, part0;
         const int* ids;
         {
             const auto g = args();
@@ -789,6 +815,7 @@ attend_kernel(AttendArgs a) {
             cols = t.cols;
             pos0 = t.pos0;
             kind = t.kind;
+            part0 = t.base + (run - t.run0) * cols;
         }
         if (p0 < p1) {
         const bool nowhere = kind & kBad;
@@ -798,8 +825,8 @@ attend_kernel(AttendArgs a) {
         const uint32_t k_from = j8 * kDim + piece, v_from = 1024 * (j8 >> 2) + kDim * (j8 & 3) + piece;
         const uint32_t k_at = c * kDim + ((h ^ (c & 7)) * 16), jv = (lane & 15) >> 1;
         const uint32_t v_at = (8 * h + jv) * kDim + 8 * (lane & 1) + ((((lane >> 4) & 1) ^ jv) * 16);
-        const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_k[wave]));
-        const uint32_t v_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_v[wave]));
+        const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_kv[wave]) + 2 * kHalf);
+        const uint32_t v_lds = __builtin_amdgcn_readfirstlane(lds_addr(s_kv[wave]));
         auto load_k = [&](uint32_t tile, int half) {
             copy_keys(a.p.k + (size_t)tile * kTileBytes8 + half * kHalf + k_from, k_lds + half * kHalf);
         };
@@ -828,18 +855,31 @@ attend_kernel(AttendArgs a) {
         int qx;
         {
             const auto g = args();
-            const int col = col0 + min(c, cols - 1);  // (lanes past the last column repeat it)
-            const int local = col / g->per_row;
+            const int cc = min(c, cols - 1);  // (lanes past the last column repeat it)
+            const int col = col0 + cc, local = col / g->per_row;
             int row = row0 + local;
-            if (kind & kPrefix) row = reinterpret_cast<const int*>(g->ws + header()->at.rows)[row];
-            const int head_of = kh * g->per_row + col - local * g->per_row;
+            if ((kind & (kPrefix | kInRow)) == kPrefix) row = reinterpret_cast<const int*>(g->ws + header()->at.rows)[row];
+            const int q_row = row * g->hq + kh * g->per_row + col - local * g->per_row;
             limit = kind & kPrefix ? INT_MAX : nowhere ? -1 : pos0 + local;
+            // Q's rows, two an instruction, as K's and V's codes: 16-byte piece p of column c in place p ^ c. (By lanes,
+            // as the operands want them, an instruction touches 64 lines; with eight waves on a CU Q then took 7600
+            // cycles of a tile, and so 4400.)
+            const float* const qs = g->q;
+            int slot = c ^ h;
+            asm volatile("" : "+v"(slot));  // (or sixteen of them are kept over the tiles)
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) {
+                if (2 * i >= cols) break;
+                const int r0 = __builtin_amdgcn_readlane(q_row, 2 * i), r1 = __builtin_amdgcn_readlane(q_row, 2 * i + 1);
+                copy_rows(qs + (size_t)(h ? r1 : r0) * kDim + 4 * (slot ^ 2 * i), v_lds + 1024 * i);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             // step s holds dims 32 (s / 2) + 16 h + 8 (s % 2) .. + 8, as K's 16-byte pieces do
-            const float* qrow = g->q + ((size_t)row * g->hq + head_of) * kDim + 16 * h;
+            const uint32_t q_at = cc * 4 * kDim + 16 * (4 * h ^ cc);
             f32x4 raw[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                raw[i] = *reinterpret_cast<const f32x4*>(qrow + 32 * (i >> 2) + 8 * ((i >> 1) & 1) + 4 * (i & 1));
+                raw[i] = *reinterpret_cast<const f32x4*>(&s_kv[wave][q_at ^ 16 * (8 * (i >> 2) + 2 * ((i >> 1) & 1) + (i & 1))]);
             // Q here, then the first page's copies on their way, then the work on Q under them. (The compiler
             // does not count the copies: a wait for an earlier load would be one for them too.)
 #pragma unroll
@@ -851,28 +891,29 @@ attend_kernel(AttendArgs a) {
             load_k(tile, 1);
             load_v(tile, 0);
             in_order();
-            const float scale = 0.08838834764831845f * kLog2e;
-            float x[8][8];
+            constexpr float kScale = 0.08838834764831845f * kLog2e;
             float qmax = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[s][j] = as_f32(raw[2 * s + (j >> 2)][j & 3] * scale);
-                    qmax = fmaxf(qmax, fabsf(x[s][j]));
-                }
-            qmax = max_h(qmax);
-            qx = (int)(__float_as_uint(qmax) >> 23) - 127 - 8;  // the row's largest to [2^8, 2^9)
+            for (int i = 0; i < 16; ++i) {
+                qmax = fmaxf(fmaxf(qmax, fabsf(raw[i][0])), fabsf(raw[i][1]));
+                qmax = fmaxf(fmaxf(qmax, fabsf(raw[i][2])), fabsf(raw[i][3]));
+            }
+            qmax = max_h(qmax) * kScale;
+            // the row's largest to [2^8, 2^9) (below 2^-112 it stays less: every score is 0 there)
+            qx = max((int)(__float_as_uint(qmax) >> 23) - 127 - 8, -120);
+            const float up = ldexpf(kScale, -qx), up11 = up * 0x1p11f;
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 half2v u[4], w[4];
                 float rest[8];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float y0 = ldexpf(x[s][2 * j], -qx), y1 = ldexpf(x[s][2 * j + 1], -qx);
-                    split(y0, y1, u[j], w[j]);
-                    rest[2 * j] = ldexpf(y0 - (float)u[j].x, 11);
-                    rest[2 * j + 1] = ldexpf(y1 - (float)u[j].y, 11);
+                    const float x0 = raw[2 * s + (j >> 1)][2 * (j & 1)], x1 = raw[2 * s + (j >> 1)][2 * (j & 1) + 1];
+                    split(x0 * up, x1 * up, u[j], w[j]);
+                    if constexpr (!EXACT) {  // (times 2^11: exact)
+                        rest[2 * j] = fmaf((float)u[j].x, -0x1p11f, x0 * up11);
+                        rest[2 * j + 1] = fmaf((float)u[j].y, -0x1p11f, x1 * up11);
+                    }
                 }
                 q.hi[s] = join(u[0], u[1], u[2], u[3]);
                 if constexpr (EXACT) {
@@ -911,13 +952,13 @@ attend_kernel(AttendArgs a) {
         i32x2 vw[2][4]; // keys 16 st + 8 (j / 4) + 4 h + j % 4 of dim 32 t + c at [st][t]
         auto read_k = [&](int half) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(&s_k[wave][half][k_at ^ 32 * i]);
+            for (int i = 0; i < 4; ++i) kw[i] = *reinterpret_cast<const u32x4*>(&s_kv[wave][(2 + half) * kHalf + (k_at ^ 32 * i)]);
         };
         auto read_v = [&](int half) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 vw[i >> 2][i & 3] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) i32x2*)&s_v[wave][half][2048 * (i >> 2) + (v_at ^ 32 * (i & 3))]);
+                    (__attribute__((address_space(3))) i32x2*)&s_kv[wave][half * kHalf + 2048 * (i >> 2) + (v_at ^ 32 * (i & 3))]);
         };
         if (!nowhere) {
             int page = p0;
@@ -959,7 +1000,7 @@ attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (8 * (i >> 2) + (i & 3) > last) s[i] = -INFINITY;
-                    hide_values(s_v[wave][half], s_nan[wave], lim1 - k0, limit - k0, acc);
+                    hide_values(&s_kv[wave][half * kHalf], s_nan[wave], lim1 - k0, limit - k0, acc);
                 }
                 float top = fmaxf(fmaxf(s[12], s[13]), fmaxf(s[14], s[15]));
 #pragma unroll
@@ -1063,33 +1104,53 @@ attend_kernel(AttendArgs a) {
         for (int i = 0; i < 4; ++i) acc[i] *= unit;
 
         // ---- out: to o, or to the parts. The lane holds dims 32 t + 8 q + 4 h + r of its column -------------
-        if (c >= cols) {
-        } else if (kind & kDirect) {
-            const int col = col0 + c, local = col / g->per_row;  // (a prefix tile is never direct)
-            const size_t at = ((size_t)(row0 + local) * g->hq + kh * g->per_row + col - local * g->per_row) * kDim;
+        // and the rows leave through the LDS, two an instruction (straight from the lanes an instruction would touch
+        // 64 lines, as Q's would).
+        const bool direct = kind & kDirect;
+        if (direct) {
             const float inv = 1.0f / lsum;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const f32x16& x = acc[i >> 2];
-                const int r = 4 * (i & 3);
-                write_o<!EXACT>(g->o, at + 32 * (i >> 2) + 2 * r + 4 * h, f32x4{x[r], x[r + 1], x[r + 2], x[r + 3]}, inv);
+            for (int i = 0; i < 4; ++i) acc[i] *= inv;
+        }
+        uint32_t o_at = c * 4 * kDim + 16 * (h ^ c), piece_at = h * 4 * kDim + 16 * (h ^ c);
+        asm volatile("" : "+v"(o_at), "+v"(piece_at));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const f32x16& x = acc[i >> 2];
+            const int r = 4 * (i & 3);
+            *reinterpret_cast<f32x4*>(&s_kv[wave][o_at ^ 16 * (8 * (i >> 2) + 2 * (i & 3))]) = f32x4{x[r], x[r + 1], x[r + 2], x[r + 3]};
+        }
+        asm volatile("" ::: "memory");
+        auto column = [&](int i) {  // columns 2 i, 2 i + 1: this lane's piece
+            return *reinterpret_cast<const f32x4*>(&s_kv[wave][(piece_at ^ 32 * i) + 8 * kDim * i]);
+        };
+        if (direct) {
+            const int col = col0 + c, local = col / g->per_row;  // (a prefix tile is never direct)
+            const int o_row = (row0 + local) * g->hq + kh * g->per_row + col - local * g->per_row;
+            void* const o = g->o;
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) {
+                if (2 * i >= cols) break;
+                const int r0 = __builtin_amdgcn_readlane(o_row, 2 * i), r1 = __builtin_amdgcn_readlane(o_row, 2 * i + 1);
+                const f32x4 x = column(i);
+                if (2 * i + h < cols) write_o<!EXACT>(o, (size_t)(h ? r1 : r0) * kDim + 4 * c, x, 1.0f);
             }
         } else {
             const auto hd = header();
-            const auto own = (Scalar<Tile>)(uintptr_t)g->tile + ti;
-            const size_t part = (size_t)kh * hd->at.cap + own->base + (size_t)(run - own->run0) * cols + c;
-            float* to = reinterpret_cast<float*>(g->ws + hd->at.acc) + part * kDim + 4 * h;
+            const size_t part = (size_t)kh * hd->at.cap + part0;
+            float* to = reinterpret_cast<float*>(g->ws + hd->at.acc) + part * kDim + 4 * lane;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const f32x16& x = acc[i >> 2];
-                const int r = 4 * (i & 3);
-                *reinterpret_cast<f32x4*>(to + 32 * (i >> 2) + 2 * r) = f32x4{x[r], x[r + 1], x[r + 2], x[r + 3]};
+            for (int i = 0; i < kCols / 2; ++i) {
+                if (2 * i >= cols) break;
+                const f32x4 x = column(i);
+                if (2 * i + h < cols) *reinterpret_cast<f32x4*>(to + 2 * kDim * i) = x;
             }
-            if (h == 0) *reinterpret_cast<f32x2*>(reinterpret_cast<float*>(g->ws + hd->at.ml) + 2 * part) = f32x2{m_used, lsum};
+            if (lane < cols) *reinterpret_cast<f32x2*>(reinterpret_cast<float*>(g->ws + hd->at.ml) + 2 * (part + lane)) = f32x2{m_used, lsum};
         }
         }
-        if (ti + 1 >= header()->tiles) break;
-        t = load_line(reinterpret_cast<const Tile*>((uintptr_t)args()->tile) + ti + 1);
+        const auto hd = header();
+        if (ti + 1 >= hd->tiles) break;
+        t = load_line(reinterpret_cast<const Tile*>(args()->ws + hd->at.tiles) + ti + 1);
     }
 }
 
@@ -1099,14 +1160,17 @@ attend_kernel(AttendArgs a) {
 // or every eighth, 16 bytes of their sums a lane and eight parts on their way at once, and then the halves
 // theirs. Bound: the chain header -> unit -> parts -> o, and for prompts the parts' bytes.
 __global__ void __launch_bounds__(kThreads)
-attend_merge_kernel(AttendArgs a) {
+attend_merge_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
     __shared__ __attribute__((aligned(16))) float s_x[kWaves][kDim];
     __shared__ f32x2 s_ml[kWaves];
-    const Plan plan = load_plan(a);
+    const Join* units = reinterpret_cast<const Join*>(ws + merges_at(runs));
+    const int kh = blockIdx.x % hkv, e0 = blockIdx.x / hkv, es = gridDim.x / hkv;
+    // (the first unit comes with the header, before it is known to be one)
+    Join j = load_line(units + e0);
+    const Plan plan = load_plan(ws, a);
     const Header& head = plan.head;
     const int lane = threadIdx.x & 63, h = lane >> 5, d = 4 * (lane & 31);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kh = blockIdx.x % a.p.hkv, e0 = blockIdx.x / a.p.hkv, es = gridDim.x / a.p.hkv;
     if (!plan.fits) {  // of another step's sizes, or none: no row is left looking like a result
         const size_t all = (size_t)a.tokens * a.hq * kDim;
         for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (size_t)gridDim.x * kThreads) {
@@ -1118,7 +1182,7 @@ attend_merge_kernel(AttendArgs a) {
     const float* ml = plan.ml + 2 * (size_t)kh * head.at.cap;
     const float* sums = plan.acc + (size_t)kh * head.at.cap * kDim + d;
     for (int e = e0; e < head.merges; e += es) {
-        const Join j = load_line(plan.merge + e);
+        if (e != e0) j = load_line(units + e);
         // this half wave's column, and its first part
         const int half = 2 * wave + h, step = j.lanes / 32;
         const int c = j.lanes == 32 ? half : j.lanes == 64 ? wave : 0, first = half & (step - 1);
@@ -1198,10 +1262,6 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
     const Layout l = layout(n, groups, tokens, hq, hkv);
     uint8_t* w = static_cast<uint8_t*>(ws);
     PlanArgs a = {};
-    a.cu = cu;
-    a.pos = pos;
-    a.group = group;
-    a.prefix = prefix;
     a.head = reinterpret_cast<Header*>(w);
     a.start = reinterpret_cast<Tile*>(w + l.starts);
     a.tile = reinterpret_cast<Tile*>(w + l.tiles);
@@ -1223,7 +1283,8 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
     auto kernel = few                                       ? attend_plan_kernel<true, kPlanFew>
                   : n <= kPlanLds && groups <= kPlanLds ? attend_plan_kernel<true, kScanThreads>
                                                         : attend_plan_kernel<false, kScanThreads>;
-    hipLaunchKernelGGL(kernel, dim3(1), dim3(few ? kPlanFew : kScanThreads), 0, stream, a);
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(few ? kPlanFew : kScanThreads), 0, stream, cu, pos, group, prefix, n,
+                       groups, a);
     return check_launch("attend_plan_kernel");
 }
 
@@ -1233,8 +1294,6 @@ int attend_launch(const float* q, const PoolArgs& pool, const int* table, int wi
     AttendArgs a = {};
     a.ws = static_cast<uint8_t*>(ws);
     a.ws_len = ws_len;
-    a.start = reinterpret_cast<const Tile*>(a.ws + l.starts);
-    a.tile = reinterpret_cast<const Tile*>(a.ws + l.tiles);
     a.q = q;
     a.p = pool;
     a.table = table;
@@ -1246,13 +1305,14 @@ int attend_launch(const float* q, const PoolArgs& pool, const int* table, int wi
     a.per_row = hq / pool.hkv;
     a.o_f16 = o_f16;
     auto kernel = o_f16 ? attend_kernel<false> : attend_kernel<true>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0,
-                       stream, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0, stream,
+                       a.ws, pool.hkv, l.runs, a);
     const int st = check_launch("attend_kernel");
     if (st != BRASA_OK) return st;
-    // a workgroup for each entry of a KV head, up to eight per CU
+    // a workgroup for each unit of a KV head, up to eight per CU
     const int wgs = std::max(std::min(l.max_merges, 2048 / pool.hkv), 1);
-    hipLaunchKernelGGL(attend_merge_kernel, dim3((unsigned)(wgs * pool.hkv)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(attend_merge_kernel, dim3((unsigned)(wgs * pool.hkv)), dim3(kThreads), 0, stream, a.ws,
+                       pool.hkv, l.runs, a);
     return check_launch("attend_merge_kernel");
 }
 
