@@ -487,6 +487,16 @@ int brasa_kv_pages_compact(brasa_kv_pool pool, const int32_t* table, const int32
                                    as_stream(stream));
 }
 
+// Arrays of a call, for what must not overlap: other workgroups read while one writes.
+struct Range {
+    const void* p;
+    size_t bytes;
+};
+static bool overlap(const Range& a, const Range& b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return x && y && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+
 // The axes of `half` pairs and the table they index.
 static int axes_check(const char* what, const brasa_rope_axes_map& m, const brasa_rope_table_view& table, size_t dim) {
     if (dim != table.dim) return set_error(BRASA_ERR_SHAPE, "RoPE table dimension");
@@ -536,6 +546,9 @@ int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, f
         return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16)
         return set_error(BRASA_ERR_ARG, "%s: the rows must be 16-byte aligned", what);
+    const Range rq{q, tokens * hq * 4 * kDim}, rk{k, tokens * pool.hkv * 4 * kDim}, rv{v, tokens * pool.hkv * 4 * kDim};
+    if (overlap(rq, rk) || overlap(rq, rv) || overlap(rk, rv))
+        return set_error(BRASA_ERR_ARG, "%s: q, k and v overlap", what);
     return norm_rope_paged_launch(p, q, k, v, q_norm, k_norm, eps, table.cos, table.sin, (int)table.max_pos, axes,
                                   rope_pos, cu, pos, pages, (int)n, (int)width, (int)tokens, (int)hq,
                                   as_stream(stream));
@@ -552,7 +565,11 @@ int brasa_kv_rows(const int32_t* add, const int32_t* len, const int32_t* table, 
     if (tokens > kMaxPositions) return set_error(BRASA_ERR_SHAPE, "%s: %zu rows", what, tokens);
     if (n == 0) return set_error(BRASA_ERR_SHAPE, "%s: no sequences", what);
     if (!add || !len || (slot && width && !table)) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
-    if (lk == len || cu == add) return set_error(BRASA_ERR_ARG, "%s: lk and cu must be arrays of their own", what);
+    const Range all[8] = {{add, 4 * n}, {len, 4 * n}, {slot ? table : nullptr, 4 * n * width}, {cu, 4 * (n + 1)}, {lk, 4 * n},
+                          {seq, 4 * tokens}, {pos, 4 * tokens}, {slot, 4 * tokens}};
+    for (int i = 3; i < 8; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(all[i], all[j])) return set_error(BRASA_ERR_ARG, "%s: an output overlaps another array", what);
     return kv_rows_launch(add, len, table, cu, lk, seq, pos, slot, (int)n, (int)width, (int)pages, (int)tokens,
                           as_stream(stream));
 }
@@ -567,6 +584,9 @@ int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_
     if (groups > kMaxSeqs) return set_error(BRASA_ERR_SHAPE, "%s: %zu groups", what, groups);
     if (groups == 0) return BRASA_OK;
     if (!group || !prefix || (n && (!len || (width && !table)))) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
+    const Range out{prefix, 4 * groups};
+    if (overlap(out, {group, 4 * (groups + 1)}) || overlap(out, {len, 4 * n}) || overlap(out, {table, 4 * n * width}))
+        return set_error(BRASA_ERR_ARG, "%s: prefix overlaps an input", what);
     return kv_pages_shared_launch(table, len, group, (int)groups, prefix, (int)n, (int)width, (int)pages,
                                   as_stream(stream));
 }
@@ -623,6 +643,10 @@ int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, cons
     if (!q || (!table && width) || !workspace || !o) return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
     if ((uintptr_t)workspace % 256 || ((uintptr_t)q | (uintptr_t)o) % 16)
         return set_error(BRASA_ERR_ARG, "%s: q and o must be 16-byte, the workspace 256-byte aligned", what);
+    const size_t values = tokens * hq * kDim;
+    const Range rq{q, 4 * values}, ro{o, (o_dtype == BRASA_OUT_F16 ? 2 : 4) * values}, rw{workspace, need};
+    if (overlap(rq, ro) || overlap(rq, rw) || overlap(ro, rw))
+        return set_error(BRASA_ERR_ARG, "%s: q, o and the workspace overlap", what);
     return attend_launch(q, p, table, (int)width, (int)n, (int)tokens, workspace, workspace_len, o,
                          o_dtype == BRASA_OUT_F16, (int)hq, as_stream(stream));
 }

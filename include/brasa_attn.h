@@ -492,7 +492,7 @@ int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t laye
  * and turned by rope_pos [axes, tokens]; k (turned) and v (as given) go into the pages as in
  * brasa_store_kv_paged. Rows of q from cu[0] to cu[n], and rows of k whose position has a page; the others
  * are left as they are. (A rotary position outside the table, a negative one too, gives NaN here.) Requires
- * table.dim == 128; rows of q, k and v 16-byte aligned.
+ * table.dim == 128; rows of q, k and v 16-byte aligned and apart.
  */
 int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, float* k, const float* v,
                                    const float* q_norm, const float* k_norm, float eps,
@@ -506,8 +506,8 @@ int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, f
  * (none where add[i] <= 0 or len[i] < 0). cu [n + 1]: its rows are cu[i] .. cu[i + 1]; lk [n]: its length after the step;
  * and for each row t < tokens its sequence seq[t], position pos[t] and slot[t] = page * 64 + position % 64 of
  * its page in the table, -1 where that is not there. Rows behind the last sequence's get -1 in all three; rows past
- * `tokens` are cut off (cu and lk too). table as above (`pages`: the pool's). Any output may be NULL; lk must not
- * be len, nor cu add.
+ * `tokens` are cut off (cu and lk too). table as above (`pages`: the pool's). Any output may be NULL; none may overlap
+ * an input or another.
  */
 int brasa_kv_rows(const int32_t* add, const int32_t* len, const int32_t* table, size_t n, size_t width,
                   size_t pages, size_t tokens, int32_t* cu, int32_t* lk, int32_t* seq, int32_t* pos,
@@ -517,7 +517,8 @@ int brasa_kv_rows(const int32_t* add, const int32_t* len, const int32_t* table, 
  * The positions that groups of sequences share: group g is sequences group[g] .. group[g + 1] (device, [groups + 1]),
  * and prefix[g] = 64 times the number of leading pages that all of its sequences with len[i] > 0 name alike and fill
  * (64 positions of each page at least; as forks of one sequence or requests behind one system prompt do); 0
- * for a group with fewer than two such sequences. Bounds of group outside [0, n] or out of order are clamped.
+ * for a group with fewer than two such sequences. Bounds of group outside [0, n] or out of order are clamped. prefix must
+ * not overlap an input.
  */
 int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_t* group, size_t groups,
                           size_t n, size_t width, size_t pages, int32_t* prefix, void* stream);
@@ -545,7 +546,7 @@ int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_
  *
  * workspace: brasa_attention_paged_workspace_len bytes, 256-byte aligned, any contents: the plan, then the partial
  * sums of one call at a time. Calls that may run at the same time need workspaces (and plans) of their own. q and o
- * 16-byte aligned; tokens * hq up to 2^29.
+ * 16-byte aligned, both and the workspace apart; tokens * hq up to 2^29.
  */
 size_t brasa_attention_paged_workspace_len(size_t n, size_t groups, size_t tokens, size_t hq, size_t hkv);
 int brasa_attention_paged_plan(const int32_t* cu, const int32_t* pos, const int32_t* group,

@@ -200,6 +200,16 @@ def test_many_sequences():
     s.check()
 
 
+@pytest.mark.parametrize("n,hq", [(250, 2), (257, 2), (300, 16), (900, 16)])
+def test_rounds_of_the_plan(n, hq):
+    """Each size of the plan's workgroup, with tiles for one round of it or more: few and many columns of a sequence
+    in a prefix that crosses tiles, and one group whose rows are not packed behind each other."""
+    new = [1] * n
+    new[n // 2] = 40
+    held = [64 + (7 * i) % 90 for i in range(n)]
+    _run(("rounds", n, hq), new=new, held=held, groups=[(n // 3, 64), (n - n // 3, 64)], hq=hq, hkv=1, seed=n)
+
+
 @pytest.mark.parametrize("out", list(OutDType))
 def test_values_that_are_not_finite(out):
     """NaN keys and values reach the rows that see them, in their places, and no others."""

@@ -93,6 +93,36 @@ def test_attention_refusals(code, over):
     _refused(code, lambda: Kernels().attention_paged(**a))
 
 
+@pytest.mark.parametrize("over", [
+    {"lk": P + 4}, {"cu": P + 68}, {"cu": P - 8}, {"lk": P + 64}, {"seq": P + 60}, {"slot": P + 512}, {"pos": P + 512 + 20},
+    {"slot": P + 192}, {"seq": P + 256, "pos": P + 272}], ids=str)
+def test_rows_overlaps(over):
+    a = {**dict(add=P + 64, lens=P, table=P + 512, n=2, width=3, pages=9, tokens=5, cu=P + 128, lk=P + 192, slot=P + 256), **over}
+    _refused(ARG, lambda: Kernels().kv_rows(**a))
+
+
+@pytest.mark.parametrize("prefix", [P, P + 4, P + 68, P + 140, P - 4])
+def test_shared_overlaps(prefix):
+    _refused(ARG, lambda: Kernels().kv_pages_shared(table=P + 128, lens=P + 64, group=P, groups=2, n=2, width=3, pages=9,
+                                                   prefix=prefix))
+
+
+@pytest.mark.parametrize("qkv", [(P, P, 1 << 30), (1 << 30, P, P), (P, 1 << 30, P), (P, P + 5 * 32 * 512 - 16, 1 << 30),
+                                 (1 << 30, P, P + 5 * 8 * 512 - 16)])
+def test_writer_overlaps(qkv):
+    _refused(ARG, lambda: Kernels().qk_norm_rope_store_paged(
+        KvPool.view(P, P, P, P, 2, 8, 8), 1, qkv, (P, P), 1e-6, RopeTable.view(P, P, 128, 10), RopeAxes([64]), P, P, P, P, 2, 3, 5, 32))
+
+
+@pytest.mark.parametrize("out,size", [(OutDType.F32, 4), (OutDType.F16, 2)])
+def test_attention_overlaps(out, size):
+    base, values = 1 << 40, 5 * 32 * 128
+    need = attention_paged_workspace_len(2, 0, 5, 32, 8)
+    for q, o, ws in ((base, base, P), (base, base + 4 * values - 16, P), (base + size * values - 16, base, P),
+                     (P, base, base), (base, P, base + 1024), (base + need - need % 16 - 16, P, base)):
+        _refused(ARG, lambda: Kernels().attention_paged(q, KvPool.view(P, P, P, P, 1, 8, 8), 0, P, 2, 4, 5, ws, need, o, 32, out))
+
+
 def test_workspace_len():
     assert attention_paged_workspace_len(2, 0, 4, 30, 8) == 0
     for n, groups, tokens, hq, hkv in ((1, 0, 1, 32, 8), (64, 3, 64, 32, 8), (3, 1, 9000, 8, 8), (100, 2, 100, 128, 1)):
