@@ -5,7 +5,8 @@
 // position p = pos[a(i)][t]: y_i = x_i c - x_{i + dim / 2} s, y_{i + dim / 2} = x_{i + dim / 2} c + x_i s,
 // with c and s the table's entries (p, i). One axis is rope_neox, bit for bit.
 //
-// Bound: HBM, 8 bytes a value in and out.
+// Bound: HBM, 8 bytes a value in and out. 16000 rows of 32 heads of 128 take 85 us (524 MB, 6.2 TB/s, in place),
+// 1027 rows of 16 heads of 72 4.9 (the chain positions -> angles -> rows).
 #include "paged.hpp"
 
 namespace brasa {
@@ -40,7 +41,8 @@ __device__ __forceinline__ RowKind row_kind(const int* pos, int axes, int tokens
     return leave ? kLeave : none ? kNone : kTurn;
 }
 
-// A thread turns V neighbouring pairs of up to kSpan heads of a token, whose angles it loads once.
+// A thread turns V neighbouring pairs of up to kSpan heads of a token, whose angles it loads once. (The rows are
+// asked for behind the angles: before them, large calls take 97 us in place of 85.)
 constexpr int kSpan = 4;
 constexpr int kRopeThreads = 256;
 template <int V>
@@ -90,7 +92,8 @@ rope_axes_kernel(RopeArgs a) {
 // A workgroup takes the new rows of one (block, KV head) of K or V, a row per wave and instruction, all
 // of them in registers (lane l holds values l and l + 64, a rotary pair and rms_norm's order of sums, so
 // the bits are those of rms_norm, rope_axes and store_kv_paged in sequence); the workgroups behind
-// them take rows of q.
+// them take rows of q. Bound: HBM for prompts (5548 rows of 32 + 8 + 8 heads in 48.3 us: 242 MB, 5.0 TB/s; with one
+// row of q a wave in place of eight 77.9), the chain lengths -> page -> scale -> codes for a step (64 rows 9.3 us).
 constexpr int kWriteWaves = 4;
 constexpr int kWriteThreads = 64 * kWriteWaves;
 constexpr int kTileRows = kPage / kWriteWaves;  // rows of a block that a wave takes
@@ -148,7 +151,7 @@ __device__ __forceinline__ void norm_turn(float& x0, float& x1, float w0, float 
     x1 = b0 * c + a0 * s;
 }
 
-template <int RPW>  // rows of q for each wave, of one token
+constexpr int kRows = 8;  // of q for each wave, of one token, whose loads travel together
 __global__ void __launch_bounds__(kWriteThreads, 5)
 norm_rope_paged_kernel(WriteArgs a) {
     const int lane = threadIdx.x & 63;
@@ -159,13 +162,13 @@ norm_rope_paged_kernel(WriteArgs a) {
         const int first = min(max(scalar(a.rows.cu)[0], 0), a.rows.tokens);
         const int last = min(max(scalar(a.rows.cu)[a.rows.n], first), a.rows.tokens);
         const unsigned unit = blockIdx.x - a.tiles;
-        const int t = a.t0 + (int)(unit / a.spans), h0 = ((int)(unit % a.spans) * kWriteWaves + wave) * RPW;
+        const int t = a.t0 + (int)(unit / a.spans), h0 = ((int)(unit % a.spans) * kWriteWaves + wave) * kRows;
         if (t < first || t >= last || h0 >= a.hq) return;
         float* q = a.q + ((size_t)t * a.hq + h0) * kDim + lane;
-        float x0[RPW], x1[RPW], c, s;
-        const int rows = min(a.hq - h0, RPW);
+        float x0[kRows], x1[kRows], c, s;
+        const int rows = min(a.hq - h0, kRows);
 #pragma unroll
-        for (int j = 0; j < RPW; ++j) {
+        for (int j = 0; j < kRows; ++j) {
             const int r = min(j, rows - 1);
             x0[j] = q[r * kDim];
             x1[j] = q[r * kDim + 64];
@@ -173,7 +176,7 @@ norm_rope_paged_kernel(WriteArgs a) {
         angle_of(a, t, lane, axis, c, s);
         const float w0 = a.qn[lane], w1 = a.qn[lane + 64];
 #pragma unroll
-        for (int j = 0; j < RPW; ++j) {
+        for (int j = 0; j < kRows; ++j) {
             if (j >= rows) break;
             norm_turn(x0[j], x1[j], w0, w1, c, s, a.eps);
             q[j * kDim] = x0[j];
@@ -310,7 +313,10 @@ int rope_axes_launch(float* x, const float* cos_t, const float* sin_t, int max_p
     a.heads = heads;
     a.half = dim / 2;
     a.max_pos = max_pos;
-    if (a.half % 4 == 0 && (uintptr_t)x % 16 == 0) return launch_rope<4>(a, stream);
+    // Four pairs a thread, 16 bytes an access, for large calls: 67M values in 83 us, a pair a thread 93. Small ones
+    // want the threads: 1.2M values 4.7 us a pair a thread and 5.3 four, 8.4M 11.2 and 11.7.
+    if (a.half % 4 == 0 && (uintptr_t)x % 16 == 0 && (long long)tokens * heads * dim > (1LL << 23))
+        return launch_rope<4>(a, stream);
     return launch_rope<1>(a, stream);
 }
 
@@ -334,10 +340,7 @@ int norm_rope_paged_launch(const PoolArgs& pool, float* q, float* k, const float
     a.hq = hq;
     a.max_pos = max_pos;
     const long long items = width ? most_blocks(n, tokens) : 0;
-    // one row of q per wave while every row can have a wave at once, else eight of a token, whose loads
-    // travel together
-    const int rpw = (long long)tokens * hq <= 256 * 32 ? 1 : 8;
-    a.spans = (hq + kWriteWaves * rpw - 1) / (kWriteWaves * rpw);
+    a.spans = (hq + kWriteWaves * kRows - 1) / (kWriteWaves * kRows);
     // A launch of 2^32 threads or more runs fewer, without an error: at most 2^30 of each kind in each.
     const long long most = (1LL << 30) / kWriteThreads / (2 * pool.hkv);
     const long long most_q = a.spans ? (1LL << 30) / kWriteThreads / a.spans : tokens;
@@ -347,10 +350,7 @@ int norm_rope_paged_launch(const PoolArgs& pool, float* q, float* k, const float
         a.tiles = (unsigned)(std::min(std::max(items - i, 0LL), most) * 2 * pool.hkv);
         const unsigned more = (unsigned)(std::min(std::max(tokens - t, 0LL), most_q) * a.spans);
         if (a.tiles + more == 0) break;
-        if (rpw == 1)
-            hipLaunchKernelGGL(norm_rope_paged_kernel<1>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
-        else
-            hipLaunchKernelGGL(norm_rope_paged_kernel<8>, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
+        hipLaunchKernelGGL(norm_rope_paged_kernel, dim3(a.tiles + more), dim3(kWriteThreads), 0, stream, a);
         const int st = check_launch("norm_rope_paged_kernel");
         if (st != BRASA_OK) return st;
     }

@@ -66,6 +66,24 @@ def test_one_axis_is_rope_neox(dim, offset):
     assert np.array_equal(a.download(np.uint32, x.size, offset), b.download(np.uint32, x.size, offset))
 
 
+@pytest.mark.parametrize("dim,heads,tokens,offset", [(128, 33, 2100, 0), (72, 37, 3200, 0), (128, 33, 2100, 4)])
+def test_many_rows(dim, heads, tokens, offset):
+    """A call over more than 2^23 values gives the bits of its rows in pieces."""
+    assert tokens * heads * dim > 1 << 23
+    rng, t, kern = np.random.default_rng(dim), RopeTable(1e4, dim, 200), Kernels()
+    x = rng.standard_normal(tokens * heads * dim).astype(np.float32)
+    pos = rng.integers(-2, 202, (3, tokens)).astype(np.int32)
+    a, b, axes = DeviceBuffer(x.nbytes + 16), DeviceBuffer(x.nbytes + 16), RopeAxes.of_pairs(rng.integers(0, 3, dim // 2), 3)
+    for buf in (a, b):
+        buf.upload(x, offset)
+    kern.rope_axes((a, offset), t, axes, ints(pos), tokens, heads, dim)
+    for i in range(0, tokens, 700):
+        n = min(700, tokens - i)
+        kern.rope_axes((b, offset + 4 * i * heads * dim), t, axes, ints(pos[:, i:i + n]), n, heads, dim)
+    synchronize()
+    assert np.array_equal(a.download(np.uint32, x.size, offset), b.download(np.uint32, x.size, offset))
+
+
 def test_gradient_of_a_rotation():
     """A rotation is linear: the differences of its values are the rotation of the differences, and the rotation
     by the opposite angles (its transpose) undoes it."""
