@@ -91,9 +91,8 @@ rope_axes_kernel(RopeArgs a) {
 //
 // A workgroup takes the new rows of one (block, KV head) of K or V, a row per wave and instruction, all
 // of them in registers (lane l holds values l and l + 64, a rotary pair and rms_norm's order of sums, so
-// the bits are those of rms_norm, rope_axes and store_kv_paged in sequence); the workgroups behind
-// them take rows of q. Bound: HBM for prompts (5548 rows of 32 + 8 + 8 heads in 48.3 us: 242 MB, 5.0 TB/s; with one
-// row of q a wave in place of eight 77.9), the chain lengths -> page -> scale -> codes for a step (64 rows 9.3 us).
+// q's bits are those of rms_norm and rope_axes in sequence); the workgroups behind them take rows of q. Bound: HBM for prompts (5548 rows of 32 + 8 + 8 heads in 50.1 us: 242 MB, 4.8 TB/s; with one row of q a wave
+// in place of eight about 80), the chain lengths -> page -> scale -> codes for a step (64 rows 9.5 us).
 constexpr int kWriteWaves = 4;
 constexpr int kWriteThreads = 64 * kWriteWaves;
 constexpr int kTileRows = kPage / kWriteWaves;  // rows of a block that a wave takes
@@ -149,6 +148,33 @@ __device__ __forceinline__ void norm_turn(float& x0, float& x1, float w0, float 
     const float a0 = (x0 * scale) * w0, b0 = (x1 * scale) * w1;
     x0 = a0 * c - b0 * s;
     x1 = b0 * c + a0 * s;
+}
+
+// A row of k, in 64 bits and rounded once. Its values become codes, and in 32 bits a few of a prompt's (one of 6M, at
+// times) came out on the other side of a border between two codes, half a step of the code away. (32 bits: 48.3 us.)
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double p) {
+    p += dpp64<0x140>(p);
+    p += dpp64<0x141>(p);
+    p += dpp64<0x1B>(p);
+    p += dpp64<0xB1>(p);
+    p += __shfl_xor(p, 16);
+    p += __shfl_xor(p, 32);
+    return p;
+}
+__device__ __forceinline__ void norm_turn64(float& x0, float& x1, float w0, float w1, float c, float s, float eps) {
+    const double m = wave_sum64((double)x0 * x0 + (double)x1 * x1) / kDim + eps;
+    double r = __builtin_amdgcn_rsq(m);
+    if (r > 0.0 && r < INFINITY) r = fma(r, 0.5 * fma(-m * r, r, 1.0), r);  // (a Newton step: the instruction has 2^-26)
+    const double a0 = x0 * r * w0, b0 = x1 * r * w1;
+    x0 = (float)(a0 * c - b0 * s);
+    x1 = (float)(b0 * c + a0 * s);
 }
 
 constexpr int kRows = 8;  // of q for each wave, of one token, whose loads travel together
@@ -230,7 +256,7 @@ norm_rope_paged_kernel(WriteArgs a) {
             for (int j = 0; j < kAhead; ++j) {
                 const int s = kWriteWaves * (j0 + j) + wave;
                 if (s < s0 || s >= s1) continue;
-                norm_turn(x0[j0 + j], x1[j0 + j], w0, w1, c[j], sn[j], a.eps);
+                norm_turn64(x0[j0 + j], x1[j0 + j], w0, w1, c[j], sn[j], a.eps);
                 dst[row_at(s)] = x0[j0 + j];
                 dst[row_at(s) + 64] = x1[j0 + j];
             }

@@ -487,10 +487,11 @@ int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t laye
                                  size_t hq, void* stream);
 
 /*
- * brasa_rms_norm of the heads of q and k, brasa_rope_axes and brasa_store_kv_paged in one launch, with their bits: q
- * [tokens, hq, 128] and k [tokens, hkv, 128] (f32, in place) are normalised with q_norm / k_norm [128] and eps
- * and turned by rope_pos [axes, tokens]; k (turned) and v (as given) go into the pages as in
- * brasa_store_kv_paged. Rows of q from cu[0] to cu[n], and rows of k whose position has a page; the others
+ * brasa_rms_norm of the heads of q and k, brasa_rope_axes and brasa_store_kv_paged in one launch: q [tokens, hq,
+ * 128] and k [tokens, hkv, 128] (f32, in place) are normalised with q_norm / k_norm [128] and eps and turned by
+ * rope_pos [axes, tokens], q with the bits of those two calls, k in 64 bits and rounded once, so that its codes are
+ * those of the exact value; k (turned) and v (as given) go into the pages as in brasa_store_kv_paged, with its
+ * bits. Rows of q from cu[0] to cu[n], and rows of k whose position has a page; the others
  * are left as they are. (A rotary position outside the table, a negative one too, gives NaN here.) Requires
  * table.dim == 128; rows of q, k and v 16-byte aligned and apart.
  */

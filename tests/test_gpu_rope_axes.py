@@ -1,8 +1,10 @@
 """GPU: rotary positions with several axes, and the paged cache's writer fused with the norms and the rotation.
 
 Tolerance of a rotation: two products and their sum, each rounded to f32 (half a step, 2^-24 of each term's
-size): 2^-22 (|a| + |b|). With one axis the bits are rope_neox's, and the fused call's are those of rms_norm,
-rope_axes and store_kv_paged in sequence.
+size): 2^-22 (|a| + |b|). With one axis the bits are rope_neox's. The fused call's q has the bits of rms_norm and
+rope_axes in sequence; its k is computed in 64 bits (at most 2^-40 of a term with the root's, far more than its 20
+roundings of 2^-53 and a Newton step from 2^-26) and rounded once, half a step of 2^-24; and its pages have the
+bits of store_kv_paged on that k.
 """
 import numpy as np
 import pytest
@@ -118,16 +120,18 @@ def _writer(seed, new, old, hq, hkv, axes=3, layers=1, layer=0, spoil=None, stre
     if spoil:
         spoil(table, pos, cu, rope_pos, x)
     w = [rng.uniform(0.5, 1.5, DIM).astype(np.float32) for _ in range(2)]
-    t, of = RopeTable(1e6, DIM, 300), RopeAxes.of_pairs(rng.integers(0, axes, 64), axes)
+    axis = rng.integers(0, axes, 64)
+    t, of = RopeTable(1e6, DIM, 300), RopeAxes.of_pairs(axis, axes)
     gcu, gpos, gt, gr = ints(cu), ints(pos), ints(table), ints(rope_pos)
     gw = [_f32(a) for a in w]
     one, two = upload_pool(pool), upload_pool(pool)
     a, b = [_f32(v) for v in x], [_f32(v) for v in x]
     kern.qk_norm_rope_store_paged(one, layer, a, gw, 1e-6, t, of, gr, gcu, gpos, gt, n, width, tokens, hq)
-    for buf, weight, heads in ((b[0], gw[0], hq), (b[1], gw[1], hkv)):
-        kern.rms_norm(buf, weight, buf, tokens * heads, DIM, 1e-6)
-        kern.rope_axes(buf, t, of, gr, tokens, heads, DIM)
-    kern.store_kv_paged(two, layer, b[1], b[2], gcu, gpos, gt, n, width, tokens)
+    kern.rms_norm(b[0], gw[0], b[0], tokens * hq, DIM, 1e-6)
+    kern.rope_axes(b[0], t, of, gr, tokens, hq, DIM)
+    if stream:
+        stream.synchronize()
+    kern.store_kv_paged(two, layer, a[1], b[2], gcu, gpos, gt, n, width, tokens)
     if stream:
         stream.synchronize()
     synchronize()
@@ -140,10 +144,18 @@ def _writer(seed, new, old, hq, hkv, axes=3, layers=1, layer=0, spoil=None, stre
         for j in range(cu[i + 1] - cu[i]):
             p = int(pos[i]) + j
             stored[cu[i] + j] = pos[i] >= 0 and p < width * PAGE and 0 <= table[i, p // PAGE] < pages
-    for got, seq, given, on in ((a[0], b[0], x[0], inside), (a[1], b[1], x[1], stored)):
-        got, seq = got.download(np.float32).reshape(given.shape), seq.download(np.float32).reshape(given.shape)
-        same = (bits(got) == bits(seq)) | (np.isnan(got) & np.isnan(seq))
-        assert same[on].all() and np.array_equal(bits(got[~on]), bits(given[~on]))
+    q, seq = (buf.download(np.float32).reshape(x[0].shape) for buf in (a[0], b[0]))
+    same = (bits(q) == bits(seq)) | (np.isnan(q) & np.isnan(seq))
+    assert same[inside].all() and np.array_equal(bits(q[~inside]), bits(x[0][~inside]))
+    got, given = a[1].download(np.float32).reshape(x[1].shape), x[1].astype(np.float64)
+    assert np.array_equal(bits(got[~stored]), bits(x[1][~stored]))
+    with np.errstate(invalid="ignore"):
+        norm = given / np.sqrt((given ** 2).mean(-1, keepdims=True) + np.float64(np.float32(1e-6))) * w[1]
+        want = step_ref.rope(norm, *rope_table(1e6, DIM, 300), axis, rope_pos)
+        size = np.abs(norm[..., :64]) + np.abs(norm[..., 64:])
+        tol = 2.0 ** -24 * np.abs(want) + 2.0 ** -40 * np.concatenate([size, size], -1) + 2.0 ** -150
+        close = (np.abs(got - want) <= tol) | (np.isnan(got) & np.isnan(want))
+    assert close[stored].all()
     return got
 
 
