@@ -5,8 +5,8 @@
 // position p = pos[a(i)][t]: y_i = x_i c - x_{i + dim / 2} s, y_{i + dim / 2} = x_{i + dim / 2} c + x_i s,
 // with c and s the table's entries (p, i). One axis is rope_neox, bit for bit.
 //
-// Bound: HBM, 8 bytes a value in and out. 16000 rows of 32 heads of 128 take 85 us (524 MB, 6.2 TB/s, in place),
-// 1027 rows of 16 heads of 72 4.9 (the chain positions -> angles -> rows).
+// Bound: HBM, 8 bytes a value in and out. 16000 rows of 32 heads of 128 take 100 us (524 MB, 5.2 TB/s; 85 just
+// behind another pass over them), 1027 rows of 16 heads of 72 4.9 (the chain positions -> angles -> rows).
 #include "paged.hpp"
 
 namespace brasa {
@@ -91,8 +91,9 @@ rope_axes_kernel(RopeArgs a) {
 //
 // A workgroup takes the new rows of one (block, KV head) of K or V, a row per wave and instruction, all
 // of them in registers (lane l holds values l and l + 64, a rotary pair and rms_norm's order of sums, so
-// q's bits are those of rms_norm and rope_axes in sequence); the workgroups behind them take rows of q. Bound: HBM for prompts (5548 rows of 32 + 8 + 8 heads in 50.1 us: 242 MB, 4.8 TB/s; with one row of q a wave
-// in place of eight about 80), the chain lengths -> page -> scale -> codes for a step (64 rows 9.5 us).
+// q's bits are those of rms_norm and rope_axes in sequence); the workgroups behind them take rows of q.
+// Bound: HBM for prompts (5548 rows of 32 + 8 + 8 heads: 242 MB in 51.9 us, 4.7 TB/s; with one row of q a wave in
+// place of eight half as long again), the chain lengths -> page -> scale -> codes for a step (64 rows 8.6 us).
 constexpr int kWriteWaves = 4;
 constexpr int kWriteThreads = 64 * kWriteWaves;
 constexpr int kTileRows = kPage / kWriteWaves;  // rows of a block that a wave takes
@@ -124,6 +125,11 @@ __device__ __forceinline__ float wave_sum(float p) {
     return __int_as_float(b[0]) + __int_as_float(b[1]);
 }
 
+// Rows pass the caches by: 5548 of them in HBM 51.9 us in place of 59.6. (What reads q next finds less of it there: a copy
+// of it right behind takes 6 us longer, so 2 are left.)
+__device__ __forceinline__ float read_once(const float* p) { return __builtin_nontemporal_load(p); }
+__device__ __forceinline__ void write_once(float* p, float x) { __builtin_nontemporal_store(x, p); }
+
 // This lane's angle for row t (NaN where a position is outside the table).
 __device__ __forceinline__ void angle_of(const WriteArgs& a, int t, int lane, int axis, float& c, float& s) {
     bool there = true;
@@ -151,7 +157,7 @@ __device__ __forceinline__ void norm_turn(float& x0, float& x1, float w0, float 
 }
 
 // A row of k, in 64 bits and rounded once. Its values become codes, and in 32 bits a few of a prompt's (one of 6M, at
-// times) came out on the other side of a border between two codes, half a step of the code away. (32 bits: 48.3 us.)
+// times) came out on the other side of a border between two codes, half a step of the code away. (It takes 1.8 us of 50.)
 template <int CTRL>
 __device__ __forceinline__ double dpp64(double x) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
@@ -196,8 +202,8 @@ norm_rope_paged_kernel(WriteArgs a) {
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             const int r = min(j, rows - 1);
-            x0[j] = q[r * kDim];
-            x1[j] = q[r * kDim + 64];
+            x0[j] = read_once(q + r * kDim);
+            x1[j] = read_once(q + r * kDim + 64);
         }
         angle_of(a, t, lane, axis, c, s);
         const float w0 = a.qn[lane], w1 = a.qn[lane + 64];
@@ -205,8 +211,8 @@ norm_rope_paged_kernel(WriteArgs a) {
         for (int j = 0; j < kRows; ++j) {
             if (j >= rows) break;
             norm_turn(x0[j], x1[j], w0, w1, c, s, a.eps);
-            q[j * kDim] = x0[j];
-            q[j * kDim + 64] = x1[j];
+            write_once(q + j * kDim, x0[j]);
+            write_once(q + j * kDim + 64, x1[j]);
         }
         return;
     }
@@ -236,8 +242,8 @@ norm_rope_paged_kernel(WriteArgs a) {
         const int s = kWriteWaves * j + wave;
         x0[j] = x1[j] = 0.0f;
         if (s >= s0 && s < s1) {
-            x0[j] = src[row_at(s)];
-            x1[j] = src[row_at(s) + 64];
+            x0[j] = read_once(src + row_at(s));
+            x1[j] = read_once(src + row_at(s) + 64);
         }
     }
     if (!is_v) {
@@ -257,8 +263,8 @@ norm_rope_paged_kernel(WriteArgs a) {
                 const int s = kWriteWaves * (j0 + j) + wave;
                 if (s < s0 || s >= s1) continue;
                 norm_turn64(x0[j0 + j], x1[j0 + j], w0, w1, c[j], sn[j], a.eps);
-                dst[row_at(s)] = x0[j0 + j];
-                dst[row_at(s) + 64] = x1[j0 + j];
+                write_once(dst + row_at(s), x0[j0 + j]);
+                write_once(dst + row_at(s) + 64, x1[j0 + j]);
             }
         }
     }
