@@ -208,15 +208,6 @@ __device__ __forceinline__ int block_max(int x, int before, int* s, int& all) {
     }
     return x;
 }
-__device__ __forceinline__ Tile read_lane(const Tile& t, int lane) {
-    union {
-        Tile t;
-        uint32_t w[sizeof(Tile) / 4];
-    } u = {t};
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(Tile) / 4); ++i) u.w[i] = __builtin_amdgcn_readlane(u.w[i], lane);
-    return u.t;
-}
 // x / d for 0 <= x < 2^52, d > 0, with inv = 1.0 / d
 __device__ __forceinline__ long long div_by(long long x, long long d, double inv) {
     long long q = (long long)((double)x * inv);
@@ -247,10 +238,9 @@ attend_plan_kernel(const int* cu, const int* pos, const int* group, const int* p
     };
     __shared__ long long s_scan[W];
     __shared__ int s_scan32[W];
-    __shared__ int s_merges;
-    __shared__ int s_parts[THREADS], s_cols[THREADS], s_base[THREADS];  // of the tiles, where there is one a thread
+    __shared__ Tile s_tile[THREADS];  // one a thread
+    __shared__ int s_unit[THREADS];   // first unit of each tile's columns to join
     const int tid = threadIdx.x;
-    if (tid == 0) s_merges = 0;
     const int per_row = a.per_row;
     // (the first of each list at once: what follows then waits for one trip to memory, not for three)
     struct In {
@@ -423,19 +413,20 @@ attend_plan_kernel(const int* cu, const int* pos, const int* group, const int* p
         t = make_tile(i);
         mine += kOver + t.b1 - t.b0;
     }
-    block_scan64<W>(mine, s_scan, total);
+    const long long before = block_scan64<W>(mine, s_scan, total);
     const long long size = max((total + a.runs - 1) / a.runs, least_run(total));
     const double inv = 1.0 / (double)size;
 
-    // ---- the tiles --------------------------------------------------------------------------------
+    // ---- the tiles, and the tile where each run starts ----------------------------------------------
+    const bool one_round = ntiles <= THREADS;
     long long line = 0, cols = 0;
     for (int t0 = 0; t0 < ntiles; t0 += THREADS) {
-        const int at = t0 + tid;
+        const int at = t0 + tid, many = min(ntiles - t0, THREADS);
         const bool on = at < ntiles;
-        if (on && ntiles > THREADS) t = make_tile(at);  // (else it is at hand)
-        const long long len = on ? t.b1 - t.b0 : 0;
-        long long sum;
-        t.start = line + block_scan64<W>(on ? len + kOver : 0, s_scan, sum) + kOver;
+        if (on && !one_round) t = make_tile(at);  // (else it is at hand)
+        const long long len = on ? t.b1 - t.b0 : 0, line0 = line;
+        long long sum = total;
+        t.start = (one_round ? before : line + block_scan64<W>(on ? len + kOver : 0, s_scan, sum)) + kOver;
         line += sum;
         t.run0 = (int)div_by(t.start, size, inv);
         const int last = on ? (int)div_by(t.start + len - 1, size, inv) : 0;
@@ -444,58 +435,79 @@ attend_plan_kernel(const int* cu, const int* pos, const int* group, const int* p
         const long long part_cols = on && !(t.kind & kDirect) ? (long long)t.cols * t.parts : 0;
         t.base = (int)(cols + block_scan64<W>(part_cols, s_scan, sum));
         cols += sum;
-        if (on) {
-            a.tile[at] = t;
-            s_parts[tid] = t.parts;
-            s_cols[tid] = t.cols;
-            s_base[tid] = t.base;
+        if (on) s_tile[tid] = t;
+        __syncthreads();
+        // (through the LDS: written by their threads, 64 lines an instruction, and a tile of many runs by one thread, both
+        // took 13 of 29 thousand cycles for drafts)
+        for (int k = tid; k < 4 * many; k += THREADS)
+            reinterpret_cast<u32x4*>(a.tile + t0)[k] = reinterpret_cast<const u32x4*>(s_tile)[k];
+        const int w1 = (int)div_by(line + size - 1, size, inv);
+        for (int w = (int)div_by(line0 + size - 1, size, inv) + tid; w < w1; w += THREADS) {
+            int lo = 0, hi = many - 1;  // the first tile that ends behind the run's start
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (s_tile[mid].start + (s_tile[mid].b1 - s_tile[mid].b0) > w * size) hi = mid;
+                else lo = mid + 1;
+            }
+            a.start[w] = s_tile[lo];
         }
-        // the runs that start in it, or in the pages' worth before it; a wave together where they are many
-        int w = on ? (int)div_by(t.start - kOver + size - 1, size, inv) : 1;
-        for (uint64_t many = __builtin_amdgcn_ballot_w64(last - w >= 4); many; many &= many - 1) {
-            const int from = __builtin_ctzll(many), w1 = __builtin_amdgcn_readlane(last, from);
-            const Tile u = read_lane(t, from);
-            for (int k = __builtin_amdgcn_readlane(w, from) + (tid & 63); k <= w1; k += 64) a.start[k] = u;
-        }
-        if (last - w < 4)
-            for (; w <= last; ++w) a.start[w] = t;
     }
-    if (ntiles > THREADS) stores_barrier();
-    else __syncthreads();
+    if (!one_round) stores_barrier();
 
     // ---- the columns to join ----------------------------------------------------------------------
-    for (int at = tid; at < ntiles; at += THREADS) {
-        if (ntiles > THREADS) t = a.tile[at];
-        if (t.kind & (kPrefix | kDirect)) continue;
-        const int border = t.ptile >= 0 ? min(kCols - t.pcol, t.cols) : t.cols;  // (the rest in the next prefix tile)
-        for (int c0 = 0; c0 < t.cols; c0 = border) {
-            const int c1 = c0 < border ? border : t.cols;
-            Join j = {};
-            j.parts = t.parts;
-            j.cols = t.cols;
-            j.base = t.base + c0;
-            if (t.ptile >= 0) {
-                const int pt = t.ptile + (c0 > 0);
-                j.pparts = ntiles > THREADS ? brasa::ld_l2(&a.tile[pt].parts) : s_parts[pt];
-                j.pcols = ntiles > THREADS ? brasa::ld_l2(&a.tile[pt].cols) : s_cols[pt];
-                j.pbase = (ntiles > THREADS ? brasa::ld_l2(&a.tile[pt].base) : s_base[pt]) + (c0 > 0 ? 0 : t.pcol);
-            }
-            j.row0 = t.row0;
-            j.col0 = t.col0 + c0;
-            j.lanes = join_lanes(j.parts + j.pparts);
-            const int each = kThreads / j.lanes;
-            int to = atomicAdd(&s_merges, (c1 - c0 + each - 1) / each);
-            for (int c = c0; c < c1; c += each) {
-                j.many = min(c1 - c, each);
-                a.merge[to++] = j;
-                j.base += each;
-                j.pbase += each;
-                j.col0 += each;
-            }
-            if (c1 == t.cols) break;
+    // A tile's columns in its first prefix tile, or all (side 0), and those in the next one.
+    auto join_of = [&](const Tile& x, int side) {
+        const int border = x.ptile >= 0 ? min(kCols - x.pcol, x.cols) : x.cols, c0 = side ? border : 0;
+        Join j = {};
+        j.base = x.base + c0;
+        j.parts = x.parts;
+        j.cols = x.cols;
+        j.row0 = x.row0;
+        j.col0 = x.col0 + c0;
+        j.many = side ? x.cols - border : border;
+        if (x.ptile >= 0 && j.many > 0) {
+            const int pt = x.ptile + side;
+            j.pparts = one_round ? s_tile[pt].parts : brasa::ld_l2(&a.tile[pt].parts);
+            j.pcols = one_round ? s_tile[pt].cols : brasa::ld_l2(&a.tile[pt].cols);
+            j.pbase = (one_round ? s_tile[pt].base : brasa::ld_l2(&a.tile[pt].base)) + (side ? 0 : x.pcol);
         }
+        j.lanes = join_lanes(j.parts + j.pparts);
+        return j;
+    };
+    auto units_of = [](const Join& j) { return (j.many * j.lanes + kThreads - 1) / kThreads; };
+    int merges = 0;
+    for (int t0 = 0; t0 < ntiles; t0 += THREADS) {
+        const int many = min(ntiles - t0, THREADS);
+        int units = 0, sum;
+        if (tid < many) {
+            if (!one_round) t = a.tile[t0 + tid];
+            if (!(t.kind & (kPrefix | kDirect))) units = units_of(join_of(t, 0)) + units_of(join_of(t, 1));
+        }
+        s_unit[tid] = block_scan<W>(units, s_scan32, sum);
+        __syncthreads();
+        for (int u = tid; u < sum; u += THREADS) {
+            int lo = 0, hi = many;  // the last tile that starts at or before u: one with units
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (s_unit[mid] <= u) lo = mid;
+                else hi = mid;
+            }
+            const Tile x = one_round ? s_tile[lo] : a.tile[t0 + lo];
+            Join j = join_of(x, 0);
+            int r = u - s_unit[lo];
+            if (r >= units_of(j)) {
+                r -= units_of(j);
+                j = join_of(x, 1);
+            }
+            const int each = kThreads / j.lanes;
+            j.base += r * each;
+            j.pbase += r * each;
+            j.col0 += r * each;
+            j.many = min(j.many - r * each, each);
+            a.merge[merges + u] = j;
+        }
+        merges += sum;
     }
-    __syncthreads();
     if (tid == 0) {
         a.head->magic = kMagic;
         a.head->n = a.n;
@@ -505,7 +517,7 @@ attend_plan_kernel(const int* cu, const int* pos, const int* group, const int* p
         a.head->hkv = a.hkv;
         a.head->runs = a.runs;
         a.head->tiles = ntiles;
-        a.head->merges = s_merges;
+        a.head->merges = merges;
         a.head->size = size;
         a.head->total = line;
         a.head->at.tiles = a.at.tiles;
