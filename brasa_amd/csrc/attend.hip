@@ -16,10 +16,10 @@
 // in order, so the result does not depend on timing.
 //
 // Bound, 32 query heads over 8: for prompts and chunks the matrix cores at the clock that they and the vector units
-// leave (4988 rows over up to 13K positions, 333 GFLOP: 460 to 500 us, 0.69 PFLOP/s at about 1.5 GHz, where a large
-// product reaches 1.2). For a step's single rows latency: four rows over 16K shared positions (33 MB) take 15.7 us, of
+// leave (4988 rows over up to 13K positions, 333 GFLOP: 460 to 510 us, 0.69 PFLOP/s at about 1.5 GHz, where a large
+// product reaches 1.2). For a step's single rows latency: four rows over 16K shared positions (33 MB) take 15.3 us, of
 // which the eight half pages of a wave are half and the loads header -> page ids and Q -> codes -> sums, each a
-// trip of 0.6 to 1.5 us, the rest; 64 sequences behind 8192 shared positions (71 MB) 31.5 us.
+// trip of 0.6 to 1.5 us, the rest; 64 sequences behind 8192 shared positions (71 MB) 31 us.
 #include <climits>
 #include <type_traits>
 
@@ -216,9 +216,9 @@ __device__ __forceinline__ long long div_by(long long x, long long d, double inv
     return q;
 }
 // IN_LDS: the lists of sequences and groups fit the LDS (up to kPlanLds of each); else they stand in the
-// workspace, and every look at one costs a trip to the L2 (64 sequences in one group 19.6 us in place of 14.4).
-// Up to kPlanFew sequences and tiles take as many threads, whose scans wait for four waves only (the same 64 in 11.3
-// us; one sequence 5.3 in place of 8.7, 24 sequences' drafts 13.8 in place of 17.2).
+// workspace, and every look at one costs a trip to the L2 (64 sequences in one group 15.9 us in place of 11.8).
+// Up to kPlanFew sequences and tiles take as many threads, whose scans wait for four waves only (the same 64 in 8.7
+// us; one sequence 5.2 in place of 8.2, 24 sequences' drafts 9.2 in place of 11.9).
 constexpr int kPlanLds = 1024, kPlanFew = 256;
 template <bool IN_LDS, int THREADS>
 __global__ void __launch_bounds__(THREADS)
