@@ -40,7 +40,8 @@ __device__ __forceinline__ uintptr_t again(T p) {
     asm volatile("" : "+s"(x));
     return x;
 }
-// ---- workgroup scans of 1024 threads ------------------------------------------------------------
+
+// ---- workgroup scans, of 1024 threads unless W says otherwise ------------------------------------------------------------
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / 64;
 
