@@ -123,8 +123,8 @@ Layout layout(int n, int groups, int tokens, int hq, int hkv) {
     const long long shared = groups ? std::min(cols, seqs * (kCols - 1)) : 0;
     l.runs = std::max(kRuns / hkv, kWaves);
     l.max_tiles = (int)(seqs + cols / kCols + (groups ? std::min((long long)groups, seqs) + shared / kCols : 0));
-    // all shared columns, and those of the tiles that a run's border cuts
-    l.max_merges = (int)(shared + (long long)l.runs * std::min((long long)kCols, cols));
+    // all shared columns, and those of the tiles that a run's border cuts; each column once
+    l.max_merges = (int)std::min(shared + (long long)l.runs * std::min((long long)kCols, cols), cols);
     // shared columns once in each of the two tiles, and for each border a tile's columns once or twice
     l.cap = 2 * shared + 2LL * l.runs * std::min((long long)kCols, cols);
     size_t at = up256(sizeof(Header));

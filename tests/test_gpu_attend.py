@@ -255,6 +255,18 @@ def test_bad_sequences():
     assert np.isnan(got[s.cu[2]:s.cu[3]]).all()
 
 
+@pytest.mark.parametrize("out", list(OutDType))
+def test_table_without_columns(out):
+    """No position has a page: NaN in every row of a sequence, as many as there are."""
+    s = Step(new=[1, 40, 0, 3], held=[5, 0, 7, 200], groups=[(4, 64)], hq=8, hkv=2, seed=17, out=out)
+    s.width = 0
+    s.upload()
+    s.plan()
+    s.call()
+    synchronize()
+    s.check(nan=(0, 1, 3))
+
+
 def test_bounds_out_of_order():
     """cu and group are raised to the largest before them: no row of o outside is touched."""
     s = Step(new=[4, 3, 5, 2], held=[70, 80, 64, 90], groups=[(2, 64), (2, 64)], hq=4, hkv=1, seed=11)
