@@ -37,13 +37,20 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 32;     // columns of a tile
 constexpr int kRuns = 2048;   // waves of a launch: two per SIMD
-// Pages whose time a tile costs beside its own: with 4 a batch of 64 sequences takes 33.2 us, four drafts each
-// 26.9, prompts' rows over 16K to 64K positions 458; with 2 34.2, 27.6 and 461, with 6 33.3, 27.4 and 475.
-constexpr int kOver = 4;
-// Least length of a run, of a line of `total` pages, as a part costs its joining: one short sequence takes 10.1 us
-// with runs of 2 and 13.0 with 4, four rows over 16K positions 17.0 + 5.9 us with 2 and 15.8 + 4.8 with 4.
-constexpr int kShortLine = 64;
-__device__ __forceinline__ long long least_run(long long total) { return total <= kShortLine ? 2 : 4; }
+// Pages whose time a tile costs beside its own: with 6 eight sequences of 4 to 5K positions take 23.0 us a layer, 32
+// behind 4096 shared ones 23.5, a batch of 64 behind 8192 35.8; with 4 24.1, 24.6 and 35.8, with 8 22.0, 24.6 and 36.2,
+// with 2 the batch 39.
+constexpr int kOver = 6;
+// Length of a run in a line of `total` pages cut into at most `runs`: one wave per SIMD while that leaves it up to
+// kLongRun pages, and else two waves. A wave more costs its way to the first product, 4 us,
+// and its parts their joining; between one wave and two for each SIMD most wait for few. (Two waves throughout: four
+// rows over 16K positions 18.9 us a layer in place of 18.0, a batch of 64 38.0 in place of 35.7, drafts 40.1 in
+// place of 37.6; one throughout: prompts 251 in place of 243, chunks 522 in place of 482.)
+constexpr int kLongRun = 48;
+__device__ __forceinline__ long long run_pages(long long total, int runs) {
+    const long long half = (total + runs / 2 - 1) / (runs / 2);
+    return half <= kLongRun ? half : (total + runs - 1) / runs;
+}
 
 struct Tile {
     int seq;          // table row whose pages it reads
@@ -414,7 +421,7 @@ attend_plan_kernel(const int* cu, const int* pos, const int* group, const int* p
         mine += kOver + t.b1 - t.b0;
     }
     const long long before = block_scan64<W>(mine, s_scan, total);
-    const long long size = max((total + a.runs - 1) / a.runs, least_run(total));
+    const long long size = run_pages(total, a.runs);
     const double inv = 1.0 / (double)size;
 
     // ---- the tiles, and the tile where each run starts ----------------------------------------------
