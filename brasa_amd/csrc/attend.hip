@@ -17,9 +17,9 @@
 //
 // Bound, 32 query heads over 8: for prompts and chunks the matrix cores at the clock that they and the vector units
 // leave (4988 rows over up to 13K positions, 333 GFLOP: 460 to 510 us, 0.69 PFLOP/s at about 1.5 GHz, where a large
-// product reaches 1.2). For a step's single rows latency: four rows over 16K shared positions (33 MB) take 15.3 us, of
-// which the eight half pages of a wave are half and the loads header -> page ids and Q -> codes -> sums, each a
-// trip of 0.6 to 1.5 us, the rest; 64 sequences behind 8192 shared positions (71 MB) 31 us.
+// product reaches 1.2). For a step's single rows latency: four rows over 16K shared positions (33 MB) take 14.2 us, of
+// which the six half pages of a wave are half and the loads header -> page ids and Q -> codes -> sums, each a
+// trip of 0.6 to 1.5 us, the rest; 64 sequences behind 8192 shared positions (71 MB) 29 to 32 us.
 #include <climits>
 #include <type_traits>
 
@@ -77,14 +77,14 @@ struct Join {
     int base, parts, cols;     // own parts: columns base + part * cols + column
     int pbase, pparts, pcols;  // the prefix tile's
     int row0, col0, many;      // columns from col0 on of the sequence whose first packed row is row0
-    int lanes;                 // of a column: 32, 64 or all
+    int lanes;                 // of a column: 32 or all
     int unused0, unused1;
 };
 static_assert(sizeof(Join) % 16 == 0, "read in wide pieces");
-// Half a wave has eight parts on their way at once and takes two turns before more of them pay: the joining takes 4.1
-// us for four rows over 16K positions (64 parts a column), 6.9 for a batch of 64 (20), 20.1 for prompts (3); with half
-// waves only 12.0, 7.3 and 19.2, waves only 8.0, 6.9 and 39.3, workgroups only 4.1, 7.6 and 90.5.
-__host__ __device__ constexpr int join_lanes(int parts) { return parts <= 8 ? 32 : parts <= 32 ? 64 : kThreads; }
+// Half a wave has eight parts on their way at once, and up to 32 of a column in four turns; more take the workgroup. The
+// joining takes 4.0 us for four rows over 16K positions (about 80 parts a column), 5.0 for a batch of 64 (8 to 30), 18.6 for
+// prompts (2 or 3); with half waves throughout 11.2, 5.0 and 19.4, with workgroups 4.0, 6.8 and 84.
+__host__ __device__ constexpr int join_lanes(int parts) { return parts <= 32 ? 32 : kThreads; }
 
 // Where the plan and the partials stand in the workspace.
 struct Places {
@@ -1197,9 +1197,8 @@ attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
 
 // ---- parts into rows ----------------------------------------------------------------------------
 //
-// Half a wave per column, a wave or a workgroup, by the number of its parts: each half wave joins every second,
-// or every eighth, 16 bytes of their sums a lane and eight parts on their way at once, and then the halves
-// theirs. Bound: the chain header -> unit -> parts -> o, and for prompts the parts' bytes.
+// Half a wave per column, or a workgroup where it has many parts: each half wave joins them all, or every
+// eighth, 16 bytes of their sums a lane and eight parts on their way at once, and then the halves theirs. Bound: the chain header -> unit -> parts -> o, and for prompts the parts' bytes.
 __global__ void __launch_bounds__(kThreads)
 attend_merge_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
     __shared__ __attribute__((aligned(16))) float s_x[kWaves][kDim];
@@ -1226,7 +1225,7 @@ attend_merge_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
         if (e != e0) j = load_line(units + e);
         // this half wave's column, and its first part
         const int half = 2 * wave + h, step = j.lanes / 32;
-        const int c = j.lanes == 32 ? half : j.lanes == 64 ? wave : 0, first = half & (step - 1);
+        const int c = j.lanes == 32 ? half : 0, first = half & (step - 1);
         const int parts = c < j.many ? j.pparts + j.parts : 0;
         float m = -INFINITY, l = 0.0f;
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1257,14 +1256,12 @@ attend_merge_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
                 for (int r = 0; r < 4; ++r) x[r] = fmaf(y[k][r], f, x[r]);
             }
         }
-        if (j.lanes > 32) {
+        if (j.lanes > 32) {  // the halves, and the waves
             const float top = max_h(m), f = part_weight(m, top);
             l = sum_h(l * f);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = sum_h(x[r] * f);
             m = top;
-        }
-        if (j.lanes > 64) {
             if (h == 0) *reinterpret_cast<f32x4*>(&s_x[wave][d]) = x;
             if (lane == 0) s_ml[wave] = f32x2{m, l};
             __syncthreads();
