@@ -42,10 +42,10 @@ constexpr int kRuns = 2048;   // waves of a launch: two per SIMD
 // with 2 the batch 39.
 constexpr int kOver = 6;
 // Length of a run in a line of `total` pages cut into at most `runs`: one wave per SIMD while that leaves it up to
-// kLongRun pages, and else two waves. A wave more costs its way to the first product, 4 us,
-// and its parts their joining; between one wave and two for each SIMD most wait for few. (Two waves throughout: four
-// rows over 16K positions 18.9 us a layer in place of 18.0, a batch of 64 38.0 in place of 35.7, drafts 40.1 in
-// place of 37.6; one throughout: prompts 251 in place of 243, chunks 522 in place of 482.)
+// kLongRun pages, and else two waves. A wave more costs its way to the first product, 4 us, and its parts their
+// joining; with more waves than SIMDs but fewer than two each, most wait for few. (Two waves throughout, in runs of four
+// pages at least: four rows over 16K positions 18.9 us a layer in place of 18.0, a batch of 64 38.0 in place of
+// 35.7, drafts 40.1 in place of 37.6; one throughout: prompts 251 in place of 243, chunks 522 in place of 482.)
 constexpr int kLongRun = 48;
 __device__ __forceinline__ long long run_pages(long long total, int runs) {
     const long long half = (total + runs / 2 - 1) / (runs / 2);
@@ -58,7 +58,7 @@ struct Tile {
     int col0, cols;   // its columns among the sequence's, or the group's
     int b0, b1;       // pages
     int pos0;         // own tile: position of the sequence's first new row
-    int kind;         // kPrefix, kDirect, kBad
+    int kind;         // TileKind
     long long start;  // of its pages in the line
     int base, parts;  // partials: columns base + part * cols + column; parts of it
     int run0;         // run of its first part
@@ -1198,7 +1198,8 @@ attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
 // ---- parts into rows ----------------------------------------------------------------------------
 //
 // Half a wave per column, or a workgroup where it has many parts: each half wave joins them all, or every
-// eighth, 16 bytes of their sums a lane and eight parts on their way at once, and then the halves theirs. Bound: the chain header -> unit -> parts -> o, and for prompts the parts' bytes.
+// eighth, 16 bytes of their sums a lane and eight parts on their way at once, and then the halves theirs.
+// Bound: the chain header -> unit -> parts -> o, and for prompts the parts' bytes.
 __global__ void __launch_bounds__(kThreads)
 attend_merge_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
     __shared__ __attribute__((aligned(16))) float s_x[kWaves][kDim];
