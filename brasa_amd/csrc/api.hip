@@ -71,7 +71,7 @@ size_t attend_workspace_len(int n, int groups, int tokens, int hq, int hkv);
 int attend_plan_launch(const int* cu, const int* pos, const int* group, const int* prefix, int groups, int n,
                        int width, int tokens, int hq, int hkv, void* ws, hipStream_t stream);
 int attend_launch(const float* q, const PoolArgs& pool, const int* table, int width, int n, int tokens,
-                  void* ws, size_t ws_len, void* o, int o_f16, int hq, hipStream_t stream);
+                  void* ws, size_t ws_len, void* o, int o_f16, int exact, int hq, hipStream_t stream);
 
 namespace {
 thread_local char g_err[512] = "";
@@ -630,7 +630,8 @@ int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, cons
                           size_t hq, void* stream) {
     g_err[0] = 0;
     const char* what = "attention_paged";
-    if (o_dtype != BRASA_OUT_F32 && o_dtype != BRASA_OUT_F16)
+    const bool o_f16 = o_dtype == BRASA_OUT_F16 || o_dtype == BRASA_OUT_F16_SHORT;
+    if (o_dtype != BRASA_OUT_F32 && !o_f16)
         return set_error(BRASA_ERR_ARG, "%s: invalid output dtype %d", what, o_dtype);
     PoolArgs p;
     int st = pool_check(what, pool, layer, &p);
@@ -644,11 +645,11 @@ int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, cons
     if ((uintptr_t)workspace % 256 || ((uintptr_t)q | (uintptr_t)o) % 16)
         return set_error(BRASA_ERR_ARG, "%s: q and o must be 16-byte, the workspace 256-byte aligned", what);
     const size_t values = tokens * hq * kDim;
-    const Range rq{q, 4 * values}, ro{o, (o_dtype == BRASA_OUT_F16 ? 2 : 4) * values}, rw{workspace, need};
+    const Range rq{q, 4 * values}, ro{o, (o_f16 ? 2 : 4) * values}, rw{workspace, need};
     if (overlap(rq, ro) || overlap(rq, rw) || overlap(ro, rw))
         return set_error(BRASA_ERR_ARG, "%s: q, o and the workspace overlap", what);
-    return attend_launch(q, p, table, (int)width, (int)n, (int)tokens, workspace, workspace_len, o,
-                         o_dtype == BRASA_OUT_F16, (int)hq, as_stream(stream));
+    return attend_launch(q, p, table, (int)width, (int)n, (int)tokens, workspace, workspace_len, o, o_f16,
+                         o_dtype != BRASA_OUT_F16_SHORT, (int)hq, as_stream(stream));
 }
 
 int brasa_rope_table(double theta, size_t dim, size_t max_pos, float* cos_out, float* sin_out) {

@@ -726,8 +726,8 @@ __device__ __forceinline__ void add_pv(const i32x2 (&v)[2][4], const half8v (&hi
 }
 
 // Q of a wave's columns as the B operands of S^T = K Q^T: f16 values, and what they leave over, as f16 values
-// too (EXACT: 22 bits together) or as e4m3 codes of 2^11 times it (15 bits, at half the matrix cores' time,
-// and K's codes are the other operand as they are).
+// too (EXACT: 22 bits together, as the paged decode takes them) or, where the caller asks for fewer bits, as e4m3 codes of 2^11
+// times it (15 bits, at half the matrix cores' time, and K's codes are the other operand as they are).
 template <bool EXACT>
 struct QueryOps {
     half8v hi[8];
@@ -815,7 +815,7 @@ __device__ __forceinline__ void hide_values(uint8_t* v, int* first, int last1, i
     }
 }
 
-template <bool EXACT>
+template <bool EXACT, bool F16>
 __global__ void __launch_bounds__(kThreads, 2)
 attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
     constexpr int kHalf = 32 * kDim;  // codes of half a page
@@ -1174,7 +1174,7 @@ attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
                 if (2 * i >= cols) break;
                 const int r0 = __builtin_amdgcn_readlane(o_row, 2 * i), r1 = __builtin_amdgcn_readlane(o_row, 2 * i + 1);
                 const f32x4 x = column(i);
-                if (2 * i + h < cols) write_o<!EXACT>(o, (size_t)(h ? r1 : r0) * kDim + 4 * c, x, 1.0f);
+                if (2 * i + h < cols) write_o<F16>(o, (size_t)(h ? r1 : r0) * kDim + 4 * c, x, 1.0f);
             }
         } else {
             const auto hd = header();
@@ -1328,7 +1328,7 @@ int attend_plan_launch(const int* cu, const int* pos, const int* group, const in
 }
 
 int attend_launch(const float* q, const PoolArgs& pool, const int* table, int width, int n, int tokens,
-                  void* ws, size_t ws_len, void* o, int o_f16, int hq, hipStream_t stream) {
+                  void* ws, size_t ws_len, void* o, int o_f16, int exact, int hq, hipStream_t stream) {
     const Layout l = layout(n, n, tokens, hq, pool.hkv);  // (the most entries: the plan's may have fewer groups)
     AttendArgs a = {};
     a.ws = static_cast<uint8_t*>(ws);
@@ -1343,7 +1343,7 @@ int attend_launch(const float* q, const PoolArgs& pool, const int* table, int wi
     a.hq = hq;
     a.per_row = hq / pool.hkv;
     a.o_f16 = o_f16;
-    auto kernel = o_f16 ? attend_kernel<false> : attend_kernel<true>;
+    auto kernel = !o_f16 ? attend_kernel<true, false> : exact ? attend_kernel<true, true> : attend_kernel<false, true>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((l.runs + kWaves - 1) / kWaves * pool.hkv)), dim3(kThreads), 0, stream,
                        a.ws, pool.hkv, l.runs, a);
     const int st = check_launch("attend_kernel");

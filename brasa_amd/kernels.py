@@ -68,6 +68,9 @@ class OutDType(enum.IntEnum):
     F16 = 1
 
 
+OUT_F16_SHORT = 2  # ``attention_paged`` with ``short``
+
+
 @dataclass(frozen=True)
 class AttnShape:
     """lib.rs:1354-1364."""
@@ -359,10 +362,15 @@ class Kernels:
                                                _stream(stream or self.stream)))
 
     def attention_paged(self, q, pool, layer: int, table, n: int, width: int, tokens: int, workspace,
-                        workspace_len: int, o, hq: int, out: OutDType = OutDType.F32, stream=None) -> None:
-        """Attention of a step's new rows over the paged cache, on the plan in ``workspace``."""
+                        workspace_len: int, o, hq: int, out: OutDType = OutDType.F32, stream=None,
+                        short: bool = False) -> None:
+        """Attention of a step's new rows over the paged cache, on the plan in ``workspace``. ``short``: f16 results
+        from 15 bits of q and f16 weights, in less time."""
+        if short and out != OutDType.F16:
+            raise BrasaError(5, "attention_paged: short is for f16 results")
         check(lib().brasa_attention_paged(_ptr(q), pool.c(), layer, _ptr(table), width, n, tokens, _ptr(workspace),
-                                          workspace_len, _ptr(o), int(out), hq, _stream(stream or self.stream)))
+                                          workspace_len, _ptr(o), OUT_F16_SHORT if short else int(out), hq,
+                                          _stream(stream or self.stream)))
 
     def kv_pages_fork(self, parent, table, lens, ref, table_out, lens_out, ref_out, n: int,
                       width: int, pages: int, stream=None) -> None:

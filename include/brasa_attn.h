@@ -68,6 +68,8 @@ extern "C" {
  * f16 (RNE) is offered for callers whose next GEMM reads f16. */
 #define BRASA_OUT_F32 0
 #define BRASA_OUT_F16 1
+/* brasa_attention_paged alone: f16 from shorter operands. */
+#define BRASA_OUT_F16_SHORT 2
 
 /* AttnShape (crates/kernels/src/lib.rs:1354-1364). */
 typedef struct brasa_attn_shape {
@@ -528,9 +530,10 @@ int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_
  * Attention of new rows over the paged cache, theirs included (store them first): row t of sequence i (cu[i] <= t <
  * cu[i + 1], at position pos[i] + t - cu[i]) over positions 0 .. its own in `layer`. One row for each sequence (a decode
  * step), a few (drafts under verification) or many (a prompt, or a chunk of one behind what is cached) take the
- * same call. q: [tokens, hq, 128] f32, o: [tokens, hq, 128] in o_dtype. Sums and softmax are f32. For
- * BRASA_OUT_F32, q and the weights are contracted as two f16 halves (22 bits); for BRASA_OUT_F16 with 15 bits of q and f16
- * weights, whose rounding is of the size of the result's own. Any hq a multiple of hkv.
+ * same call. q: [tokens, hq, 128] f32, o: [tokens, hq, 128] in o_dtype. Sums and softmax are f32, q and the weights are
+ * contracted as two f16 halves (22 bits). With BRASA_OUT_F16_SHORT for o_dtype (f16 results) q keeps 15 bits and the weights
+ * are f16 values, whose rounding is of the size of the result's own: prompts take about two thirds of the time. Any hq a
+ * multiple of hkv.
  *
  * The plan of a step is laid out on the device by brasa_attention_paged_plan, once for all layers:
  * sequences group[g] .. group[g + 1] (as in brasa_kv_pages_shared) are taken to name the same pages in their first
