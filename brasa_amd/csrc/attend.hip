@@ -987,7 +987,7 @@ attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-        int vref = 0;     // acc stands in units of 2^(vref - 127)
+        int vref = 0;     // this lane's column of acc stands in units of 2^(vref - 127)
 
         u32x4 kw[4];    // key c, dims 32 i + 16 h .. + 16
         i32x2 vw[2][4]; // keys 16 st + 8 (j / 4) + 4 h + j % 4 of dim 32 t + c at [st][t]
@@ -1046,28 +1046,31 @@ attend_kernel(uint8_t* ws, int hkv, int runs, AttendArgs a) {
                 float top = fmaxf(fmaxf(s[12], s[13]), fmaxf(s[14], s[15]));
 #pragma unroll
                 for (int i = 0; i < 12; i += 3) top = fmaxf(top, fmaxf(fmaxf(s[i], s[i + 1]), s[i + 2]));
-                // a reference point that moves only when the maximum has grown by 2^8: p stays below
-                // 2^15 with the bias of 2^7 that keeps small p out of f16's subnormals
-                if (__builtin_amdgcn_ballot_w64(top * sc > m_used + 8.0f)) {
+                // Two reference points of each column, both powers of two: m_used for l, which moves when the largest
+                // score has grown by 2^8 past it, and m_used + vref for acc, which moves when a weight times its page's
+                // V scale has. So a key's f16 weight, p = 2^(score - m_used + 7 - less), keeps its bits wherever
+                // its part of the sum is not far below the largest part, whatever scales the other pages have; p stays
+                // below 2^15, and its bias of 2^7 keeps small p out of f16's subnormals.
+                int less = vref - vx;
+                if (__builtin_amdgcn_ballot_w64(top * sc > m_used + (float)(8 + min(less, 0)))) {
                     top = max_h(top) * sc;
                     const bool grow = top > m_used + 8.0f;
-                    const float alpha = grow ? __builtin_amdgcn_exp2f(m_used - top) : 1.0f;
-                    if (grow) m_used = top;
-                    lsum *= alpha;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[i] *= alpha;
-                }
-                // V's scale: acc's unit grows with it, and where it is smaller p shrinks, through its
-                // exponent (by 2^100 at most: p is 0 in f16 from 2^40 on)
-                if (vx > vref) {
-                    const float f = ldexpf(1.0f, vref - vx);
+                    const float m = grow ? floorf(top) : m_used;
+                    const int by = grow ? (int)fminf(m - m_used, 1000.0f) : 0;  // (from -inf: both sums are 0)
+                    const int before = vref - by;
+                    const float over = top - m;
+                    vref = over + (float)(vx - 8) > (float)before ? vx + (int)floorf(over) : before;
+                    m_used = m;
+                    lsum *= ldexpf(1.0f, -by);
+                    const float f = ldexpf(1.0f, before - vref);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[i] *= f;
-                    vref = vx;
+                    less = vref - vx;
                 }
-                const int less = min(vref - vx, 100);
+                // (from 2^40 on every p is 0 in f16; the limit is for l's sake)
+                less = min(less, 64);
                 // (a column that has seen no key yet: its scores are all -inf, and p 0)
-                const float mb = m_used == -INFINITY ? 0.0f : 7.0f - (float)less - m_used;
+                const float mb = m_used == -INFINITY ? 0.0f : (float)(7 - less) - m_used;
                 in_order();
                 f32x16 next;
                 float p[16], psum = 0.0f;

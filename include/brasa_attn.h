@@ -531,7 +531,8 @@ int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_
  * cu[i + 1], at position pos[i] + t - cu[i]) over positions 0 .. its own in `layer`. One row for each sequence (a decode
  * step), a few (drafts under verification) or many (a prompt, or a chunk of one behind what is cached) take the
  * same call. q: [tokens, hq, 128] f32, o: [tokens, hq, 128] in o_dtype. Sums and softmax are f32, q and the weights are
- * contracted as two f16 halves (22 bits). With BRASA_OUT_F16_SHORT for o_dtype (f16 results) q keeps 15 bits and the weights
+ * contracted as two f16 halves (22 bits; a weight's error is at least 2^-32 of the row's largest weight times its page's V scale, so
+ * a page's values keep their bits beside pages of a larger scale whose weights are small). With BRASA_OUT_F16_SHORT for o_dtype (f16 results) q keeps 15 bits and the weights
  * are f16 values, whose rounding is of the size of the result's own: prompts take about two thirds of the time. Any hq a
  * multiple of hkv.
  *
