@@ -645,7 +645,9 @@ int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, cons
     if ((uintptr_t)workspace % 256 || ((uintptr_t)q | (uintptr_t)o) % 16)
         return set_error(BRASA_ERR_ARG, "%s: q and o must be 16-byte, the workspace 256-byte aligned", what);
     const size_t values = tokens * hq * kDim;
-    const Range rq{q, 4 * values}, ro{o, (o_f16 ? 2 : 4) * values}, rw{workspace, need};
+    // (what a plan of these sizes with any number of groups takes of the workspace)
+    const size_t most = attend_workspace_len((int)n, (int)kMaxSeqs, (int)tokens, (int)hq, p.hkv);
+    const Range rq{q, 4 * values}, ro{o, (o_f16 ? 2 : 4) * values}, rw{workspace, std::min(workspace_len, most)};
     if (overlap(rq, ro) || overlap(rq, rw) || overlap(ro, rw))
         return set_error(BRASA_ERR_ARG, "%s: q, o and the workspace overlap", what);
     return attend_launch(q, p, table, (int)width, (int)n, (int)tokens, workspace, workspace_len, o, o_f16,
