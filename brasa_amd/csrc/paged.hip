@@ -34,7 +34,7 @@ store_paged_kernel(StoreArgs a) {
     const int kh = blockIdx.x % a.p.hkv;
     const bool is_v = blockIdx.y;
     TouchedBlock t;
-    if (!touched_block(a.rows, a.item0 + blockIdx.x / a.p.hkv, a.p.pages, t)) return;
+    if (!touched_block<false>(a.rows, a.item0 + blockIdx.x / a.p.hkv, a.p.pages, t)) return;
     // slots [s0, s1) of the block are new, [0, s0) hold earlier rows
     const int s0 = t.s0, s1 = t.s1;
     const size_t tile = (size_t)t.page * a.p.hkv + kh;

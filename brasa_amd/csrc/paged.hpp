@@ -87,28 +87,46 @@ struct NewRows {
     int n, width, tokens;
 };
 
-// the blocks that sequence i's new rows touch: [pos / kPage, + count)
-__device__ __forceinline__ int touched_blocks(const NewRows& a, int i, int& c0, int& c1, int& pos) {
-    c0 = min(max(a.cu[i], 0), a.tokens);
-    c1 = min(max(a.cu[i + 1], c0), a.tokens);
-    pos = a.pos[i];
+// how many blocks a sequence's rows [c0, c1) touch from position pos on: [pos / kPage, + count)
+__device__ __forceinline__ int touched_blocks(const NewRows& a, int c0, int c1, int pos) {
     // (a negative position, or one past what the table can hold, has no block)
     if (c1 == c0 || pos < 0 || pos >= a.width * kPage) return 0;
     return min((pos + (c1 - c0) - 1) / kPage, a.width - 1) - pos / kPage + 1;
 }
+// inclusive maximum over the lanes of a wave
+__device__ __forceinline__ int wave_max(int x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x = max(x, y);
+    }
+    return x;
+}
 
 // The item-th block of all that new rows touch: its page, its slots [s0, s1) that are new, and the
 // packed row of its slot 0. Every wave walks the sequences' block counts, 64 at a time. False: there
-// is no such block, or it has no page.
+// is no such block, or it has no page. APART: bounds out of order are raised to the largest before them, so
+// that no row is in two blocks, for rows that are rewritten in place; else each sequence's are clamped alone.
 struct TouchedBlock {
     int page, s0, s1, row0;
 };
+template <bool APART>
 __device__ __forceinline__ bool touched_block(const NewRows& a, int item, int pages, TouchedBlock& t) {
     const int lane = threadIdx.x & 63;
-    int seq = -1, before = 0, c0 = 0, c1 = 0, pos = 0;
+    int seq = -1, before = 0, top = 0, c0 = 0, c1 = 0, pos = 0;
     for (int i0 = 0; i0 < a.n; i0 += 64) {
         int nb = 0;
-        if (i0 + lane < a.n) nb = touched_blocks(a, i0 + lane, c0, c1, pos);
+        const int i = i0 + lane;
+        if (i < a.n) {
+            c0 = min(max(a.cu[i], 0), a.tokens);
+            c1 = min(max(a.cu[i + 1], 0), a.tokens);
+            pos = a.pos[i];
+        }
+        if (APART && __builtin_amdgcn_ballot_w64(i < a.n && (c0 < top || c1 < c0))) c0 = max(wave_max(c0), top);
+        c1 = max(c1, c0);
+        if (APART) top = __builtin_amdgcn_readlane(c1, 63);  // (where another round follows, all lanes have a sequence)
+        if (i < a.n) nb = touched_blocks(a, c0, c1, pos);
         const int incl = wave_scan(nb) + before;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(incl > item);
         if (past) {

@@ -220,7 +220,7 @@ norm_rope_paged_kernel(WriteArgs a) {
     const int kh = blockIdx.x / 2 % a.p.hkv;
     const bool is_v = blockIdx.x & 1;
     TouchedBlock t;
-    if (!touched_block(a.rows, (int)(a.item0 + blockIdx.x / 2 / a.p.hkv), a.p.pages, t)) return;
+    if (!touched_block<true>(a.rows, (int)(a.item0 + blockIdx.x / 2 / a.p.hkv), a.p.pages, t)) return;
     const int s0 = t.s0, s1 = t.s1;
     const size_t tile = (size_t)t.page * a.p.hkv + kh;
     uint8_t* codes = (is_v ? a.p.v : a.p.k) + tile * kTileBytes8;

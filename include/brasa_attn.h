@@ -494,7 +494,7 @@ int brasa_decode_attention_paged(const float* q, brasa_kv_pool pool, size_t laye
  * rope_pos [axes, tokens], q with the bits of those two calls, k in 64 bits and rounded once, so that its codes are
  * those of the exact value; k (turned) and v (as given) go into the pages as in brasa_store_kv_paged, with its
  * bits. Rows of q from cu[0] to cu[n], and rows of k whose position has a page; the others
- * are left as they are. (A rotary position outside the table, a negative one too, gives NaN here.) Requires
+ * are left as they are. For k and v, values of cu out of order are raised to the largest before them. (A rotary position outside the table, a negative one too, gives NaN here.) Requires
  * table.dim == 128; rows of q, k and v 16-byte aligned and apart.
  */
 int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, float* k, const float* v,
