@@ -621,6 +621,10 @@ int brasa_attention_paged_plan(const int32_t* cu, const int32_t* pos, const int3
     if (!workspace || (n && (!cu || !pos)) || (groups && (!group || !prefix)))
         return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
     if ((uintptr_t)workspace % 256) return set_error(BRASA_ERR_ARG, "%s: the workspace must be 256-byte aligned", what);
+    const Range rw{workspace, need};
+    for (const Range& r : {Range{n ? cu : nullptr, 4 * (n + 1)}, Range{pos, 4 * n}, Range{groups ? group : nullptr, 4 * (groups + 1)},
+                           Range{prefix, 4 * groups}})
+        if (overlap(rw, r)) return set_error(BRASA_ERR_ARG, "%s: an input overlaps the workspace", what);
     return attend_plan_launch(cu, pos, group, prefix, (int)groups, (int)n, (int)width, (int)tokens, (int)hq, (int)hkv,
                               workspace, as_stream(stream));
 }

@@ -23,3 +23,13 @@ def test_attention_inside_a_grouped_workspace(groups):
         for q, o in ((base + at, P), (P, base + at)):
             _refused(lambda: Kernels().attention_paged(q, KvPool.view(P, P, P, P, 1, 8, hkv), 0, P, n, 4, tokens, base, size, o, hq,
                                                        OutDType.F32))
+
+
+@pytest.mark.parametrize("name,size", [("cu", 4 * 65), ("pos", 4 * 64), ("group", 16), ("prefix", 12)])
+def test_plan_inputs_inside_the_workspace(name, size):
+    n, groups, tokens, hq, hkv, base = 64, 3, 64, 32, 8, 1 << 40
+    need = attention_paged_workspace_len(n, groups, tokens, hq, hkv)
+    for at in (base, base + 4096, base + need - 4, base - size + 4):
+        a = {**dict(cu=P, pos=P, group=P, prefix=P), name: at}
+        _refused(lambda: Kernels().attention_paged_plan(**a, groups=groups, n=n, width=4, tokens=tokens, hq=hq, hkv=hkv,
+                                                        workspace=base, workspace_len=need))
