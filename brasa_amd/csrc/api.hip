@@ -520,6 +520,9 @@ int brasa_rope_axes(float* x, brasa_rope_table_view table, brasa_rope_axes_map a
     if (!x || !pos || (table.max_pos && (!table.cos || !table.sin)))
         return set_error(BRASA_ERR_ARG, "%s: null pointer", what);
     if ((uintptr_t)x % 4) return set_error(BRASA_ERR_ARG, "%s: x must be 4-byte aligned", what);
+    const Range rx{x, tokens * heads * dim * 4}, angles{table.cos, table.max_pos * dim * 2}, sines{table.sin, angles.bytes};
+    if (overlap(rx, {pos, 4 * axes.axes * tokens}) || overlap(rx, angles) || overlap(rx, sines))
+        return set_error(BRASA_ERR_ARG, "%s: x overlaps an input", what);
     return rope_axes_launch(x, table.cos, table.sin, (int)table.max_pos, axes, pos, (int)tokens, (int)heads, (int)dim,
                             as_stream(stream));
 }
@@ -549,6 +552,11 @@ int brasa_qk_norm_rope_store_paged(brasa_kv_pool pool, size_t layer, float* q, f
     const Range rq{q, tokens * hq * 4 * kDim}, rk{k, tokens * pool.hkv * 4 * kDim}, rv{v, tokens * pool.hkv * 4 * kDim};
     if (overlap(rq, rk) || overlap(rq, rv) || overlap(rk, rv))
         return set_error(BRASA_ERR_ARG, "%s: q, k and v overlap", what);
+    const Range inputs[] = {{q_norm, 4 * kDim}, {k_norm, 4 * kDim}, {table.cos, table.max_pos * 2 * kDim},
+                            {table.sin, table.max_pos * 2 * kDim}, {rope_pos, 4 * axes.axes * tokens}, {cu, 4 * (n + 1)},
+                            {pos, 4 * n}, {pages, 4 * n * width}};
+    for (const Range& r : inputs)
+        if (overlap(rq, r) || overlap(rk, r)) return set_error(BRASA_ERR_ARG, "%s: q or k overlaps an input", what);
     return norm_rope_paged_launch(p, q, k, v, q_norm, k_norm, eps, table.cos, table.sin, (int)table.max_pos, axes,
                                   rope_pos, cu, pos, pages, (int)n, (int)width, (int)tokens, (int)hq,
                                   as_stream(stream));
@@ -654,6 +662,8 @@ int brasa_attention_paged(const float* q, brasa_kv_pool pool, size_t layer, cons
     const Range rq{q, 4 * values}, ro{o, (o_f16 ? 2 : 4) * values}, rw{workspace, std::min(workspace_len, most)};
     if (overlap(rq, ro) || overlap(rq, rw) || overlap(ro, rw))
         return set_error(BRASA_ERR_ARG, "%s: q, o and the workspace overlap", what);
+    const Range rt{table, 4 * n * width};
+    if (overlap(rt, ro) || overlap(rt, rw)) return set_error(BRASA_ERR_ARG, "%s: the table overlaps o or the workspace", what);
     return attend_launch(q, p, table, (int)width, (int)n, (int)tokens, workspace, workspace_len, o, o_f16,
                          o_dtype != BRASA_OUT_F16_SHORT, (int)hq, as_stream(stream));
 }

@@ -551,7 +551,7 @@ int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_
  *
  * workspace: brasa_attention_paged_workspace_len bytes, 256-byte aligned, any contents: the plan, then the partial
  * sums of one call at a time. Calls that may run at the same time need workspaces (and plans) of their own. q and o
- * 16-byte aligned; q, the plan's inputs, o and the workspace apart; tokens * hq up to 2^29.
+ * 16-byte aligned; q, the plan's inputs, the table, o and the workspace apart; tokens * hq up to 2^29.
  */
 size_t brasa_attention_paged_workspace_len(size_t n, size_t groups, size_t tokens, size_t hq, size_t hkv);
 int brasa_attention_paged_plan(const int32_t* cu, const int32_t* pos, const int32_t* group,

@@ -1,7 +1,7 @@
 """CPU: arrays of a step's calls that overlap what the call writes are refused before the device is touched."""
 import pytest
 
-from brasa_amd import BrasaError, Kernels, KvPool, OutDType, attention_paged_workspace_len
+from brasa_amd import BrasaError, Kernels, KvPool, OutDType, RopeAxes, RopeTable, attention_paged_workspace_len
 
 P = 4096  # an address that passes the checks of null and alignment; never followed here
 ARG = 5
@@ -33,3 +33,30 @@ def test_plan_inputs_inside_the_workspace(name, size):
         a = {**dict(cu=P, pos=P, group=P, prefix=P), name: at}
         _refused(lambda: Kernels().attention_paged_plan(**a, groups=groups, n=n, width=4, tokens=tokens, hq=hq, hkv=hkv,
                                                         workspace=base, workspace_len=need))
+
+
+@pytest.mark.parametrize("out,size", [(OutDType.F32, 4), (OutDType.F16, 2)])
+def test_attention_over_its_table(out, size):
+    n, width, tokens, hq, base, ws = 3, 5, 7, 32, 1 << 40, 1 << 36
+    need = attention_paged_workspace_len(n, 0, tokens, hq, 8)
+    for table in (base, base - 4 * n * width + 4, base + size * tokens * hq * 128 - 4, ws + 4096, ws + need - 4):
+        _refused(lambda: Kernels().attention_paged(P, KvPool.view(P, P, P, P, 1, 8, 8), 0, table, n, width, tokens, ws, need, base, hq, out))
+
+
+@pytest.mark.parametrize("name,size", [("rope_pos", 4 * 2 * 9), ("cu", 4 * 4), ("pos", 4 * 3), ("pages", 4 * 3 * 5), ("qn", 512), ("kn", 512),
+                                       ("cos", 4 * 64 * 10), ("sin", 4 * 64 * 10)])
+def test_writer_over_its_inputs(name, size):
+    n, width, tokens, hq, hkv, q, k = 3, 5, 9, 32, 8, 1 << 40, 1 << 41
+    for at in (q, q - size + 4, q + 4 * tokens * hq * 128 - 4, k, k - size + 4, k + 4 * tokens * hkv * 128 - 4):
+        a = {**dict(rope_pos=P, cu=P, pos=P, pages=P, qn=P, kn=P, cos=P, sin=P), name: at}
+        _refused(lambda: Kernels().qk_norm_rope_store_paged(
+            KvPool.view(P, P, P, P, 1, 8, hkv), 0, (q, k, 1 << 42), (a["qn"], a["kn"]), 1e-6, RopeTable.view(a["cos"], a["sin"], 128, 10),
+            RopeAxes([60, 4]), a["rope_pos"], a["cu"], a["pos"], a["pages"], n, width, tokens, hq))
+
+
+@pytest.mark.parametrize("name,size", [("pos", 4 * 2 * 9), ("cos", 4 * 36 * 10), ("sin", 4 * 36 * 10)])
+def test_rotation_over_its_inputs(name, size):
+    tokens, heads, dim, x = 9, 3, 72, 1 << 40
+    for at in (x, x - size + 4, x + 4 * tokens * heads * dim - 4):
+        a = {**dict(pos=P, cos=P, sin=P), name: at}
+        _refused(lambda: Kernels().rope_axes(x, RopeTable.view(a["cos"], a["sin"], dim, 10), RopeAxes([30, 6]), a["pos"], tokens, heads, dim))
