@@ -132,6 +132,8 @@ def rope_table(theta: float, dim: int, max_pos: int):
 class RopeTable:
     """``RopeTable::new`` (lib.rs:1376-1386): the f64-computed table uploaded to the device."""
 
+    owned = True  # the arrays are the table's own
+
     def __init__(self, theta: float, dim: int, max_pos: int):
         cos, sin = rope_table(theta, dim, max_pos)
         self.cos = DeviceBuffer(max(cos.nbytes, 4))
@@ -144,15 +146,17 @@ class RopeTable:
     def view(cls, cos, sin, dim: int, max_pos: int) -> "RopeTable":
         """A table over the caller's device arrays [max_pos, dim / 2] f32."""
         t = cls.__new__(cls)
-        t.cos, t.sin, t.dim, t.max_pos = cos, sin, dim, max_pos
+        t.cos, t.sin, t.dim, t.max_pos, t.owned = cos, sin, dim, max_pos, False
         return t
 
     def c(self) -> RopeTableC:
         return RopeTableC(_ptr(self.cos), _ptr(self.sin), self.dim, self.max_pos)
 
     def free(self) -> None:
-        self.cos.free()
-        self.sin.free()
+        """Frees the table's own arrays (a view's are its caller's)."""
+        if self.owned:
+            self.cos.free()
+            self.sin.free()
 
 
 class RopeAxes:
