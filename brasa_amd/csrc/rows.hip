@@ -13,8 +13,8 @@
 namespace brasa {
 namespace {
 
-// a + b up to a cap, for a, b in [0, 2^30]: associative, so scans may group the terms at will
-__device__ __forceinline__ int add_cap(int a, int b, int cap) { return min(a + b, cap); }
+// a + b up to a cap, for a, b in [0, 2^30], whose sum may be 2^31: associative, so scans may group the terms at will
+__device__ __forceinline__ int add_cap(int a, int b, int cap) { return (int)min((unsigned)a + (unsigned)b, (unsigned)cap); }
 
 struct RowsArgs {
     const int* add;
