@@ -15,11 +15,11 @@
 // whose sequence has a prefix tile, leaves (m, l, acc) in the workspace and a second launch joins them
 // in order, so the result does not depend on timing.
 //
-// Bound, 32 query heads over 8: for prompts and chunks the matrix cores at the clock that they and the vector units
-// leave (4988 rows over up to 13K positions, 333 GFLOP: 460 to 510 us, 0.69 PFLOP/s at about 1.5 GHz, where a large
-// product reaches 1.2). For a step's single rows latency: four rows over 16K shared positions (33 MB) take 14.2 us, of
+// Bound, 32 query heads over 8: for prompts and chunks the matrix cores and the vector instructions beside them
+// (4988 rows over up to 13K positions, 333 GFLOP, each product twice: 670 us, 0.50 PFLOP/s, where a large product reaches 1.2;
+// the short form 493, 0.68). For a step's single rows latency: four rows over 16K shared positions (33 MB) take 14.4 us, of
 // which the six half pages of a wave are half and the loads header -> page ids and Q -> codes -> sums, each a
-// trip of 0.6 to 1.5 us, the rest; 64 sequences behind 8192 shared positions (71 MB) 29 to 32 us.
+// trip of 0.6 to 1.5 us, the rest; 64 sequences behind 8192 shared positions (71 MB) 41 to 43 us, 32 to 34 in the short form.
 #include <climits>
 #include <type_traits>
 
@@ -37,15 +37,15 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 32;     // columns of a tile
 constexpr int kRuns = 2048;   // waves of a launch: two per SIMD
-// Pages whose time a tile costs beside its own: with 6 eight sequences of 4 to 5K positions take 23.0 us a layer, 32
-// behind 4096 shared ones 23.5, a batch of 64 behind 8192 35.8; with 4 24.1, 24.6 and 35.8, with 8 22.0, 24.6 and 36.2,
-// with 2 the batch 39.
+// Pages whose time a tile costs beside its own. 32 heads over 8, us a layer with its share of the plan: with 6 eight
+// sequences of 4 to 5K positions take 22.8, 32 behind 4096 shared ones 23.3, a batch of 64 behind 8192 46.0, drafts 40.6; with
+// 4 23.8, 23.8, 45.8 and 40.4, with 8 23.7, 24.9, 46.7 and 41.7, with 2 24.4, 23.1, 45.3 and 42.9.
 constexpr int kOver = 6;
 // Length of a run in a line of `total` pages cut into at most `runs`: one wave per SIMD while that leaves it up to
 // kLongRun pages, and else two waves. A wave more costs its way to the first product, 4 us, and its parts their
-// joining; with more waves than SIMDs but fewer than two each, most wait for few. (Two waves throughout, in runs of four
-// pages at least: four rows over 16K positions 18.9 us a layer in place of 18.0, a batch of 64 38.0 in place of
-// 35.7, drafts 40.1 in place of 37.6; one throughout: prompts 251 in place of 243, chunks 522 in place of 482.)
+// joining; with more waves than SIMDs but fewer than two each, most wait for few. (32 heads over 8. Two waves throughout: four
+// rows over 16K positions 20.8 us a layer in place of 18.2, a batch of 64 48.9 in place of 46.0, drafts 43.0 in place of
+// 40.6; one throughout: prompts 354 in place of 335, chunks 717 in place of 673.)
 constexpr int kLongRun = 48;
 __device__ __forceinline__ long long run_pages(long long total, int runs) {
     const long long half = (total + runs / 2 - 1) / (runs / 2);
@@ -67,9 +67,10 @@ struct Tile {
 };
 static_assert(sizeof(Tile) == 64, "a tile is one line");
 // kInRow: a prefix tile whose group's sharing rows are all packed behind each other (a load less before Q's).
-// kOnce: no other tile reads its pages, which then pass the caches by (four rows over 16K positions 18.9 us a
-// layer in place of 19.9, a batch of 64 40.4 in place of 41.4; for all tiles the batch takes 48, chunks 650 in place
-// of 490).
+// kOnce: the tile holds all columns of its sequence or group, and its pages pass the caches by (four rows over 16K positions
+// 18.2 us a layer in place of 19.5, eight sequences of 4 to 5K 22.8 in place of 25.0, a batch of 64 46.0 in place of 47.1; for
+// all tiles prompts take 371 in place of 335, chunks 821 in place of 673). (Another sequence may name the same pages, where it
+// is in no group, has positions below the group's prefix or just a tile's columns: its tile reads them from HBM too.)
 enum TileKind { kPrefix = 1, kDirect = 2, kBad = 4, kInRow = 8, kOnce = 16 };
 
 // Columns whose parts a workgroup of the merge joins: `many` of one tile, which continue in one prefix tile or in none.
@@ -82,8 +83,9 @@ struct Join {
 };
 static_assert(sizeof(Join) % 16 == 0, "read in wide pieces");
 // Half a wave has eight parts on their way at once, and up to 32 of a column in four turns; more take the workgroup. The
-// joining takes 4.0 us for four rows over 16K positions (about 80 parts a column), 5.0 for a batch of 64 (8 to 30), 18.6 for
-// prompts (2 or 3); with half waves throughout 11.2, 5.0 and 19.4, with workgroups 4.0, 6.8 and 84.
+// joining takes 4.0 us for four rows over 16K positions (about 80 parts a column), 5.1 for a batch of 64 (8 to 30), 19 to 22 for
+// prompts (2 or 3). With half waves throughout the four rows' pass of 36 layers takes 904 us in place of 657, with workgroups the
+// prompts' 401 in place of 335.
 __host__ __device__ constexpr int join_lanes(int parts) { return parts <= 32 ? 32 : kThreads; }
 
 // Where the plan and the partials stand in the workspace.

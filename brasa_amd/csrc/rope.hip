@@ -6,7 +6,7 @@
 // with c and s the table's entries (p, i). One axis is rope_neox, bit for bit.
 //
 // Bound: HBM, 8 bytes a value in and out. 16000 rows of 32 heads of 128 take 100 us (524 MB, 5.2 TB/s; 85 just
-// behind another pass over them), 1027 rows of 16 heads of 72 4.9 (the chain positions -> angles -> rows).
+// behind another pass over them), 1027 rows of 16 heads of 72 4.4 to 4.9 (the chain positions -> angles -> rows).
 #include "paged.hpp"
 
 namespace brasa {
@@ -345,8 +345,9 @@ int rope_axes_launch(float* x, const float* cos_t, const float* sin_t, int max_p
     a.heads = heads;
     a.half = dim / 2;
     a.max_pos = max_pos;
-    // Four pairs a thread, 16 bytes an access, for large calls: 67M values in 83 us, a pair a thread 93. Small ones
-    // want the threads: 1.2M values 4.7 us a pair a thread and 5.3 four, 8.4M 11.2 and 11.7.
+    // Four pairs a thread, 16 bytes an access, for large calls: 67M values that HBM holds in 100 us, a pair a thread 110; 16.8M
+    // 30.6 and 31.3, 10.2M 21.3 and 22.4. Small ones want the threads: 8.4M 19.1 and 18.4, 4.1M 10.7 and 9.8. (Two
+    // times the same rows, which the caches then hold: 67M 87 and 110, 16.8M 26.0 and 26.8, 8.4M 12.2 and 14.5, 4.1M 7.8 and 7.6.)
     if (a.half % 4 == 0 && (uintptr_t)x % 16 == 0 && (long long)tokens * heads * dim > (1LL << 23))
         return launch_rope<4>(a, stream);
     return launch_rope<1>(a, stream);

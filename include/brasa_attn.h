@@ -530,18 +530,22 @@ int brasa_kv_pages_shared(const int32_t* table, const int32_t* len, const int32_
  * Attention of new rows over the paged cache, theirs included (store them first): row t of sequence i (cu[i] <= t <
  * cu[i + 1], at position pos[i] + t - cu[i]) over positions 0 .. its own in `layer`. One row for each sequence (a decode
  * step), a few (drafts under verification) or many (a prompt, or a chunk of one behind what is cached) take the
- * same call. q: [tokens, hq, 128] f32, o: [tokens, hq, 128] in o_dtype. Sums and softmax are f32, q and the weights are
- * contracted as two f16 halves (22 bits; a weight's error is at least 2^-32 of the row's largest weight times its page's V scale, so
- * a page's values keep their bits beside pages of a larger scale whose weights are small). With BRASA_OUT_F16_SHORT for o_dtype (f16 results) q keeps 15 bits and the weights
- * are f16 values, whose rounding is of the size of the result's own: prompts take about two thirds of the time. Any hq a
- * multiple of hkv.
+ * same call. q: [tokens, hq, 128] f32, o: [tokens, hq, 128] in o_dtype. Any hq a multiple of hkv.
+ *
+ * Sums and softmax are f32, q and the weights are contracted as two f16 halves: 22 bits, down to 2^-32 of the row's largest
+ * weight times its page's V scale. BRASA_OUT_F16_SHORT as o_dtype takes 15 bits of q and f16 weights for f16 results: an error
+ * up to 1.4 times the results' own rounding, and for prompts three quarters of the time.
+ *
+ * (One row for each sequence and no shared prefix is brasa_decode_attention_paged's case too, which needs no plan. With 32 heads
+ * over 8, us a layer: one sequence of 257 positions 8.2 there and 12.0 here, of 16384 14.9 and 17.1, 128 of 100 14.0 and 15.2; 8
+ * of 4000 to 5000 23.1 and 22.8; 64 of 300 to 16000 104 and 94, 256 of 500 to 3000 191 and 177; a step's plan 6 to 11.)
  *
  * The plan of a step is laid out on the device by brasa_attention_paged_plan, once for all layers:
  * sequences group[g] .. group[g + 1] (as in brasa_kv_pages_shared) are taken to name the same pages in their first
  * prefix[g] positions (rounded down to whole pages; not checked: they may be brasa_kv_pages_shared's or a server's
- * own), and those pages are read and multiplied once for all rows of the group, but for sequences with too
- * many rows to gain from it or with positions below the prefix. groups == 0: none are shared. The calls that
- * follow take the plan's workspace and its n, width, tokens, hq and hkv; one whose sizes are not the plan's, or
+ * own), and those pages are read and multiplied once for all rows of the group, but for sequences whose rows
+ * together have 32 or more query heads of a KV head (with hq = 32 hkv a single row has) or that have positions below the prefix.
+ * groups == 0: none are shared. The calls that follow take the plan's workspace and its n, width, tokens, hq and hkv; one whose sizes are not the plan's, or
  * without a plan, fills o with NaN.
  *
  * Rows outside all sequences are left as they were in o. A sequence with a negative pos, one past the table, or a
